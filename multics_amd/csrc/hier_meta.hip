@@ -550,6 +550,140 @@ __global__ __launch_bounds__(kThreads) void meta_build_kernel(HierTopo t, HierMe
   }
 }
 
+// ---- windows of more frames than the arrays above hold ----------------------
+//
+// One block's (a cached call's) tile list over any number of runs, the runs in
+// chunks of kMaxRuns with the entries so far carried along.  The reference
+// formats are not made for such windows.
+
+__device__ void eval_chunk(const Topo& c, int kind, int s, int r0, int m, Shared& sh) {
+  for (int i = threadIdx.x; i < m; i += kThreads) {
+    const Run u = decode(c, kind, s, r0 + i);
+    uint32_t mask = 0;
+    for (int j = 0; j < c.t->n_frames; ++j)
+      if (u.width > 0 && allowed(c, kind, s, u, j)) mask |= 1u << j;
+    sh.mask[i] = mask;
+    sh.width[i] = u.width;
+    sh.val[i] = mask ? u.width : 0;
+    sh.doff[i] = mask ? tile_base(c, u) : 0;
+  }
+  __syncthreads();
+}
+
+__global__ __launch_bounds__(kThreads) void meta_count_long_kernel(HierTopo t, HierMetaCounts out) {
+  __shared__ Shared sh;
+  __shared__ int seg[32], logical[32], uni, dense;
+  Topo c;
+  c.t = &t;
+  c.b = 0;
+  const int s = blockIdx.x;
+  c.fa = t.fa[0]; c.fl = t.no_local ? 0 : t.fl[0]; c.fg = t.fg[0];
+  const int kind = stream_kind(t, s);
+  if (kind == kLocal && t.no_local) return;
+  const int R = num_runs(c, kind), n = t.n_frames;
+  if (threadIdx.x < 32) seg[threadIdx.x] = logical[threadIdx.x] = 0;
+  if (threadIdx.x == 0) uni = dense = 0;
+  __syncthreads();
+  for (int r = threadIdx.x; r < R; r += kThreads) {     // (integer sums: any order)
+    const Run u = decode(c, kind, s, r);
+    bool any = false;
+    for (int j = 0; j < n; ++j)
+      if (u.width > 0 && allowed(c, kind, s, u, j)) {
+        any = true;
+        atomicAdd(&seg[j], u.width);
+        if (u.present) atomicAdd(&logical[j], u.width);
+      }
+    if (any) atomicAdd(&uni, u.width);
+    if (u.present) atomicAdd(&dense, u.width);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) out.tile_count[s] = (uni + kTileKeys - 1) / kTileKeys * kTileKeys;
+  for (int j = threadIdx.x; j < n; j += kThreads) {
+    const int o = seg_id(t, kind, s, j);
+    out.seg_count[o] = seg[j];
+    out.logical_count[o] = logical[j];
+    out.dense_count[o] = dense;
+    out.tiled_count[o] = 0;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void meta_build_long_kernel(HierTopo t, HierMetaOut out) {
+  __shared__ Shared sh;
+  __shared__ int first;          // the first live run's first token
+  Topo c;
+  c.t = &t;
+  c.b = 0;
+  const int s = blockIdx.x;
+  c.fa = t.fa[0]; c.fl = t.no_local ? 0 : t.fl[0]; c.fg = t.fg[0];
+  const int kind = stream_kind(t, s);
+  if (kind == kLocal && t.no_local) return;
+  const int R = num_runs(c, kind), n = t.n_frames, qlen = qlen_of(t, kind);
+  const int tix = kind == kAgent ? 0 : (kind == kLocal ? 1 : 2);
+  const int64_t base = out.tile_kv_off[s];
+  if (threadIdx.x == 0) first = 0;
+  int done = 0;
+  for (int r0 = 0; r0 < R; r0 += kMaxRuns) {
+    const int m = min(kMaxRuns, R - r0);
+    __syncthreads();             // the last chunk's readers are done
+    eval_chunk(c, kind, s, r0, m, sh);
+    const int uni = lds_excl_prefix(sh.val, sh.off, m, sh.tmp4);
+    if (done == 0 && uni > 0 && threadIdx.x == 0) first = sh.doff[find_run(sh.off, m, 0)];
+    for (int i0 = 4 * threadIdx.x; i0 < uni; i0 += 4 * kThreads) {
+      int r = find_run(sh.off, m, i0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = i0 + e;
+        if (i >= uni) break;
+        while (r + 1 < m && sh.off[r + 1] <= i) ++r;
+        out.tile_kv_idx[base + done + i] = sh.doff[r] + (i - sh.off[r]);
+        out.tile_kv_mask[base + done + i] = sh.mask[r];
+      }
+    }
+    done += uni;
+  }
+  __syncthreads();
+  const int padded = (done + kTileKeys - 1) / kTileKeys * kTileKeys;
+  for (int i = done + threadIdx.x; i < padded; i += kThreads) {
+    out.tile_kv_idx[base + i] = first;
+    out.tile_kv_mask[base + i] = 0;
+  }
+  __syncthreads();               // every mask is written
+  const int lane = threadIdx.x & 63;
+  for (int k = threadIdx.x >> 6; k < padded / kTileKeys; k += kThreads / 64) {
+    uint32_t a = out.tile_kv_mask[base + k * kTileKeys + lane];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) a &= (uint32_t)__shfl_xor((int)a, d, 64);
+    if (lane == 0) out.tile_blk_and[base / kTileKeys + k] = a;
+  }
+  if (out.tile_items) {
+    const int rows = n * qlen, rpi = out.rows_per_item, nit = (rows + rpi - 1) / rpi;
+    for (int it = threadIdx.x; it < nit; it += kThreads) {
+      int32_t* d = out.tile_items + ((int64_t)out.tile_item_off[s] + it) * 8;
+      d[0] = t.tile_qbase[s];
+      d[1] = t.tile_qstride[tix];
+      d[2] = qlen;
+      d[3] = it * rpi;
+      d[4] = min(rpi, rows - it * rpi);
+      d[5] = (int32_t)base;
+      d[6] = padded;
+      d[7] = n;
+    }
+  }
+}
+
+// Runs and dense slots that a stream can have at most.
+int64_t most_runs(const HierTopo& t) {
+  return (int64_t)t.P * t.fa_max + (int64_t)t.N * t.fl_max + t.fg_max +
+         (int64_t)(t.P - 1) * t.n_frames;
+}
+int64_t most_slots(const HierTopo& t) {
+  return (int64_t)t.P * t.fa_max * t.L + (int64_t)t.N * t.fl_max * t.KL +
+         (int64_t)t.fg_max * t.KG + (int64_t)t.P * t.n_frames * t.L;
+}
+bool is_long(const HierTopo& t) {
+  return most_runs(t) > kMaxRuns || most_slots(t) > (int64_t)kMaxChunks * kTiledN;
+}
+
 int validate(const HierTopo* t) {
   HIER_REQUIRE(t != nullptr, HIER_EINVAL, "topology is NULL");
   HIER_REQUIRE(t->P >= 1 && t->N >= 1 && t->L >= 1 && t->KL >= 0 && t->KG >= 0, HIER_EINVAL,
@@ -561,10 +695,12 @@ int validate(const HierTopo* t) {
   HIER_REQUIRE(t->fa_max >= 0 && t->fl_max >= 0 && t->fg_max >= 0, HIER_EINVAL,
                "invalid frame pitches fa_max=%d fl_max=%d fg_max=%d", t->fa_max, t->fl_max,
                t->fg_max);
-  // bounds that keep every size product below in 64 bits (the run bound
-  // below implies P, N, fa_max, fl_max, fg_max <= kMaxRuns + 1 anyway)
-  HIER_REQUIRE(t->P <= kMaxRuns + 1 && t->N <= kMaxRuns + 1 && t->fa_max <= kMaxRuns &&
-                   t->fl_max <= kMaxRuns && t->fg_max <= kMaxRuns && t->L <= (1 << 20) &&
+  // bounds that keep every size product below in 64 bits (with the run bound
+  // below P, N, fa_max, fl_max, fg_max <= kMaxRuns + 1 anyway; one block alone,
+  // a cached window, may have more frames)
+  const int frames = t->B == 1 ? 1 << 20 : kMaxRuns;
+  HIER_REQUIRE(t->P <= kMaxRuns + 1 && t->N <= kMaxRuns + 1 && t->fa_max <= frames &&
+                   t->fl_max <= frames && t->fg_max <= frames && t->L <= (1 << 20) &&
                    t->KL <= (1 << 20) && t->KG <= (1 << 20) && t->B <= (1 << 20),
                HIER_EUNSUPPORTED, "topology too large (P=%d N=%d L=%d B=%d)", t->P, t->N, t->L,
                t->B);
@@ -580,16 +716,16 @@ int validate(const HierTopo* t) {
   HIER_REQUIRE(t->no_local || (t->local_frames && t->local_active && t->ref_local_base &&
                                t->tile_local_base),
                HIER_EINVAL, "local stream arrays missing");
-  int NS = t->P + t->N + 1;
-  int64_t rmax = (int64_t)t->P * t->fa_max + (int64_t)t->N * t->fl_max + t->fg_max +
-                 (int64_t)(t->P - 1) * t->n_frames;
+  const int64_t rmax = most_runs(*t), dmax = most_slots(*t);
+  if (t->B == 1) {
+    HIER_REQUIRE(dmax < (1ll << 31) - kTileKeys && rmax < (1ll << 31), HIER_EUNSUPPORTED,
+                 "too many cached tokens (%lld)", (long long)dmax);
+    return HIER_OK;
+  }
   HIER_REQUIRE(rmax <= kMaxRuns, HIER_EUNSUPPORTED, "too many cached frame runs (%lld > %d)",
                (long long)rmax, kMaxRuns);
-  int64_t dmax = (int64_t)t->P * t->fa_max * t->L + (int64_t)t->N * t->fl_max * t->KL +
-                 (int64_t)t->fg_max * t->KG + (int64_t)t->P * t->n_frames * t->L;
   HIER_REQUIRE(dmax <= (int64_t)kMaxChunks * kTiledN, HIER_EUNSUPPORTED,
                "dense slot list too long (%lld)", (long long)dmax);
-  (void)NS;
   return HIER_OK;
 }
 
@@ -603,6 +739,11 @@ extern "C" int hier_meta_count(const HierTopo* topo, const HierMetaCounts* count
                    counts->logical_count && counts->tile_count,
                HIER_EINVAL, "count output pointer is NULL");
   int grid = topo->B * (topo->P + topo->N + 1);
+  if (is_long(*topo)) {
+    hipLaunchKernelGGL(meta_count_long_kernel, dim3(grid), dim3(kThreads), 0, (hipStream_t)stream,
+                       *topo, *counts);
+    return hier::check_launch("meta_count_long_kernel");
+  }
   hipLaunchKernelGGL(meta_count_kernel, dim3(grid), dim3(kThreads), 0, (hipStream_t)stream,
                      *topo, *counts);
   return hier::check_launch("meta_count_kernel");
@@ -630,6 +771,14 @@ extern "C" int hier_meta_build(const HierTopo* topo, const HierMetaOut* out, voi
                      out->tiled_kv_off && out->tiled_max_k,
                  HIER_EINVAL, "tiled arrays incomplete");
   int grid = topo->B * (topo->P + topo->N + 1);
+  if (is_long(*topo)) {
+    HIER_REQUIRE(out->tile_kv_idx && !out->seg_kv_index && !out->tiled_kv_index, HIER_EUNSUPPORTED,
+                 "a window of this many frames has a tile list only (%lld runs, %lld slots)",
+                 (long long)most_runs(*topo), (long long)most_slots(*topo));
+    hipLaunchKernelGGL(meta_build_long_kernel, dim3(grid), dim3(kThreads), 0, (hipStream_t)stream,
+                       *topo, *out);
+    return hier::check_launch("meta_build_long_kernel");
+  }
   hipLaunchKernelGGL(meta_build_kernel, dim3(grid), dim3(kThreads), 0, (hipStream_t)stream,
                      *topo, *out);
   return hier::check_launch("meta_build_kernel");

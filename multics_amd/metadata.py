@@ -89,6 +89,7 @@ class TileList:
     fwd_items: Optional[torch.Tensor] = None
     fwd_n_items: int = 0
     row_table: Optional[torch.Tensor] = None
+    max_keys: int = 0            # entries of the longest built list; 0 = unknown
 
     def kept_tensors(self):
         """The list's tensors and those of its launch list."""
@@ -907,6 +908,7 @@ def build(topo: BlockTopology, device, *, segmented_block_m: Optional[int] = Non
                          rows_exact_cover=exact, fwd_items=fwd,
                          fwd_n_items=merge.fwd_n_items if merge is not None else 0,
                          row_table=merge.row_table if merge is not None else None)
+    tiles.max_keys = int(np.diff(tile_off).max(initial=0))
     tiles._keepalive = (dv, keep, merge)  # device inputs must outlive the async build
     # the fold plan, which the key-major list can take too (folded_key_list)
     tiles._fold = merge if merge is not None and merge.key_fold else None
