@@ -571,6 +571,133 @@ typedef struct HierGateArgs {
 
 int hier_gated_residual(const HierGateArgs* args, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Per-head RMSNorm, gain and rotation of the q and k projections in one     */
+/* pass (the projection tail of models that norm each head instead of the    */
+/* whole model dim; cf. attention.py:231-242, rope.py:248-254).  Per token   */
+/* and head: y = x / sqrt(mean(x^2) + eps) * w, then pairs (y[2i], y[2i+1])  */
+/* turned by (cos[i], sin[i]).  fp32 inside, one rounding to bf16.  q and k  */
+/* may have different numbers of heads; a projection's heads lie D apart in  */
+/* its row, the rows any stride apart (e.g. columns of one fused matrix).    */
+/* ------------------------------------------------------------------------ */
+typedef struct HierHeadNormArgs {
+  int64_t S;                       /* tokens                                   */
+  int32_t Hq, Hk, D;               /* heads of q and of k, head dim (64 or 128) */
+  float eps;
+  int32_t gain_bf16;               /* gains in bf16 (else fp32)                */
+  int32_t reserved;
+  const uint16_t* qx;              /* bf16 [S] rows of Hq * D                  */
+  const uint16_t* kx;              /* bf16 [S] rows of Hk * D                  */
+  int64_t qx_ss, kx_ss;            /* elements between rows                    */
+  const void* norm_q_w;            /* [D]                                      */
+  const void* norm_k_w;
+  const float* rope_cos;           /* [S][D/2]                                 */
+  const float* rope_sin;
+  uint16_t* q_out;                 /* bf16, element (s, h, d) at s*_ss + h*_sh + d */
+  uint16_t* k_out;
+  int64_t q_ss, q_sh, k_ss, k_sh;
+} HierHeadNormArgs;
+
+int hier_head_prologue(const HierHeadNormArgs* args, void* stream);
+
+/* Its gradient, recomputed from the inputs: dqx / dkx (contiguous rows) and   */
+/* the gains' gradients, summed over tokens and heads in a fixed order        */
+/* through partial, fp32 [hier_head_prologue_bwd_rows][D].                    */
+typedef struct HierHeadNormBwdArgs {
+  int64_t S;
+  int32_t Hq, Hk, D;
+  float eps;
+  int32_t gain_bf16, reserved;
+  const uint16_t* qx;
+  const uint16_t* kx;
+  int64_t qx_ss, kx_ss;
+  const void* norm_q_w;
+  const void* norm_k_w;
+  const float* rope_cos;
+  const float* rope_sin;
+  const uint16_t* dq;              /* bf16 gradients of q_out / k_out          */
+  const uint16_t* dk;
+  int64_t dq_ss, dq_sh, dk_ss, dk_sh;
+  uint16_t* dqx;                   /* bf16 [S][Hq * D]                         */
+  uint16_t* dkx;                   /* bf16 [S][Hk * D]                         */
+  float* dnorm_q;                  /* [D]                                      */
+  float* dnorm_k;
+  float* partial;
+} HierHeadNormBwdArgs;
+
+/* Rows of partial, or a negative error code.                                 */
+int hier_head_prologue_bwd_rows(const HierHeadNormBwdArgs* args);
+int hier_head_prologue_bwd(const HierHeadNormBwdArgs* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Paged KV cache held in 8 bits: e4m3 codes with one scale for each block    */
+/* of 16 pool rows (HIER_FP8_BLOCK) and head.  A scale is a power of two,     */
+/* stored as its exponent + 127 (e8m0): the smallest, not below 2^-100, that  */
+/* takes the block's largest magnitude to at most 448 (1 for a block of       */
+/* zeros), so that a code times its scale is exact in bf16.  A token whose K  */
+/* or V holds a value that is not finite in a head is kept as not a number    */
+/* there: K codes NaN, V codes 0 (it counts as zeros for the scales); V codes */
+/* are therefore always numbers, and a key that a query does not see adds     */
+/* nothing to it.                                                             */
+/* ------------------------------------------------------------------------ */
+enum { HIER_FP8_BLOCK = 16 };
+
+/* Append: source rows [src, src + count) of block-table row (src, dst, count) */
+/* go to pool rows [dst, dst + count), 1 <= count <= 16, dst a multiple of 16, */
+/* and set that block's scales.  Rows of the pool behind count are left as     */
+/* they are.  A table row outside these bounds or outside the pool is skipped.  */
+typedef struct HierPageFp8Args {
+  int32_t H, D;                    /* heads, head dim (64 or 128)              */
+  int32_t n_blocks;                /* rows of the block table                  */
+  int32_t n_rows;                  /* source rows                              */
+  int64_t pool_rows;               /* rows of each pool (multiple of 16)       */
+  const uint16_t* k_src;           /* bf16 rows of the block                   */
+  const uint16_t* v_src;
+  int64_t k_src_ss, k_src_sh, v_src_ss, v_src_sh;
+  const int32_t* blocks;           /* [n_blocks][3] DEVICE: src, dst, count    */
+  uint8_t* k_pool;                 /* e4m3 [pool_rows] rows                    */
+  uint8_t* v_pool;
+  int64_t pool_ss, pool_sh;        /* strides of both pools, bytes             */
+  uint8_t* k_scale;                /* e8m0 [pool_rows / 16]                    */
+  uint8_t* v_scale;
+  int64_t scale_ss, scale_sh;      /* strides of both scale arrays, bytes      */
+} HierPageFp8Args;
+
+int hier_kv_append_fp8(const HierPageFp8Args* args, void* stream);
+
+/* hier_attn_fwd over such a pool: the same lists, rows and results for K and */
+/* V the values that the pool stands for.  Query head h reads key head        */
+/* h / (H / Hk).  With splits > 1 every item's key list is cut into that many */
+/* parts, computed by workgroups of their own into part_o / part_ml, and      */
+/* joined in a fixed order by a second launch.                                */
+typedef struct HierFwdFp8Args {
+  int32_t H, Hk, D;                /* query heads, key heads, head dim         */
+  int32_t n_items;
+  float scale;                     /* softmax scale                            */
+  int32_t splits;                  /* >= 1                                     */
+  int64_t kv_rows;                 /* rows of each pool                        */
+  int64_t q_rows;                  /* rows of q / o                            */
+  const uint16_t* q;               /* bf16                                     */
+  const uint8_t* k;                /* e4m3 pools                               */
+  const uint8_t* v;
+  const uint8_t* k_scale;          /* e8m0                                     */
+  const uint8_t* v_scale;
+  uint16_t* o;                     /* bf16                                     */
+  float* lse;                      /* fp32 [H][lse_stride_h] or NULL           */
+  int64_t q_ss, q_sh, o_ss, o_sh, lse_stride_h;      /* elements               */
+  int64_t kv_ss, kv_sh;            /* bytes, of both pools                     */
+  int64_t scale_ss, scale_sh;      /* bytes, of both scale arrays              */
+  const int32_t* tile_items;       /* the list, as for hier_attn_fwd           */
+  const int32_t* tile_kv_idx;
+  const uint32_t* tile_kv_mask;
+  const uint32_t* tile_blk_and;
+  const int32_t* row_table;
+  float* part_o;                   /* [splits][H][q_rows][D] (splits > 1)      */
+  float* part_ml;                  /* [splits][H][q_rows][2] running max, sum  */
+} HierFwdFp8Args;
+
+int hier_attn_fwd_fp8(const HierFwdFp8Args* args, void* stream);
+
 /* Last error message of the calling thread ("" if none).                    */
 const char* hier_last_error(void);
 

@@ -162,6 +162,41 @@ class HierTrimArgs(C.Structure):
                [(n, vp) for n in ("items", "kv_mask", "row_table", "out_items")]
 
 
+class HierHeadNormArgs(C.Structure):
+    _fields_ = [("S", i64), ("Hq", i32), ("Hk", i32), ("D", i32), ("eps", f32),
+                ("gain_bf16", i32), ("reserved", i32), ("qx", vp), ("kx", vp), ("qx_ss", i64), ("kx_ss", i64)] + \
+               [(n, vp) for n in ("norm_q_w", "norm_k_w", "rope_cos", "rope_sin", "q_out",
+                                  "k_out")] + \
+               [(n, i64) for n in ("q_ss", "q_sh", "k_ss", "k_sh")]
+
+
+class HierHeadNormBwdArgs(C.Structure):
+    _fields_ = [("S", i64), ("Hq", i32), ("Hk", i32), ("D", i32), ("eps", f32),
+                ("gain_bf16", i32), ("reserved", i32), ("qx", vp), ("kx", vp), ("qx_ss", i64), ("kx_ss", i64)] + \
+               [(n, vp) for n in ("norm_q_w", "norm_k_w", "rope_cos", "rope_sin", "dq", "dk")] + \
+               [(n, i64) for n in ("dq_ss", "dq_sh", "dk_ss", "dk_sh")] + \
+               [(n, vp) for n in ("dqx", "dkx", "dnorm_q", "dnorm_k", "partial")]
+
+
+class HierPageFp8Args(C.Structure):
+    _fields_ = [("H", i32), ("D", i32), ("n_blocks", i32), ("n_rows", i32), ("pool_rows", i64),
+                ("k_src", vp), ("v_src", vp)] + \
+               [(n, i64) for n in ("k_src_ss", "k_src_sh", "v_src_ss", "v_src_sh")] + \
+               [(n, vp) for n in ("blocks", "k_pool", "v_pool")] + \
+               [("pool_ss", i64), ("pool_sh", i64), ("k_scale", vp), ("v_scale", vp),
+                ("scale_ss", i64), ("scale_sh", i64)]
+
+
+class HierFwdFp8Args(C.Structure):
+    _fields_ = [(n, i32) for n in ("H", "Hk", "D", "n_items")] + \
+               [("scale", f32), ("splits", i32), ("kv_rows", i64), ("q_rows", i64)] + \
+               [(n, vp) for n in ("q", "k", "v", "k_scale", "v_scale", "o", "lse")] + \
+               [(n, i64) for n in ("q_ss", "q_sh", "o_ss", "o_sh", "lse_stride_h", "kv_ss", "kv_sh",
+                                   "scale_ss", "scale_sh")] + \
+               [(n, vp) for n in ("tile_items", "tile_kv_idx", "tile_kv_mask", "tile_blk_and",
+                                  "row_table", "part_o", "part_ml")]
+
+
 EXPORTS = {
     "hier_meta_count": [C.POINTER(HierTopo), C.POINTER(HierMetaCounts), vp],
     "hier_meta_build": [C.POINTER(HierTopo), C.POINTER(HierMetaOut), vp],
@@ -185,6 +220,11 @@ EXPORTS = {
     "hier_kv_append": [C.POINTER(HierPageArgs), vp],
     "hier_frame_attn": [C.POINTER(HierFrameAttnArgs), vp],
     "hier_gated_residual": [C.POINTER(HierGateArgs), vp],
+    "hier_head_prologue": [C.POINTER(HierHeadNormArgs), vp],
+    "hier_head_prologue_bwd_rows": [C.POINTER(HierHeadNormBwdArgs)],
+    "hier_head_prologue_bwd": [C.POINTER(HierHeadNormBwdArgs), vp],
+    "hier_kv_append_fp8": [C.POINTER(HierPageFp8Args), vp],
+    "hier_attn_fwd_fp8": [C.POINTER(HierFwdFp8Args), vp],
     "hier_last_error": [],
     "hier_version": [],
 }
@@ -238,3 +278,15 @@ def stream_of(device: torch.device) -> int:
 
 def call(name: str, *args) -> None:
     check(getattr(lib(), name)(*args), name)
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """``call`` with the current stream of ``device`` as the last argument,
+    launched with that device current (a stream belongs to its device)."""
+    if device.type != "cuda":
+        raise ValueError(f"expected a GPU, got device {device}")
+    if device.index is None or device.index == torch.cuda.current_device():
+        call(name, *args, stream_of(device))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, stream_of(device))

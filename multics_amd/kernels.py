@@ -113,6 +113,15 @@ def _uncleared(like: torch.Tensor = None, *, size=None, dtype=None, device=None)
     return t
 
 
+def _attn_out(tiles, s, H, D, device):
+    """Output buffer of a forward: uncleared when the list's items own every
+    one of the s rows (the kernel then writes each, 0 for a row that sees no
+    key), zero-filled otherwise."""
+    if tiles.rows_exact_cover and tiles.row_extent == s:
+        return _uncleared(size=(s, H, D), dtype=torch.bfloat16, device=device)
+    return torch.zeros((s, H, D), dtype=torch.bfloat16, device=device)
+
+
 def _covers_all_rows(tiles: TileList) -> bool:
     """Whether the items of a full-sequence list own every row of
     [0, row_extent) exactly once, with queries and keys the same rows.  The
@@ -675,3 +684,268 @@ def qk_prologue_train(qx, kx, *, norm_q_w, norm_k_w, rope_cos, rope_sin, num_hea
     camc = None if cam is None else cam.to(torch.bfloat16).contiguous()
     return QKPrologueFunction.apply(qx.contiguous(), kx.contiguous(), norm_q_w, norm_k_w, camc,
                                     w_cam_q, w_cam_k, cs, sn, int(num_heads), float(eps))
+
+
+# --------------------------------------------------------------------------
+# per-head norms with rotation
+# --------------------------------------------------------------------------
+
+def _head_rows(name: str, t: torch.Tensor, dev) -> tuple:
+    """``t`` [S, H*D] bf16 as rows that the kernels read in place: unit channel
+    stride, 16-byte rows."""
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be [S, H*D], got {tuple(t.shape)}")
+    if t.dtype != torch.bfloat16:
+        raise NotImplementedError(f"{name} must be bf16, got {t.dtype}")
+    if not t.is_cuda:
+        raise NotImplementedError("per-head norms require GPU tensors")
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, expected {dev}")
+    if t.stride(1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
+        t = t.contiguous()
+    return t
+
+
+def _head_args(qx, kx, norm_q_w, norm_k_w, rope_cos, rope_sin, num_heads, num_kv_heads):
+    """The checked arguments that the per-head prologue and its gradient share:
+    (qx, kx, gains, cos, sin, Hq, Hk, D)."""
+    dev = qx.device
+    qx, kx = _head_rows("qx", qx, dev), _head_rows("kx", kx, dev)
+    Hq = int(num_heads)
+    Hk = Hq if num_kv_heads is None else int(num_kv_heads)
+    S, dim = qx.shape
+    if Hq < 1 or Hk < 1 or dim % Hq:
+        raise ValueError(f"{dim} channels do not divide into {Hq} heads (and {Hk} key heads)")
+    D = dim // Hq
+    if D not in (64, 128):
+        raise NotImplementedError(f"per-head norms support head_dim 64/128, got {D}")
+    if kx.shape != (S, Hk * D):
+        raise ValueError(f"kx must be [{S}, {Hk}*{D}], got {tuple(kx.shape)}")
+    gains = []
+    for name, w in (("norm_q_w", norm_q_w), ("norm_k_w", norm_k_w)):
+        if w.shape != (D,) or w.dtype not in (torch.bfloat16, torch.float32) or w.device != dev:
+            raise ValueError(f"{name} must be [{D}] bf16 or fp32 on {dev}, got {tuple(w.shape)} "
+                             f"{w.dtype} on {w.device}")
+        gains.append(w)
+    if gains[0].dtype != gains[1].dtype:
+        gains = [w.float() for w in gains]
+    gains = [w.contiguous() if w.data_ptr() % 16 == 0 else w.clone() for w in gains]
+    tables = []
+    for name, t in (("rope_cos", rope_cos), ("rope_sin", rope_sin)):
+        if t.shape != (S, D // 2) or t.device != dev:
+            raise ValueError(f"{name} must be [S, D/2] = {(S, D // 2)} on {dev}, got "
+                             f"{tuple(t.shape)} on {t.device}")
+        t = t.contiguous().float()
+        tables.append(t if t.data_ptr() % 16 == 0 else t.clone())
+    return qx, kx, gains, tables[0], tables[1], Hq, Hk, D
+
+
+def _head_common(qx, kx, gains, cs, sn, Hq, Hk, D, eps):
+    return dict(S=qx.shape[0], Hq=Hq, Hk=Hk, D=D, eps=float(eps),
+                gain_bf16=int(gains[0].dtype == torch.bfloat16), reserved=0, qx=qx.data_ptr(),
+                kx=kx.data_ptr(), qx_ss=qx.stride(0), kx_ss=kx.stride(0),
+                norm_q_w=gains[0].data_ptr(), norm_k_w=gains[1].data_ptr(),
+                rope_cos=cs.data_ptr(), rope_sin=sn.data_ptr())
+
+
+def qk_head_prologue(qx: torch.Tensor, kx: torch.Tensor, *, norm_q_w: torch.Tensor,
+                     norm_k_w: torch.Tensor, rope_cos: torch.Tensor, rope_sin: torch.Tensor,
+                     num_heads: int, eps: float, num_kv_heads: Optional[int] = None,
+                     out_layout: str = "shd"):
+    """RMSNorm of every head of q and k, gain and rotation in one HIP pass
+    (``hier_head_prologue``): per token and head
+    ``y = x / sqrt(mean(x^2) + eps) * w``, then the pairs (y[2i], y[2i+1])
+    turned by (cos[i], sin[i]); fp32 inside, rounded once.
+
+    ``qx`` [S, H*D] and ``kx`` [S, Hk*D] are bf16 projections (Hk =
+    ``num_kv_heads`` or H; D 64 or 128), contiguous or columns of one fused
+    projection, read in place.  Gains [D] are bf16 or fp32, shared by the
+    heads; the tables are [S, D/2].  Returns ``(q, k)`` bf16 [S, H, D] /
+    [S, Hk, D] of token-major (``out_layout="shd"``) or head-major (``"hsd"``)
+    storage.  No gradient: ``qk_head_prologue_train``."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (qx, kx, norm_q_w, norm_k_w)):
+        raise RuntimeError("qk_head_prologue gives no gradient: use qk_head_prologue_train")
+    qx, kx, gains, cs, sn, Hq, Hk, D = _head_args(qx, kx, norm_q_w, norm_k_w, rope_cos, rope_sin,
+                                                  num_heads, num_kv_heads)
+    S, dev = qx.shape[0], qx.device
+    if out_layout == "shd":
+        mk = lambda H: torch.empty((S, H, D), dtype=torch.bfloat16, device=dev)  # noqa: E731
+    elif out_layout == "hsd":
+        mk = lambda H: torch.empty((H, S, D), dtype=torch.bfloat16, device=dev).transpose(0, 1)  # noqa: E731
+    else:
+        raise ValueError(f"unknown layout {out_layout!r}")
+    q, k = mk(Hq), mk(Hk)
+    if S:
+        args = _capi.HierHeadNormArgs(
+            q_out=q.data_ptr(), k_out=k.data_ptr(), q_ss=q.stride(0), q_sh=q.stride(1),
+            k_ss=k.stride(0), k_sh=k.stride(1), **_head_common(qx, kx, gains, cs, sn, Hq, Hk, D, eps))
+        _capi.call_on(dev, "hier_head_prologue", C.byref(args))
+    return q, k
+
+
+def qk_head_prologue_backward(dq: torch.Tensor, dk: torch.Tensor, qx: torch.Tensor,
+                              kx: torch.Tensor, *, norm_q_w: torch.Tensor, norm_k_w: torch.Tensor,
+                              rope_cos: torch.Tensor, rope_sin: torch.Tensor, num_heads: int,
+                              eps: float, num_kv_heads: Optional[int] = None):
+    """Gradient of ``qk_head_prologue`` (``hier_head_prologue_bwd``) from its
+    inputs and the gradients ``dq`` [S, H, D] / ``dk`` [S, Hk, D] (bf16) of its
+    outputs: ``(dqx, dkx, dnorm_q, dnorm_k)``, bf16 [S, H*D] / [S, Hk*D] and
+    fp32 [D].  The gains' sums over tokens and heads are taken in a fixed
+    order: equal inputs give equal bits."""
+    qx, kx, gains, cs, sn, Hq, Hk, D = _head_args(qx, kx, norm_q_w, norm_k_w, rope_cos, rope_sin,
+                                                  num_heads, num_kv_heads)
+    S, dev = qx.shape[0], qx.device
+    outs = []
+    for name, g, H in (("dq", dq, Hq), ("dk", dk, Hk)):
+        if g.shape != (S, H, D) or g.dtype != torch.bfloat16 or g.device != dev:
+            raise ValueError(f"{name} must be bf16 [{S}, {H}, {D}] on {dev}, got "
+                             f"{tuple(g.shape)} {g.dtype} on {g.device}")
+        if g.stride(2) != 1 or g.stride(0) % 8 or g.stride(1) % 8 or g.data_ptr() % 16:
+            g = g.contiguous()
+        outs.append(g)
+    dq, dk = outs
+    dqx = torch.empty((S, Hq * D), dtype=torch.bfloat16, device=dev)
+    dkx = torch.empty((S, Hk * D), dtype=torch.bfloat16, device=dev)
+    if S == 0:
+        return (dqx, dkx) + tuple(torch.zeros(D, device=dev) for _ in range(2))
+    dw = torch.empty((2, D), dtype=torch.float32, device=dev)
+    args = _capi.HierHeadNormBwdArgs(
+        dq=dq.data_ptr(), dk=dk.data_ptr(), dq_ss=dq.stride(0), dq_sh=dq.stride(1),
+        dk_ss=dk.stride(0), dk_sh=dk.stride(1), dqx=dqx.data_ptr(), dkx=dkx.data_ptr(),
+        dnorm_q=dw[0].data_ptr(), dnorm_k=dw[1].data_ptr(),
+        **_head_common(qx, kx, gains, cs, sn, Hq, Hk, D, eps))
+    rows = int(_capi.lib().hier_head_prologue_bwd_rows(C.byref(args)))
+    part = torch.empty((max(rows, 1), D), dtype=torch.float32, device=dev)
+    args.partial = part.data_ptr()
+    _capi.call_on(dev, "hier_head_prologue_bwd", C.byref(args))
+    return dqx, dkx, dw[0], dw[1]
+
+
+class QKHeadPrologueFunction(torch.autograd.Function):
+    """Differentiable ``qk_head_prologue``: gradients for the projections and
+    the gains (none for the tables)."""
+
+    @staticmethod
+    def forward(ctx, qx, kx, norm_q_w, norm_k_w, rope_cos, rope_sin, num_heads, num_kv_heads, eps,
+                out_layout):
+        ctx.save_for_backward(qx, kx, norm_q_w, norm_k_w, rope_cos, rope_sin)
+        ctx.heads = dict(num_heads=num_heads, num_kv_heads=num_kv_heads, eps=eps)
+        return qk_head_prologue(qx, kx, norm_q_w=norm_q_w, norm_k_w=norm_k_w, rope_cos=rope_cos,
+                                rope_sin=rope_sin, out_layout=out_layout, **ctx.heads)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        qx, kx, wq, wk, cs, sn = ctx.saved_tensors
+        dqx, dkx, dwq, dwk = qk_head_prologue_backward(
+            dq.to(torch.bfloat16), dk.to(torch.bfloat16), qx, kx, norm_q_w=wq, norm_k_w=wk,
+            rope_cos=cs, rope_sin=sn, **ctx.heads)
+        return (dqx, dkx, dwq.to(wq.dtype), dwk.to(wk.dtype)) + (None,) * 6
+
+
+def qk_head_prologue_train(qx, kx, *, norm_q_w, norm_k_w, rope_cos, rope_sin, num_heads, eps,
+                           num_kv_heads=None, out_layout="shd"):
+    """``qk_head_prologue`` under autograd: differentiable in the projections
+    and the gains.  The same arguments and results."""
+    return QKHeadPrologueFunction.apply(qx, kx, norm_q_w, norm_k_w, rope_cos, rope_sin,
+                                        int(num_heads),
+                                        None if num_kv_heads is None else int(num_kv_heads),
+                                        float(eps), out_layout)
+
+
+# --------------------------------------------------------------------------
+# attention over a cache held in 8 bits
+# --------------------------------------------------------------------------
+
+def _fp8_splits(workgroups: int, max_tiles: int) -> int:
+    """Parts that every item's key list is cut into: one where the items fill
+    the 512 workgroups that run at once (two a CU), else enough to fill them,
+    of two 64-key tiles at least, at most 32."""
+    if workgroups >= 512:
+        return 1
+    return max(1, min(32, -(-512 // workgroups), max_tiles // 2))
+
+
+def hier_cached_attention_fp8(q: torch.Tensor, cache, tiles: TileList, *,
+                              out: Optional[torch.Tensor] = None,
+                              lse: Optional[torch.Tensor] = None,
+                              scale: Optional[float] = None) -> torch.Tensor:
+    """Hierarchical attention of a rollout block over a ``HierPagedKVCache``
+    held in 8 bits (``hier_attn_fwd_fp8``): what ``hier_attention_forward``
+    computes over the values that the cache stands for
+    (``cache.dequantised()``), read from the codes.
+
+    ``q`` is bf16 [S, H, D] (or [1, S, H, D]) in the cached query order with a
+    unit-stride head dimension; H is the cache's ``batch * num_heads`` or a
+    multiple of it (query heads g*i .. g*i + g-1 then share the cache's head i).
+    ``tiles`` is the block's list over the cache's pool
+    (``metadata.cached_window_tiles``).  Returns ``out``, bf16 [S, H, D] (made
+    here when not given; rows of no item are 0 then, and left as they were in
+    a given one); a row that sees no key is 0.  ``lse`` (optional, fp32 [H, S])
+    receives the natural-log softmax normaliser.  Inference only."""
+    if torch.is_grad_enabled() and q.requires_grad:
+        raise RuntimeError("attention over an 8-bit cache is inference-only (q requires grad)")
+    if not getattr(cache, "fp8", False):
+        raise ValueError("the cache is not held in 8 bits: use hier_attention_forward")
+    if q.dtype != torch.bfloat16:
+        raise NotImplementedError(f"q must be bf16, got {q.dtype}")
+    if not q.is_cuda:
+        raise NotImplementedError("hierarchical attention requires a GPU tensor")
+    dev = q.device
+    if cache.k.device != dev or tiles.items.device != dev:
+        raise ValueError(f"q is on {dev}, the cache on {cache.k.device}, the tile list on "
+                         f"{tiles.items.device}")
+    q3, q_ss, q_sh = _rows_view(q)
+    S, H, D = q3.shape
+    if q_ss % 8 or q_sh % 8 or q3.data_ptr() % 16:
+        q3 = q3.contiguous()
+        q_ss, q_sh = q3.stride(0), q3.stride(1)
+    rows, Hk = cache.k.shape[:2]
+    if D != cache.D or H % Hk:
+        raise ValueError(f"q has {H} heads of {D}, the cache {Hk} of {cache.D}: the heads must be "
+                         "a multiple of the cache's")
+    if tiles.rows_per_item != 128:
+        raise ValueError("hier_attn_fwd_fp8 processes work items of up to 128 query rows")
+    if rows < tiles.key_extent:
+        raise ValueError(f"the cache holds {rows} rows, the tile list addresses {tiles.key_extent}")
+    if S < tiles.row_extent:
+        raise ValueError(f"q holds {S} rows, the tile list addresses {tiles.row_extent}")
+    if out is None:
+        out = _attn_out(tiles, S, H, D, dev)
+    elif out.dtype != torch.bfloat16 or out.device != dev or out.shape not in (q.shape, q3.shape):
+        raise ValueError(f"out must be bf16 {tuple(q3.shape)} on {dev}, got {tuple(out.shape)} "
+                         f"{out.dtype} on {out.device}")
+    o3 = out[0] if out.dim() == 4 else out
+    if o3.stride(2) != 1 or o3.stride(0) % 8 or o3.stride(1) % 8 or o3.data_ptr() % 16:
+        raise ValueError("out must have a unit-stride head dimension and 16-byte rows")
+    if lse is not None and (lse.dtype != torch.float32 or lse.dim() != 2 or lse.shape[0] != H or
+                            lse.shape[1] < tiles.row_extent or lse.stride(1) != 1 or
+                            lse.device != dev):
+        raise ValueError("lse must be fp32 [H, >=rows] with unit row stride")
+    run = M.launch_list(tiles)
+    items, n_items = (run.items, tiles.n_items) if run.fwd_items is None else \
+        (run.fwd_items, tiles.fwd_n_items)
+    if n_items == 0:
+        return out
+    max_tiles = (tiles.max_keys or tiles.kv_idx.numel()) // M.TILE_KEYS
+    splits = _fp8_splits(n_items * H, max_tiles)
+    part = torch.empty(splits * H * tiles.row_extent * (D + 2), dtype=torch.float32, device=dev) \
+        if splits > 1 else None
+    table = tiles.row_table
+    args = _capi.HierFwdFp8Args(
+        H=H, Hk=Hk, D=D, n_items=n_items,
+        scale=float(scale if scale is not None else 1.0 / math.sqrt(D)), splits=splits,
+        kv_rows=rows, q_rows=tiles.row_extent, q=q3.data_ptr(), k=cache.k.data_ptr(),
+        v=cache.v.data_ptr(), k_scale=cache.k_scale.data_ptr(), v_scale=cache.v_scale.data_ptr(),
+        o=o3.data_ptr(), lse=None if lse is None else lse.data_ptr(), q_ss=q_ss, q_sh=q_sh,
+        o_ss=o3.stride(0), o_sh=o3.stride(1), lse_stride_h=0 if lse is None else lse.stride(0),
+        kv_ss=cache.k.stride(0), kv_sh=cache.k.stride(1), scale_ss=cache.k_scale.stride(0),
+        scale_sh=cache.k_scale.stride(1), tile_items=items.data_ptr(),
+        tile_kv_idx=tiles.kv_idx.data_ptr(), tile_kv_mask=tiles.kv_mask.data_ptr(),
+        tile_blk_and=tiles.blk_and.data_ptr(),
+        row_table=None if table is None else table.data_ptr())
+    if part is not None:
+        args.part_o = part.data_ptr()
+        args.part_ml = part.data_ptr() + 4 * splits * H * tiles.row_extent * D
+    _capi.call_on(dev, "hier_attn_fwd_fp8", C.byref(args))
+    return out

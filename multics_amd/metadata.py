@@ -1815,7 +1815,7 @@ def cached_window_tiles(cache, end_frame: int, *, device, n_frames, n_block, loc
     them."""
     raw = lambda x: None if x is None else (np.shape(x), np.asarray(x).tobytes())
     key = ("window", str(device), cache.P, cache.N, cache.L, cache.KL, cache.KG, cache.R,
-           cache.no_local, int(end_frame), cache.slot_frame.tobytes(),
+           cache.pages, cache.no_local, int(end_frame), cache.slot_frame.tobytes(),
            cache.local_active.tobytes(), n_frames, n_block, local_attn, raw(labels), raw(q_active),
            bool(direct_player), bool(hier_no_local_hub), raw(membership), raw(global_only))
     hit = _lru_get(_META_CACHE, key)

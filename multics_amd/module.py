@@ -24,6 +24,9 @@ cam_q, cam_k``), mutable attributes and call signatures as the reference module
 Q/K/V projection: with autograd active, torch ops with the reference's
 rounding points (camera adapter, RMSNorm in fp32, RoPE in float64); without
 autograd, the fused HIP prologue (camera + RMSNorm + gain + RoPE in one pass).
+With ``qk_norm="head"`` (an addition to the reference's constructor) q and k are
+normed for each head, on ``kernels.qk_head_prologue`` with and without autograd.
+A cache held in 8 bits runs on ``kernels.hier_cached_attention_fp8``.
 """
 
 from __future__ import annotations
@@ -34,8 +37,9 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import metadata as M
-from .kernels import (_uncleared, gated_residual, hier_attention,
-                      hier_attention_forward, qk_prologue_train, qkv_prologue)
+from .kernels import (_attn_out, gated_residual, hier_attention, hier_attention_forward,
+                      hier_cached_attention_fp8, qk_head_prologue, qk_head_prologue_train,
+                      qk_prologue_train, qkv_prologue)
 from .hier_masks import HierBlockMask
 from .kv_cache import stream_pool
 from .paged_cache import HierPagedKVCache
@@ -91,27 +95,24 @@ def rope_apply(x: torch.Tensor, freqs: torch.Tensor, num_heads: int) -> torch.Te
     return torch.view_as_real(xc * freqs.to(x.device)).flatten(2).to(x.dtype)
 
 
-def _attn_out(tiles, s, H, D, device):
-    """Output buffer of a forward: uncleared when the list's items own every
-    one of the s rows (the kernel then writes each, 0 for a row that sees no
-    key), zero-filled otherwise."""
-    if tiles.rows_exact_cover and tiles.row_extent == s:
-        return _uncleared(size=(s, H, D), dtype=torch.bfloat16, device=device)
-    return torch.zeros((s, H, D), dtype=torch.bfloat16, device=device)
-
-
 class SelfAttention(nn.Module):
-    def __init__(self, dim: int, num_heads: int, eps: float = 1e-06):
+    def __init__(self, dim: int, num_heads: int, eps: float = 1e-06, qk_norm: str = "model"):
+        """``qk_norm``: RMSNorm of q and k over the whole model dim
+        (``"model"``, the reference's) or over each head (``"head"``: gains of
+        one head's channels, shared by the heads)."""
         super().__init__()
+        if qk_norm not in ("model", "head"):
+            raise ValueError(f"qk_norm must be 'model' or 'head', got {qk_norm!r}")
         self.dim = dim
+        self.qk_norm = qk_norm
         self.num_heads = num_heads
         self.head_dim = dim // num_heads
         self.q = nn.Linear(dim, dim)
         self.k = nn.Linear(dim, dim)
         self.v = nn.Linear(dim, dim)
         self.o = nn.Linear(dim, dim)
-        self.norm_q = RMSNorm(dim, eps=eps)
-        self.norm_k = RMSNorm(dim, eps=eps)
+        self.norm_q = RMSNorm(dim if qk_norm == "model" else self.head_dim, eps=eps)
+        self.norm_k = RMSNorm(dim if qk_norm == "model" else self.head_dim, eps=eps)
         self.eps = eps
         self.sink_size = 0
         self.local_attn_size = 6
@@ -167,8 +168,10 @@ class SelfAttention(nn.Module):
     def _project_self_attn_qkv(self, x, freqs, cam_tokens=None):
         """Differentiable Q/K/V (attention.py:355-365)."""
         qx, kx = self._apply_camera_qk(self.q(x), self.k(x), cam_tokens)
-        q = rope_apply(self.norm_q(qx), freqs, self.num_heads)
-        k = rope_apply(self.norm_k(kx), freqs, self.num_heads)
+        norm = lambda m, t: m(t) if self.qk_norm == "model" else \
+            m(t.unflatten(-1, (self.num_heads, self.head_dim))).flatten(-2)
+        q = rope_apply(norm(self.norm_q, qx), freqs, self.num_heads)
+        k = rope_apply(norm(self.norm_k, kx), freqs, self.num_heads)
         return q, k, self.v(x)
 
     def _fused_ok(self, x, cam_tokens) -> bool:
@@ -183,6 +186,8 @@ class SelfAttention(nn.Module):
         keys one contiguous slab: the K gathers fetch fewer bytes from HBM,
         at the same speed), V the v projection itself, read in place (the
         attention kernels take any row / head strides)."""
+        if self.qk_norm == "head":
+            return self._project_heads(x, freqs, cam_tokens, qk_head_prologue)
         cam = self._check_cam(x, cam_tokens)
         qx, kx, vx = (lin(x)[0].contiguous() for lin in (self.q, self.k, self.v))
         cs, sn = freqs_to_cos_sin(freqs, device=x.device)
@@ -194,15 +199,30 @@ class SelfAttention(nn.Module):
             w_cam_k=None if cam is None else self.cam_k.weight, out_layout="hsd")
         return q, k, vx.view(vx.shape[0], self.num_heads, self.head_dim)
 
+    def _project_heads(self, x, freqs, cam_tokens, prologue):
+        """[S, H, D] Q/K/V with per-head norms: the GEMMs, the camera adapter's
+        product where there are camera tokens, and ``prologue`` (the HIP pass,
+        with or without its gradient) on q and k."""
+        s, H, D = x.shape[1], self.num_heads, self.head_dim
+        qx, kx = self._apply_camera_qk(self.q(x), self.k(x), cam_tokens)
+        cs, sn = freqs_to_cos_sin(freqs, device=x.device)
+        q, k = prologue(qx.view(s, H * D), kx.view(s, H * D), norm_q_w=self.norm_q.weight,
+                        norm_k_w=self.norm_k.weight, rope_cos=cs, rope_sin=sn, num_heads=H,
+                        eps=self.norm_q.eps, out_layout="hsd")
+        return q, k, self.v(x).view(s, H, D)
+
     def _project_train(self, x, freqs, cam_tokens):
         """Differentiable [S, H, D] bf16 Q/K/V.  On the GPU, for bf16 weights and
-        model dims that are multiples of 512 (up to 4096), the q / k tail runs
-        on the HIP prologue forward and backward (``qk_prologue_train``) after
-        the three GEMMs; otherwise the reference's torch ops
+        model dims that are multiples of 512 (up to 4096; any with per-head
+        norms), the q / k tail runs on the HIP prologue forward and backward
+        (``qk_prologue_train``, ``qk_head_prologue_train``) after the three
+        GEMMs; otherwise the reference's torch ops
         (``_project_self_attn_qkv``)."""
         s = x.shape[1]
         H, D = self.num_heads, self.head_dim
         dim = H * D
+        if self.qk_norm == "head" and self._fused_ok(x, cam_tokens):
+            return self._project_heads(x, freqs, cam_tokens, qk_head_prologue_train)
         if self._fused_ok(x, cam_tokens) and dim % 512 == 0 and dim <= 4096:
             cam = self._check_cam(x, cam_tokens)
             # (views of the [1, s, dim] projections: the backward of an index
@@ -451,8 +471,11 @@ class SelfAttention(nn.Module):
             labels=None if labels is None else labels.numpy(), q_active=act.numpy(),
             direct_player=bool(direct_player), membership=mem.numpy() if use_mem else None,
             global_only=go.numpy() if use_mem else None, hier_no_local_hub=no_local)
-        out = _attn_out(tiles, s, b * H, D, x.device)
-        hier_attention_forward(q, kv_cache.k, kv_cache.v, tiles, out)
+        if kv_cache.fp8:
+            out = hier_cached_attention_fp8(q, kv_cache, tiles)
+        else:
+            out = _attn_out(tiles, s, b * H, D, x.device)
+            hier_attention_forward(q, kv_cache.k, kv_cache.v, tiles, out)
         out = out.view(s, b, dim).transpose(0, 1)
         return self.o(out.to(self.o.weight.dtype))
 

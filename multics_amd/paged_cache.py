@@ -19,6 +19,13 @@ overwrites the same pages, which is the reference's refresh-in-place; a new
 frame overwrites the page of frame f - R, which is the reference's eviction.
 No row ever moves and nothing is concatenated: the attention tile list
 addresses the pool rows directly.
+
+With ``dtype=torch.float8_e4m3fn`` the pools hold 8-bit codes and, for every 16
+rows and head, a power-of-two scale (``k_scale`` / ``v_scale``, e8m0
+``[rows / 16, batch * H]``); a value is its code times its scale.  Pages are
+padded to whole blocks of 16 rows, so that a block belongs to one page and is
+always written as a whole (220 tokens: 224 rows).  ``append`` quantises
+(``hier_kv_append_fp8``), ``kernels.hier_cached_attention_fp8`` reads the codes.
 """
 
 from __future__ import annotations
@@ -34,6 +41,8 @@ from . import _capi
 
 _stream = _capi.stream_of
 
+FP8_BLOCK = 16      # rows that share a scale (HIER_FP8_BLOCK)
+
 
 class HierPagedKVCache:
     """One layer's hierarchical KV cache (pools + ring bookkeeping).
@@ -48,6 +57,9 @@ class HierPagedKVCache:
     pair of caches (wan_video_Nplayers.py:645-648, one model call per prompt
     at :739-776) then shares the ring bookkeeping, the tile list and one
     kernel launch per block, which sees ``batch * H`` heads.
+
+    ``dtype`` is bf16, or ``torch.float8_e4m3fn`` for a cache held in 8 bits
+    (half the memory; head dim 64 or 128).
     """
 
     def __init__(self, *, num_players: int, num_groups: int, num_patches: int,
@@ -73,13 +85,31 @@ class HierPagedKVCache:
             if self.W < self.n:
                 raise ValueError("hier_hub requires local_attn_size=-1 or >= num_frame_per_block")
             self.R = self.W + self.n
-        self.a_rows = self.P * self.R * self.L
-        self.l_rows = 0 if self.no_local else self.N * self.R * self.KL
-        self.g_rows = self.R * self.KG
+        self.fp8 = dtype == torch.float8_e4m3fn
+        if dtype.itemsize == 1 and not self.fp8:
+            raise NotImplementedError(f"an 8-bit cache holds float8_e4m3fn, got {dtype}")
+        if self.fp8 and self.D not in (64, 128):
+            raise NotImplementedError(f"an 8-bit cache supports head_dim 64/128, got {self.D}")
+        # rows of a page: the frame's tokens, in whole blocks when they share scales
+        page = (lambda w: -(-w // FP8_BLOCK) * FP8_BLOCK) if self.fp8 else (lambda w: w)
+        self.pages = (page(self.L), page(self.KL), page(self.KG))
+        self.a_rows = self.P * self.R * self.pages[0]
+        self.l_rows = 0 if self.no_local else self.N * self.R * self.pages[1]
+        self.g_rows = self.R * self.pages[2]
         rows = self.a_rows + self.l_rows + self.g_rows
         self.device = torch.device(device)
-        self.k = torch.zeros((rows, self.B * self.H, self.D), dtype=dtype, device=self.device)
-        self.v = torch.zeros_like(self.k)
+        heads = self.B * self.H
+        if self.fp8:
+            # head-major storage: a head's codes of a page lie in one piece
+            code = lambda: torch.zeros((heads, rows, self.D), dtype=torch.uint8,  # noqa: E731
+                                       device=self.device).view(dtype).transpose(0, 1)
+            one = lambda: torch.full((heads, rows // FP8_BLOCK), 127, dtype=torch.uint8,  # noqa: E731
+                                     device=self.device).view(torch.float8_e8m0fnu).t()
+            self.k, self.v, self.k_scale, self.v_scale = code(), code(), one(), one()
+        else:
+            self.k = torch.zeros((rows, heads, self.D), dtype=dtype, device=self.device)
+            self.v = torch.zeros_like(self.k)
+            self.k_scale = self.v_scale = None
         self.slot_frame = np.full(self.R, -1, dtype=np.int64)
         self.local_active = np.zeros((max(self.N, 1), self.R), dtype=bool)
         self._dst_cache = {}
@@ -105,27 +135,44 @@ class HierPagedKVCache:
     # ---- addressing ----------------------------------------------------------------
 
     def agent_row(self, p: int, frame: int) -> int:
-        return (p * self.R + frame % self.R) * self.L
+        return (p * self.R + frame % self.R) * self.pages[0]
 
     def local_row(self, g: int, frame: int) -> int:
-        return self.a_rows + (g * self.R + frame % self.R) * self.KL
+        return self.a_rows + (g * self.R + frame % self.R) * self.pages[1]
 
     def global_row(self, frame: int) -> int:
-        return self.a_rows + self.l_rows + (frame % self.R) * self.KG
+        return self.a_rows + self.l_rows + (frame % self.R) * self.pages[2]
 
     def block_rows(self, start_frame: int, n: int) -> np.ndarray:
         """Pool row of every token of a block in the cached query order
         [P*n*L agents | n*N*KL locals | n*KG global]."""
         P, N, L, KL, KG = self.P, self.N, self.L, self.KL, self.KG
+        pa, pl, pg = self.pages
         fr = start_frame + np.arange(n)
         slot = fr % self.R
-        agent = ((np.arange(P)[:, None, None] * self.R + slot[None, :, None]) * L +
+        agent = ((np.arange(P)[:, None, None] * self.R + slot[None, :, None]) * pa +
                  np.arange(L)[None, None, :]).reshape(-1)
-        local = (self.a_rows + (np.arange(N)[None, :, None] * self.R + slot[:, None, None]) * KL +
+        local = (self.a_rows + (np.arange(N)[None, :, None] * self.R + slot[:, None, None]) * pl +
                  np.arange(KL)[None, None, :]).reshape(-1) if not self.no_local else \
             np.zeros(0, np.int64)
-        glob = (self.a_rows + self.l_rows + slot[:, None] * KG + np.arange(KG)[None, :]).reshape(-1)
+        glob = (self.a_rows + self.l_rows + slot[:, None] * pg + np.arange(KG)[None, :]).reshape(-1)
         return np.concatenate([agent, local, glob]).astype(np.int32)
+
+    def block_table(self, start_frame: int, n: int) -> np.ndarray:
+        """``[n_blocks, 3]`` int32 (source row, pool row, rows) of the blocks of
+        16 pool rows that a block's tokens fill: every page's tokens in runs
+        of 16, the last shorter."""
+        rows = self.block_rows(start_frame, n)
+        widths = [self.L] * (self.P * n) + \
+            ([] if self.no_local else [self.KL] * (n * self.N)) + [self.KG] * n
+        src, count, at = [], [], 0
+        for w in widths:
+            first = np.arange(0, w, FP8_BLOCK)
+            src.append(at + first)
+            count.append(np.minimum(FP8_BLOCK, w - first))
+            at += w
+        src = np.concatenate(src)
+        return np.stack([src, rows[src], np.concatenate(count)], axis=1).astype(np.int32)
 
     # ---- append ----------------------------------------------------------------------
 
@@ -140,8 +187,12 @@ class HierPagedKVCache:
         if k_blk.shape != (S, HB, self.D) or v_blk.shape != (S, HB, self.D):
             raise ValueError(f"block K/V must be [{S}, {HB}, {self.D}], "
                              f"got {tuple(k_blk.shape)}, {tuple(v_blk.shape)}")
-        if k_blk.dtype != self.k.dtype or v_blk.dtype != self.k.dtype:
-            raise ValueError("block K/V dtype must match the cache")
+        want = torch.bfloat16 if self.fp8 else self.k.dtype
+        if k_blk.dtype != want or v_blk.dtype != want:
+            raise ValueError("block K/V dtype must match the cache" if not self.fp8 else
+                             "an 8-bit cache takes bf16 K/V")
+        if self.fp8 and (k_blk.device != self.k.device or v_blk.device != self.k.device):
+            raise ValueError(f"block K/V must be on the cache's device {self.k.device}")
         if n > self.R:
             raise ValueError(f"a block of {n} frames does not fit a window of {self.R} frames")
         if self.W == -1 and (start_frame < 0 or start_frame + n > self.R):
@@ -152,8 +203,22 @@ class HierPagedKVCache:
         key = (start_frame % self.R, n)
         dst = self._dst_cache.get(key)
         if dst is None:
-            dst = torch.from_numpy(self.block_rows(start_frame, n)).to(self.device)
+            dst = torch.from_numpy(self.block_table(start_frame, n) if self.fp8 else
+                                   self.block_rows(start_frame, n)).to(self.device)
             self._dst_cache[key] = dst
+        if self.fp8:
+            self._append_fp8(k_blk, v_blk, dst)
+        else:
+            self._append_rows(k_blk, v_blk, dst)
+        act = np.asarray(active_block, dtype=bool).reshape(n, -1)
+        for j in range(n):
+            slot = (start_frame + j) % self.R
+            self.slot_frame[slot] = start_frame + j
+            if not self.no_local:
+                self.local_active[:, slot] = act[j, :self.N]
+
+    def _append_rows(self, k_blk, v_blk, dst) -> None:
+        S, HB = k_blk.shape[:2]
         if k_blk.stride(2) != 1 or v_blk.stride(2) != 1:
             k_blk, v_blk = k_blk.contiguous(), v_blk.contiguous()
         args = _capi.HierPageArgs(
@@ -163,12 +228,28 @@ class HierPagedKVCache:
             k_pool=self.k.data_ptr(), v_pool=self.v.data_ptr(), pool_ss=self.k.stride(0),
             pool_sh=self.k.stride(1))
         _capi.call("hier_kv_append", C.byref(args), _stream(self.device))
-        act = np.asarray(active_block, dtype=bool).reshape(n, -1)
-        for j in range(n):
-            slot = (start_frame + j) % self.R
-            self.slot_frame[slot] = start_frame + j
-            if not self.no_local:
-                self.local_active[:, slot] = act[j, :self.N]
+
+    def _append_fp8(self, k_blk, v_blk, blocks) -> None:
+        k_blk, v_blk = (t if t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and
+                        t.data_ptr() % 16 == 0 else t.contiguous() for t in (k_blk, v_blk))
+        args = _capi.HierPageFp8Args(
+            H=k_blk.shape[1], D=self.D, n_blocks=blocks.shape[0], n_rows=k_blk.shape[0],
+            pool_rows=self.k.shape[0], k_src=k_blk.data_ptr(), v_src=v_blk.data_ptr(),
+            k_src_ss=k_blk.stride(0), k_src_sh=k_blk.stride(1), v_src_ss=v_blk.stride(0),
+            v_src_sh=v_blk.stride(1), blocks=blocks.data_ptr(), k_pool=self.k.data_ptr(),
+            v_pool=self.v.data_ptr(), pool_ss=self.k.stride(0), pool_sh=self.k.stride(1),
+            k_scale=self.k_scale.data_ptr(), v_scale=self.v_scale.data_ptr(),
+            scale_ss=self.k_scale.stride(0), scale_sh=self.k_scale.stride(1))
+        _capi.call_on(self.k.device, "hier_kv_append_fp8", C.byref(args))
+
+    def dequantised(self):
+        """The ``(k, v)`` that an 8-bit cache stands for, bf16 ``[rows,
+        batch * H, D]`` (exact: a code and a power of two fit a bf16)."""
+        if not self.fp8:
+            return self.k, self.v
+        wide = lambda c, s: (c.float() * s.float().repeat_interleave(FP8_BLOCK, 0)[..., None]).to(  # noqa: E731
+            torch.bfloat16)
+        return wide(self.k, self.k_scale), wide(self.v, self.v_scale)
 
     # ---- window ----------------------------------------------------------------------
 

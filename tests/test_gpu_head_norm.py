@@ -1,0 +1,244 @@
+"""Per-head RMSNorm with rotation on the GPU, forward and gradient, against the
+formula in 64 bits.
+
+Bounds.  The result is rounded to bf16 once: half a step, 2^-8 of the value.
+Before that everything is fp32: the inverse RMS (a sum of D squares, a square
+root, a division), three products and a sum err by less than 16 roundings of
+2^-24 of the terms, 2^-20 of |a| + |b| for a rotated pair (a, b); the gradient
+goes through one more such sum, 2^-18 of the sum of its terms' magnitudes.
+"""
+
+import pytest
+import torch
+
+from multics_amd.kernels import (qk_head_prologue, qk_head_prologue_backward,
+                                 qk_head_prologue_train)
+from multics_amd.module import SelfAttention, rope_apply
+from tests.gpu_util import need_gpu, say
+
+pytestmark = pytest.mark.gpu
+EPS = 1e-6
+STEP, F32 = 2.0 ** -8, 2.0 ** -20
+
+CASES = [
+    # S, Hq, Hk, D, fused projection, gain dtype, layout
+    (1, 1, 1, 128, False, torch.float32, "shd"),
+    (1, 24, 24, 128, False, torch.bfloat16, "hsd"),
+    (2, 7, 1, 64, True, torch.float32, "shd"),
+    (37, 25, 25, 128, False, torch.bfloat16, "hsd"),    # one head past a wave's groups
+    (131, 49, 7, 64, True, torch.float32, "hsd"),
+    (513, 20, 5, 64, False, torch.bfloat16, "shd"),
+    (1999, 12, 2, 128, True, torch.float32, "shd"),
+]
+
+
+def _inputs(S, Hq, Hk, D, fused, gain, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    rows = (rnd(S, (Hq + 2 * Hk) * D) * torch.exp(rnd(S, 1))).to(torch.bfloat16)
+    qx, kx = rows[:, :Hq * D], rows[:, Hq * D:(Hq + Hk) * D]
+    if not fused:
+        qx, kx = qx.contiguous(), kx.contiguous()
+    angle = rnd(S, D // 2) * 3
+    kw = dict(norm_q_w=(1 + 0.3 * rnd(D)).to(gain), norm_k_w=(1 + 0.3 * rnd(D)).to(gain),
+              rope_cos=torch.cos(angle), rope_sin=torch.sin(angle), num_heads=Hq, num_kv_heads=Hk,
+              eps=EPS)
+    dq, dk = rnd(S, Hq, D).to(torch.bfloat16), rnd(S, Hk, D).to(torch.bfloat16)
+    return qx, kx, kw, dq, dk
+
+
+def _formula(x, w, cos, sin, H):
+    """(y, |a| + |b| of each element's pair) in 64 bits."""
+    S, D = x.shape[0], x.shape[1] // H
+    h = x.double().reshape(S, H, D)
+    n = h / torch.sqrt((h * h).mean(-1, keepdim=True) + EPS) * w.double()
+    z = torch.view_as_complex(n.reshape(S, H, D // 2, 2).contiguous()) * \
+        torch.complex(cos.double(), sin.double())[:, None]
+    size = n.abs().reshape(S, H, D // 2, 2).sum(-1, keepdim=True).expand(-1, -1, -1, 2)
+    return torch.view_as_real(z).flatten(-2), size.reshape(S, H, D)
+
+
+@pytest.mark.parametrize("S,Hq,Hk,D,fused,gain,layout", CASES)
+def test_forward_matches_the_formula(S, Hq, Hk, D, fused, gain, layout):
+    need_gpu()
+    qx, kx, kw, _, _ = _inputs(S, Hq, Hk, D, fused, gain)
+    say("head norm", S, Hq, Hk, D, fused, gain, layout)
+    q, k = qk_head_prologue(qx, kx, out_layout=layout, **kw)
+    torch.cuda.synchronize()
+    for got, x, w, H in ((q, qx, kw["norm_q_w"], Hq), (k, kx, kw["norm_k_w"], Hk)):
+        ref, size = _formula(x, w, kw["rope_cos"], kw["rope_sin"], H)
+        assert got.shape == (S, H, D) and got.dtype == torch.bfloat16
+        off = (got.double() - ref).abs()
+        assert bool((off <= STEP * ref.abs() + 2 * F32 * size).all()), float((off / size).max())
+
+
+def _grad_formula(x, dy, w, cos, sin, H):
+    """(dx, bound of its fp32 error, dw, sum of |terms| of dw) in 64 bits."""
+    S, D = x.shape[0], x.shape[1] // H
+    h = x.double().reshape(S, H, D)
+    r = 1 / torch.sqrt((h * h).mean(-1, keepdim=True) + EPS)
+    z = torch.view_as_complex(dy.double().reshape(S, H, D // 2, 2).contiguous()) * \
+        torch.complex(cos.double(), -sin.double())[:, None]
+    dn = torch.view_as_real(z).flatten(-2)
+    big = dy.double().abs().reshape(S, H, D // 2, 2).sum(-1, keepdim=True).expand(
+        -1, -1, -1, 2).reshape(S, H, D)                      # bounds |dn| and its terms
+    xh, dh = h * r, dn * w.double()
+    dx = r * (dh - xh * (dh * xh).mean(-1, keepdim=True))
+    bh = big * w.double().abs()
+    size = r * (bh + xh.abs() * (bh * xh.abs()).mean(-1, keepdim=True))
+    return dx, 2.0 ** -18 * size, (dn * xh).sum((0, 1)), (big * xh.abs()).sum((0, 1))
+
+
+@pytest.mark.parametrize("S,Hq,Hk,D,fused,gain,layout", CASES)
+def test_gradient_matches_the_formula(S, Hq, Hk, D, fused, gain, layout):
+    need_gpu()
+    qx, kx, kw, dq, dk = _inputs(S, Hq, Hk, D, fused, gain)
+    if layout == "hsd":         # gradients of head-major storage
+        dq, dk = (t.transpose(0, 1).contiguous().transpose(0, 1) for t in (dq, dk))
+    say("head norm gradient", S, Hq, Hk, D, fused, gain, layout)
+    got = qk_head_prologue_backward(dq, dk, qx, kx, **kw)
+    again = qk_head_prologue_backward(dq, dk, qx, kx, **kw)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    for x, dy, w, H, dx, dw in ((qx, dq, kw["norm_q_w"], Hq, got[0], got[2]),
+                                (kx, dk, kw["norm_k_w"], Hk, got[1], got[3])):
+        ref, slack, rw, terms = _grad_formula(x, dy, w, kw["rope_cos"], kw["rope_sin"], H)
+        assert dx.shape == x.shape
+        off = (dx.double().reshape(ref.shape) - ref).abs()
+        assert bool((off <= STEP * (ref.abs() + slack) + slack).all()), float((off / slack).max())
+        # fp32 sums of fewer than 256 terms in a row at these sizes, each term
+        # itself within 2^-20: 2^-15 of the terms' magnitudes
+        assert dw.dtype == torch.float32
+        assert bool(((dw.double() - rw).abs() <= 2.0 ** -15 * terms).all())
+
+
+def test_gradient_matches_differences():
+    """Along a random direction, against the 64-bit formula's central difference."""
+    need_gpu()
+    S, Hq, Hk, D = 33, 6, 3, 64
+    qx, kx, kw, dq, dk = _inputs(S, Hq, Hk, D, False, torch.float32, seed=4)
+    got = qk_head_prologue_backward(dq, dk, qx, kx, **kw)
+    g = torch.Generator(device="cuda").manual_seed(9)
+    for x, dy, w, H, dx, dw in ((qx, dq, kw["norm_q_w"], Hq, got[0], got[2]),
+                                (kx, dk, kw["norm_k_w"], Hk, got[1], got[3])):
+        u = torch.randn(x.shape, generator=g, device="cuda", dtype=torch.float64)
+        uw = torch.randn(D, generator=g, device="cuda", dtype=torch.float64)
+        loss = lambda t: (_formula(x.double() + t * u, w.double() + t * uw,  # noqa: E731
+                                   kw["rope_cos"], kw["rope_sin"], H)[0] * dy.double()).sum()
+        h = 1e-5
+        slope = (loss(h) - loss(-h)) / (2 * h)
+        mine = (dx.double() * u).sum() + (dw.double() * uw).sum()
+        _, slack, _, terms = _grad_formula(x, dy, w, kw["rope_cos"], kw["rope_sin"], H)
+        bound = ((STEP * dx.double().abs() + 2 * slack.reshape(dx.shape)) * u.abs()).sum() + \
+            (2.0 ** -15 * terms * uw.abs()).sum() + 1e-7 * slope.abs()
+        assert (slope - mine).abs() <= bound
+
+
+def test_autograd_and_module_gradients():
+    """The training entry gives the raw gradient, for strided columns too, and
+    SelfAttention(qk_norm="head") reaches it: its q and k equal the torch tail
+    (which rounds after the norm, the gain and the rotation: three roundings)."""
+    need_gpu()
+    qx, kx, kw, dq, dk = _inputs(45, 8, 2, 64, True, torch.bfloat16)
+    leaves = [t.detach().requires_grad_() for t in (qx, kx, kw["norm_q_w"], kw["norm_k_w"])]
+    q, k = qk_head_prologue_train(leaves[0], leaves[1], **{**kw, "norm_q_w": leaves[2],
+                                                           "norm_k_w": leaves[3]})
+    got = torch.autograd.grad([q, k], leaves, [dq, dk])
+    want = qk_head_prologue_backward(dq, dk, qx, kx, **kw)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert torch.equal(got[2], want[2].bfloat16()) and torch.equal(got[3], want[3].bfloat16())
+    with pytest.raises(RuntimeError, match="qk_head_prologue_train"):
+        qk_head_prologue(leaves[0], leaves[1], **kw)
+
+    torch.manual_seed(0)
+    m = SelfAttention(320, 5, qk_norm="head").to("cuda", torch.bfloat16)     # dim not k * 512
+    m.enable_camera_pose_qk(12, dropout_p=0.0)
+    torch.nn.init.normal_(m.cam_q.weight, std=0.1)
+    torch.nn.init.normal_(m.norm_q.weight, mean=1.0, std=0.2)
+    assert m.norm_q.weight.shape == (64,)
+    x = torch.randn(1, 70, 320, device="cuda").to(torch.bfloat16).requires_grad_()
+    cam = torch.randn(1, 70, 12, device="cuda").to(torch.bfloat16)
+    freqs = torch.polar(torch.ones(70, 1, 32, dtype=torch.float64, device="cuda"),
+                        torch.rand(70, 1, 32, dtype=torch.float64, device="cuda"))
+    q, k, v = m._project_train(x, freqs, cam)
+    pq, pk, pv = (t.view(70, 5, 64) for t in m._project_self_attn_qkv(x, freqs, cam))
+    for a, b in ((q, pq), (k, pk)):
+        # three roundings against one, and the rotation mixes a pair's
+        pair = b.double().reshape(70, 5, 32, 2).abs().sum(-1, keepdim=True).expand(
+            -1, -1, -1, 2).reshape(b.shape)
+        assert bool(((a.double() - b.double()).abs() <= 4 * STEP * 1.5 * pair).all())
+    assert torch.equal(v, pv)
+    (q.float().square().sum() + k.float().sum()).backward()
+    for p in (x, m.q.weight, m.k.weight, m.norm_q.weight, m.norm_k.weight, m.cam_q.weight):
+        assert p.grad is not None and bool(torch.isfinite(p.grad).all()) and bool((p.grad != 0).any())
+    with torch.no_grad():
+        fq, fk, _ = m._qkv_blocks(x, freqs, cam)
+    assert torch.equal(fq, q) and torch.equal(fk, k)
+
+
+def test_values_that_are_not_finite_stay_in_their_head():
+    need_gpu()
+    qx, kx, kw, _, _ = _inputs(9, 4, 4, 64, False, torch.float32)
+    ref = qk_head_prologue(qx, kx, **kw)
+    bad = qx.clone()
+    bad[3, 64 + 5] = float("nan")
+    bad[5, 130] = float("inf")
+    q, k = qk_head_prologue(bad, kx, **kw)
+    keep = torch.ones(9, 4, dtype=torch.bool, device="cuda")
+    keep[3, 1] = keep[5, 2] = False
+    assert torch.equal(q[keep], ref[0][keep]) and torch.equal(k, ref[1])
+    assert bool(torch.isnan(q[3, 1]).all()) and bool(torch.isnan(q[5, 2, 2:4]).any())
+    zero = qk_head_prologue(torch.zeros_like(qx), kx, **kw)[0]
+    assert torch.count_nonzero(zero) == 0
+
+
+def test_captured_on_a_side_stream():
+    """Forward and gradient recorded into a graph, replayed on new inputs."""
+    need_gpu()
+    args = [_inputs(77, 6, 2, 128, False, torch.float32, seed=i) for i in range(3)]
+    qx, kx, kw, dq, dk = (t.clone() if torch.is_tensor(t) else t for t in args[0])
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        qk_head_prologue(qx, kx, **kw)
+        qk_head_prologue_backward(dq, dk, qx, kx, **kw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = qk_head_prologue(qx, kx, **kw) + qk_head_prologue_backward(dq, dk, qx, kx, **kw)
+    for new in args + args:
+        for to, t in zip((qx, kx, dq, dk), (new[0], new[1], new[3], new[4])):
+            to.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = qk_head_prologue(qx, kx, **kw) + qk_head_prologue_backward(dq, dk, qx, kx, **kw)
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_refusals_and_empty():
+    need_gpu()
+    qx, kx, kw, dq, dk = _inputs(8, 4, 2, 64, False, torch.float32)
+    bad = [
+        (ValueError, dict(num_heads=3)), (ValueError, dict(num_kv_heads=4)),
+        (ValueError, dict(num_heads=0)), (NotImplementedError, dict(num_heads=8, num_kv_heads=4)),
+        (ValueError, dict(norm_q_w=kw["norm_q_w"][:32])),
+        (ValueError, dict(norm_q_w=kw["norm_q_w"].half())),
+        (ValueError, dict(rope_cos=kw["rope_cos"][:7])),
+        (ValueError, dict(rope_sin=kw["rope_sin"].cpu())), (ValueError, dict(out_layout="sdh")),
+    ]
+    for exc, change in bad:
+        with pytest.raises(exc):
+            qk_head_prologue(qx, kx, **{**kw, **change})
+    with pytest.raises(NotImplementedError):
+        qk_head_prologue(qx.float(), kx, **kw)
+    with pytest.raises(ValueError):
+        qk_head_prologue(qx, kx[:7], **kw)
+    with pytest.raises(ValueError):
+        qk_head_prologue_backward(dq[:, :3], dk, qx, kx, **kw)
+    with pytest.raises(ValueError):
+        qk_head_prologue_backward(dq.float(), dk, qx, kx, **kw)
+    none = {**kw, "rope_cos": kw["rope_cos"][:0], "rope_sin": kw["rope_sin"][:0]}
+    q, k = qk_head_prologue(qx[:0], kx[:0], **none)
+    assert q.shape == (0, 4, 64) and k.shape == (0, 2, 64)
+    grads = qk_head_prologue_backward(dq[:0], dk[:0], qx[:0], kx[:0], **none)
+    assert grads[0].shape == (0, 256) and torch.count_nonzero(grads[2]) == 0
