@@ -48,8 +48,19 @@ template <int D>
 struct Geo8 {
   static constexpr int NS = D / 64;          // 64-wide d-steps of Q K^T
   static constexpr int CPR = D / 16;         // 16-byte chunks of a row of codes
-  static constexpr int NL = kSlab * CPR / kThreads;   // chunks of a thread per tile
+  static constexpr int RPC = 64 / CPR;       // rows of a wave's copy instruction
+  static constexpr int NL = 16 / RPC;        // copies of a wave (its 16 rows) per tile
   static constexpr int KTILEB = kSlab * D;
+};
+
+// LDS stages of a workgroup: codes of K, V in bf16, masks and K scales (one
+// dword a key), two of each, every one its own array (the copies into one
+// stage then never make the compiler wait before it reads another).
+struct Stages {
+  char* k[2];
+  char* v[2];
+  char* m[2];
+  int* s[2];
 };
 
 // XOR mask on the 16-byte chunk index of row `row` of a K tile: 8 consecutive
@@ -148,19 +159,32 @@ __device__ __forceinline__ void rows_init(Rows<D>& R, const HierFwdFp8Args& a, c
   R.alpha = 1.f;
 }
 
-// S^T of 32-key block kb: lane l holds key 32 kb + l % 32, d 64 s + 32 (l / 32) .. + 32.
+// Per-lane LDS byte offsets of the MFMA operand reads (tile-relative).
 template <int D>
-__device__ __forceinline__ f32x16 qk_block(const Rows<D>& R, const char* ktile, const int* kscale,
-                                           int kb, int lane) {
-  const int key = kb * 32 + (lane & 31);
-  const char* row = ktile + key * D;
-  const int sw = kswz<D>(key), sk = kscale[key];
+struct ReadAddr {
+  int k[2 * Geo8<D>::NS];   // codes of key lane % 32, d 64 s + 32 (lane / 32) .. + 32: two chunks
+  int v[Geo<D>::NDB];       // first transposed V read of d-block db, key chunk 0
+  __device__ __forceinline__ void init(int lane) {
+    const int key = lane & 31;
+#pragma unroll
+    for (int i = 0; i < 2 * Geo8<D>::NS; ++i)
+      k[i] = key * D + 16 * ((4 * (i >> 1) + 2 * (lane >> 5) + (i & 1)) ^ kswz<D>(key));
+#pragma unroll
+    for (int db = 0; db < Geo<D>::NDB; ++db) v[db] = tr_read_off<D, kTrRead>(lane, db, 0);
+  }
+};
+
+// S^T of 32-key block kb of a tile.
+template <int D>
+__device__ __forceinline__ f32x16 qk_block(const Rows<D>& R, const char* kslot, const int* kscale,
+                                           const ReadAddr<D>& ra, int kb, int lane) {
+  const char* base = kslot + kb * 32 * D;
+  const int sk = kscale[kb * 32 + (lane & 31)];
   f32x16 acc = {};
 #pragma unroll
   for (int s = 0; s < Geo8<D>::NS; ++s) {
-    const int c = 4 * s + 2 * (lane >> 5);
-    const u32x4 x = *reinterpret_cast<const u32x4*>(row + 16 * (c ^ sw));
-    const u32x4 y = *reinterpret_cast<const u32x4*>(row + 16 * ((c + 1) ^ sw));
+    const u32x4 x = *reinterpret_cast<const u32x4*>(base + ra.k[2 * s]);
+    const u32x4 y = *reinterpret_cast<const u32x4*>(base + ra.k[2 * s + 1]);
     const i32x8 k = {(int)x[0], (int)x[1], (int)x[2], (int)x[3],
                      (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
     acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, R.hi[s], acc, 0, 0, 0, sk, 0, R.e_hi);
@@ -170,8 +194,9 @@ __device__ __forceinline__ f32x16 qk_block(const Rows<D>& R, const char* ktile, 
 }
 
 // Set the scores of block kb that the lane's query frame may not see to -inf.
-__device__ __forceinline__ void mask_block(f32x16& s, const uint32_t* mk, int kb, int qframe,
+__device__ __forceinline__ void mask_block(f32x16& s, const char* mslot, int kb, int qframe,
                                            int lane) {
+  const uint32_t* mk = reinterpret_cast<const uint32_t*>(mslot);
 #pragma unroll
   for (int g4 = 0; g4 < 4; ++g4) {
     const u32x4 w = *reinterpret_cast<const u32x4*>(&mk[kb * 32 + 8 * g4 + 4 * (lane >> 5)]);
@@ -202,11 +227,12 @@ __device__ __forceinline__ float p_block(const f32x16& s, bf16x8* p, float c2, f
   return ps0 + ps1;
 }
 
-// Online softmax of one block with the lazily refreshed running max; true:
-// O is to be scaled by R.alpha before the block's P V.
+// Online softmax, second half: ps is the lane's sum of a block's P taken
+// against the running max.  True: the max was refreshed and P recomputed; O is
+// to be scaled by R.alpha before the block's P V.
 template <int D>
-__device__ __forceinline__ bool softmax_block(Rows<D>& R, const f32x16& s, bf16x8* p, float c2) {
-  const float ps = p_block(s, p, c2, -R.m);
+__device__ __forceinline__ bool softmax_fix(Rows<D>& R, const f32x16& s, bf16x8* p, float c2,
+                                            float ps) {
   if (__ballot(!(ps <= kSumMax)) == 0) {
     R.l += ps;
     R.alpha = 1.f;
@@ -224,23 +250,28 @@ __device__ __forceinline__ bool softmax_block(Rows<D>& R, const f32x16& s, bf16x
 }
 
 template <int D>
-__device__ __forceinline__ void rescale(Rows<D>& R) {
+__device__ __forceinline__ bool softmax_block(Rows<D>& R, const f32x16& s, bf16x8* p, float c2) {
+  return softmax_fix<D>(R, s, p, c2, p_block(s, p, c2, -R.m));
+}
+
+template <int D>
+__device__ __forceinline__ void rescale(Rows<D>& R, float alpha) {
 #pragma unroll
   for (int db = 0; db < Geo<D>::NDB; ++db)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) R.o[db][i] *= R.alpha;
+    for (int i = 0; i < 16; ++i) R.o[db][i] *= alpha;
 }
 
 // O^T += V^T P^T over the two 16-key chunks of block kb.
 template <int D>
-__device__ __forceinline__ void pv_block(Rows<D>& R, const bf16x8* p, const char* vtile, int kb,
-                                         int lane) {
+__device__ __forceinline__ void pv_block(Rows<D>& R, const bf16x8* p, const char* vslot,
+                                         const ReadAddr<D>& ra, int kb) {
   constexpr int HALF = (8 / Geo<D>::NI) * Geo<D>::ROWB;   // rows of keys +8
 #pragma unroll
   for (int j = 0; j < 2; ++j)
 #pragma unroll
     for (int db = 0; db < Geo<D>::NDB; ++db) {
-      const char* p0 = vtile + (2 * kb + j) * 16 * Geo<D>::ROWB + tr_read_off<D, kTrRead>(lane, db, 0);
+      const char* p0 = vslot + (2 * kb + j) * 16 * Geo<D>::ROWB + ra.v[db];
       R.o[db] = mfma(tr_read(p0, p0 + HALF), p[j], R.o[db]);
     }
 }
@@ -278,75 +309,288 @@ __device__ __forceinline__ void store_rows(const Rows<D>& R, const HierFwdFp8Arg
     a.lse[(int64_t)head * a.lse_stride_h + R.qtok] = l > 0.f ? fmaf(R.m, kLn2, __logf(l)) : -INFINITY;
 }
 
+// ---- staging ------------------------------------------------------------------
+//
+// A wave stages rows 16 w .. + 16 of a tile: lane l chunk l % CPR of rows
+// 16 w + RPC e + l / CPR.  K's codes are copied to LDS as they are; V's go
+// through registers (loaded while the tile before is multiplied, converted and
+// written at the end of it).
+
+template <int D>
+struct Ctx {
+  const char* gk;            // the head's codes
+  const char* gv;
+  const uint8_t* sk;         // the head's scales
+  const uint8_t* sv;
+  const int32_t* kv_idx;     // of the part's first tile
+  const uint32_t* kv_mask;
+  const uint32_t* blk;
+  uint32_t ss_b, scale_b;    // bytes between rows of codes, between scales
+  float c2;
+  int nt, wave, lane;
+  bool active;
+  int row0;                  // the lane's first row of a tile
+  uint32_t k16, v16;         // byte offsets of its chunk in a row: K's swizzled source, V's
+  int vst[2 * Geo8<D>::NL];  // where its chunks of V go
+  ReadAddr<D> ra;
+};
+
+template <int D>
+struct Row {
+  int v[Geo8<D>::NL];
+};
+template <int D>
+struct VRegs {
+  u32x4 w[Geo8<D>::NL];
+  uint32_t s[Geo8<D>::NL];
+};
+
+template <int D>
+__device__ __forceinline__ Row<D> load_rows(const Ctx<D>& c, int tile) {
+  Row<D> r;
+#pragma unroll
+  for (int e = 0; e < Geo8<D>::NL; ++e)
+    r.v[e] = c.kv_idx[tile * kSlab + c.row0 + Geo8<D>::RPC * e];
+  return r;
+}
+
+template <int D>
+__device__ __forceinline__ void copy_k(const Ctx<D>& c, const Row<D>& r, char* slot) {
+#pragma unroll
+  for (int e = 0; e < Geo8<D>::NL; ++e)
+    dma16(c.gk, __umul24((uint32_t)r.v[e], c.ss_b) + c.k16,
+          slot + (16 * c.wave + Geo8<D>::RPC * e) * D);
+}
+
+template <int D>
+__device__ __forceinline__ void load_scales(const Ctx<D>& c, const uint8_t* sc, const Row<D>& r,
+                                            uint32_t* s) {
+#pragma unroll
+  for (int e = 0; e < Geo8<D>::NL; ++e)
+    s[e] = sc[__umul24((uint32_t)r.v[e] / HIER_FP8_BLOCK, c.scale_b)];
+}
+
+template <int D>
+__device__ __forceinline__ void store_scales(const Ctx<D>& c, const uint32_t* s, int* slot) {
+  if (c.lane % Geo8<D>::CPR == 0)
+#pragma unroll
+    for (int e = 0; e < Geo8<D>::NL; ++e) slot[c.row0 + Geo8<D>::RPC * e] = (int)s[e];
+}
+
+template <int D>
+__device__ __forceinline__ void load_v(const Ctx<D>& c, const Row<D>& r, VRegs<D>& v) {
+#pragma unroll
+  for (int e = 0; e < Geo8<D>::NL; ++e)
+    v.w[e] = *reinterpret_cast<const u32x4*>(c.gv + (__umul24((uint32_t)r.v[e], c.ss_b) + c.v16));
+  load_scales<D>(c, c.sv, r, v.s);
+}
+
+// Sixteen codes as bf16 (exact) into two chunks of the tile.
+template <int D>
+__device__ __forceinline__ void store_v(const Ctx<D>& c, const VRegs<D>& v, char* slot) {
+#pragma unroll
+  for (int e = 0; e < Geo8<D>::NL; ++e) {
+    const float sv = pow2_of(v.s[e]);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      u32x4 b;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t w = v.w[e][2 * p + i];
+        b[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, sv, false));
+        b[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, sv, true));
+      }
+      *reinterpret_cast<u32x4*>(slot + c.vst[2 * e + p]) = b;
+    }
+  }
+}
+
+// The lane's offsets, the part's key list and the first tiles: K(0), K(1) with
+// masks and scales, V(0) resident; the rows of tiles 1 and 2 and the flags of
+// tile 1 loaded (nt >= 1).
+template <int D>
+__device__ __forceinline__ void setup(Ctx<D>& c, const HierFwdFp8Args& a, const int32_t* it, int head,
+                                      int split, int tid) {
+  using G = Geo8<D>;
+  c.lane = tid & 63;
+  c.wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int nt = it[6] / kSlab;
+  const int t0 = (int)((int64_t)nt * split / a.splits), t1 = (int)((int64_t)nt * (split + 1) / a.splits);
+  c.nt = t1 - t0;
+  const int64_t off = (int64_t)it[5] + (int64_t)t0 * kSlab;
+  const int kh = head / (a.H / a.Hk);
+  c.gk = reinterpret_cast<const char*>(a.k + kh * a.kv_sh);
+  c.gv = reinterpret_cast<const char*>(a.v + kh * a.kv_sh);
+  c.sk = a.k_scale + kh * a.scale_sh;
+  c.sv = a.v_scale + kh * a.scale_sh;
+  c.kv_idx = a.tile_kv_idx + off;
+  c.kv_mask = a.tile_kv_mask + off;
+  c.blk = a.tile_blk_and + off / kSlab;
+  c.ss_b = (uint32_t)a.kv_ss;
+  c.scale_b = (uint32_t)a.scale_ss;
+  c.c2 = a.scale * 1.4426950408889634f;
+  const int chunk = c.lane % G::CPR;
+  c.row0 = 16 * c.wave + c.lane / G::CPR;
+  c.k16 = 16u * (uint32_t)(chunk ^ kswz<D>(c.row0));   // (the same for each of its rows)
+  c.v16 = 16u * (uint32_t)chunk;
+#pragma unroll
+  for (int e = 0; e < G::NL; ++e)
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int row = c.row0 + G::RPC * e;
+      c.vst[2 * e + p] = prow<D>(row) * Geo<D>::ROWB + 16 * ((2 * chunk + p) ^ swz<D, kTrRead>(row));
+    }
+  c.ra.init(c.lane);
+}
+
+template <int D>
+__device__ __forceinline__ void first_tiles(Ctx<D>& c, Row<D>& ik, Row<D>& iv, uint32_t& blk,
+                                            const Stages& st) {
+  const Row<D> r0 = load_rows<D>(c, 0);
+  iv = load_rows<D>(c, min(1, c.nt - 1));
+  ik = load_rows<D>(c, min(2, c.nt - 1));
+  blk = c.blk[min(1, c.nt - 1)];
+  uint32_t s[Geo8<D>::NL];
+  VRegs<D> v;
+  copy_k<D>(c, r0, st.k[0]);
+  if (c.wave == 0) copy_dwords(c.kv_mask, st.m[0], c.lane);
+  load_scales<D>(c, c.sk, r0, s);
+  load_v<D>(c, r0, v);
+  store_scales<D>(c, s, st.s[0]);
+  if (c.nt > 1) {
+    copy_k<D>(c, iv, st.k[1]);
+    if (c.wave == 0) copy_dwords(c.kv_mask + kSlab, st.m[1], c.lane);
+    load_scales<D>(c, c.sk, iv, s);
+    store_scales<D>(c, s, st.s[1]);
+  }
+  store_v<D>(c, v, st.v[0]);
+  wait_copies();
+  __syncthreads();
+}
+
+// ---- the kernel ---------------------------------------------------------------
+
+// Half-step j = 2t + B of the pipeline: QK of block B of tile t+1 into sq,
+// softmax of block j+1 (sc) into pn, P V of block B of tile t with pv; then the
+// masks of sq (blk_cur: visibility flags of tile t+1).  The three are
+// independent, so one scheduling region interleaves them.  PAR = t & 1: K(t+1),
+// its masks and scales in stage PAR^1, V(t) in PAR.
+template <int D, int PAR, int B>
+__device__ __forceinline__ void half_step(Ctx<D>& c, Rows<D>& R, f32x16& sq, const f32x16& sc,
+                                          const bf16x8* pv, bf16x8* pn, bool& resc,
+                                          float& alpha_pend, uint32_t blk_cur, const Stages& st) {
+  if (resc) rescale<D>(R, alpha_pend);
+  sq = qk_block<D>(R, st.k[PAR ^ 1], st.s[PAR ^ 1], c.ra, B, c.lane);
+  float ps = p_block(sc, pn, c.c2, -R.m);
+  pv_block<D>(R, pv, st.v[PAR], c.ra, B);
+  // keep the softmax results in this region (otherwise they sink past the
+  // branches below, away from the MFMAs they are meant to overlap)
+  asm volatile("" : "+v"(pn[0]), "+v"(pn[1]), "+v"(ps));
+  resc = softmax_fix<D>(R, sc, pn, c.c2, ps);
+  alpha_pend = R.alpha;
+  if ((blk_cur & R.bits) != R.bits) mask_block(sq, st.m[PAR ^ 1], B, R.qframe, c.lane);
+}
+
+// Tile iteration t (t + 1 < nt): K(t+2) with masks and scales on its way into
+// stage PAR and V(t+1) into registers, half-steps 2t and 2t+1, V(t+1)
+// converted into stage PAR^1.  On entry K(t+1) and V(t) are resident, S(2t+1)
+// (sb) is masked, P(2t) (pa) ready with its rescale pending; ik / iv are the
+// rows of tiles min(t+2, nt-1) / t+1, blk the flags of tile t+1.
+template <int D, int PAR>
+__device__ __forceinline__ void tile_iter(Ctx<D>& c, Rows<D>& R, int t, f32x16& sa, f32x16& sb,
+                                          bf16x8* pa, bf16x8* pb, bool& resc, float& alpha_pend,
+                                          Row<D>& ik, Row<D>& iv, uint32_t& blk, const Stages& st) {
+  const bool more = t + 2 < c.nt;
+  uint32_t s[Geo8<D>::NL];
+  VRegs<D> v;
+  load_v<D>(c, iv, v);
+  if (more) {
+    copy_k<D>(c, ik, st.k[PAR]);
+    if (c.wave == 0) copy_dwords(c.kv_mask + (t + 2) * kSlab, st.m[PAR], c.lane);
+  }
+  load_scales<D>(c, c.sk, ik, s);
+  iv = ik;
+  ik = load_rows<D>(c, min(t + 3, c.nt - 1));
+  const uint32_t blk_pre = c.blk[min(t + 2, c.nt - 1)];
+  if (c.active) {
+    half_step<D, PAR, 0>(c, R, sa, sb, pa, pb, resc, alpha_pend, blk, st);
+    half_step<D, PAR, 1>(c, R, sb, sa, pb, pa, resc, alpha_pend, blk, st);
+  }
+  store_v<D>(c, v, st.v[PAR ^ 1]);
+  if (more) store_scales<D>(c, s, st.s[PAR]);
+  wait_copies();
+  __syncthreads();
+  blk = blk_pre;
+}
+
+// Last tile (t = nt - 1): softmax of its block 1 (sb) into pb, P V of both.
+template <int D, int PAR>
+__device__ __forceinline__ void last_tile(Ctx<D>& c, Rows<D>& R, const f32x16& sb, const bf16x8* pa,
+                                          bf16x8* pb, bool resc, float alpha_pend,
+                                          const Stages& st) {
+  if (resc) rescale<D>(R, alpha_pend);
+  resc = softmax_block<D>(R, sb, pb, c.c2);
+  alpha_pend = R.alpha;
+  pv_block<D>(R, pa, st.v[PAR], c.ra, 0);
+  if (resc) rescale<D>(R, alpha_pend);
+  pv_block<D>(R, pb, st.v[PAR], c.ra, 1);
+}
+
 template <int D>
 __global__ __launch_bounds__(kThreads, 2) void attn_fp8_kernel(HierFwdFp8Args a, int total) {
-  using G = Geo8<D>;
-  __shared__ __align__(16) char lds_k[G::KTILEB];
-  __shared__ __align__(16) char lds_v[Geo<D>::TILEB];
-  __shared__ __align__(16) uint32_t lds_m[kSlab];
-  __shared__ int lds_s[kSlab];
+  __shared__ __align__(16) char lds_k0[Geo8<D>::KTILEB], lds_k1[Geo8<D>::KTILEB];
+  __shared__ __align__(16) char lds_v0[Geo<D>::TILEB], lds_v1[Geo<D>::TILEB];
+  __shared__ __align__(16) char lds_m0[Geo<D>::MBYTES], lds_m1[Geo<D>::MBYTES];
+  __shared__ int lds_s0[kSlab], lds_s1[kSlab];
+  const Stages st = {{lds_k0, lds_k1}, {lds_v0, lds_v1}, {lds_m0, lds_m1}, {lds_s0, lds_s1}};
   const int logical = hier::xcd_logical(blockIdx.x, gridDim.x);
   if (logical >= total) return;
   const int per_head = a.n_items * a.splits;
   const int head = logical / per_head, rest = logical - head * per_head;
   const int item = rest / a.splits, split = rest - item * a.splits;
   const int32_t* it = a.tile_items + (int64_t)item * 8;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kv_off = it[5], nt = it[6] / kSlab;
-  const int t0 = (int)((int64_t)nt * split / a.splits), t1 = (int)((int64_t)nt * (split + 1) / a.splits);
-  const bool active = wave * 32 < it[4];
-  const int kh = head / (a.H / a.Hk);
-  const uint8_t* kp = a.k + kh * a.kv_sh;
-  const uint8_t* vp = a.v + kh * a.kv_sh;
-  const uint8_t* ksp = a.k_scale + kh * a.scale_sh;
-  const uint8_t* vsp = a.v_scale + kh * a.scale_sh;
-  const int32_t* idx = a.tile_kv_idx + kv_off;
-  const uint32_t* masks = a.tile_kv_mask + kv_off;
-  const uint32_t* blk = a.tile_blk_and + kv_off / kSlab;
-  const float c2 = a.scale * 1.4426950408889634f;
+  Ctx<D> c;
+  setup<D>(c, a, it, head, split, threadIdx.x);
+  c.active = c.wave * 32 < it[4];
   Rows<D> R;
-  rows_init<D>(R, a, it, head, wave * 32, lane);
-  for (int t = t0; t < t1; ++t) {
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < G::NL; ++e) {
-      const int ci = e * kThreads + tid, j = ci / G::CPR, c = ci % G::CPR;
-      const int64_t row = idx[t * kSlab + j];
-      const u32x4 kw = *reinterpret_cast<const u32x4*>(kp + row * a.kv_ss + 16 * c);
-      const u32x4 vw = *reinterpret_cast<const u32x4*>(vp + row * a.kv_ss + 16 * c);
-      const float sv = pow2_of(vsp[row / HIER_FP8_BLOCK * a.scale_ss]);
-      *reinterpret_cast<u32x4*>(lds_k + j * D + 16 * (c ^ kswz<D>(j))) = kw;
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        u32x4 b;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          b[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(vw[2 * p + i], sv, false));
-          b[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(vw[2 * p + i], sv, true));
-        }
-        *reinterpret_cast<u32x4*>(lds_v + prow<D>(j) * Geo<D>::ROWB +
-                                  16 * ((2 * c + p) ^ swz<D, kTrRead>(j))) = b;
-      }
-    }
-    if (tid < kSlab) {
-      const int64_t row = idx[t * kSlab + tid];
-      lds_s[tid] = ksp[row / HIER_FP8_BLOCK * a.scale_ss];
-      lds_m[tid] = masks[t * kSlab + tid];
-    }
-    __syncthreads();
-    if (!active) continue;
-    const bool masked = (blk[t] & R.bits) != R.bits;
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      f32x16 s = qk_block<D>(R, lds_k, lds_s, kb, lane);
-      if (masked) mask_block(s, lds_m, kb, R.qframe, lane);
-      bf16x8 p[2];
-      if (softmax_block<D>(R, s, p, c2)) rescale<D>(R);
-      pv_block<D>(R, p, lds_v, kb, lane);
-    }
+  rows_init<D>(R, a, it, head, c.wave * 32, c.lane);
+  const int nt = c.nt;
+  if (nt == 0) {
+    if (c.active) store_rows<D>(R, a, head, split, c.lane);
+    return;
   }
-  if (active) store_rows<D>(R, a, head, split, lane);
+  Row<D> ik, iv;
+  uint32_t blk;
+  first_tiles<D>(c, ik, iv, blk, st);
+  // S of both blocks of tile 0 computed and masked; P of block 0
+  f32x16 sa, sb;
+  bf16x8 pa[2], pb[2];
+  bool resc = false;
+  float alpha_pend = 1.f;
+  if (c.active) {
+    sa = qk_block<D>(R, st.k[0], st.s[0], c.ra, 0, c.lane);
+    sb = qk_block<D>(R, st.k[0], st.s[0], c.ra, 1, c.lane);
+    if ((c.blk[0] & R.bits) != R.bits) {
+      mask_block(sa, st.m[0], 0, R.qframe, c.lane);
+      mask_block(sb, st.m[0], 1, R.qframe, c.lane);
+    }
+    resc = softmax_block<D>(R, sa, pa, c.c2);
+    alpha_pend = R.alpha;
+  }
+  __syncthreads();   // every wave has read stage 0 of K, masks and scales
+  // two tile iterations per trip, so that every stage is a compile-time constant
+  int t = 0;
+  for (; t + 2 < nt; t += 2) {
+    tile_iter<D, 0>(c, R, t, sa, sb, pa, pb, resc, alpha_pend, ik, iv, blk, st);
+    tile_iter<D, 1>(c, R, t + 1, sa, sb, pa, pb, resc, alpha_pend, ik, iv, blk, st);
+  }
+  if (t + 1 < nt) {
+    tile_iter<D, 0>(c, R, t, sa, sb, pa, pb, resc, alpha_pend, ik, iv, blk, st);
+    if (c.active) last_tile<D, 1>(c, R, sb, pa, pb, resc, alpha_pend, st);
+  } else if (c.active) {
+    last_tile<D, 0>(c, R, sb, pa, pb, resc, alpha_pend, st);
+  }
+  if (c.active) store_rows<D>(R, a, head, split, c.lane);
 }
 
 // Joins the splits of one item and head: rows in turn, D / 4 lanes a row.
@@ -421,6 +665,12 @@ extern "C" int hier_attn_fwd_fp8(const HierFwdFp8Args* args, void* stream) {
   HIER_REQUIRE(a.q_ss % 8 == 0 && a.q_sh % 8 == 0 && a.kv_ss % 16 == 0 && a.kv_sh % 16 == 0 &&
                    a.o_ss % 4 == 0 && a.o_sh % 4 == 0,
                HIER_EINVAL, "strides must keep 16-byte rows aligned");
+  // rows of codes are addressed with 32-bit byte offsets from their head's
+  // first (one 24 x 24-bit multiply)
+  HIER_REQUIRE(a.kv_ss >= 0 && a.scale_ss >= 0 && a.kv_rows <= (1ll << 24) && a.kv_ss < (1ll << 24) &&
+                   a.scale_ss < (1ll << 24) && a.kv_rows * a.kv_ss <= (1ll << 32),
+               HIER_EUNSUPPORTED,
+               "a head's codes must span at most 4 GiB, of 2^24 rows and strides below 2^24 bytes");
   const int64_t total = (int64_t)a.n_items * a.splits * a.H;
   HIER_REQUIRE((int64_t)a.n_items * a.splits < (1ll << 31) && total < (1ll << 24), HIER_EUNSUPPORTED,
                "too many work items");
