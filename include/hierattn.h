@@ -674,7 +674,7 @@ typedef struct HierFwdFp8Args {
   int32_t H, Hk, D;                /* query heads, key heads, head dim         */
   int32_t n_items;
   float scale;                     /* softmax scale                            */
-  int32_t splits;                  /* >= 1                                     */
+  int32_t splits;                  /* 1 .. 32                                  */
   int64_t kv_rows;                 /* rows of each pool                        */
   int64_t q_rows;                  /* rows of q / o                            */
   const uint16_t* q;               /* bf16                                     */

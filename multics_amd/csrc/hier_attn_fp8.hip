@@ -82,7 +82,7 @@ struct Rows {
   int e_hi, e_lo;                            // their scales (exponent + 127)
   f32x16 o[Geo<D>::NDB];
   float m, l, alpha;                         // m in exp2 units
-  int qtok, qframe;
+  int qtok, qframe, head;
   bool valid;
   uint32_t bits;   // OR over the sub-block's valid rows of 1 << query frame
 };
@@ -104,12 +104,16 @@ __device__ __forceinline__ void row_of(R& r, const HierFwdFp8Args& a, const int3
   }
 }
 
+// ``pack`` > 1: the sub-block holds that many query heads, from ``head`` on, of
+// every row (they share a key head); R.head is the lane's.
 template <int D>
 __device__ __forceinline__ void rows_init(Rows<D>& R, const HierFwdFp8Args& a, const int32_t* it,
-                                          int head, int rrel, int lane) {
-  row_of(R, a, it, rrel + (lane & 31));
+                                          int head, int rrel, int lane, int pack = 1) {
+  const int rel = rrel + (lane & 31);
+  row_of(R, a, it, pack == 1 ? rel : rel / pack);
+  R.head = head + (pack == 1 ? 0 : rel % pack);
   R.bits = wave_or(R.valid ? (1u << R.qframe) : 0u);
-  const uint16_t* qp = a.q + (int64_t)R.qtok * a.q_ss + (int64_t)head * a.q_sh + 32 * (lane >> 5);
+  const uint16_t* qp = a.q + (int64_t)R.qtok * a.q_ss + (int64_t)R.head * a.q_sh + 32 * (lane >> 5);
   u32x4 w[Geo8<D>::NS][4];
   uint32_t mag = 0;
 #pragma unroll
@@ -277,10 +281,11 @@ __device__ __forceinline__ void pv_block(Rows<D>& R, const bf16x8* p, const char
 }
 
 template <int D>
-__device__ __forceinline__ void store_rows(const Rows<D>& R, const HierFwdFp8Args& a, int head,
-                                           int split, int lane) {
+__device__ __forceinline__ void store_rows(const Rows<D>& R, const HierFwdFp8Args& a, int split,
+                                           int lane) {
   const float l = pair_sum(R.l);
   if (!R.valid) return;
+  const int head = R.head;
   const int half = lane >> 5;
   if (a.splits > 1) {
     const int64_t at = ((int64_t)split * a.H + head) * a.q_rows + R.qtok;
@@ -385,23 +390,26 @@ __device__ __forceinline__ void load_v(const Ctx<D>& c, const Row<D>& r, VRegs<D
   load_scales<D>(c, c.sv, r, v.s);
 }
 
-// Sixteen codes as bf16 (exact) into two chunks of the tile.
+// Codes 8 p .. 8 p + 7 of a chunk as bf16 (exact).
+__device__ __forceinline__ u32x4 wide_codes(const u32x4& v, int p, float scale) {
+  u32x4 b;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t w = v[2 * p + i];
+    b[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
+    b[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true));
+  }
+  return b;
+}
+
 template <int D>
 __device__ __forceinline__ void store_v(const Ctx<D>& c, const VRegs<D>& v, char* slot) {
 #pragma unroll
   for (int e = 0; e < Geo8<D>::NL; ++e) {
     const float sv = pow2_of(v.s[e]);
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      u32x4 b;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t w = v.w[e][2 * p + i];
-        b[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, sv, false));
-        b[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, sv, true));
-      }
-      *reinterpret_cast<u32x4*>(slot + c.vst[2 * e + p]) = b;
-    }
+    for (int p = 0; p < 2; ++p)
+      *reinterpret_cast<u32x4*>(slot + c.vst[2 * e + p]) = wide_codes(v.w[e], p, sv);
   }
 }
 
@@ -536,6 +544,149 @@ __device__ __forceinline__ void last_tile(Ctx<D>& c, Rows<D>& R, const f32x16& s
   pv_block<D>(R, pb, st.v[PAR], c.ra, 1);
 }
 
+// ---- items of at most 32 rows --------------------------------------------------
+//
+// A hub's rows, a player's last rows or a single token fill one 32-row
+// sub-block.  All four waves take it, each on every fourth tile of the list
+// with a softmax state of its own, and nothing to wait for in the others: K
+// goes from memory straight into the MFMA operand (a lane holds 32 codes of
+// one key twice), V through 32 rows of LDS that are the wave's own.  The next
+// block's loads are in flight while one is multiplied.  The four states are
+// joined through LDS.  Query heads that share a key head are packed into the
+// sub-block when they fit, so that its K and V are read once.
+
+template <int D>
+struct Block {               // what a wave loads of a 32-key block
+  static constexpr int NV = 32 / Geo8<D>::RPC;   // 16-byte loads of V
+  u32x4 k[2 * Geo8<D>::NS];
+  u32x4 v[NV];
+  uint32_t sk, sv[NV];
+};
+template <int D>
+struct BlockRow {
+  int k, v[Block<D>::NV];    // pool rows: of the lane's key, of its chunks of V
+};
+
+template <int D>
+__device__ __forceinline__ BlockRow<D> block_rows(const Ctx<D>& c, int b) {
+  BlockRow<D> r;
+  const int32_t* p = c.kv_idx + b * 32;
+  r.k = p[c.lane & 31];
+#pragma unroll
+  for (int e = 0; e < Block<D>::NV; ++e) r.v[e] = p[Geo8<D>::RPC * e + c.lane / Geo8<D>::CPR];
+  return r;
+}
+
+template <int D>
+__device__ __forceinline__ void block_load(const Ctx<D>& c, const BlockRow<D>& r, Block<D>& x) {
+  const char* k = c.gk + (__umul24((uint32_t)r.k, c.ss_b) + 32u * (uint32_t)(c.lane >> 5));
+#pragma unroll
+  for (int i = 0; i < 2 * Geo8<D>::NS; ++i)
+    x.k[i] = *reinterpret_cast<const u32x4*>(k + 64 * (i >> 1) + 16 * (i & 1));
+#pragma unroll
+  for (int e = 0; e < Block<D>::NV; ++e)
+    x.v[e] = *reinterpret_cast<const u32x4*>(c.gv + (__umul24((uint32_t)r.v[e], c.ss_b) + c.v16));
+  x.sk = c.sk[__umul24((uint32_t)r.k / HIER_FP8_BLOCK, c.scale_b)];
+#pragma unroll
+  for (int e = 0; e < Block<D>::NV; ++e)
+    x.sv[e] = c.sv[__umul24((uint32_t)r.v[e] / HIER_FP8_BLOCK, c.scale_b)];
+}
+
+// Set the scores that the lane's query frame may not see to -inf, masks from
+// the list.
+__device__ __forceinline__ void mask_from(f32x16& s, const uint32_t* mk, int qframe, int lane) {
+  mask_block(s, reinterpret_cast<const char*>(mk), 0, qframe, lane);
+}
+
+template <int D>
+__device__ __forceinline__ void few_rows(const HierFwdFp8Args& a, const int32_t* it, Ctx<D>& c,
+                                         int head, int pack, int split, const Stages& st) {
+  using B = Block<D>;
+  Rows<D> R;
+  rows_init<D>(R, a, it, head, 0, c.lane, pack);
+  char* const vslot = (c.wave < 2 ? st.v[0] : st.v[1]) + (c.wave & 1) * 32 * Geo<D>::ROWB;
+  int vst[2 * B::NV];
+#pragma unroll
+  for (int e = 0; e < B::NV; ++e)
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int row = Geo8<D>::RPC * e + c.lane / Geo8<D>::CPR;
+      vst[2 * e + p] = prow<D>(row) * Geo<D>::ROWB +
+                       16 * ((2 * (c.lane % Geo8<D>::CPR) + p) ^ swz<D, kTrRead>(row));
+    }
+  // block b of the wave: 32-key block b & 1 of tile wave + 4 (b >> 1)
+  const int mine = c.nt > c.wave ? 2 * ((c.nt - c.wave + kWaves - 1) / kWaves) : 0;
+  const auto at = [&](int b) { return 2 * (c.wave + kWaves * (b >> 1)) + (b & 1); };
+  if (mine > 0) {
+    Block<D> x;
+    block_load<D>(c, block_rows<D>(c, at(0)), x);
+    BlockRow<D> next = block_rows<D>(c, at(1));
+    for (int b = 0; b < mine; ++b) {
+      // S^T
+      f32x16 s = {};
+#pragma unroll
+      for (int i = 0; i < Geo8<D>::NS; ++i) {
+        const u32x4 u = x.k[2 * i], w = x.k[2 * i + 1];
+        const i32x8 k = {(int)u[0], (int)u[1], (int)u[2], (int)u[3],
+                         (int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+        s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, R.hi[i], s, 0, 0, 0, (int)x.sk, 0, R.e_hi);
+        s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, R.lo[i], s, 0, 0, 0, (int)x.sk, 0, R.e_lo);
+      }
+      // V to LDS in bf16
+#pragma unroll
+      for (int e = 0; e < B::NV; ++e) {
+        const float sv = pow2_of(x.sv[e]);
+#pragma unroll
+        for (int p = 0; p < 2; ++p) *reinterpret_cast<u32x4*>(vslot + vst[2 * e + p]) = wide_codes(x.v[e], p, sv);
+      }
+      const int blk = at(b);
+      const bool masked = (c.blk[blk >> 1] & R.bits) != R.bits;
+      // the next block's loads (past the last: the last again)
+      if (b + 1 < mine) {
+        block_load<D>(c, next, x);
+        next = block_rows<D>(c, at(min(b + 2, mine - 1)));
+      }
+      if (masked) mask_from(s, c.kv_mask + blk * 32, R.qframe, c.lane);
+      bf16x8 p[2];
+      if (softmax_block<D>(R, s, p, c.c2)) rescale<D>(R, R.alpha);
+      pv_block<D>(R, p, vslot, c.ra, 0);
+    }
+  }
+  // join: waves 2, 3 into 0, 1, then 1 into 0 (O^T as fp32 [element][lane] in
+  // the V stages, m and l in the mask stages)
+  float* const ml = reinterpret_cast<float*>(st.m[0]);     // [64 lanes]: m, and
+  float* const ll = reinterpret_cast<float*>(st.m[1]);     // l, of one wave
+#pragma unroll
+  for (int half = 2; half >= 1; half >>= 1) {
+    __syncthreads();
+    if (c.wave >= half && c.wave < 2 * half) {
+      float* o = reinterpret_cast<float*>(c.wave == half ? st.v[0] : st.v[1]);
+#pragma unroll
+      for (int db = 0; db < Geo<D>::NDB; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[(db * 16 + e) * 64 + c.lane] = R.o[db][e];
+      // both halves of a row's lanes hold the same m; each its part of l
+      st.s[0][(c.wave - half) * 32 + (c.lane & 31)] = __float_as_int(R.m);
+      (c.wave == half ? ml : ll)[c.lane] = R.l;
+    }
+    __syncthreads();
+    if (c.wave < half) {
+      const float* o = reinterpret_cast<const float*>(c.wave == 0 ? st.v[0] : st.v[1]);
+      const float m2 = __int_as_float(st.s[0][c.wave * 32 + (c.lane & 31)]);
+      const float m = fmaxf(R.m, m2);
+      const float w1 = __builtin_amdgcn_exp2f(R.m - m), w2 = __builtin_amdgcn_exp2f(m2 - m);
+      R.l = R.l * w1 + (c.wave == 0 ? ml : ll)[c.lane] * w2;
+      R.m = m;
+#pragma unroll
+      for (int db = 0; db < Geo<D>::NDB; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          R.o[db][e] = R.o[db][e] * w1 + o[(db * 16 + e) * 64 + c.lane] * w2;
+    }
+  }
+  if (c.wave == 0) store_rows<D>(R, a, split, c.lane);
+}
+
 template <int D>
 __global__ __launch_bounds__(kThreads, 2) void attn_fp8_kernel(HierFwdFp8Args a, int total) {
   __shared__ __align__(16) char lds_k0[Geo8<D>::KTILEB], lds_k1[Geo8<D>::KTILEB];
@@ -551,12 +702,17 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fp8_kernel(HierFwdFp8Args a,
   const int32_t* it = a.tile_items + (int64_t)item * 8;
   Ctx<D> c;
   setup<D>(c, a, it, head, split, threadIdx.x);
+  if (it[4] <= 32) {
+    const int group = a.H / a.Hk, pack = group * it[4] <= 32 ? group : 1;
+    if (head % pack == 0) few_rows<D>(a, it, c, head, pack, split, st);
+    return;
+  }
   c.active = c.wave * 32 < it[4];
   Rows<D> R;
   rows_init<D>(R, a, it, head, c.wave * 32, c.lane);
   const int nt = c.nt;
   if (nt == 0) {
-    if (c.active) store_rows<D>(R, a, head, split, c.lane);
+    if (c.active) store_rows<D>(R, a, split, c.lane);
     return;
   }
   Row<D> ik, iv;
@@ -590,42 +746,70 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fp8_kernel(HierFwdFp8Args a,
   } else if (c.active) {
     last_tile<D, 0>(c, R, sb, pa, pb, resc, alpha_pend, st);
   }
-  if (c.active) store_rows<D>(R, a, head, split, c.lane);
+  if (c.active) store_rows<D>(R, a, split, c.lane);
 }
 
-// Joins the splits of one item and head: rows in turn, D / 4 lanes a row.
+// Joins the parts of one item and head, kJoinRows rows a workgroup, D / 4 lanes
+// a row: the parts' maxima and sums are read at once, one or two a lane (at
+// most 32 parts), and their O's eight at a time, so that a row costs a few
+// memory latencies and not one a part.
+constexpr int kMaxSplits = 32;
 template <int D>
 __global__ __launch_bounds__(kThreads) void join_fp8_kernel(HierFwdFp8Args a) {
-  constexpr int LPR = D / 4;
+  constexpr int LPR = D / 4, ROWS = kThreads / LPR, PER = kMaxSplits / LPR;
   struct { int qtok, qframe; bool valid; } r;
   const int head = blockIdx.x / a.n_items, item = blockIdx.x - head * a.n_items;
   const int32_t* it = a.tile_items + (int64_t)item * 8;
-  const int d = 4 * (threadIdx.x % LPR);
-  const int64_t step = (int64_t)a.H * a.q_rows;
-  for (int rel = threadIdx.x / LPR; rel < it[4]; rel += kThreads / LPR) {
-    row_of(r, a, it, rel);
-    if (!r.valid) continue;
-    const int64_t at = (int64_t)head * a.q_rows + r.qtok;
-    float m = kNoMax;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (at + s * step)]);
-    float l = 0.f;
-    f32x4 o = {};
-    for (int s = 0; s < a.splits; ++s) {
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (at + s * step));
-      const float w = __builtin_amdgcn_exp2f(ml.x - m);
-      const f32x4 p = *reinterpret_cast<const f32x4*>(a.part_o + (at + s * step) * D + d);
-      l = fmaf(ml.y, w, l);
+  const int rel = blockIdx.y * ROWS + threadIdx.x / LPR, sub = threadIdx.x % LPR;
+  if (blockIdx.y * ROWS >= it[4]) return;
+  row_of(r, a, it, rel);
+  const int64_t at = (int64_t)head * a.q_rows + r.qtok, step = (int64_t)a.H * a.q_rows;
+  float ms[PER], ls[PER], m = kNoMax;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = fmaf(p[i], w, o[i]);
+  for (int i = 0; i < PER; ++i) {
+    const int s = sub + i * LPR;
+    ms[i] = kNoMax, ls[i] = 0.f;
+    if (r.valid && s < a.splits) {
+      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (at + s * step));
+      ms[i] = ml.x, ls[i] = ml.y;
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    u32x2 w;
-    w[0] = (uint32_t)f2bf(o[0] * inv) | ((uint32_t)f2bf(o[1] * inv) << 16);
-    w[1] = (uint32_t)f2bf(o[2] * inv) | ((uint32_t)f2bf(o[3] * inv) << 16);
-    *reinterpret_cast<u32x2*>(a.o + (int64_t)r.qtok * a.o_ss + (int64_t)head * a.o_sh + d) = w;
-    if (a.lse && d == 0)
-      a.lse[(int64_t)head * a.lse_stride_h + r.qtok] = l > 0.f ? fmaf(m, kLn2, __logf(l)) : -INFINITY;
+    m = fmaxf(m, ms[i]);
   }
+#pragma unroll
+  for (int d = 1; d < LPR; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, LPR));
+  float l = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    ms[i] = __builtin_amdgcn_exp2f(ms[i] - m);       // a part's weight
+    l = fmaf(ls[i], ms[i], l);
+  }
+#pragma unroll
+  for (int d = 1; d < LPR; d <<= 1) l += __shfl_xor(l, d, LPR);
+  f32x4 o = {};
+  const float* p = a.part_o + at * D + 4 * sub;
+  for (int s0 = 0; s0 < a.splits; s0 += 8) {
+    f32x4 x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = f32x4{};
+      if (r.valid && s0 + i < a.splits) x[i] = *reinterpret_cast<const f32x4*>(p + (s0 + i) * step * D);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      // (a row's lanes hold parts sub and sub + LPR)
+      const float w = __shfl(PER == 2 && s0 + i >= LPR ? ms[PER - 1] : ms[0], (s0 + i) % LPR, LPR);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = s0 + i < a.splits ? fmaf(x[i][j], w, o[j]) : o[j];
+    }
+  }
+  if (!r.valid) return;
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  u32x2 w;
+  w[0] = (uint32_t)f2bf(o[0] * inv) | ((uint32_t)f2bf(o[1] * inv) << 16);
+  w[1] = (uint32_t)f2bf(o[2] * inv) | ((uint32_t)f2bf(o[3] * inv) << 16);
+  *reinterpret_cast<u32x2*>(a.o + (int64_t)r.qtok * a.o_ss + (int64_t)head * a.o_sh + 4 * sub) = w;
+  if (a.lse && sub == 0)
+    a.lse[(int64_t)head * a.lse_stride_h + r.qtok] = l > 0.f ? fmaf(m, kLn2, __logf(l)) : -INFINITY;
 }
 
 template <int D>
@@ -634,8 +818,8 @@ int launch(const HierFwdFp8Args& a, int64_t total, hipStream_t stream) {
                      stream, a, (int)total);
   const int rc = hier::check_launch("attn_fp8_kernel");
   if (rc != HIER_OK || a.splits == 1) return rc;
-  hipLaunchKernelGGL(join_fp8_kernel<D>, dim3((unsigned)(a.n_items * a.H)), dim3(kThreads), 0, stream,
-                     a);
+  hipLaunchKernelGGL(join_fp8_kernel<D>, dim3((unsigned)(a.n_items * a.H), 128 * (D / 4) / kThreads),
+                     dim3(kThreads), 0, stream, a);
   return hier::check_launch("join_fp8_kernel");
 }
 
@@ -648,7 +832,9 @@ extern "C" int hier_attn_fwd_fp8(const HierFwdFp8Args* args, void* stream) {
   HIER_REQUIRE(a.D == 128 || a.D == 64, HIER_EUNSUPPORTED, "head_dim must be 64 or 128, got %d", a.D);
   HIER_REQUIRE(a.H >= 1 && a.Hk >= 1 && a.H % a.Hk == 0, HIER_EINVAL,
                "H=%d must be a multiple of Hk=%d", a.H, a.Hk);
-  HIER_REQUIRE(a.n_items >= 0 && a.kv_rows >= 0 && a.q_rows >= 0 && a.splits >= 1, HIER_EINVAL,
+  HIER_REQUIRE(a.n_items >= 0 && a.kv_rows >= 0 && a.q_rows >= 0 && a.splits >= 1 &&
+                   a.splits <= kMaxSplits,
+               HIER_EINVAL,
                "invalid n_items=%d kv_rows=%lld q_rows=%lld splits=%d", a.n_items,
                (long long)a.kv_rows, (long long)a.q_rows, a.splits);
   if (a.n_items == 0) return HIER_OK;
