@@ -63,11 +63,27 @@ struct Stages {
   int* s[2];
 };
 
-// XOR mask on the 16-byte chunk index of row `row` of a K tile: 8 consecutive
-// rows at one chunk column fall into different banks.
+// XOR masks on the 16-byte chunk index of a row.  LDS serves 16 lanes of a
+// 16-byte access at once from 64 banks (256 bytes).
+// K tile (D bytes a row, 2 or 4 rows per 256): 16 consecutive rows at one chunk
+// column fall into different banks.
 template <int D>
-__device__ __forceinline__ int kswz(int row) {
-  return D == 128 ? (row & 7) : ((row >> 1) & 3);
+__device__ __forceinline__ constexpr int kswz(int row) {
+  return D == 128 ? ((row >> 1) & 7) : ((row >> 2) & 3);
+}
+// V tile: the swizzle of the transposed reads, and its lowest bit turned in
+// odd rows, so that the writes of two rows' even (or odd) chunks do not meet;
+// the reads take whole groups of four chunks and stay free of conflicts.
+template <int D>
+__device__ __forceinline__ constexpr int vswz(int row) {
+  return swz<D, kTrRead>(row) ^ (row & 1);
+}
+// tr_read_off over that swizzle.
+template <int D>
+__device__ __forceinline__ int v_read_off(int lane, int db) {
+  const int i = lane & 15, row = 4 * (lane >> 5) + (i >> 2);
+  const int q = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+  return prow<D>(row) * Geo<D>::ROWB + 16 * ((4 * db + q) ^ vswz<D>(row)) + 8 * (i & 1);
 }
 
 __device__ __forceinline__ float pow2_of(uint32_t byte) { return __uint_as_float(byte << 23); }
@@ -174,7 +190,7 @@ struct ReadAddr {
     for (int i = 0; i < 2 * Geo8<D>::NS; ++i)
       k[i] = key * D + 16 * ((4 * (i >> 1) + 2 * (lane >> 5) + (i & 1)) ^ kswz<D>(key));
 #pragma unroll
-    for (int db = 0; db < Geo<D>::NDB; ++db) v[db] = tr_read_off<D, kTrRead>(lane, db, 0);
+    for (int db = 0; db < Geo<D>::NDB; ++db) v[db] = v_read_off<D>(lane, db);
   }
 };
 
@@ -335,7 +351,7 @@ struct Ctx {
   int nt, wave, lane;
   bool active;
   int row0;                  // the lane's first row of a tile
-  uint32_t k16, v16;         // byte offsets of its chunk in a row: K's swizzled source, V's
+  uint32_t k16[Geo8<D>::NL], v16;   // byte offsets of its chunk in a row: K's swizzled source, V's
   int vst[2 * Geo8<D>::NL];  // where its chunks of V go
   ReadAddr<D> ra;
 };
@@ -363,7 +379,7 @@ template <int D>
 __device__ __forceinline__ void copy_k(const Ctx<D>& c, const Row<D>& r, char* slot) {
 #pragma unroll
   for (int e = 0; e < Geo8<D>::NL; ++e)
-    dma16(c.gk, __umul24((uint32_t)r.v[e], c.ss_b) + c.k16,
+    dma16(c.gk, __umul24((uint32_t)r.v[e], c.ss_b) + c.k16[e],
           slot + (16 * c.wave + Geo8<D>::RPC * e) * D);
 }
 
@@ -439,15 +455,15 @@ __device__ __forceinline__ void setup(Ctx<D>& c, const HierFwdFp8Args& a, const 
   c.c2 = a.scale * 1.4426950408889634f;
   const int chunk = c.lane % G::CPR;
   c.row0 = 16 * c.wave + c.lane / G::CPR;
-  c.k16 = 16u * (uint32_t)(chunk ^ kswz<D>(c.row0));   // (the same for each of its rows)
   c.v16 = 16u * (uint32_t)chunk;
 #pragma unroll
-  for (int e = 0; e < G::NL; ++e)
+  for (int e = 0; e < G::NL; ++e) {
+    const int row = c.row0 + G::RPC * e;
+    c.k16[e] = 16u * (uint32_t)(chunk ^ kswz<D>(row));
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const int row = c.row0 + G::RPC * e;
-      c.vst[2 * e + p] = prow<D>(row) * Geo<D>::ROWB + 16 * ((2 * chunk + p) ^ swz<D, kTrRead>(row));
-    }
+    for (int p = 0; p < 2; ++p)
+      c.vst[2 * e + p] = prow<D>(row) * Geo<D>::ROWB + 16 * ((2 * chunk + p) ^ vswz<D>(row));
+  }
   c.ra.init(c.lane);
 }
 
@@ -491,8 +507,9 @@ __device__ __forceinline__ void half_step(Ctx<D>& c, Rows<D>& R, f32x16& sq, con
   sq = qk_block<D>(R, st.k[PAR ^ 1], st.s[PAR ^ 1], c.ra, B, c.lane);
   float ps = p_block(sc, pn, c.c2, -R.m);
   pv_block<D>(R, pv, st.v[PAR], c.ra, B);
-  // keep the softmax results in this region (otherwise they sink past the
-  // branches below, away from the MFMAs they are meant to overlap)
+  // keep S and the softmax results in this region (otherwise they sink past the
+  // branches below, away from what they are meant to overlap)
+  asm volatile("" : "+v"(sq));
   asm volatile("" : "+v"(pn[0]), "+v"(pn[1]), "+v"(ps));
   resc = softmax_fix<D>(R, sc, pn, c.c2, ps);
   alpha_pend = R.alpha;
@@ -612,7 +629,7 @@ __device__ __forceinline__ void few_rows(const HierFwdFp8Args& a, const int32_t*
     for (int p = 0; p < 2; ++p) {
       const int row = Geo8<D>::RPC * e + c.lane / Geo8<D>::CPR;
       vst[2 * e + p] = prow<D>(row) * Geo<D>::ROWB +
-                       16 * ((2 * (c.lane % Geo8<D>::CPR) + p) ^ swz<D, kTrRead>(row));
+                       16 * ((2 * (c.lane % Geo8<D>::CPR) + p) ^ vswz<D>(row));
     }
   // block b of the wave: 32-key block b & 1 of tile wave + 4 (b >> 1)
   const int mine = c.nt > c.wave ? 2 * ((c.nt - c.wave + kWaves - 1) / kWaves) : 0;
