@@ -63,27 +63,27 @@ struct Stages {
   int* s[2];
 };
 
-// XOR masks on the 16-byte chunk index of a row.  LDS serves 16 lanes of a
-// 16-byte access at once from 64 banks (256 bytes).
-// K tile (D bytes a row, 2 or 4 rows per 256): 16 consecutive rows at one chunk
-// column fall into different banks.
+// Where the 16-byte chunks of a row stand in its tile.
+// K tile (D bytes a row): XOR mask on the chunk index, so that 16 consecutive
+// rows at one chunk column fall into different banks of a read (256 bytes).
 template <int D>
 __device__ __forceinline__ constexpr int kswz(int row) {
   return D == 128 ? ((row >> 1) & 7) : ((row >> 2) & 3);
 }
-// V tile: the swizzle of the transposed reads, and its lowest bit turned in
-// odd rows, so that the writes of two rows' even (or odd) chunks do not meet;
-// the reads take whole groups of four chunks and stay free of conflicts.
+// V tile: the swizzle of the transposed reads, and the lowest bit turned in the
+// upper half of a row (D = 64: in odd rows), so that the even chunks that eight
+// lanes write at once fall into different banks of a write (128 bytes); a read
+// takes whole groups of four chunks and does not see it.
 template <int D>
-__device__ __forceinline__ constexpr int vswz(int row) {
-  return swz<D, kTrRead>(row) ^ (row & 1);
+__device__ __forceinline__ constexpr int v_chunk(int row, int chunk) {
+  return chunk ^ swz<D, kTrRead>(row) ^ (D == 128 ? (chunk >> 3) & 1 : row & 1);
 }
-// tr_read_off over that swizzle.
+// tr_read_off over it.
 template <int D>
 __device__ __forceinline__ int v_read_off(int lane, int db) {
   const int i = lane & 15, row = 4 * (lane >> 5) + (i >> 2);
   const int q = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-  return prow<D>(row) * Geo<D>::ROWB + 16 * ((4 * db + q) ^ vswz<D>(row)) + 8 * (i & 1);
+  return prow<D>(row) * Geo<D>::ROWB + 16 * v_chunk<D>(row, 4 * db + q) + 8 * (i & 1);
 }
 
 __device__ __forceinline__ float pow2_of(uint32_t byte) { return __uint_as_float(byte << 23); }
@@ -462,7 +462,7 @@ __device__ __forceinline__ void setup(Ctx<D>& c, const HierFwdFp8Args& a, const 
     c.k16[e] = 16u * (uint32_t)(chunk ^ kswz<D>(row));
 #pragma unroll
     for (int p = 0; p < 2; ++p)
-      c.vst[2 * e + p] = prow<D>(row) * Geo<D>::ROWB + 16 * ((2 * chunk + p) ^ vswz<D>(row));
+      c.vst[2 * e + p] = prow<D>(row) * Geo<D>::ROWB + 16 * v_chunk<D>(row, 2 * chunk + p);
   }
   c.ra.init(c.lane);
 }
@@ -629,7 +629,7 @@ __device__ __forceinline__ void few_rows(const HierFwdFp8Args& a, const int32_t*
     for (int p = 0; p < 2; ++p) {
       const int row = Geo8<D>::RPC * e + c.lane / Geo8<D>::CPR;
       vst[2 * e + p] = prow<D>(row) * Geo<D>::ROWB +
-                       16 * ((2 * (c.lane % Geo8<D>::CPR) + p) ^ vswz<D>(row));
+                       16 * v_chunk<D>(row, 2 * (c.lane % Geo8<D>::CPR) + p);
     }
   // block b of the wave: 32-key block b & 1 of tile wave + 4 (b >> 1)
   const int mine = c.nt > c.wave ? 2 * ((c.nt - c.wave + kWaves - 1) / kWaves) : 0;
