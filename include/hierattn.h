@@ -602,7 +602,8 @@ int hier_head_prologue(const HierHeadNormArgs* args, void* stream);
 
 /* Its gradient, recomputed from the inputs: dqx / dkx (contiguous rows) and   */
 /* the gains' gradients, summed over tokens and heads in a fixed order        */
-/* through partial, fp32 [hier_head_prologue_bwd_rows][D].                    */
+/* through partial, fp32 [partial_rows][D], partial_rows at least             */
+/* min(2 * ceil(S / 8), 2050).                                                */
 typedef struct HierHeadNormBwdArgs {
   int64_t S;
   int32_t Hq, Hk, D;
@@ -623,10 +624,9 @@ typedef struct HierHeadNormBwdArgs {
   float* dnorm_q;                  /* [D]                                      */
   float* dnorm_k;
   float* partial;
+  int64_t partial_rows;
 } HierHeadNormBwdArgs;
 
-/* Rows of partial, or a negative error code.                                 */
-int hier_head_prologue_bwd_rows(const HierHeadNormBwdArgs* args);
 int hier_head_prologue_bwd(const HierHeadNormBwdArgs* args, void* stream);
 
 /* ------------------------------------------------------------------------ */

@@ -128,7 +128,7 @@ __device__ __forceinline__ void rows_init(Rows<D>& R, const HierFwdFp8Args& a, c
   const int rel = rrel + (lane & 31);
   row_of(R, a, it, pack == 1 ? rel : rel / pack);
   R.head = head + (pack == 1 ? 0 : rel % pack);
-  R.bits = wave_or(R.valid ? (1u << R.qframe) : 0u);
+  R.bits = __builtin_amdgcn_readfirstlane(wave_or(R.valid ? (1u << R.qframe) : 0u));
   const uint16_t* qp = a.q + (int64_t)R.qtok * a.q_ss + (int64_t)R.head * a.q_sh + 32 * (lane >> 5);
   u32x4 w[Geo8<D>::NS][4];
   uint32_t mag = 0;
@@ -247,26 +247,46 @@ __device__ __forceinline__ float p_block(const f32x16& s, bf16x8* p, float c2, f
   return ps0 + ps1;
 }
 
+// x = y where x stands: the rare path writes into the registers of the common
+// one, which so needs no copies where the two meet.  (The s_nop are the wait
+// states behind an exp and in front of an MFMA, which the compiler does not add
+// around assembly.)
+__device__ __forceinline__ void put(float& x, float y) {
+  asm volatile("s_nop 1\n\tv_mov_b32 %0, %2\n\ts_nop 1" : "=v"(x) : "0"(x), "v"(y));
+}
+__device__ __forceinline__ void put(bf16x8& x, const bf16x8& y) {
+  u32x4 u = __builtin_bit_cast(u32x4, x);
+  const u32x4 w = __builtin_bit_cast(u32x4, y);
+  asm volatile("s_nop 1\n\tv_mov_b32 %0, %8\n\tv_mov_b32 %1, %9\n\tv_mov_b32 %2, %10\n\tv_mov_b32 %3, %11\n\ts_nop 1"
+               : "=&v"(u[0]), "=&v"(u[1]), "=&v"(u[2]), "=&v"(u[3])
+               : "0"(u[0]), "1"(u[1]), "2"(u[2]), "3"(u[3]), "v"(w[0]), "v"(w[1]), "v"(w[2]), "v"(w[3]));
+  x = __builtin_bit_cast(bf16x8, u);
+}
+
 // Online softmax, second half: ps is the lane's sum of a block's P taken
 // against the running max.  True: the max was refreshed and P recomputed; O is
 // to be scaled by R.alpha before the block's P V.
 template <int D>
 __device__ __forceinline__ bool softmax_fix(Rows<D>& R, const f32x16& s, bf16x8* p, float c2,
                                             float ps) {
-  if (__ballot(!(ps <= kSumMax)) == 0) {
-    R.l += ps;
-    R.alpha = 1.f;
-    return false;
-  }
-  float mx = s[0];
+  float alpha = 1.f;
+  const bool refresh = __ballot(!(ps <= kSumMax)) != 0;
+  if (__builtin_expect(refresh, 0)) {
+    float mx = s[0];
 #pragma unroll
-  for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-  mx = pair_max(mx);
-  const float m_new = fmaxf(R.m, mx * c2);
-  R.alpha = __builtin_amdgcn_exp2f(R.m - m_new);
-  R.m = m_new;
-  R.l = R.l * R.alpha + p_block(s, p, c2, -m_new);
-  return true;
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    mx = pair_max(mx);
+    const float m = fmaxf(R.m, mx * c2);
+    bf16x8 q[2];
+    put(ps, p_block(s, q, c2, -m));
+    put(p[0], q[0]);
+    put(p[1], q[1]);
+    put(alpha, __builtin_amdgcn_exp2f(R.m - m));
+    put(R.m, m);
+  }
+  R.l = fmaf(R.l, alpha, ps);
+  R.alpha = alpha;
+  return refresh;
 }
 
 template <int D>
@@ -369,9 +389,9 @@ struct VRegs {
 template <int D>
 __device__ __forceinline__ Row<D> load_rows(const Ctx<D>& c, int tile) {
   Row<D> r;
+  const int32_t* p = c.kv_idx + tile * kSlab;
 #pragma unroll
-  for (int e = 0; e < Geo8<D>::NL; ++e)
-    r.v[e] = c.kv_idx[tile * kSlab + c.row0 + Geo8<D>::RPC * e];
+  for (int e = 0; e < Geo8<D>::NL; ++e) r.v[e] = p[(uint32_t)c.row0 + Geo8<D>::RPC * e];
   return r;
 }
 
@@ -388,7 +408,7 @@ __device__ __forceinline__ void load_scales(const Ctx<D>& c, const uint8_t* sc, 
                                             uint32_t* s) {
 #pragma unroll
   for (int e = 0; e < Geo8<D>::NL; ++e)
-    s[e] = sc[__umul24((uint32_t)r.v[e] / HIER_FP8_BLOCK, c.scale_b)];
+    s[e] = sc[(uint32_t)__umul24((uint32_t)r.v[e] / HIER_FP8_BLOCK, c.scale_b)];
 }
 
 template <int D>
@@ -473,7 +493,7 @@ __device__ __forceinline__ void first_tiles(Ctx<D>& c, Row<D>& ik, Row<D>& iv, u
   const Row<D> r0 = load_rows<D>(c, 0);
   iv = load_rows<D>(c, min(1, c.nt - 1));
   ik = load_rows<D>(c, min(2, c.nt - 1));
-  blk = c.blk[min(1, c.nt - 1)];
+  blk = __builtin_amdgcn_readfirstlane(c.blk[min(1, c.nt - 1)]);
   uint32_t s[Geo8<D>::NL];
   VRegs<D> v;
   copy_k<D>(c, r0, st.k[0]);
@@ -545,7 +565,7 @@ __device__ __forceinline__ void tile_iter(Ctx<D>& c, Rows<D>& R, int t, f32x16& 
   if (more) store_scales<D>(c, s, st.s[PAR]);
   wait_copies();
   __syncthreads();
-  blk = blk_pre;
+  blk = __builtin_amdgcn_readfirstlane(blk_pre);   // (not before: it waits for the load)
 }
 
 // Last tile (t = nt - 1): softmax of its block 1 (sb) into pb, P V of both.
@@ -603,10 +623,10 @@ __device__ __forceinline__ void block_load(const Ctx<D>& c, const BlockRow<D>& r
 #pragma unroll
   for (int e = 0; e < Block<D>::NV; ++e)
     x.v[e] = *reinterpret_cast<const u32x4*>(c.gv + (__umul24((uint32_t)r.v[e], c.ss_b) + c.v16));
-  x.sk = c.sk[__umul24((uint32_t)r.k / HIER_FP8_BLOCK, c.scale_b)];
+  x.sk = c.sk[(uint32_t)__umul24((uint32_t)r.k / HIER_FP8_BLOCK, c.scale_b)];
 #pragma unroll
   for (int e = 0; e < Block<D>::NV; ++e)
-    x.sv[e] = c.sv[__umul24((uint32_t)r.v[e] / HIER_FP8_BLOCK, c.scale_b)];
+    x.sv[e] = c.sv[(uint32_t)__umul24((uint32_t)r.v[e] / HIER_FP8_BLOCK, c.scale_b)];
 }
 
 // Set the scores that the lane's query frame may not see to -inf, masks from
@@ -657,7 +677,7 @@ __device__ __forceinline__ void few_rows(const HierFwdFp8Args& a, const int32_t*
         for (int p = 0; p < 2; ++p) *reinterpret_cast<u32x4*>(vslot + vst[2 * e + p]) = wide_codes(x.v[e], p, sv);
       }
       const int blk = at(b);
-      const bool masked = (c.blk[blk >> 1] & R.bits) != R.bits;
+      const bool masked = (__builtin_amdgcn_readfirstlane(c.blk[blk >> 1]) & R.bits) != R.bits;
       // the next block's loads (past the last: the last again)
       if (b + 1 < mine) {
         block_load<D>(c, next, x);

@@ -261,14 +261,6 @@ extern "C" int hier_head_prologue(const HierHeadNormArgs* args, void* stream) {
   return hier::check_launch("head_norm_kernel");
 }
 
-extern "C" int hier_head_prologue_bwd_rows(const HierHeadNormBwdArgs* args) {
-  if (args == nullptr || args->S < 1 || args->Hq < 1 || args->Hk < 1 ||
-      (int64_t)args->Hq + args->Hk > (1 << 30))
-    return HIER_EINVAL;
-  const int H = args->Hq + args->Hk;
-  return bwd_rows(args->S, args->Hq, H) + bwd_rows(args->S, args->Hk, H);
-}
-
 extern "C" int hier_head_prologue_bwd(const HierHeadNormBwdArgs* args, void* stream) {
   hier::clear_error();
   HIER_REQUIRE(args != nullptr, HIER_EINVAL, "args is NULL");
@@ -288,6 +280,8 @@ extern "C" int hier_head_prologue_bwd(const HierHeadNormBwdArgs* args, void* str
                HIER_EINVAL, "strides must keep 16-byte rows aligned");
   HIER_REQUIRE(a.S <= (1ll << 31), HIER_EUNSUPPORTED, "too many tokens");
   const int rows_q = bwd_rows(a.S, a.Hq, a.Hq + a.Hk), rows_k = bwd_rows(a.S, a.Hk, a.Hq + a.Hk);
+  HIER_REQUIRE(a.partial_rows >= (int64_t)rows_q + rows_k, HIER_EINVAL, "partial has %lld rows, needs %d",
+               (long long)a.partial_rows, rows_q + rows_k);
   if (a.D == 128)
     hipLaunchKernelGGL(head_norm_bwd_kernel<128>, dim3(rows_q + rows_k), dim3(kThreads), 0,
                        (hipStream_t)stream, a, rows_q, rows_k);

@@ -690,62 +690,69 @@ def qk_prologue_train(qx, kx, *, norm_q_w, norm_k_w, rope_cos, rope_sin, num_hea
 # per-head norms with rotation
 # --------------------------------------------------------------------------
 
-def _head_rows(name: str, t: torch.Tensor, dev) -> tuple:
-    """``t`` [S, H*D] bf16 as rows that the kernels read in place: unit channel
-    stride, 16-byte rows."""
-    if t.dim() != 2:
-        raise ValueError(f"{name} must be [S, H*D], got {tuple(t.shape)}")
-    if t.dtype != torch.bfloat16:
+_pack_head = _capi.packer(_capi.HierHeadNormArgs)
+_pack_head_bwd = _capi.packer(_capi.HierHeadNormBwdArgs)
+_pack_fwd_fp8 = _capi.packer(_capi.HierFwdFp8Args)
+
+
+def _head_rows(name: str, t: torch.Tensor, gpu: int) -> tuple:
+    """``t`` [S, H*D] bf16 as rows that the kernels read in place (unit channel
+    stride, 16-byte rows) and their stride."""
+    if t.dtype is not torch.bfloat16:
         raise NotImplementedError(f"{name} must be bf16, got {t.dtype}")
-    if not t.is_cuda:
-        raise NotImplementedError("per-head norms require GPU tensors")
-    if t.device != dev:
-        raise ValueError(f"{name} is on {t.device}, expected {dev}")
-    if t.stride(1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
+    if t.get_device() != gpu:
+        raise ValueError(f"{name} is on {t.device}, qx on another device")
+    ss, unit = t.stride()
+    if unit != 1 or ss % 8 or t.data_ptr() % 16:
         t = t.contiguous()
-    return t
+        ss = t.stride(0)
+    return t, ss
 
 
-def _head_args(qx, kx, norm_q_w, norm_k_w, rope_cos, rope_sin, num_heads, num_kv_heads):
-    """The checked arguments that the per-head prologue and its gradient share:
-    (qx, kx, gains, cos, sin, Hq, Hk, D)."""
-    dev = qx.device
-    qx, kx = _head_rows("qx", qx, dev), _head_rows("kx", kx, dev)
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _head_args(qx, kx, norm_q_w, norm_k_w, rope_cos, rope_sin, num_heads, num_kv_heads, eps):
+    """The checked arguments that the per-head prologue and its gradient
+    share: (S, Hq, Hk, D, values of the structures' common fields, what keeps
+    their memory)."""
+    if qx.dim() != 2 or kx.dim() != 2:
+        raise ValueError(f"qx, kx must be [S, H*D], got {tuple(qx.shape)}, {tuple(kx.shape)}")
+    gpu = qx.get_device()
+    if gpu < 0:
+        raise NotImplementedError("per-head norms require GPU tensors")
     Hq = int(num_heads)
     Hk = Hq if num_kv_heads is None else int(num_kv_heads)
     S, dim = qx.shape
     if Hq < 1 or Hk < 1 or dim % Hq:
         raise ValueError(f"{dim} channels do not divide into {Hq} heads (and {Hk} key heads)")
     D = dim // Hq
-    if D not in (64, 128):
+    if D != 128 and D != 64:
         raise NotImplementedError(f"per-head norms support head_dim 64/128, got {D}")
     if kx.shape != (S, Hk * D):
         raise ValueError(f"kx must be [{S}, {Hk}*{D}], got {tuple(kx.shape)}")
-    gains = []
+    qx, q_ss = _head_rows("qx", qx, gpu)
+    kx, k_ss = _head_rows("kx", kx, gpu)
     for name, w in (("norm_q_w", norm_q_w), ("norm_k_w", norm_k_w)):
-        if w.shape != (D,) or w.dtype not in (torch.bfloat16, torch.float32) or w.device != dev:
-            raise ValueError(f"{name} must be [{D}] bf16 or fp32 on {dev}, got {tuple(w.shape)} "
-                             f"{w.dtype} on {w.device}")
-        gains.append(w)
-    if gains[0].dtype != gains[1].dtype:
-        gains = [w.float() for w in gains]
-    gains = [w.contiguous() if w.data_ptr() % 16 == 0 else w.clone() for w in gains]
-    tables = []
+        if w.shape != (D,) or w.get_device() != gpu or \
+                w.dtype is not torch.float32 and w.dtype is not torch.bfloat16:
+            raise ValueError(f"{name} must be [{D}] bf16 or fp32 on {qx.device}, got "
+                             f"{tuple(w.shape)} {w.dtype} on {w.device}")
+    bf16 = norm_q_w.dtype is torch.bfloat16
+    if bf16 != (norm_k_w.dtype is torch.bfloat16):
+        norm_q_w, norm_k_w, bf16 = norm_q_w.float(), norm_k_w.float(), False
     for name, t in (("rope_cos", rope_cos), ("rope_sin", rope_sin)):
-        if t.shape != (S, D // 2) or t.device != dev:
-            raise ValueError(f"{name} must be [S, D/2] = {(S, D // 2)} on {dev}, got "
+        if t.shape != (S, D // 2) or t.get_device() != gpu:
+            raise ValueError(f"{name} must be [S, D/2] = {(S, D // 2)} on {qx.device}, got "
                              f"{tuple(t.shape)} on {t.device}")
-        t = t.contiguous().float()
-        tables.append(t if t.data_ptr() % 16 == 0 else t.clone())
-    return qx, kx, gains, tables[0], tables[1], Hq, Hk, D
-
-
-def _head_common(qx, kx, gains, cs, sn, Hq, Hk, D, eps):
-    return dict(S=qx.shape[0], Hq=Hq, Hk=Hk, D=D, eps=float(eps),
-                gain_bf16=int(gains[0].dtype == torch.bfloat16), reserved=0, qx=qx.data_ptr(),
-                kx=kx.data_ptr(), qx_ss=qx.stride(0), kx_ss=kx.stride(0),
-                norm_q_w=gains[0].data_ptr(), norm_k_w=gains[1].data_ptr(),
-                rope_cos=cs.data_ptr(), rope_sin=sn.data_ptr())
+        if t.dtype is not torch.float32:
+            rope_cos, rope_sin = rope_cos.float(), rope_sin.float()
+    wq, wk, cs, sn = _aligned(norm_q_w), _aligned(norm_k_w), _aligned(rope_cos), _aligned(rope_sin)
+    common = (S, Hq, Hk, D, float(eps), int(bf16), 0, qx.data_ptr(), kx.data_ptr(), q_ss, k_ss,
+              wq.data_ptr(), wk.data_ptr(), cs.data_ptr(), sn.data_ptr())
+    return S, Hq, Hk, D, common, (qx, kx, wq, wk, cs, sn)
 
 
 def qk_head_prologue(qx: torch.Tensor, kx: torch.Tensor, *, norm_q_w: torch.Tensor,
@@ -763,23 +770,22 @@ def qk_head_prologue(qx: torch.Tensor, kx: torch.Tensor, *, norm_q_w: torch.Tens
     heads; the tables are [S, D/2].  Returns ``(q, k)`` bf16 [S, H, D] /
     [S, Hk, D] of token-major (``out_layout="shd"``) or head-major (``"hsd"``)
     storage.  No gradient: ``qk_head_prologue_train``."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (qx, kx, norm_q_w, norm_k_w)):
+    if torch.is_grad_enabled() and (qx.requires_grad or kx.requires_grad or
+                                    norm_q_w.requires_grad or norm_k_w.requires_grad):
         raise RuntimeError("qk_head_prologue gives no gradient: use qk_head_prologue_train")
-    qx, kx, gains, cs, sn, Hq, Hk, D = _head_args(qx, kx, norm_q_w, norm_k_w, rope_cos, rope_sin,
-                                                  num_heads, num_kv_heads)
-    S, dev = qx.shape[0], qx.device
+    S, Hq, Hk, D, common, keep = _head_args(qx, kx, norm_q_w, norm_k_w, rope_cos, rope_sin, num_heads,
+                                            num_kv_heads, eps)
     if out_layout == "shd":
-        mk = lambda H: torch.empty((S, H, D), dtype=torch.bfloat16, device=dev)  # noqa: E731
+        q, k = qx.new_empty((S, Hq, D)), qx.new_empty((S, Hk, D))
+        strides = (Hq * D, D, Hk * D, D)
     elif out_layout == "hsd":
-        mk = lambda H: torch.empty((H, S, D), dtype=torch.bfloat16, device=dev).transpose(0, 1)  # noqa: E731
+        q, k = (qx.new_empty((H, S, D)).transpose(0, 1) for H in (Hq, Hk))
+        strides = (D, S * D, D, S * D)
     else:
         raise ValueError(f"unknown layout {out_layout!r}")
-    q, k = mk(Hq), mk(Hk)
     if S:
-        args = _capi.HierHeadNormArgs(
-            q_out=q.data_ptr(), k_out=k.data_ptr(), q_ss=q.stride(0), q_sh=q.stride(1),
-            k_ss=k.stride(0), k_sh=k.stride(1), **_head_common(qx, kx, gains, cs, sn, Hq, Hk, D, eps))
-        _capi.call_on(dev, "hier_head_prologue", C.byref(args))
+        _capi.call_on(qx.device, "hier_head_prologue",
+                      _pack_head(*common, q.data_ptr(), k.data_ptr(), *strides))
     return q, k
 
 
@@ -792,33 +798,31 @@ def qk_head_prologue_backward(dq: torch.Tensor, dk: torch.Tensor, qx: torch.Tens
     outputs: ``(dqx, dkx, dnorm_q, dnorm_k)``, bf16 [S, H*D] / [S, Hk*D] and
     fp32 [D].  The gains' sums over tokens and heads are taken in a fixed
     order: equal inputs give equal bits."""
-    qx, kx, gains, cs, sn, Hq, Hk, D = _head_args(qx, kx, norm_q_w, norm_k_w, rope_cos, rope_sin,
-                                                  num_heads, num_kv_heads)
-    S, dev = qx.shape[0], qx.device
-    outs = []
+    S, Hq, Hk, D, common, keep = _head_args(qx, kx, norm_q_w, norm_k_w, rope_cos, rope_sin, num_heads,
+                                            num_kv_heads, eps)
+    gpu, grads = qx.get_device(), []
     for name, g, H in (("dq", dq, Hq), ("dk", dk, Hk)):
-        if g.shape != (S, H, D) or g.dtype != torch.bfloat16 or g.device != dev:
-            raise ValueError(f"{name} must be bf16 [{S}, {H}, {D}] on {dev}, got "
+        if g.shape != (S, H, D) or g.dtype is not torch.bfloat16 or g.get_device() != gpu:
+            raise ValueError(f"{name} must be bf16 [{S}, {H}, {D}] on {qx.device}, got "
                              f"{tuple(g.shape)} {g.dtype} on {g.device}")
-        if g.stride(2) != 1 or g.stride(0) % 8 or g.stride(1) % 8 or g.data_ptr() % 16:
+        ss, sh, unit = g.stride()
+        if unit != 1 or ss % 8 or sh % 8 or g.data_ptr() % 16:
             g = g.contiguous()
-        outs.append(g)
-    dq, dk = outs
-    dqx = torch.empty((S, Hq * D), dtype=torch.bfloat16, device=dev)
-    dkx = torch.empty((S, Hk * D), dtype=torch.bfloat16, device=dev)
+            ss, sh, _ = g.stride()
+        grads.append((g, ss, sh))
+    (dq, dq_ss, dq_sh), (dk, dk_ss, dk_sh) = grads
+    dqx, dkx = qx.new_empty((S, Hq * D)), qx.new_empty((S, Hk * D))
     if S == 0:
-        return (dqx, dkx) + tuple(torch.zeros(D, device=dev) for _ in range(2))
-    dw = torch.empty((2, D), dtype=torch.float32, device=dev)
-    args = _capi.HierHeadNormBwdArgs(
-        dq=dq.data_ptr(), dk=dk.data_ptr(), dq_ss=dq.stride(0), dq_sh=dq.stride(1),
-        dk_ss=dk.stride(0), dk_sh=dk.stride(1), dqx=dqx.data_ptr(), dkx=dkx.data_ptr(),
-        dnorm_q=dw[0].data_ptr(), dnorm_k=dw[1].data_ptr(),
-        **_head_common(qx, kx, gains, cs, sn, Hq, Hk, D, eps))
-    rows = int(_capi.lib().hier_head_prologue_bwd_rows(C.byref(args)))
-    part = torch.empty((max(rows, 1), D), dtype=torch.float32, device=dev)
-    args.partial = part.data_ptr()
-    _capi.call_on(dev, "hier_head_prologue_bwd", C.byref(args))
-    return dqx, dkx, dw[0], dw[1]
+        return dqx, dkx, *torch.zeros((2, D), device=qx.device).unbind(0)
+    # a row of sums for each workgroup: of eight tokens at least, about 2,048 in
+    # all (checked by the entry)
+    rows = min(2 * -(-S // 8), 2050)
+    part = qx.new_empty((rows, D), dtype=torch.float32)
+    dwq, dwk = qx.new_empty((2, D), dtype=torch.float32).unbind(0)
+    _capi.call_on(qx.device, "hier_head_prologue_bwd", _pack_head_bwd(
+        *common, dq.data_ptr(), dk.data_ptr(), dq_ss, dq_sh, dk_ss, dk_sh, dqx.data_ptr(),
+        dkx.data_ptr(), dwq.data_ptr(), dwk.data_ptr(), part.data_ptr(), rows))
+    return dqx, dkx, dwq, dwk
 
 
 class QKHeadPrologueFunction(torch.autograd.Function):
@@ -932,20 +936,15 @@ def hier_cached_attention_fp8(q: torch.Tensor, cache, tiles: TileList, *,
     part = torch.empty(splits * H * tiles.row_extent * (D + 2), dtype=torch.float32, device=dev) \
         if splits > 1 else None
     table = tiles.row_table
-    args = _capi.HierFwdFp8Args(
-        H=H, Hk=Hk, D=D, n_items=n_items,
-        scale=float(scale if scale is not None else 1.0 / math.sqrt(D)), splits=splits,
-        kv_rows=rows, q_rows=tiles.row_extent, q=q3.data_ptr(), k=cache.k.data_ptr(),
-        v=cache.v.data_ptr(), k_scale=cache.k_scale.data_ptr(), v_scale=cache.v_scale.data_ptr(),
-        o=o3.data_ptr(), lse=None if lse is None else lse.data_ptr(), q_ss=q_ss, q_sh=q_sh,
-        o_ss=o3.stride(0), o_sh=o3.stride(1), lse_stride_h=0 if lse is None else lse.stride(0),
-        kv_ss=cache.k.stride(0), kv_sh=cache.k.stride(1), scale_ss=cache.k_scale.stride(0),
-        scale_sh=cache.k_scale.stride(1), tile_items=items.data_ptr(),
-        tile_kv_idx=tiles.kv_idx.data_ptr(), tile_kv_mask=tiles.kv_mask.data_ptr(),
-        tile_blk_and=tiles.blk_and.data_ptr(),
-        row_table=None if table is None else table.data_ptr())
-    if part is not None:
-        args.part_o = part.data_ptr()
-        args.part_ml = part.data_ptr() + 4 * splits * H * tiles.row_extent * D
-    _capi.call_on(dev, "hier_attn_fwd_fp8", C.byref(args))
+    k, v, k_scale, v_scale, kv_ss, kv_sh, scale_ss, scale_sh = cache._pool
+    at = 0 if part is None else part.data_ptr()
+    args = _pack_fwd_fp8(
+        H, Hk, D, n_items, float(scale if scale is not None else 1.0 / math.sqrt(D)), splits, rows,
+        tiles.row_extent, q3.data_ptr(), k, v, k_scale, v_scale, o3.data_ptr(),
+        0 if lse is None else lse.data_ptr(), q_ss, q_sh, o3.stride(0), o3.stride(1),
+        0 if lse is None else lse.stride(0), kv_ss, kv_sh, scale_ss, scale_sh, items.data_ptr(),
+        tiles.kv_idx.data_ptr(), tiles.kv_mask.data_ptr(), tiles.blk_and.data_ptr(),
+        0 if table is None else table.data_ptr(), at,
+        at and at + 4 * splits * H * tiles.row_extent * D)
+    _capi.call_on(dev, "hier_attn_fwd_fp8", args)
     return out

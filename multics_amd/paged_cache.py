@@ -42,6 +42,7 @@ from . import _capi
 _stream = _capi.stream_of
 
 FP8_BLOCK = 16      # rows that share a scale (HIER_FP8_BLOCK)
+_pack_page = _capi.packer(_capi.HierPageFp8Args)
 
 
 class HierPagedKVCache:
@@ -230,17 +231,25 @@ class HierPagedKVCache:
         _capi.call("hier_kv_append", C.byref(args), _stream(self.device))
 
     def _append_fp8(self, k_blk, v_blk, blocks) -> None:
-        k_blk, v_blk = (t if t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and
-                        t.data_ptr() % 16 == 0 else t.contiguous() for t in (k_blk, v_blk))
-        args = _capi.HierPageFp8Args(
-            H=k_blk.shape[1], D=self.D, n_blocks=blocks.shape[0], n_rows=k_blk.shape[0],
-            pool_rows=self.k.shape[0], k_src=k_blk.data_ptr(), v_src=v_blk.data_ptr(),
-            k_src_ss=k_blk.stride(0), k_src_sh=k_blk.stride(1), v_src_ss=v_blk.stride(0),
-            v_src_sh=v_blk.stride(1), blocks=blocks.data_ptr(), k_pool=self.k.data_ptr(),
-            v_pool=self.v.data_ptr(), pool_ss=self.k.stride(0), pool_sh=self.k.stride(1),
-            k_scale=self.k_scale.data_ptr(), v_scale=self.v_scale.data_ptr(),
-            scale_ss=self.k_scale.stride(0), scale_sh=self.k_scale.stride(1))
-        _capi.call_on(self.k.device, "hier_kv_append_fp8", C.byref(args))
+        rows = []
+        for t in (k_blk, v_blk):
+            ss, sh, unit = t.stride()
+            if unit != 1 or ss % 8 or sh % 8 or t.data_ptr() % 16:
+                t = t.contiguous()
+                ss, sh, _ = t.stride()
+            rows.append((t, ss, sh))
+        (k, k_ss, k_sh), (v, v_ss, v_sh) = rows
+        k_pool, v_pool, k_scale, v_scale, pool_ss, pool_sh, scale_ss, scale_sh = self._pool
+        _capi.call_on(self.k.device, "hier_kv_append_fp8", _pack_page(
+            self.B * self.H, self.D, blocks.shape[0], k.shape[0], self.k.shape[0], k.data_ptr(),
+            v.data_ptr(), k_ss, k_sh, v_ss, v_sh, blocks.data_ptr(), k_pool, v_pool, pool_ss, pool_sh,
+            k_scale, v_scale, scale_ss, scale_sh))
+
+    @property
+    def _pool(self):
+        """Addresses and strides of the 8-bit pools and their scales."""
+        return (self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(),
+                self.v_scale.data_ptr(), *self.k.stride()[:2], *self.k_scale.stride())
 
     def dequantised(self):
         """The ``(k, v)`` that an 8-bit cache stands for, bf16 ``[rows,
