@@ -603,7 +603,7 @@ int hier_head_prologue(const HierHeadNormArgs* args, void* stream);
 /* Its gradient, recomputed from the inputs: dqx / dkx (contiguous rows) and   */
 /* the gains' gradients, summed over tokens and heads in a fixed order        */
 /* through partial, fp32 [partial_rows][D], partial_rows at least             */
-/* min(2 * ceil(S / 8), 2050).                                                */
+/* min(2 * ceil(S / 8), 1026).                                                */
 typedef struct HierHeadNormBwdArgs {
   int64_t S;
   int32_t Hq, Hk, D;

@@ -814,9 +814,9 @@ def qk_head_prologue_backward(dq: torch.Tensor, dk: torch.Tensor, qx: torch.Tens
     dqx, dkx = qx.new_empty((S, Hq * D)), qx.new_empty((S, Hk * D))
     if S == 0:
         return dqx, dkx, *torch.zeros((2, D), device=qx.device).unbind(0)
-    # a row of sums for each workgroup: of eight tokens at least, about 2,048 in
-    # all (checked by the entry)
-    rows = min(2 * -(-S // 8), 2050)
+    # a row of sums for each workgroup: of eight tokens at least, 1,024 in all
+    # (checked by the entry)
+    rows = min(2 * -(-S // 8), 1026)
     part = qx.new_empty((rows, D), dtype=torch.float32)
     dwq, dwk = qx.new_empty((2, D), dtype=torch.float32).unbind(0)
     _capi.call_on(qx.device, "hier_head_prologue_bwd", _pack_head_bwd(
@@ -863,11 +863,15 @@ def qk_head_prologue_train(qx, kx, *, norm_q_w, norm_k_w, rope_cos, rope_sin, nu
 
 def _fp8_splits(workgroups: int, max_tiles: int) -> int:
     """Parts that every item's key list is cut into: one where the items fill
-    the 512 workgroups that run at once (two a CU), else enough to fill them,
-    of two 64-key tiles at least, at most 32."""
+    the 512 workgroups that run at once (two a CU), else enough for 768 of
+    them, of eight 64-key tiles at least (a part costs a second launch, and
+    its rows of O written and read in fp32), at most 32.  324 items of 163
+    tiles: 161 us in one part, 154 in two, 137 in three, 141 in four; 96 items
+    of 228 tiles: 251 in one, 85 in six, 87 in eight, 102 in 24; 1,560 items:
+    568 in one, 618 in two."""
     if workgroups >= 512:
         return 1
-    return max(1, min(32, -(-512 // workgroups), max_tiles // 2))
+    return max(1, min(32, -(-768 // workgroups), max_tiles // 8))
 
 
 def hier_cached_attention_fp8(q: torch.Tensor, cache, tiles: TileList, *,
