@@ -213,20 +213,23 @@ __device__ __forceinline__ f32x16 qk_block(const Rows<D>& R, const char* kslot, 
   return acc;
 }
 
-// Set the scores of block kb that the lane's query frame may not see to -inf.
+// Set the scores that the lane's query frame may not see to -inf: w, the masks
+// of keys 8 g4 + 4 (lane / 32) .. + 4.
+__device__ __forceinline__ void mask_four(f32x16& s, int g4, const u32x4& w, int qframe) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t sel = (uint32_t)__builtin_amdgcn_sbfe((int)w[e], qframe, 1);
+    const uint32_t x = __float_as_uint(s[4 * g4 + e]);
+    s[4 * g4 + e] = __uint_as_float((x & sel) | (0xff800000u & ~sel));
+  }
+}
+// The same of block kb of a tile.
 __device__ __forceinline__ void mask_block(f32x16& s, const char* mslot, int kb, int qframe,
                                            int lane) {
   const uint32_t* mk = reinterpret_cast<const uint32_t*>(mslot);
 #pragma unroll
-  for (int g4 = 0; g4 < 4; ++g4) {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(&mk[kb * 32 + 8 * g4 + 4 * (lane >> 5)]);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t sel = (uint32_t)__builtin_amdgcn_sbfe((int)w[e], qframe, 1);
-      const uint32_t x = __float_as_uint(s[4 * g4 + e]);
-      s[4 * g4 + e] = __uint_as_float((x & sel) | (0xff800000u & ~sel));
-    }
-  }
+  for (int g4 = 0; g4 < 4; ++g4)
+    mask_four(s, g4, *reinterpret_cast<const u32x4*>(&mk[kb * 32 + 8 * g4 + 4 * (lane >> 5)]), qframe);
 }
 
 // P of one 32-key block: exp2(s * c2 + nb) rounded to bf16, as the two P^T
@@ -598,10 +601,12 @@ struct Block {               // what a wave loads of a 32-key block
   u32x4 k[2 * Geo8<D>::NS];
   u32x4 v[NV];
   uint32_t sk, sv[NV];
+  u32x4 m[4];                // masks of the lane's 16 keys, where the block needs them
 };
 template <int D>
 struct BlockRow {
   int k, v[Block<D>::NV];    // pool rows: of the lane's key, of its chunks of V
+  uint32_t flags;            // of the block's tile
 };
 
 template <int D>
@@ -611,11 +616,19 @@ __device__ __forceinline__ BlockRow<D> block_rows(const Ctx<D>& c, int b) {
   r.k = p[c.lane & 31];
 #pragma unroll
   for (int e = 0; e < Block<D>::NV; ++e) r.v[e] = p[Geo8<D>::RPC * e + c.lane / Geo8<D>::CPR];
+  r.flags = c.blk[b >> 1];
   return r;
 }
 
 template <int D>
-__device__ __forceinline__ void block_load(const Ctx<D>& c, const BlockRow<D>& r, Block<D>& x) {
+__device__ __forceinline__ bool block_masked(const BlockRow<D>& r, uint32_t bits) {
+  return ((uint32_t)__builtin_amdgcn_readfirstlane(r.flags) & bits) != bits;
+}
+
+// Loads of block b (rows r), with its masks if it is ``masked``.
+template <int D>
+__device__ __forceinline__ void block_load(const Ctx<D>& c, int b, const BlockRow<D>& r, bool masked,
+                                           Block<D>& x) {
   const char* k = c.gk + (__umul24((uint32_t)r.k, c.ss_b) + 32u * (uint32_t)(c.lane >> 5));
 #pragma unroll
   for (int i = 0; i < 2 * Geo8<D>::NS; ++i)
@@ -627,12 +640,12 @@ __device__ __forceinline__ void block_load(const Ctx<D>& c, const BlockRow<D>& r
 #pragma unroll
   for (int e = 0; e < Block<D>::NV; ++e)
     x.sv[e] = c.sv[(uint32_t)__umul24((uint32_t)r.v[e] / HIER_FP8_BLOCK, c.scale_b)];
-}
-
-// Set the scores that the lane's query frame may not see to -inf, masks from
-// the list.
-__device__ __forceinline__ void mask_from(f32x16& s, const uint32_t* mk, int qframe, int lane) {
-  mask_block(s, reinterpret_cast<const char*>(mk), 0, qframe, lane);
+  if (masked) {
+    const uint32_t* m = c.kv_mask + b * 32;
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4)
+      x.m[g4] = *reinterpret_cast<const u32x4*>(m + (8 * g4 + 4 * (uint32_t)(c.lane >> 5)));
+  }
 }
 
 template <int D>
@@ -655,38 +668,50 @@ __device__ __forceinline__ void few_rows(const HierFwdFp8Args& a, const int32_t*
   const int mine = c.nt > c.wave ? 2 * ((c.nt - c.wave + kWaves - 1) / kWaves) : 0;
   const auto at = [&](int b) { return 2 * (c.wave + kWaves * (b >> 1)) + (b & 1); };
   if (mine > 0) {
-    Block<D> x;
-    block_load<D>(c, block_rows<D>(c, at(0)), x);
-    BlockRow<D> next = block_rows<D>(c, at(1));
-    for (int b = 0; b < mine; ++b) {
-      // S^T
-      f32x16 s = {};
+    constexpr int N = 1;       // blocks whose loads are in flight
+    Block<D> x[N];
+    bool masked[N];
 #pragma unroll
-      for (int i = 0; i < Geo8<D>::NS; ++i) {
-        const u32x4 u = x.k[2 * i], w = x.k[2 * i + 1];
-        const i32x8 k = {(int)u[0], (int)u[1], (int)u[2], (int)u[3],
-                         (int)w[0], (int)w[1], (int)w[2], (int)w[3]};
-        s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, R.hi[i], s, 0, 0, 0, (int)x.sk, 0, R.e_hi);
-        s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, R.lo[i], s, 0, 0, 0, (int)x.sk, 0, R.e_lo);
-      }
-      // V to LDS in bf16
+    for (int i = 0; i < N; ++i) {
+      const int u = at(min(i, mine - 1));
+      const BlockRow<D> r = block_rows<D>(c, u);
+      masked[i] = block_masked<D>(r, R.bits);
+      block_load<D>(c, u, r, masked[i], x[i]);
+    }
+    BlockRow<D> next = block_rows<D>(c, at(min(N, mine - 1)));
+    for (int b0 = 0; b0 < mine; b0 += N) {
 #pragma unroll
-      for (int e = 0; e < B::NV; ++e) {
-        const float sv = pow2_of(x.sv[e]);
+      for (int i = 0; i < N; ++i) {
+        const int b = b0 + i;
+        // S^T
+        f32x16 s = {};
 #pragma unroll
-        for (int p = 0; p < 2; ++p) *reinterpret_cast<u32x4*>(vslot + vst[2 * e + p]) = wide_codes(x.v[e], p, sv);
+        for (int j = 0; j < Geo8<D>::NS; ++j) {
+          const u32x4 u = x[i].k[2 * j], w = x[i].k[2 * j + 1];
+          const i32x8 k = {(int)u[0], (int)u[1], (int)u[2], (int)u[3],
+                           (int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+          s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, R.hi[j], s, 0, 0, 0, (int)x[i].sk, 0, R.e_hi);
+          s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, R.lo[j], s, 0, 0, 0, (int)x[i].sk, 0, R.e_lo);
+        }
+        // V to LDS in bf16
+#pragma unroll
+        for (int e = 0; e < B::NV; ++e) {
+          const float sv = pow2_of(x[i].sv[e]);
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+            *reinterpret_cast<u32x4*>(vslot + vst[2 * e + p]) = wide_codes(x[i].v[e], p, sv);
+        }
+        if (masked[i])
+#pragma unroll
+          for (int g4 = 0; g4 < 4; ++g4) mask_four(s, g4, x[i].m[g4], R.qframe);
+        // block b + N's loads, and the rows of the one after it (past the last: the last)
+        masked[i] = block_masked<D>(next, R.bits);
+        block_load<D>(c, at(min(b + N, mine - 1)), next, masked[i], x[i]);
+        next = block_rows<D>(c, at(min(b + N + 1, mine - 1)));
+        bf16x8 p[2];
+        if (softmax_block<D>(R, s, p, c.c2)) rescale<D>(R, R.alpha);
+        pv_block<D>(R, p, vslot, c.ra, 0);
       }
-      const int blk = at(b);
-      const bool masked = (__builtin_amdgcn_readfirstlane(c.blk[blk >> 1]) & R.bits) != R.bits;
-      // the next block's loads (past the last: the last again)
-      if (b + 1 < mine) {
-        block_load<D>(c, next, x);
-        next = block_rows<D>(c, at(min(b + 2, mine - 1)));
-      }
-      if (masked) mask_from(s, c.kv_mask + blk * 32, R.qframe, c.lane);
-      bf16x8 p[2];
-      if (softmax_block<D>(R, s, p, c.c2)) rescale<D>(R, R.alpha);
-      pv_block<D>(R, p, vslot, c.ra, 0);
     }
   }
   // join: waves 2, 3 into 0, 1, then 1 into 0 (O^T as fp32 [element][lane] in

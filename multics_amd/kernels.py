@@ -930,9 +930,8 @@ def hier_cached_attention_fp8(q: torch.Tensor, cache, tiles: TileList, *,
                             lse.shape[1] < tiles.row_extent or lse.stride(1) != 1 or
                             lse.device != dev):
         raise ValueError("lse must be fp32 [H, >=rows] with unit row stride")
-    run = M.launch_list(tiles)
-    items, n_items = (run.items, tiles.n_items) if run.fwd_items is None else \
-        (run.fwd_items, tiles.fwd_n_items)
+    run = M.costly_first(tiles)
+    items, n_items = run.items, run.n_items
     if n_items == 0:
         return out
     max_tiles = (tiles.max_keys or tiles.kv_idx.numel()) // M.TILE_KEYS

@@ -1377,6 +1377,35 @@ def launch_list(tiles: TileList) -> TileList:
     return _set_launch(tiles, items, fwd)
 
 
+def costly_first(tiles: TileList) -> TileList:
+    """``launch_list(tiles)`` with the forward's own items (``items`` is the
+    list that a forward runs) in the order of what they cost, the costliest
+    first: a launch of a few rounds of workgroups ends on its short items then.
+    The cost of an item is the length of the list it was built with (equal for
+    the items of a stream, which so stay together and share what they read),
+    two fifths of it for at most 32 rows.  Made on the current stream on first
+    use and kept on the launch list; not under graph capture, which then runs
+    the items in their own order (each item's result is the same anywhere)."""
+    run = launch_list(tiles)
+    hit = run.__dict__.get("_costly")
+    if hit is not None:
+        _use_derived(run, hit)
+        return hit
+    fwd = run.fwd_items is not None
+    items, n = (run.fwd_items, tiles.fwd_n_items) if fwd else (run.items, tiles.n_items)
+    if _ready.capturing(items.device):
+        return dataclasses.replace(run, items=items, n_items=n, fwd_items=None)
+    built = (tiles.fwd_items if fwd else tiles.items)[:n]
+    cost = built[:, 6] * torch.where(built[:, 4] <= 32, 2, 5)
+    order = torch.argsort(cost, descending=True, stable=True)
+    piece = dataclasses.replace(run, items=items[:n].index_select(0, order), n_items=n, fwd_items=None)
+    piece.__dict__["_is_launch"] = True
+    _derived_on(run, piece)
+    if _keeps(run):
+        run.__dict__["_costly"] = piece
+    return piece
+
+
 def _launch_pair(a: TileList, b: TileList) -> None:
     """``launch_list`` of two new device lists without folded rows, in one
     launch."""
