@@ -305,3 +305,21 @@ def call_on(device: torch.device, name: str, *args) -> None:
     else:
         with torch.cuda.device(device):
             call(name, *args, stream_of(device))
+
+
+def aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous from a 16-byte address, copied if it is not."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def head_strides(t: torch.Tensor) -> tuple:
+    """``t`` [S, H, D] readable in 16-byte rows (copied if it is not), and its
+    strides over tokens and heads (0 where there is one only)."""
+    for _ in range(2):
+        ss, sh, unit = t.stride()
+        ss, sh = ss if t.shape[0] > 1 else 0, sh if t.shape[1] > 1 else 0
+        if unit == 1 and ss % 8 == 0 and sh % 8 == 0 and t.data_ptr() % 16 == 0:
+            break
+        t = aligned(t)
+    return t, ss, sh

@@ -916,9 +916,10 @@ extern "C" int hier_attn_fwd_fp8(const HierFwdFp8Args* args, void* stream) {
   // rows of codes are addressed with 32-bit byte offsets from their head's
   // first (one 24 x 24-bit multiply)
   HIER_REQUIRE(a.kv_ss >= 0 && a.scale_ss >= 0 && a.kv_rows <= (1ll << 24) && a.kv_ss < (1ll << 24) &&
-                   a.scale_ss < (1ll << 24) && a.kv_rows * a.kv_ss <= (1ll << 32),
+                   a.scale_ss < (1ll << 24) && a.kv_rows * a.kv_ss <= (1ll << 32) &&
+                   a.kv_rows / HIER_FP8_BLOCK * a.scale_ss <= (1ll << 32),
                HIER_EUNSUPPORTED,
-               "a head's codes must span at most 4 GiB, of 2^24 rows and strides below 2^24 bytes");
+               "a head's codes and scales must span at most 4 GiB, of 2^24 rows and strides below 2^24");
   const int64_t total = (int64_t)a.n_items * a.splits * a.H;
   HIER_REQUIRE((int64_t)a.n_items * a.splits < (1ll << 31) && total < (1ll << 24), HIER_EUNSUPPORTED,
                "too many work items");

@@ -690,6 +690,7 @@ def qk_prologue_train(qx, kx, *, norm_q_w, norm_k_w, rope_cos, rope_sin, num_hea
 # per-head norms with rotation
 # --------------------------------------------------------------------------
 
+_aligned, _head_strides = _capi.aligned, _capi.head_strides
 _pack_head = _capi.packer(_capi.HierHeadNormArgs)
 _pack_head_bwd = _capi.packer(_capi.HierHeadNormBwdArgs)
 _pack_fwd_fp8 = _capi.packer(_capi.HierFwdFp8Args)
@@ -703,15 +704,12 @@ def _head_rows(name: str, t: torch.Tensor, gpu: int) -> tuple:
     if t.get_device() != gpu:
         raise ValueError(f"{name} is on {t.device}, qx on another device")
     ss, unit = t.stride()
+    if t.shape[0] < 2:          # (the stride of one row says nothing)
+        ss = t.shape[1]
     if unit != 1 or ss % 8 or t.data_ptr() % 16:
-        t = t.contiguous()
-        ss = t.stride(0)
+        t = _aligned(t)
+        ss = t.shape[1]
     return t, ss
-
-
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _head_args(qx, kx, norm_q_w, norm_k_w, rope_cos, rope_sin, num_heads, num_kv_heads, eps):
@@ -805,11 +803,7 @@ def qk_head_prologue_backward(dq: torch.Tensor, dk: torch.Tensor, qx: torch.Tens
         if g.shape != (S, H, D) or g.dtype is not torch.bfloat16 or g.get_device() != gpu:
             raise ValueError(f"{name} must be bf16 [{S}, {H}, {D}] on {qx.device}, got "
                              f"{tuple(g.shape)} {g.dtype} on {g.device}")
-        ss, sh, unit = g.stride()
-        if unit != 1 or ss % 8 or sh % 8 or g.data_ptr() % 16:
-            g = g.contiguous()
-            ss, sh, _ = g.stride()
-        grads.append((g, ss, sh))
+        grads.append(_head_strides(g))
     (dq, dq_ss, dq_sh), (dk, dk_ss, dk_sh) = grads
     dqx, dkx = qx.new_empty((S, Hq * D)), qx.new_empty((S, Hk * D))
     if S == 0:
@@ -903,11 +897,12 @@ def hier_cached_attention_fp8(q: torch.Tensor, cache, tiles: TileList, *,
     if cache.k.device != dev or tiles.items.device != dev:
         raise ValueError(f"q is on {dev}, the cache on {cache.k.device}, the tile list on "
                          f"{tiles.items.device}")
-    q3, q_ss, q_sh = _rows_view(q)
-    S, H, D = q3.shape
-    if q_ss % 8 or q_sh % 8 or q3.data_ptr() % 16:
-        q3 = q3.contiguous()
-        q_ss, q_sh = q3.stride(0), q3.stride(1)
+    if q.dim() == 4 and q.shape[0] == 1:
+        q = q[0]
+    if q.dim() != 3:
+        raise ValueError(f"q must be [S, H, D] or [1, S, H, D], got {tuple(q.shape)}")
+    q, q_ss, q_sh = _head_strides(q)
+    S, H, D = q.shape
     rows, Hk = cache.k.shape[:2]
     if D != cache.D or H % Hk:
         raise ValueError(f"q has {H} heads of {D}, the cache {Hk} of {cache.D}: the heads must be "
@@ -920,12 +915,18 @@ def hier_cached_attention_fp8(q: torch.Tensor, cache, tiles: TileList, *,
         raise ValueError(f"q holds {S} rows, the tile list addresses {tiles.row_extent}")
     if out is None:
         out = _attn_out(tiles, S, H, D, dev)
-    elif out.dtype != torch.bfloat16 or out.device != dev or out.shape not in (q.shape, q3.shape):
-        raise ValueError(f"out must be bf16 {tuple(q3.shape)} on {dev}, got {tuple(out.shape)} "
-                         f"{out.dtype} on {out.device}")
-    o3 = out[0] if out.dim() == 4 else out
-    if o3.stride(2) != 1 or o3.stride(0) % 8 or o3.stride(1) % 8 or o3.data_ptr() % 16:
-        raise ValueError("out must have a unit-stride head dimension and 16-byte rows")
+        o = out
+    else:
+        o = out[0] if out.dim() == 4 and out.shape[0] == 1 else out
+        if o.shape != q.shape or o.dtype != torch.bfloat16 or o.device != dev:
+            raise ValueError(f"out must be bf16 {tuple(q.shape)} on {dev}, got {tuple(out.shape)} "
+                             f"{out.dtype} on {out.device}")
+    own, o_ss, o_sh = _head_strides(o)
+    if own is not o or o_ss == 0 and S > 1 or o_sh == 0 and H > 1:
+        raise ValueError("out must have rows of its own, a unit-stride head dimension and 16-byte rows")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not 0.0 < scale <= 1e30:
+        raise ValueError(f"the softmax scale must be positive, got {scale}")
     if lse is not None and (lse.dtype != torch.float32 or lse.dim() != 2 or lse.shape[0] != H or
                             lse.shape[1] < tiles.row_extent or lse.stride(1) != 1 or
                             lse.device != dev):
@@ -942,9 +943,8 @@ def hier_cached_attention_fp8(q: torch.Tensor, cache, tiles: TileList, *,
     k, v, k_scale, v_scale, kv_ss, kv_sh, scale_ss, scale_sh = cache._pool
     at = 0 if part is None else part.data_ptr()
     args = _pack_fwd_fp8(
-        H, Hk, D, n_items, float(scale if scale is not None else 1.0 / math.sqrt(D)), splits, rows,
-        tiles.row_extent, q3.data_ptr(), k, v, k_scale, v_scale, o3.data_ptr(),
-        0 if lse is None else lse.data_ptr(), q_ss, q_sh, o3.stride(0), o3.stride(1),
+        H, Hk, D, n_items, scale, splits, rows, tiles.row_extent, q.data_ptr(), k, v, k_scale,
+        v_scale, o.data_ptr(), 0 if lse is None else lse.data_ptr(), q_ss, q_sh, o_ss, o_sh,
         0 if lse is None else lse.stride(0), kv_ss, kv_sh, scale_ss, scale_sh, items.data_ptr(),
         tiles.kv_idx.data_ptr(), tiles.kv_mask.data_ptr(), tiles.blk_and.data_ptr(),
         0 if table is None else table.data_ptr(), at,

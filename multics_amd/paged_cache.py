@@ -231,14 +231,8 @@ class HierPagedKVCache:
         _capi.call("hier_kv_append", C.byref(args), _stream(self.device))
 
     def _append_fp8(self, k_blk, v_blk, blocks) -> None:
-        rows = []
-        for t in (k_blk, v_blk):
-            ss, sh, unit = t.stride()
-            if unit != 1 or ss % 8 or sh % 8 or t.data_ptr() % 16:
-                t = t.contiguous()
-                ss, sh, _ = t.stride()
-            rows.append((t, ss, sh))
-        (k, k_ss, k_sh), (v, v_ss, v_sh) = rows
+        k, k_ss, k_sh = _capi.head_strides(k_blk)
+        v, v_ss, v_sh = _capi.head_strides(v_blk)
         k_pool, v_pool, k_scale, v_scale, pool_ss, pool_sh, scale_ss, scale_sh = self._pool
         _capi.call_on(self.k.device, "hier_kv_append_fp8", _pack_page(
             self.B * self.H, self.D, blocks.shape[0], k.shape[0], self.k.shape[0], k.data_ptr(),

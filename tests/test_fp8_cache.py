@@ -140,3 +140,70 @@ def test_struct_layouts_match_c(tmp_path, monkeypatch):
         n: getattr(_capi, n) for n in ("HierHeadNormArgs", "HierHeadNormBwdArgs", "HierPageFp8Args",
                                        "HierFwdFp8Args")})
     test_capi.test_ctypes_struct_layout_matches_c(tmp_path)
+
+
+def test_c_entries_refuse_before_a_launch():
+    """Bad sizes, pointers and strides of the C calls: an error each, and no
+    launch (made-up addresses, never read)."""
+    from multics_amd import _capi
+    lib, at = _capi.lib(), 0x7f0000000000
+    EINVAL, EUNSUP = _capi.HIER_EINVAL, _capi.HIER_EUNSUPPORTED
+    import ctypes as C
+
+    def fill(cls, **kw):
+        a = cls()
+        for i, (name, t) in enumerate(cls._fields_):
+            setattr(a, name, at + 4096 * i if t is _capi.vp else 0)
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return a
+
+    good = {
+        "hier_head_prologue": (_capi.HierHeadNormArgs, dict(S=4, Hq=2, Hk=1, D=64, eps=1e-6)),
+        "hier_head_prologue_bwd": (_capi.HierHeadNormBwdArgs,
+                                   dict(S=4, Hq=2, Hk=1, D=64, eps=1e-6, partial_rows=2)),
+        "hier_kv_append_fp8": (_capi.HierPageFp8Args, dict(H=2, D=64, n_blocks=1, n_rows=4,
+                                                           pool_rows=64)),
+        "hier_attn_fwd_fp8": (_capi.HierFwdFp8Args, dict(H=4, Hk=2, D=128, n_items=3, scale=1.0,
+                                                         splits=2, kv_rows=64, q_rows=8)),
+    }
+    bad = {
+        "hier_head_prologue": [(dict(D=96), EUNSUP), (dict(Hq=0), EINVAL), (dict(S=-1), EINVAL),
+                               (dict(qx=0), EINVAL), (dict(kx=at + 8), EINVAL),
+                               (dict(qx_ss=7), EINVAL), (dict(S=1 << 33), EUNSUP)],
+        "hier_head_prologue_bwd": [(dict(D=32), EUNSUP), (dict(S=0), EINVAL), (dict(dq=0), EINVAL),
+                                   (dict(dk_sh=4), EINVAL), (dict(partial_rows=1), EINVAL),
+                                   (dict(S=100), EINVAL)],
+        "hier_kv_append_fp8": [(dict(D=80), EUNSUP), (dict(pool_rows=40), EINVAL),
+                               (dict(blocks=0), EINVAL), (dict(k_pool=at + 1), EINVAL),
+                               (dict(v_src_ss=3), EINVAL), (dict(pool_ss=8), EINVAL),
+                               (dict(n_blocks=1 << 30), EUNSUP)],
+        "hier_attn_fwd_fp8": [(dict(D=256), EUNSUP), (dict(H=3), EINVAL), (dict(splits=0), EINVAL),
+                              (dict(splits=33), EINVAL), (dict(part_o=0), EINVAL),
+                              (dict(scale=0.0), EINVAL), (dict(v_scale=0), EINVAL),
+                              (dict(kv_ss=8), EINVAL), (dict(kv_rows=1 << 25), EUNSUP),
+                              (dict(kv_rows=1 << 24, kv_ss=1024), EUNSUP),
+                              (dict(kv_rows=1 << 24, scale_ss=8192), EUNSUP),
+                              (dict(n_items=1 << 24), EUNSUP)],
+    }
+    for name, cases in bad.items():
+        cls, base = good[name]
+        assert getattr(lib, name)(None, None) == EINVAL
+        for change, want in cases:
+            assert getattr(lib, name)(C.byref(fill(cls, **{**base, **change})), None) == want, \
+                (name, change, lib.hier_last_error())
+            assert lib.hier_last_error()
+    # nothing to do is no error, whatever the rest holds
+    assert lib.hier_head_prologue(C.byref(fill(_capi.HierHeadNormArgs, S=0, Hq=1, Hk=1, D=64)), None) == 0
+    assert lib.hier_kv_append_fp8(C.byref(fill(_capi.HierPageFp8Args, H=1, D=64)), None) == 0
+    assert lib.hier_attn_fwd_fp8(C.byref(fill(_capi.HierFwdFp8Args, H=1, Hk=1, D=64, splits=1)), None) == 0
+
+
+def test_packed_arguments_are_the_structures():
+    from multics_amd import _capi
+    import ctypes as C
+    for cls in (_capi.HierHeadNormArgs, _capi.HierHeadNormBwdArgs, _capi.HierPageFp8Args,
+                _capi.HierFwdFp8Args):
+        vals = [0.5 if t is _capi.f32 else 3 + 7 * i for i, (_, t) in enumerate(cls._fields_)]
+        a = cls.from_buffer_copy(_capi.packer(cls)(*vals))
+        assert [getattr(a, n) for n, _ in cls._fields_] == vals

@@ -314,6 +314,24 @@ def test_rows_of_no_item_and_views():
     assert torch.equal(four[0], out)
 
 
+def test_one_token_of_one_head_with_strides_of_no_meaning():
+    """A dimension of one element may have any stride."""
+    need_gpu()
+    case = CASES[3]
+    c, q, tiles = _rollout(case)
+    S, H, D = q.shape
+    assert H == 1
+    want = hier_cached_attention_fp8(q, c, tiles)
+    odd = q.as_strided((S, 1, D), (D, 1, 1))
+    got = hier_cached_attention_fp8(odd, c, tiles, out=torch.zeros_like(q).as_strided((S, 1, D), (D, 3, 1)))
+    assert torch.equal(got, want)
+    one, two = _cache(1, 1, 1, 1, 1, 1, 64, 4, 1), _cache(1, 1, 1, 1, 1, 1, 64, 4, 1)
+    k = torch.randn(3, 1, 64, device="cuda").to(torch.bfloat16)
+    one.append(k, k, 0, 1, [[True]])
+    two.append(k.as_strided((3, 1, 64), (64, 5, 1)), k, 0, 1, [[True]])
+    assert torch.equal(one.k.view(torch.uint8), two.k.view(torch.uint8))
+
+
 def test_refusals():
     need_gpu()
     c, q, tiles = _rollout(CASES[0])
@@ -327,6 +345,7 @@ def test_refusals():
         (ValueError, (q, c, tiles), {"lse": torch.empty(H, S - 1, device="cuda")}),
         (ValueError, (q, c, tiles), {"lse": torch.empty(H, S)}),
         (ValueError, (q, c, tiles), {"scale": 0.0}), (ValueError, (q, c, tiles), {"scale": -1.0}),
+        (ValueError, (q, c, tiles), {"scale": float("nan")}), (ValueError, (q[0], c, tiles), {}),
         (NotImplementedError, (q.half(), c, tiles), {}),
         (ValueError, (q, _cache(2, 1, 33, 2, 1, 3, 128, 2, 2), tiles), {}),
     ]:

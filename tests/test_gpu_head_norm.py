@@ -215,6 +215,16 @@ def test_captured_on_a_side_stream():
         assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_one_row_with_a_stride_of_no_meaning():
+    need_gpu()
+    qx, kx, kw, dq, dk = _inputs(1, 3, 1, 64, False, torch.float32)
+    want = qk_head_prologue(qx, kx, **kw) + qk_head_prologue_backward(dq, dk, qx, kx, **kw)
+    odd, one = qx.as_strided((1, 192), (1, 1)), kx.as_strided((1, 64), (7, 1))
+    got = qk_head_prologue(odd, one, **kw) + qk_head_prologue_backward(
+        dq.as_strided((1, 3, 64), (3, 64, 1)), dk.as_strided((1, 1, 64), (1, 5, 1)), odd, one, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_refusals_and_empty():
     need_gpu()
     qx, kx, kw, dq, dk = _inputs(8, 4, 2, 64, False, torch.float32)
