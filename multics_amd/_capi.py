@@ -295,16 +295,25 @@ def call(name: str, *args) -> None:
     check(getattr(lib(), name)(*args), name)
 
 
+_functions = {}
+
+
 def call_on(device: torch.device, name: str, *args) -> None:
     """``call`` with the current stream of ``device`` as the last argument,
     launched with that device current (a stream belongs to its device)."""
     if device.type != "cuda":
         raise ValueError(f"expected a GPU, got device {device}")
-    if device.index is None or device.index == torch.cuda.current_device():
-        call(name, *args, stream_of(device))
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(lib(), name)
+    index, now = device.index, torch.cuda.current_device()
+    if index is None or index == now:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(now))
     else:
         with torch.cuda.device(device):
-            call(name, *args, stream_of(device))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, name)
 
 
 def aligned(t: torch.Tensor) -> torch.Tensor:
