@@ -645,7 +645,8 @@ enum { HIER_FP8_BLOCK = 16 };
 /* Append: source rows [src, src + count) of block-table row (src, dst, count) */
 /* go to pool rows [dst, dst + count), 1 <= count <= 16, dst a multiple of 16, */
 /* and set that block's scales.  Rows of the pool behind count are left as     */
-/* they are.  A table row outside these bounds or outside the pool is skipped.  */
+/* they are.  A table row outside these bounds or outside the pool is skipped;  */
+/* no two rows of a table name the same dst.                                   */
 typedef struct HierPageFp8Args {
   int32_t H, D;                    /* heads, head dim (64 or 128)              */
   int32_t n_blocks;                /* rows of the block table                  */

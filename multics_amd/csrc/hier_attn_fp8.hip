@@ -23,6 +23,17 @@
 // rounded to bf16; the row sum adds the rounded weights, so a weight's
 // rounding (at most 2^-8 of it) reaches the result only as the spread of such
 // roundings over the keys.  m, l and O are fp32.
+//
+// A workgroup is four waves of 32 rows, two workgroups a CU: with 128 rows a
+// tile's K and V are staged (V converted) once for four waves' products, and
+// 32 rows a wave leave room for S, P, O and the query's codes without spills
+// (three waves a SIMD spill: twice the time).  Full items are bound by the
+// matrix units and the softmax beside them at the card's power limit: 6,678
+// rows against their windows (24 heads of 128, 507 GFLOP) 530 us, 956 TFLOP/s
+// of what rows see, where the bf16 kernel takes 631 over the same lists; the
+// same instructions on queries of zeros, which draw less power, take 447.
+// Few items are cut into parts (the caller's ``splits``; parts and their join
+// below), items of at most 32 rows shared by the four waves (few_rows).
 #include "hier_common.h"
 #include "hier_launch.h"
 #include "hier_tile.h"
@@ -250,10 +261,10 @@ __device__ __forceinline__ float p_block(const f32x16& s, bf16x8* p, float c2, f
   return ps0 + ps1;
 }
 
-// x = y where x stands: the rare path writes into the registers of the common
-// one, which so needs no copies where the two meet.  (The s_nop are the wait
-// states behind an exp and in front of an MFMA, which the compiler does not add
-// around assembly.)
+// x = y in x's own register: the rare path writes into the registers of the
+// common one, so that no copies are needed where the two meet.  (s_nop 1: the
+// wait states that an exp's result and an MFMA's operand need, which the
+// compiler does not add around assembly.)
 __device__ __forceinline__ void put(float& x, float y) {
   asm volatile("s_nop 1\n\tv_mov_b32 %0, %2\n\ts_nop 1" : "=v"(x) : "0"(x), "v"(y));
 }
@@ -591,9 +602,12 @@ __device__ __forceinline__ void last_tile(Ctx<D>& c, Rows<D>& R, const f32x16& s
 // with a softmax state of its own, and nothing to wait for in the others: K
 // goes from memory straight into the MFMA operand (a lane holds 32 codes of
 // one key twice), V through 32 rows of LDS that are the wave's own.  The next
-// block's loads are in flight while one is multiplied.  The four states are
-// joined through LDS.  Query heads that share a key head are packed into the
-// sub-block when they fit, so that its K and V are read once.
+// block's loads are in flight while one is multiplied (two blocks ahead: the
+// same time).  The four states are joined through LDS.  Query heads that share
+// a key head are packed into the sub-block when they fit, so that its K and V
+// are read once.  Bound by the latency of a wave's loads: one token of 32 heads
+// of 128 over 8 key heads, 4,096 cached frames, 20.6 us with the join of its
+// eight parts (99 as an item whose waves share each tile).
 
 template <int D>
 struct Block {               // what a wave loads of a 32-key block
@@ -668,50 +682,40 @@ __device__ __forceinline__ void few_rows(const HierFwdFp8Args& a, const int32_t*
   const int mine = c.nt > c.wave ? 2 * ((c.nt - c.wave + kWaves - 1) / kWaves) : 0;
   const auto at = [&](int b) { return 2 * (c.wave + kWaves * (b >> 1)) + (b & 1); };
   if (mine > 0) {
-    constexpr int N = 1;       // blocks whose loads are in flight
-    Block<D> x[N];
-    bool masked[N];
+    B x;
+    const BlockRow<D> first = block_rows<D>(c, at(0));
+    bool masked = block_masked<D>(first, R.bits);
+    block_load<D>(c, at(0), first, masked, x);
+    BlockRow<D> next = block_rows<D>(c, at(min(1, mine - 1)));
+    for (int b = 0; b < mine; ++b) {
+      // S^T
+      f32x16 s = {};
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int u = at(min(i, mine - 1));
-      const BlockRow<D> r = block_rows<D>(c, u);
-      masked[i] = block_masked<D>(r, R.bits);
-      block_load<D>(c, u, r, masked[i], x[i]);
-    }
-    BlockRow<D> next = block_rows<D>(c, at(min(N, mine - 1)));
-    for (int b0 = 0; b0 < mine; b0 += N) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int b = b0 + i;
-        // S^T
-        f32x16 s = {};
-#pragma unroll
-        for (int j = 0; j < Geo8<D>::NS; ++j) {
-          const u32x4 u = x[i].k[2 * j], w = x[i].k[2 * j + 1];
-          const i32x8 k = {(int)u[0], (int)u[1], (int)u[2], (int)u[3],
-                           (int)w[0], (int)w[1], (int)w[2], (int)w[3]};
-          s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, R.hi[j], s, 0, 0, 0, (int)x[i].sk, 0, R.e_hi);
-          s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, R.lo[j], s, 0, 0, 0, (int)x[i].sk, 0, R.e_lo);
-        }
-        // V to LDS in bf16
-#pragma unroll
-        for (int e = 0; e < B::NV; ++e) {
-          const float sv = pow2_of(x[i].sv[e]);
-#pragma unroll
-          for (int p = 0; p < 2; ++p)
-            *reinterpret_cast<u32x4*>(vslot + vst[2 * e + p]) = wide_codes(x[i].v[e], p, sv);
-        }
-        if (masked[i])
-#pragma unroll
-          for (int g4 = 0; g4 < 4; ++g4) mask_four(s, g4, x[i].m[g4], R.qframe);
-        // block b + N's loads, and the rows of the one after it (past the last: the last)
-        masked[i] = block_masked<D>(next, R.bits);
-        block_load<D>(c, at(min(b + N, mine - 1)), next, masked[i], x[i]);
-        next = block_rows<D>(c, at(min(b + N + 1, mine - 1)));
-        bf16x8 p[2];
-        if (softmax_block<D>(R, s, p, c.c2)) rescale<D>(R, R.alpha);
-        pv_block<D>(R, p, vslot, c.ra, 0);
+      for (int j = 0; j < Geo8<D>::NS; ++j) {
+        const u32x4 u = x.k[2 * j], w = x.k[2 * j + 1];
+        const i32x8 k = {(int)u[0], (int)u[1], (int)u[2], (int)u[3],
+                         (int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+        s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, R.hi[j], s, 0, 0, 0, (int)x.sk, 0, R.e_hi);
+        s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, R.lo[j], s, 0, 0, 0, (int)x.sk, 0, R.e_lo);
       }
+      // V to LDS in bf16
+#pragma unroll
+      for (int e = 0; e < B::NV; ++e) {
+        const float sv = pow2_of(x.sv[e]);
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          *reinterpret_cast<u32x4*>(vslot + vst[2 * e + p]) = wide_codes(x.v[e], p, sv);
+      }
+      if (masked)
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4) mask_four(s, g4, x.m[g4], R.qframe);
+      // the next block's loads, and the rows of the one after it (past the last: the last)
+      masked = block_masked<D>(next, R.bits);
+      block_load<D>(c, at(min(b + 1, mine - 1)), next, masked, x);
+      next = block_rows<D>(c, at(min(b + 2, mine - 1)));
+      bf16x8 p[2];
+      if (softmax_block<D>(R, s, p, c.c2)) rescale<D>(R, R.alpha);
+      pv_block<D>(R, p, vslot, c.ra, 0);
     }
   }
   // join: waves 2, 3 into 0, 1, then 1 into 0 (O^T as fp32 [element][lane] in
@@ -814,7 +818,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fp8_kernel(HierFwdFp8Args a,
 // Joins the parts of one item and head, kJoinRows rows a workgroup, D / 4 lanes
 // a row: the parts' maxima and sums are read at once, one or two a lane (at
 // most 32 parts), and their O's eight at a time, so that a row costs a few
-// memory latencies and not one a part.
+// memory latencies and not one a part.  324 items of three parts: 12 of the
+// call's 130 us.
 constexpr int kMaxSplits = 32;
 template <int D>
 __global__ __launch_bounds__(kThreads) void join_fp8_kernel(HierFwdFp8Args a) {

@@ -9,6 +9,13 @@
 //   dn = the inverse rotation of dy;  dw_d = sum over tokens and heads of dn_d x_d r
 //   dh = dn w;  dx = r (dh - x r mean_d(dh x r))
 // All of it in fp32, one rounding to bf16 at the store.
+//
+// Both are bound by HBM: every input is read once and every output written
+// once, a lane holding eight neighbouring channels (16 bytes, four rotated
+// pairs), a head 8 or 16 lanes, so that its sums are DPP adds and nothing goes
+// through LDS.  6,678 tokens of 24 + 24 heads of 128 (167 MB): 35.5 us,
+// 4.7 TB/s; the gradient of 18,816 such tokens (703 MB): 149 us, 4.7 TB/s; a
+// large copy reaches 4.8 to 5.0.
 #include "hier_common.h"
 
 namespace {
@@ -84,8 +91,9 @@ __device__ __forceinline__ float inv_rms(const float* x, float eps) {
   return 1.f / sqrtf(fmaf(head_sum<D>(ss), 1.f / D, eps));
 }
 
-// One wave per token, tensor and kGroups groups of heads; cos, sin and the
-// gain stay in registers over the groups.
+// One wave per token, tensor and kGroups groups of heads (24 heads of 128 or 48
+// of 64): the groups' loads are all in flight at once, and cos, sin and the gain
+// stay in registers over them.
 template <int D>
 __global__ __launch_bounds__(kThreads) void head_norm_kernel(HierHeadNormArgs a, int units_q,
                                                              int units, int64_t waves) {

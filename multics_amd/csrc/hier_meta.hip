@@ -571,7 +571,6 @@ __device__ void eval_chunk(const Topo& c, int kind, int s, int r0, int m, Shared
 }
 
 __global__ __launch_bounds__(kThreads) void meta_count_long_kernel(HierTopo t, HierMetaCounts out) {
-  __shared__ Shared sh;
   __shared__ int seg[32], logical[32], uni, dense;
   Topo c;
   c.t = &t;

