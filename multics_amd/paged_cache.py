@@ -135,13 +135,14 @@ class HierPagedKVCache:
 
     # ---- addressing ----------------------------------------------------------------
 
-    def agent_row(self, p: int, frame: int) -> int:
+    def agent_row(self, p: int, frame):
+        """First pool row of a frame's page (or of each of an array of frames)."""
         return (p * self.R + frame % self.R) * self.pages[0]
 
-    def local_row(self, g: int, frame: int) -> int:
+    def local_row(self, g: int, frame):
         return self.a_rows + (g * self.R + frame % self.R) * self.pages[1]
 
-    def global_row(self, frame: int) -> int:
+    def global_row(self, frame):
         return self.a_rows + self.l_rows + (frame % self.R) * self.pages[2]
 
     def block_rows(self, start_frame: int, n: int) -> np.ndarray:
@@ -164,14 +165,13 @@ class HierPagedKVCache:
         16 pool rows that a block's tokens fill: every page's tokens in runs
         of 16, the last shorter."""
         rows = self.block_rows(start_frame, n)
-        widths = [self.L] * (self.P * n) + \
-            ([] if self.no_local else [self.KL] * (n * self.N)) + [self.KG] * n
         src, count, at = [], [], 0
-        for w in widths:
-            first = np.arange(0, w, FP8_BLOCK)
-            src.append(at + first)
-            count.append(np.minimum(FP8_BLOCK, w - first))
-            at += w
+        for pages, width in ((self.P * n, self.L), (0 if self.no_local else n * self.N, self.KL),
+                             (n, self.KG)):
+            first = np.arange(0, width, FP8_BLOCK)
+            src.append((at + np.arange(pages)[:, None] * width + first).reshape(-1))
+            count.append(np.tile(np.minimum(FP8_BLOCK, width - first), pages))
+            at += pages * width
         src = np.concatenate(src)
         return np.stack([src, rows[src], np.concatenate(count)], axis=1).astype(np.int32)
 
@@ -261,14 +261,13 @@ class HierPagedKVCache:
         frames up to it), their pool bases per stream and the local-hub active
         flag of each cached local frame."""
         f = self.slot_frame
-        frames = sorted(int(x) for x in f[(f >= 0) & (f <= end_frame) & (f > end_frame - self.R)])
-        agent = [[self.agent_row(p, x) for x in frames] for p in range(self.P)]
-        local = [] if self.no_local else [[self.local_row(g, x) for x in frames]
-                                          for g in range(self.N)]
-        glob = [self.global_row(x) for x in frames] if self.KG > 0 else []
-        lact = [] if self.no_local else [[bool(self.local_active[g, x % self.R]) for x in frames]
-                                         for g in range(self.N)]
-        return frames, (agent, local, glob), lact
+        frames = np.sort(f[(f >= 0) & (f <= end_frame) & (f > end_frame - self.R)])
+        groups = 0 if self.no_local else self.N
+        agent = [self.agent_row(p, frames).tolist() for p in range(self.P)]
+        local = [self.local_row(g, frames).tolist() for g in range(groups)]
+        glob = self.global_row(frames).tolist() if self.KG > 0 else []
+        lact = [self.local_active[g, frames % self.R].tolist() for g in range(groups)]
+        return frames.tolist(), (agent, local, glob), lact
 
 
 def init_hier_paged_kv_cache(*, num_layers: int, **kw):
