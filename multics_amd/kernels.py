@@ -860,9 +860,9 @@ def _fp8_splits(workgroups: int, max_tiles: int) -> int:
     the 512 workgroups that run at once (two a CU), else enough for 768 of
     them, of eight 64-key tiles at least (a part costs a second launch, and
     its rows of O written and read in fp32), at most 32.  324 items of 163
-    tiles: 161 us in one part, 154 in two, 137 in three, 141 in four; 96 items
-    of 228 tiles: 251 in one, 85 in six, 87 in eight, 102 in 24; 1,560 items:
-    568 in one, 618 in two."""
+    tiles: 151 us in one part, 153 in two, 129 in three, 135 in four; 96 items
+    of 228 tiles: 248 in one, 74 in six, 71 in eight, 83 in ten, 94 in 24;
+    1,560 items: 511 in one, 577 in two."""
     if workgroups >= 512:
         return 1
     return max(1, min(32, -(-768 // workgroups), max_tiles // 8))

@@ -332,6 +332,24 @@ def test_two_calls_at_once_on_two_streams():
     _check(qs[1], c, tiles)
 
 
+def test_in_and_out_of_inference_mode():
+    """A cache, its list and the list's launch order made in inference mode serve
+    calls outside of it, and the other way round."""
+    need_gpu()
+    case, outs = CASES[0], []
+    for made, called in ((True, False), (False, True), (False, False)):
+        M.clear_metadata_cache()
+        with torch.inference_mode(made):
+            c, q, tiles = _rollout(case)
+            outs.append(hier_cached_attention_fp8(q, c, tiles))
+        with torch.inference_mode(called), torch.no_grad():
+            c.append(q, q, case[11] - case[6], case[6], [case[13]] * case[6])
+            outs.append(hier_cached_attention_fp8(q, c, tiles))
+    assert torch.equal(outs[0], outs[2]) and torch.equal(outs[0], outs[4])
+    assert torch.equal(outs[1], outs[3]) and torch.equal(outs[1], outs[5])
+    assert not torch.equal(outs[0], outs[1])
+
+
 def test_rows_of_no_item_and_views():
     need_gpu()
     c, q, tiles = _rollout(CASES[0])
