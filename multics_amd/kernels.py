@@ -844,7 +844,10 @@ class QKHeadPrologueFunction(torch.autograd.Function):
 def qk_head_prologue_train(qx, kx, *, norm_q_w, norm_k_w, rope_cos, rope_sin, num_heads, eps,
                            num_kv_heads=None, out_layout="shd"):
     """``qk_head_prologue`` under autograd: differentiable in the projections
-    and the gains.  The same arguments and results."""
+    and the gains.  The same arguments and results.  A backward pass is
+    captured into a graph only when no eager pass over the same leaves is held
+    any more (outputs or a loss of it): autograd would join the two passes'
+    streams, which ends the process."""
     return QKHeadPrologueFunction.apply(qx, kx, norm_q_w, norm_k_w, rope_cos, rope_sin,
                                         int(num_heads),
                                         None if num_kv_heads is None else int(num_kv_heads),

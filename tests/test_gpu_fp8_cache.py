@@ -350,6 +350,32 @@ def test_in_and_out_of_inference_mode():
     assert not torch.equal(outs[0], outs[1])
 
 
+def test_a_pool_past_32_bits():
+    """Pools of more than 2^32 bytes, the rows in use at their far end: codes,
+    scales and outputs as in a small cache that holds the same frames."""
+    need_gpu()
+    kw = dict(P=1, N=1, L=1000, KL=1, KG=1, H=32, D=128, n=1)
+    small, big = _cache(W=2, **kw), _cache(W=1100, **kw)
+    assert big.k.shape[0] * 32 * 128 > 2 ** 32
+    g = torch.Generator(device="cuda").manual_seed(11)
+    S = _rows(big, 1)
+    mk = lambda: torch.randn(S, 32, 128, generator=g, device="cuda").to(torch.bfloat16)  # noqa: E731
+    for f in range(big.R - 3, big.R):          # the last pages of the ring
+        k, v = mk(), mk()
+        big.append(k, v, f, 1, [[True]])
+        small.append(k, v, f, 1, [[True]])
+    q, outs = mk(), []
+    for c in (small, big):
+        tiles = M.cached_window_tiles(c, big.R - 1, device="cuda", n_frames=1, n_block=1, local_attn=2,
+                                      labels=[[0]], q_active=[[True]], direct_player=True)
+        outs.append(hier_cached_attention_fp8(q, c, tiles))
+        rows = [torch.from_numpy(c.block_rows(f, 1)).long().cuda() for f in range(big.R - 3, big.R)]
+        outs.append([(t.view(torch.uint8)[r].clone(), s.view(torch.uint8)[r // 16].clone())
+                     for t, s in ((c.k, c.k_scale), (c.v, c.v_scale)) for r in rows])
+    assert torch.equal(outs[0], outs[2]) and torch.count_nonzero(outs[0]) > 0
+    assert all(torch.equal(a, b) for x, y in zip(outs[1], outs[3]) for a, b in zip(x, y))
+
+
 def test_rows_of_no_item_and_views():
     need_gpu()
     c, q, tiles = _rollout(CASES[0])

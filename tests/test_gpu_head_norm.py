@@ -192,6 +192,32 @@ def test_values_that_are_not_finite_stay_in_their_head():
     assert torch.count_nonzero(zero) == 0
 
 
+def test_more_than_2_31_elements():
+    """The last tokens of a long sequence, forward and gradient, equal those of
+    the same tokens alone (the gains' gradients are sums over all: not compared)."""
+    need_gpu()
+    S, H, D, last = 2 ** 31 // (24 * 128) + 100, 24, 128, 64
+    g = torch.Generator(device="cuda").manual_seed(4)
+    some = torch.randn(997, H * D, generator=g, device="cuda").to(torch.bfloat16)
+    qx = some.repeat(-(-S // 997), 1)[:S]
+    kx = qx[:, :D].contiguous()
+    angle = torch.rand(S, D // 2, generator=g, device="cuda")
+    cs, sn = angle.cos(), angle.sin()
+    w = 1 + 0.1 * torch.randn(D, generator=g, device="cuda")
+    kw = dict(norm_q_w=w, norm_k_w=w, num_heads=H, num_kv_heads=1, eps=1e-6)
+    end = lambda t: t[-last:]  # noqa: E731
+    tail = dict(kw, rope_cos=end(cs), rope_sin=end(sn))
+    full = dict(kw, rope_cos=cs, rope_sin=sn)
+    q, k = qk_head_prologue(qx, kx, **full)
+    q2, k2 = qk_head_prologue(end(qx), end(kx), **tail)
+    assert torch.equal(end(q), q2) and torch.equal(end(k), k2)
+    del q, k
+    dq, dk = qx.view(S, H, D), kx.view(S, 1, D)
+    got = qk_head_prologue_backward(dq, dk, qx, kx, **full)
+    want = qk_head_prologue_backward(end(dq), end(dk), end(qx), end(kx), **tail)
+    assert torch.equal(end(got[0]), want[0]) and torch.equal(end(got[1]), want[1])
+
+
 def test_captured_on_a_side_stream():
     """Forward and gradient recorded into a graph, replayed on new inputs."""
     need_gpu()
@@ -213,6 +239,45 @@ def test_captured_on_a_side_stream():
         torch.cuda.synchronize()
         want = qk_head_prologue(qx, kx, **kw) + qk_head_prologue_backward(dq, dk, qx, kx, **kw)
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_a_training_step_captured():
+    """Forward and ``backward()`` of the differentiable form in one graph, the
+    warm-up's graphs gone before: replayed gradients equal the eager ones."""
+    need_gpu()
+    args = [_inputs(61, 4, 2, 64, False, torch.float32, seed=i) for i in range(3)]
+    qx, kx, kw, dq, dk = (t.clone() if torch.is_tensor(t) else dict(t) for t in args[0])
+    leaves = [t.requires_grad_() for t in (qx, kx, kw["norm_q_w"].clone(), kw["norm_k_w"].clone())]
+    kw["norm_q_w"], kw["norm_k_w"] = leaves[2:]
+
+    def step():
+        q, k = qk_head_prologue_train(qx, kx, **kw)
+        torch.autograd.backward((q, k), (dq, dk))
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for _ in range(3):
+            for t in leaves:
+                t.grad = None
+            step()
+    torch.cuda.current_stream().wait_stream(stream)
+    torch.cuda.synchronize()
+    for t in leaves:
+        t.grad = None
+    graph = torch.cuda.CUDAGraph()
+    say("capture of a training step")
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    for new in args + args:
+        with torch.no_grad():
+            for to, t in zip((qx, kx, dq, dk), (new[0], new[1], new[3], new[4])):
+                to.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        with torch.no_grad():
+            want = qk_head_prologue_backward(dq, dk, qx, kx, **kw)
+        assert all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
 
 
 def test_one_row_with_a_stride_of_no_meaning():
