@@ -172,7 +172,9 @@ __global__ __launch_bounds__(kThreads) void head_norm_bwd_kernel(HierHeadNormBwd
       float x[8], g[8], dn[8], dot = 0.f;
       unpack(xw, x);
       unpack(gw, g);
-      const float r = inv_rms<D>(x, a.eps);
+      // (a lane without a head holds zeros: with eps = 0 their 0 * inf would
+      // reach the gain's sums)
+      const float rms = inv_rms<D>(x, a.eps), r = in ? rms : 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         dn[2 * i] = g[2 * i] * c[i] + g[2 * i + 1] * s[i];

@@ -317,3 +317,26 @@ def test_refusals_and_empty():
     assert q.shape == (0, 4, 64) and k.shape == (0, 2, 64)
     grads = qk_head_prologue_backward(dq[:0], dk[:0], qx[:0], kx[:0], **none)
     assert grads[0].shape == (0, 256) and torch.count_nonzero(grads[2]) == 0
+
+
+def _check_gradient(qx, kx, kw, dq, dk, Hq, Hk):
+    """The entry's gradient within the bounds of the head of this file."""
+    got = qk_head_prologue_backward(dq, dk, qx, kx, **kw)
+    for x, dy, w, H, dx, dw in ((qx, dq, kw["norm_q_w"], Hq, got[0], got[2]),
+                                (kx, dk, kw["norm_k_w"], Hk, got[1], got[3])):
+        ref, slack, rw, terms = _grad_formula(x, dy, w, kw["rope_cos"], kw["rope_sin"], H)
+        off = (dx.double().reshape(ref.shape) - ref).abs()
+        assert bool((off <= STEP * (ref.abs() + slack) + slack).all()), float((off / slack).max())
+        assert bool(((dw.double() - rw).abs() <= 2.0 ** -15 * terms).all())
+
+
+@pytest.mark.parametrize("Hq,Hk", [(1, 1), (5, 2), (7, 5), (12, 3), (24, 24)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_gradient_without_an_eps(D, Hq, Hk, monkeypatch):
+    """eps = 0, with head counts that leave lanes of a wave without a head."""
+    need_gpu()
+    monkeypatch.setitem(globals(), "EPS", 0.0)
+    qx, kx, kw, dq, dk = _inputs(19, Hq, Hk, D, False, torch.float32)
+    assert kw["eps"] == 0.0
+    say("head norm gradient, eps 0", D, Hq, Hk)
+    _check_gradient(qx, kx, kw, dq, dk, Hq, Hk)
