@@ -583,7 +583,7 @@ int hier_gated_residual(const HierGateArgs* args, void* stream);
 typedef struct HierHeadNormArgs {
   int64_t S;                       /* tokens                                   */
   int32_t Hq, Hk, D;               /* heads of q and of k, head dim (64 or 128) */
-  float eps;
+  float eps;                       /* at least 0                               */
   int32_t gain_bf16;               /* gains in bf16 (else fp32)                */
   int32_t reserved;
   const uint16_t* qx;              /* bf16 [S] rows of Hq * D                  */

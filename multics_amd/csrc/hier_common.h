@@ -23,6 +23,14 @@ inline int fail(int code, const char* fmt, ...) {
   return code;
 }
 
+// Whether v is a number of [lo, hi].  By its bits: comparisons alone do not
+// tell a NaN where the compiler may take it that there is none.
+inline bool number_in(float v, float lo, float hi) {
+  uint32_t bits;
+  memcpy(&bits, &v, 4);
+  return (bits & 0x7fffffffu) < 0x7f800000u && v >= lo && v <= hi;
+}
+
 inline void clear_error() { g_last_error[0] = 0; }
 
 // Bytes spanned by a [rows][H][D] bf16 view with element strides ss and sh:

@@ -257,6 +257,8 @@ extern "C" int hier_head_prologue(const HierHeadNormArgs* args, void* stream) {
   HIER_REQUIRE(a.D == 128 || a.D == 64, HIER_EUNSUPPORTED, "head_dim must be 64 or 128, got %d", a.D);
   HIER_REQUIRE(a.S >= 0 && a.Hq >= 1 && a.Hk >= 1, HIER_EINVAL, "invalid S=%lld Hq=%d Hk=%d",
                (long long)a.S, a.Hq, a.Hk);
+  HIER_REQUIRE(hier::number_in(a.eps, 0.f, 3.4e38f), HIER_EINVAL,
+               "eps must be a number of at least 0, got %g", (double)a.eps);
   if (a.S == 0) return HIER_OK;
   HIER_REQUIRE(a.qx && a.kx && a.norm_q_w && a.norm_k_w && a.rope_cos && a.rope_sin && a.q_out &&
                    a.k_out,
@@ -289,6 +291,8 @@ extern "C" int hier_head_prologue_bwd(const HierHeadNormBwdArgs* args, void* str
   HIER_REQUIRE(a.D == 128 || a.D == 64, HIER_EUNSUPPORTED, "head_dim must be 64 or 128, got %d", a.D);
   HIER_REQUIRE(a.S >= 1 && a.Hq >= 1 && a.Hk >= 1 && (int64_t)a.Hq + a.Hk <= (1 << 30), HIER_EINVAL,
                "invalid S=%lld Hq=%d Hk=%d", (long long)a.S, a.Hq, a.Hk);
+  HIER_REQUIRE(hier::number_in(a.eps, 0.f, 3.4e38f), HIER_EINVAL,
+               "eps must be a number of at least 0, got %g", (double)a.eps);
   HIER_REQUIRE(a.qx && a.kx && a.norm_q_w && a.norm_k_w && a.rope_cos && a.rope_sin && a.dq &&
                    a.dk && a.dqx && a.dkx && a.dnorm_q && a.dnorm_k && a.partial,
                HIER_EINVAL, "NULL tensor pointer");

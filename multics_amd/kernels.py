@@ -731,6 +731,8 @@ def _head_args(qx, kx, norm_q_w, norm_k_w, rope_cos, rope_sin, num_heads, num_kv
         raise NotImplementedError(f"per-head norms support head_dim 64/128, got {D}")
     if kx.shape != (S, Hk * D):
         raise ValueError(f"kx must be [{S}, {Hk}*{D}], got {tuple(kx.shape)}")
+    if not 0.0 <= eps <= 3.4e38:
+        raise ValueError(f"eps must be a number of at least 0, got {eps}")
     qx, q_ss = _head_rows("qx", qx, gpu)
     kx, k_ss = _head_rows("kx", kx, gpu)
     for name, w in (("norm_q_w", norm_q_w), ("norm_k_w", norm_k_w)):

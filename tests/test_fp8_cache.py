@@ -207,3 +207,28 @@ def test_packed_arguments_are_the_structures():
         vals = [0.5 if t is _capi.f32 else 3 + 7 * i for i, (_, t) in enumerate(cls._fields_)]
         a = cls.from_buffer_copy(_capi.packer(cls)(*vals))
         assert [getattr(a, n) for n, _ in cls._fields_] == vals
+
+
+def _refused(name, cls, base, bad):
+    """Every change of ``base`` (sizes; made-up addresses, never read) is refused."""
+    import ctypes as C
+    from multics_amd import _capi
+    for change in bad:
+        a = cls()
+        for i, (field, t) in enumerate(cls._fields_):
+            setattr(a, field, 0x7f0000000000 + 4096 * i if t is _capi.vp else 0)
+        for field, value in {**base, **change}.items():
+            setattr(a, field, value)
+        assert getattr(_capi.lib(), name)(C.byref(a), None) in (
+            _capi.HIER_EINVAL, _capi.HIER_EUNSUPPORTED), (name, change)
+    # (an empty call clears the message)
+    assert _capi.lib().hier_kv_append_fp8(C.byref(_capi.HierPageFp8Args(H=1, D=64)), None) == 0
+
+
+def test_c_norms_refuse_an_eps_below_0():
+    from multics_amd import _capi
+    bad = [dict(eps=x) for x in (-1e-6, -1.0, float("nan"), float("inf"), float("-inf"))]
+    size = dict(S=4, Hq=2, Hk=1, D=64, partial_rows=2)
+    _refused("hier_head_prologue_bwd", _capi.HierHeadNormBwdArgs, size, bad)
+    size.pop("partial_rows")
+    _refused("hier_head_prologue", _capi.HierHeadNormArgs, size, bad)

@@ -340,3 +340,14 @@ def test_gradient_without_an_eps(D, Hq, Hk, monkeypatch):
     assert kw["eps"] == 0.0
     say("head norm gradient, eps 0", D, Hq, Hk)
     _check_gradient(qx, kx, kw, dq, dk, Hq, Hk)
+
+
+@pytest.mark.parametrize("eps", [-1e-6, float("nan"), float("inf"), 1e300])
+def test_an_eps_below_0_is_refused(eps):
+    need_gpu()
+    qx, kx, kw, dq, dk = _inputs(3, 2, 1, 64, False, torch.float32)
+    for call in (lambda kw: qk_head_prologue(qx, kx, **kw),
+                 lambda kw: qk_head_prologue_train(qx, kx, **kw),
+                 lambda kw: qk_head_prologue_backward(dq, dk, qx, kx, **kw)):
+        with pytest.raises(ValueError, match="eps"):
+            call({**kw, "eps": eps})
