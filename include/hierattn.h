@@ -671,6 +671,8 @@ int hier_kv_append_fp8(const HierPageFp8Args* args, void* stream);
 /* h / (H / Hk).  With splits > 1 every item's key list is cut into that many */
 /* parts, computed by workgroups of their own into part_o / part_ml, and      */
 /* joined in a fixed order by a second launch.                                */
+/* q, k, v, o, tile_kv_mask, part_o and part_ml are 16-byte aligned, row_table */
+/* 8; the other arrays as their elements.                                     */
 typedef struct HierFwdFp8Args {
   int32_t H, Hk, D;                /* query heads, key heads, head dim         */
   int32_t n_items;

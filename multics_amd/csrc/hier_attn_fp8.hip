@@ -912,9 +912,11 @@ extern "C" int hier_attn_fwd_fp8(const HierFwdFp8Args* args, void* stream) {
                HIER_EINVAL, "NULL tensor pointer");
   HIER_REQUIRE(a.splits == 1 || (a.part_o && a.part_ml), HIER_EINVAL, "splits need part_o and part_ml");
   auto al16 = [](const void* p) { return ((uintptr_t)p & 15u) == 0; };
-  HIER_REQUIRE(al16(a.q) && al16(a.k) && al16(a.v) && al16(a.o) && al16(a.tile_kv_idx) &&
-                   al16(a.part_o) && al16(a.part_ml),
-               HIER_EINVAL, "q/k/v/o, the key index list and the workspace must be 16-byte aligned");
+  // (masks are read four keys at a time, row-table entries whole)
+  HIER_REQUIRE(al16(a.q) && al16(a.k) && al16(a.v) && al16(a.o) && al16(a.tile_kv_mask) &&
+                   al16(a.part_o) && al16(a.part_ml) && ((uintptr_t)a.row_table & 7u) == 0,
+               HIER_EINVAL,
+               "q/k/v/o, the key mask list and the workspace must be 16-byte aligned, the row table 8");
   HIER_REQUIRE(a.q_ss % 8 == 0 && a.q_sh % 8 == 0 && a.kv_ss % 16 == 0 && a.kv_sh % 16 == 0 &&
                    a.o_ss % 4 == 0 && a.o_sh % 4 == 0,
                HIER_EINVAL, "strides must keep 16-byte rows aligned");

@@ -232,3 +232,12 @@ def test_c_norms_refuse_an_eps_below_0():
     _refused("hier_head_prologue_bwd", _capi.HierHeadNormBwdArgs, size, bad)
     size.pop("partial_rows")
     _refused("hier_head_prologue", _capi.HierHeadNormArgs, size, bad)
+
+
+def test_c_attention_refuses_lists_that_it_cannot_read_whole():
+    """Masks are read 16 bytes at a time, row-table entries 8."""
+    from multics_amd import _capi
+    at = 0x7f0000000000
+    size = dict(H=4, Hk=2, D=128, n_items=3, scale=1.0, splits=2, kv_rows=64, q_rows=8)
+    _refused("hier_attn_fwd_fp8", _capi.HierFwdFp8Args, size,
+             [dict(tile_kv_mask=at + 4), dict(tile_kv_mask=at + 8), dict(row_table=at + 4)])

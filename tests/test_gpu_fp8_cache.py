@@ -519,3 +519,19 @@ def test_module_rollout_over_an_8_bit_cache(qk_norm, monkeypatch):
             assert torch.equal(torch.cat(ys), both)
             for i in range(2):
                 assert torch.equal(pair.k[:, i * H:(i + 1) * H].float(), caches[i].k.float())
+
+
+def test_an_index_list_may_start_anywhere():
+    """Pool rows are read one at a time: a list of them that starts at any entry of
+    an array serves; a mask list that cannot be read 16 bytes at a time is refused."""
+    need_gpu()
+    import dataclasses
+    shifted = lambda t: torch.cat((t[:1], t))[1:]  # noqa: E731
+    for case in (CASES[0], CASES[2]):
+        c, q, tiles = _rollout(case)
+        want = hier_cached_attention_fp8(q, c, tiles)
+        odd = dataclasses.replace(tiles, kv_idx=shifted(tiles.kv_idx))
+        assert odd.kv_idx.data_ptr() % 16 == 4
+        assert torch.equal(hier_cached_attention_fp8(q, c, odd), want)
+        with pytest.raises(ValueError, match="mask list"):
+            hier_cached_attention_fp8(q, c, dataclasses.replace(tiles, kv_mask=shifted(tiles.kv_mask)))
