@@ -905,8 +905,8 @@ extern "C" int hier_attn_fwd_fp8(const HierFwdFp8Args* args, void* stream) {
                "invalid n_items=%d kv_rows=%lld q_rows=%lld splits=%d", a.n_items,
                (long long)a.kv_rows, (long long)a.q_rows, a.splits);
   if (a.n_items == 0) return HIER_OK;
-  HIER_REQUIRE(a.scale > 0.f && a.scale <= 1e30f, HIER_EINVAL, "the softmax scale must be positive, got %g",
-               (double)a.scale);
+  HIER_REQUIRE(a.scale > 0.f && hier::number_in(a.scale, 0.f, 1e30f), HIER_EINVAL,
+               "the softmax scale must be positive, got %g", (double)a.scale);
   HIER_REQUIRE(a.q && a.k && a.v && a.k_scale && a.v_scale && a.o && a.tile_items && a.tile_kv_idx &&
                    a.tile_kv_mask && a.tile_blk_and,
                HIER_EINVAL, "NULL tensor pointer");

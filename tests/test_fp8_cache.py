@@ -241,3 +241,10 @@ def test_c_attention_refuses_lists_that_it_cannot_read_whole():
     size = dict(H=4, Hk=2, D=128, n_items=3, scale=1.0, splits=2, kv_rows=64, q_rows=8)
     _refused("hier_attn_fwd_fp8", _capi.HierFwdFp8Args, size,
              [dict(tile_kv_mask=at + 4), dict(tile_kv_mask=at + 8), dict(row_table=at + 4)])
+
+
+def test_c_attention_refuses_a_scale_that_is_not_a_number():
+    from multics_amd import _capi
+    size = dict(H=4, Hk=2, D=128, n_items=3, splits=2, kv_rows=64, q_rows=8)
+    _refused("hier_attn_fwd_fp8", _capi.HierFwdFp8Args, size,
+             [dict(scale=x) for x in (float("nan"), float("inf"), 2e30, -1.0, 0.0)])
