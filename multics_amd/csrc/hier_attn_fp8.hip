@@ -928,8 +928,9 @@ extern "C" int hier_attn_fwd_fp8(const HierFwdFp8Args* args, void* stream) {
                HIER_EUNSUPPORTED,
                "a head's codes and scales must span at most 4 GiB, of 2^24 rows and strides below 2^24");
   const int64_t total = (int64_t)a.n_items * a.splits * a.H;
-  HIER_REQUIRE((int64_t)a.n_items * a.splits < (1ll << 31) && total < (1ll << 24), HIER_EUNSUPPORTED,
-               "too many work items");
+  // (fewer than 2^32 threads a launch)
+  HIER_REQUIRE((int64_t)a.n_items * a.splits < (1ll << 31) && hier::xcd_grid(total) < (1ll << 24),
+               HIER_EUNSUPPORTED, "too many work items");
   return a.D == 128 ? launch<128>(a, total, (hipStream_t)stream)
                     : launch<64>(a, total, (hipStream_t)stream);
 }

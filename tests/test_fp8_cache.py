@@ -248,3 +248,11 @@ def test_c_attention_refuses_a_scale_that_is_not_a_number():
     size = dict(H=4, Hk=2, D=128, n_items=3, splits=2, kv_rows=64, q_rows=8)
     _refused("hier_attn_fwd_fp8", _capi.HierFwdFp8Args, size,
              [dict(scale=x) for x in (float("nan"), float("inf"), 2e30, -1.0, 0.0)])
+
+
+def test_c_attention_refuses_a_grid_of_2_32_threads():
+    """2^24 workgroups of 256, reached by rounding up to the number of XCDs too."""
+    from multics_amd import _capi
+    size = dict(H=1, Hk=1, D=64, scale=1.0, splits=1, kv_rows=64, q_rows=8)
+    _refused("hier_attn_fwd_fp8", _capi.HierFwdFp8Args, size,
+             [dict(n_items=(1 << 24) - i) for i in (0, 1, 7)] + [dict(n_items=(1 << 23) - 1, splits=2)])
