@@ -49,10 +49,18 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 // As in the bf16 forward: a lane's sum of a block above kSumMax refreshes the
-// running max.  Maxima are held in exp2 units (score * scale * log2 e), so that
-// no scale takes kNoMax, the max of a row that has seen no key, past fp32.
+// running max.  Maxima are held in exp2 units (score * scale * log2 e); kNoMax,
+// the max of a row that has seen no key, is below every score, so that a row's
+// first visible key refreshes it whatever its score.
 constexpr float kSumMax = 16.f * 256.f;
-constexpr float kNoMax = -1e30f;
+constexpr float kNoMax = -3.4028235e38f;
+// The running max m is a rounded product, off by up to 2^-25 of it, and the
+// weights exp2(s * c2 - m) of one rounding (an fma) carry that as a common
+// factor, which the row sum takes out again: at most 2^(1/2) where |m| < kFar =
+// 2^24, past fp32 from 2^32 on.  So from kFar on every block is refreshed
+// (Rows::lim is below any sum) and its products are rounded as m was: the
+// largest key's weight is 1 then.
+constexpr float kFar = 16777216.f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 template <int D>
@@ -109,6 +117,7 @@ struct Rows {
   int e_hi, e_lo;                            // their scales (exponent + 127)
   f32x16 o[Geo<D>::NDB];
   float m, l, alpha;                         // m in exp2 units
+  float lim;                                 // sum of a block's P that refreshes m
   int qtok, qframe, head;
   bool valid;
   uint32_t bits;   // OR over the sub-block's valid rows of 1 << query frame
@@ -188,6 +197,7 @@ __device__ __forceinline__ void rows_init(Rows<D>& R, const HierFwdFp8Args& a, c
   R.m = kNoMax;
   R.l = 0.f;
   R.alpha = 1.f;
+  R.lim = kSumMax;
 }
 
 // Per-lane LDS byte offsets of the MFMA operand reads (tile-relative).
@@ -244,11 +254,21 @@ __device__ __forceinline__ void mask_block(f32x16& s, const char* mslot, int kb,
 }
 
 // P of one 32-key block: exp2(s * c2 + nb) rounded to bf16, as the two P^T
-// operands of the block; returns the lane's sum of the rounded P.
-__device__ __forceinline__ float p_block(const f32x16& s, bf16x8* p, float c2, float nb) {
+// operands of the block; returns the lane's sum of the rounded P.  With ``far``
+// the product is rounded by itself.
+template <bool FAR = false>
+__device__ __forceinline__ float p_block(const f32x16& s, bf16x8* p, float c2, float nb,
+                                         bool far = false) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
-    p[i >> 3][i & 7] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[i], c2, nb));
+  for (int i = 0; i < 16; ++i) {
+    float x = fmaf(s[i], c2, nb);
+    if constexpr (FAR) {
+      float y = s[i] * c2;
+      asm("" : "+v"(y));        // (a product of its own: not contracted to an fma)
+      x = far ? y + nb : x;
+    }
+    p[i >> 3][i & 7] = (__bf16)__builtin_amdgcn_exp2f(x);
+  }
   const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
   float ps0 = 0.f, ps1 = 0.f;
 #pragma unroll
@@ -284,19 +304,21 @@ template <int D>
 __device__ __forceinline__ bool softmax_fix(Rows<D>& R, const f32x16& s, bf16x8* p, float c2,
                                             float ps) {
   float alpha = 1.f;
-  const bool refresh = __ballot(!(ps <= kSumMax)) != 0;
+  const bool refresh = __ballot(!(ps <= R.lim)) != 0;
   if (__builtin_expect(refresh, 0)) {
     float mx = s[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
     mx = pair_max(mx);
     const float m = fmaxf(R.m, mx * c2);
+    const bool far = fabsf(m) >= kFar && m != kNoMax;
     bf16x8 q[2];
-    put(ps, p_block(s, q, c2, -m));
+    put(ps, p_block<true>(s, q, c2, -m, far));
     put(p[0], q[0]);
     put(p[1], q[1]);
     put(alpha, __builtin_amdgcn_exp2f(R.m - m));
     put(R.m, m);
+    put(R.lim, far ? -1.f : kSumMax);
   }
   R.l = fmaf(R.l, alpha, ps);
   R.alpha = alpha;

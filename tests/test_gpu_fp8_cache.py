@@ -535,3 +535,34 @@ def test_an_index_list_may_start_anywhere():
         assert torch.equal(hier_cached_attention_fp8(q, c, odd), want)
         with pytest.raises(ValueError, match="mask list"):
             hier_cached_attention_fp8(q, c, dataclasses.replace(tiles, kv_mask=shifted(tiles.kv_mask)))
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("size,scale", [(1.0, 1e9), (1.0, 1e20), (1.0, 1e30), (1e30, 0.125), (1e30, 1e6)])
+@pytest.mark.parametrize("case", [CASES[0], CASES[1], CASES[2]], ids=lambda c: c[0])
+def test_scores_of_any_magnitude(case, size, scale, splits, monkeypatch):
+    """Scores far from 0 on either side, also below any start that a running max
+    could have: the largest takes all the weight, equal ones share it.  One channel
+    of a query is not 0 and k is positive there, so that a score is one product
+    (12 bits, exact) and unequal ones differ by 2^-4 of them or more: the weights
+    are those of the formula, whatever the arithmetic.  lse: the scale times
+    log2 e and its way back, the product and the sum round by 2^-24 of it each."""
+    need_gpu()
+    monkeypatch.setattr(kernels, "_fp8_splits", lambda workgroups, max_tiles: splits)
+
+    def positive(c, f, k, v):
+        k[:, :, 0] = k[:, :, 0].abs() + 0.25
+
+    c, q, tiles = _rollout(case, seed=6, hide=positive)
+    sign = torch.where(torch.arange(q.shape[0], device="cuda") % 3 == 0, -1.0, 1.0)
+    q[:, :, 1:] = 0
+    q[:, :, 0] = ((q[:, :, 0].float().abs() + 0.25).double() * size * sign[:, None]).to(torch.bfloat16)
+    say("fp8 scores", case[0], size, scale, splits)
+    lse = torch.full((q.shape[1], q.shape[0]), 7.0, device="cuda")
+    out = hier_cached_attention_fp8(q, c, tiles, lse=lse, scale=scale)
+    torch.cuda.synchronize()
+    ref, bound, rlse = _reference(q, c, tiles, scale)
+    assert bool(((out.double() - ref).abs() <= bound).all())
+    some = ~torch.isinf(rlse)
+    assert torch.equal(torch.isinf(lse), ~some)
+    assert bool(((lse.double() - rlse).abs() <= STEP + 2.0 ** -21 * rlse.abs())[some].all())
