@@ -352,6 +352,13 @@ __device__ __forceinline__ void pv_block(Rows<D>& R, const bf16x8* p, const char
     }
 }
 
+// Natural log of a row's sum l over its running max m (exp2 units): -inf for a
+// row that sees no key, not a number where l is not one (l = 0 is told by its
+// bits: the compiler takes it that there are no NaN).
+__device__ __forceinline__ float normaliser(float m, float l) {
+  return __float_as_uint(l) == 0u ? -INFINITY : fmaf(m, kLn2, __logf(l));
+}
+
 template <int D>
 __device__ __forceinline__ void store_rows(const Rows<D>& R, const HierFwdFp8Args& a, int split,
                                            int lane) {
@@ -383,7 +390,7 @@ __device__ __forceinline__ void store_rows(const Rows<D>& R, const HierFwdFp8Arg
       *reinterpret_cast<u32x2*>(op + db * 32 + 8 * g4 + 4 * half) = w;
     }
   if (a.lse && half == 0)
-    a.lse[(int64_t)head * a.lse_stride_h + R.qtok] = l > 0.f ? fmaf(R.m, kLn2, __logf(l)) : -INFINITY;
+    a.lse[(int64_t)head * a.lse_stride_h + R.qtok] = normaliser(R.m, l);
 }
 
 // ---- staging ------------------------------------------------------------------
@@ -898,7 +905,7 @@ __global__ __launch_bounds__(kThreads) void join_fp8_kernel(HierFwdFp8Args a) {
   w[1] = (uint32_t)f2bf(o[2] * inv) | ((uint32_t)f2bf(o[3] * inv) << 16);
   *reinterpret_cast<u32x2*>(a.o + (int64_t)r.qtok * a.o_ss + (int64_t)head * a.o_sh + 4 * sub) = w;
   if (a.lse && sub == 0)
-    a.lse[(int64_t)head * a.lse_stride_h + r.qtok] = l > 0.f ? fmaf(m, kLn2, __logf(l)) : -INFINITY;
+    a.lse[(int64_t)head * a.lse_stride_h + r.qtok] = normaliser(m, l);
 }
 
 template <int D>

@@ -889,7 +889,8 @@ def hier_cached_attention_fp8(q: torch.Tensor, cache, tiles: TileList, *,
     (``metadata.cached_window_tiles``).  Returns ``out``, bf16 [S, H, D] (made
     here when not given; rows of no item are 0 then, and left as they were in
     a given one); a row that sees no key is 0.  ``lse`` (optional, fp32 [H, S])
-    receives the natural-log softmax normaliser.  Inference only."""
+    receives the natural-log softmax normaliser: -inf for a row that sees no
+    key, NaN where the output is NaN.  Inference only."""
     if torch.is_grad_enabled() and q.requires_grad:
         raise RuntimeError("attention over an 8-bit cache is inference-only (q requires grad)")
     if not getattr(cache, "fp8", False):

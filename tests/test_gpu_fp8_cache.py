@@ -566,3 +566,18 @@ def test_scores_of_any_magnitude(case, size, scale, splits, monkeypatch):
     some = ~torch.isinf(rlse)
     assert torch.equal(torch.isinf(lse), ~some)
     assert bool(((lse.double() - rlse).abs() <= STEP + 2.0 ** -21 * rlse.abs())[some].all())
+
+
+def test_the_normaliser_of_rows_that_are_not_numbers():
+    """lse is NaN where the output is (-inf is a row that sees no key)."""
+    need_gpu()
+    for case in (CASES[0], CASES[2], CASES[4]):
+        c, q, tiles = _rollout(case)
+        q[1, q.shape[1] - 1, 3] = float("nan")
+        lse = torch.full((q.shape[1], q.shape[0]), 7.0, device="cuda")
+        for splits in (1, 2):
+            with pytest.MonkeyPatch.context() as m:
+                m.setattr(kernels, "_fp8_splits", lambda workgroups, max_tiles: splits)
+                out = hier_cached_attention_fp8(q, c, tiles, lse=lse)
+            assert bool(torch.isnan(out[1, -1]).all())
+            assert torch.equal(torch.isnan(lse), torch.isnan(out).all(-1).t()), case[0]
