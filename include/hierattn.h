@@ -112,6 +112,7 @@ typedef struct HierMetaOut {
   /* attention-kernel tile list: per (block, stream) the ordered union of its */
   /* query frames' key lists with a per-key bitmask over query frames         */
   const int64_t* tile_kv_off;     /* [B][P+N+1] key offset of each stream     */
+                                  /* (items hold it in 32 bits: sum tile_count < 2^31) */
   const int32_t* tile_item_off;   /* [B][P+N+1] first work item of each stream */
   int32_t rows_per_item;          /* query rows per work item (multiple of 32) */
   int32_t* tile_kv_idx;           /* [sum tile_count] K/V pool token index     */

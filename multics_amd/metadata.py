@@ -710,6 +710,21 @@ class _HubMerge:
         return shared, torch.cat([out[:self.n_out_items], kept]).index_select(0, self.fwd_index)
 
 
+def _fits_items(entries: int) -> None:
+    """Refuses key lists of more entries, over all streams and blocks, than a
+    work item's offset (int32) addresses."""
+    if entries >= 1 << 31:
+        raise NotImplementedError(f"key lists of {entries} entries in all: a tile list holds fewer "
+                                  "than 2^31")
+
+
+def _list_offsets(lengths) -> np.ndarray:
+    """First entry of each key list of these lengths, and the end of the last."""
+    off = np.concatenate([[0], np.cumsum(np.asarray(lengths, np.int64))])
+    _fits_items(int(off[-1]))
+    return off
+
+
 def build(topo: BlockTopology, device, *, segmented_block_m: Optional[int] = None,
           tiled: bool = False, rows_per_item: int = ROWS_PER_ITEM,
           merge_hubs: Optional[int] = None, fold_tails: Optional[bool] = None) -> BuildResult:
@@ -759,7 +774,7 @@ def build(topo: BlockTopology, device, *, segmented_block_m: Optional[int] = Non
         up.add(np.asarray(arr), dtype, lambda ptr: setattr(out, field, ptr))
 
     # ---- tile list ----------------------------------------------------------
-    tile_off = np.concatenate([[0], np.cumsum(tile_h.reshape(-1))])
+    tile_off = _list_offsets(tile_h.reshape(-1))
     n_keys = int(tile_off[-1])
     rows = np.array([[n * _qlen(topo, s) for s in range(NS)] for _ in range(B)], dtype=np.int64)
     nit = -(-rows // rows_per_item)
@@ -801,6 +816,7 @@ def build(topo: BlockTopology, device, *, segmented_block_m: Optional[int] = Non
         if merge.fwd_index is None:
             merge = None
     cap = merge.capacity if merge is not None else n_keys
+    _fits_items(cap)
     kv_idx = torch.empty(max(cap, 1), dtype=torch.int32, device=dev)
     kv_mask = torch.empty(max(cap, 1), dtype=torch.int32, device=dev)
     blk_and = torch.empty(max(cap // TILE_KEYS, 1), dtype=torch.int32, device=dev)

@@ -256,3 +256,12 @@ def test_c_attention_refuses_a_grid_of_2_32_threads():
     size = dict(H=1, Hk=1, D=64, scale=1.0, splits=1, kv_rows=64, q_rows=8)
     _refused("hier_attn_fwd_fp8", _capi.HierFwdFp8Args, size,
              [dict(n_items=(1 << 24) - i) for i in (0, 1, 7)] + [dict(n_items=(1 << 23) - 1, splits=2)])
+
+
+def test_list_offsets_are_refused_past_31_bits():
+    assert M._list_offsets([64, 0, 128]).tolist() == [0, 64, 64, 192]
+    most = (1 << 31) - 64
+    assert int(M._list_offsets([most - 64, 64])[-1]) == most
+    for lengths in ([most, 64], np.full(5, 1 << 30, np.int32), [1 << 31]):
+        with pytest.raises(NotImplementedError, match="entries"):
+            M._list_offsets(lengths)

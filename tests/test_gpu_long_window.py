@@ -95,3 +95,14 @@ def test_reference_formats_are_refused():
     topo, _ = _window(1, 1, 2, 1, 1, 1, 699, 700, [0])
     with pytest.raises(NotImplementedError, match="tile list only"):
         M.build(topo, "cuda", segmented_block_m=16)
+
+
+def test_lists_past_31_bits_are_refused():
+    """Four players' windows of 1.2e9 tokens: each stream's list fits, all of them
+    together do not fit an item's offset.  Refused from the counts, before any list
+    is made."""
+    need_gpu()
+    topo, _ = _window(4, 1, 1 << 18, 1, 1, 1, 1200, 1144, [0, 0, 0, 0])
+    say("lists past 31 bits")
+    with pytest.raises(NotImplementedError, match="2\\^31"):
+        M.build(topo, "cuda")
