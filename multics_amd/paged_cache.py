@@ -111,6 +111,9 @@ class HierPagedKVCache:
             self.k = torch.zeros((rows, heads, self.D), dtype=dtype, device=self.device)
             self.v = torch.zeros_like(self.k)
             self.k_scale = self.v_scale = None
+        # the pools' own device, whichever is current at an append ("cuda" alone
+        # would send the row tables to the device that is current then)
+        self.device = self.k.device
         self.slot_frame = np.full(self.R, -1, dtype=np.int64)
         self.local_active = np.zeros((max(self.N, 1), self.R), dtype=bool)
         self._dst_cache = {}

@@ -581,3 +581,15 @@ def test_the_normaliser_of_rows_that_are_not_numbers():
                 out = hier_cached_attention_fp8(q, c, tiles, lse=lse)
             assert bool(torch.isnan(out[1, -1]).all())
             assert torch.equal(torch.isnan(lse), torch.isnan(out).all(-1).t()), case[0]
+
+
+@pytest.mark.parametrize("dtype", [FP8, torch.bfloat16])
+def test_a_cache_keeps_the_device_that_its_pools_are_on(dtype):
+    """Made on "cuda", without an index: row tables of later appends go to the
+    pools' device, not to the one that is current then."""
+    need_gpu()
+    c = _cache(dtype=dtype)
+    assert c.device == c.k.device and c.device.index is not None
+    blk = torch.zeros(_rows(c, 2), 3, 64, dtype=torch.bfloat16, device="cuda")
+    c.append(blk, blk, 0, 2, [[True, True]] * 2)
+    assert all(t.device == c.k.device for t in c._dst_cache.values())
