@@ -176,9 +176,12 @@ class SelfAttention(nn.Module):
 
     def _fused_ok(self, x, cam_tokens) -> bool:
         dropout = cam_tokens is not None and self.training and self.cam_dropout_p > 0
+        # (the per-head pass takes fp32 gains too, e.g. norms kept in fp32)
+        gains = (torch.bfloat16,) if self.qk_norm == "model" else (torch.bfloat16, torch.float32)
         return (x.is_cuda and x.dtype == torch.bfloat16 and x.shape[0] == 1 and not dropout and
-                self.q.weight.dtype == torch.bfloat16 and self.norm_q.weight.dtype == torch.bfloat16
-                and self.head_dim in (64, 128))
+                self.q.weight.dtype == torch.bfloat16 and self.norm_q.weight.dtype in gains and
+                (self.qk_norm == "model" or self.norm_k.weight.dtype in gains) and
+                self.head_dim in (64, 128))
 
     def _project_fused(self, x, freqs, cam_tokens=None):
         """No-grad Q/K/V: GEMMs, then the fused HIP prologue on q and k.
@@ -213,8 +216,9 @@ class SelfAttention(nn.Module):
 
     def _project_train(self, x, freqs, cam_tokens):
         """Differentiable [S, H, D] bf16 Q/K/V.  On the GPU, for bf16 weights and
-        model dims that are multiples of 512 (up to 4096; any with per-head
-        norms), the q / k tail runs on the HIP prologue forward and backward
+        model dims that are multiples of 512 (up to 4096; any, and bf16 or fp32
+        gains, with per-head norms), the q / k tail runs on the HIP prologue
+        forward and backward
         (``qk_prologue_train``, ``qk_head_prologue_train``) after the three
         GEMMs; otherwise the reference's torch ops
         (``_project_self_attn_qkv``)."""

@@ -351,3 +351,36 @@ def test_an_eps_below_0_is_refused(eps):
                  lambda kw: qk_head_prologue_backward(dq, dk, qx, kx, **kw)):
         with pytest.raises(ValueError, match="eps"):
             call({**kw, "eps": eps})
+
+
+@pytest.mark.parametrize("q_gain,k_gain", [(torch.float32, torch.float32),
+                                           (torch.bfloat16, torch.float32)])
+def test_module_with_fp32_gains_runs_the_pass(q_gain, k_gain, monkeypatch):
+    """A bf16 module whose norms are kept in fp32 (or one of them): q and k come
+    from the HIP pass with and without autograd, once rounded from the formula."""
+    need_gpu()
+    from multics_amd import module as mod
+    calls = []
+    for name in ("qk_head_prologue", "qk_head_prologue_train"):
+        fn = getattr(mod, name)
+        monkeypatch.setattr(mod, name, lambda *a, fn=fn, name=name, **kw: calls.append(name) or fn(*a, **kw))
+    torch.manual_seed(3)
+    S, H, D = 41, 3, 64
+    m = SelfAttention(H * D, H, qk_norm="head").to("cuda", torch.bfloat16)
+    m.norm_q.to(q_gain), m.norm_k.to(k_gain)
+    for norm in (m.norm_q, m.norm_k):
+        torch.nn.init.normal_(norm.weight, mean=1.0, std=0.2)
+    x = torch.randn(1, S, H * D, device="cuda").to(torch.bfloat16)
+    angle = torch.rand(S, 1, D // 2, dtype=torch.float64, device="cuda").float().double()
+    freqs = torch.polar(torch.ones_like(angle), angle)
+    q, k, _ = m._project_train(x, freqs, None)
+    torch.autograd.backward((q, k), (torch.ones_like(q), torch.ones_like(k)))
+    with torch.no_grad():
+        fq, fk, _ = m._qkv_blocks(x, freqs, None)
+        assert calls == ["qk_head_prologue_train", "qk_head_prologue"]
+        assert torch.equal(fq, q) and torch.equal(fk, k)
+        cs, sn = freqs.real[:, 0].float(), freqs.imag[:, 0].float()
+        for got, lin, norm in ((q, m.q, m.norm_q), (k, m.k, m.norm_k)):
+            assert norm.weight.grad.dtype == norm.weight.dtype
+            ref, size = _formula(lin(x)[0], norm.weight, cs, sn, H)
+            assert bool(((got.double() - ref).abs() <= STEP * ref.abs() + 2 * F32 * size).all())
