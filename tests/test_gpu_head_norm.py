@@ -384,3 +384,75 @@ def test_module_with_fp32_gains_runs_the_pass(q_gain, k_gain, monkeypatch):
             assert norm.weight.grad.dtype == norm.weight.dtype
             ref, size = _formula(lin(x)[0], norm.weight, cs, sn, H)
             assert bool(((got.double() - ref).abs() <= STEP * ref.abs() + 2 * F32 * size).all())
+
+
+def test_gain_sums_of_many_tokens():
+    """More tokens than eight for each of the 1,024 workgroups, unequal head counts.
+    A sum is fewer than 256 additions in a row here too (k: 16 tokens a wave, three
+    steps over the lanes, four waves, 10 rows a thread, 16 threads)."""
+    need_gpu()
+    qx, kx, kw, dq, dk = _inputs(9001, 12, 2, 64, False, torch.float32, seed=8)
+    _check_gradient(qx, kx, kw, dq, dk, 12, 2)
+
+
+@pytest.mark.parametrize("gain", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cam_dim", [0, 12])
+def test_module_gradients_match_64_bits(cam_dim, gain):
+    """Gradients of a training projection -- the input, the q and k products, the
+    camera adapters and the gains -- against autograd in 64 bits through the same
+    module, its q and k rows those that bf16 products gave.
+
+    Bounds: a gradient of a q row is the kernel's (the bounds above, d below); a
+    product with it sums d times the other factor, fp32 sums of fewer than 2^9
+    terms (2^-15 of the terms), rounded to bf16; x gathers two such products and
+    their rounded sum."""
+    need_gpu()
+    torch.manual_seed(1)
+    S, H, D = 70, 5, 64
+    m = SelfAttention(H * D, H, qk_norm="head").to("cuda", torch.bfloat16)
+    m.norm_q.to(gain), m.norm_k.to(gain)
+    for norm in (m.norm_q, m.norm_k):
+        torch.nn.init.normal_(norm.weight, mean=1.0, std=0.2)
+    x = torch.randn(1, S, H * D, device="cuda").to(torch.bfloat16).requires_grad_()
+    cam, adapters = None, [None, None]
+    if cam_dim:
+        m.enable_camera_pose_qk(cam_dim, dropout_p=0.0)
+        adapters = [m.cam_q, m.cam_k]
+        for a in adapters:
+            torch.nn.init.normal_(a.weight, std=0.1)
+        cam = torch.randn(1, S, cam_dim, device="cuda").to(torch.bfloat16)
+    angle = torch.rand(S, 1, D // 2, dtype=torch.float64, device="cuda")
+    freqs = torch.polar(torch.ones_like(angle), angle)
+    grads = [torch.randn(S, H, D, device="cuda").to(torch.bfloat16) for _ in range(2)]
+    q, k, _ = m._project_train(x, freqs, cam)
+    torch.autograd.backward((q, k), grads)
+    with torch.no_grad():
+        rows = m._apply_camera_qk(m.q(x), m.k(x), cam)
+    cs, sn = freqs.real[:, 0].float(), freqs.imag[:, 0].float()
+    xw = x.detach().double()[0]
+    want_x, room_x = [], []
+    near = lambda got, ref, room: bool(  # noqa: E731
+        ((got.double() - ref).abs() <= STEP * (ref.abs() + room) + room).all())
+    for row, dy, lin, norm, adapter in zip(rows, grads, (m.q, m.k), (m.norm_q, m.norm_k), adapters):
+        row64 = row[0].double().requires_grad_()
+        w64 = norm.weight.detach().double().requires_grad_()
+        y, _ = _formula(row64, w64, cs, sn, H)
+        drow, dw = torch.autograd.grad(y, (row64, w64), dy.double())
+        _, slack, _, terms = _grad_formula(row[0], dy, norm.weight.detach(), cs, sn, H)
+        slack = slack.reshape(drow.shape)
+        d = STEP * (drow.abs() + slack) + slack            # of a row's gradient
+        for name, got, other in (("weight", lin.weight, xw), ("bias", lin.bias, torch.ones_like(xw[:, :1])),
+                                 ("camera", None if adapter is None else adapter.weight,
+                                  None if cam is None else cam[0].double())):
+            if got is None:
+                continue
+            ref = (drow.t() @ other).reshape(got.shape)
+            room = ((d + 2.0 ** -15 * drow.abs()).t() @ other.abs()).reshape(got.shape)
+            assert near(got.grad, ref, room), name
+        w = lin.weight.detach().double()
+        want_x.append(drow @ w)
+        room = (d + 2.0 ** -15 * drow.abs()) @ w.abs()
+        room_x.append(STEP * (want_x[-1].abs() + room) + room)
+        assert bool(((norm.weight.grad.double() - dw).abs() <=
+                     STEP * dw.abs() + (1 + STEP) * 2.0 ** -15 * terms).all())
+    assert near(x.grad[0], sum(want_x), sum(room_x))
