@@ -1399,9 +1399,13 @@ def costly_first(tiles: TileList) -> TileList:
     first: a launch of a few rounds of workgroups ends on its short items then.
     The cost of an item is the length of the list it was built with (equal for
     the items of a stream, which so stay together and share what they read),
-    two fifths of it for at most 32 rows.  Made on the current stream on first
-    use and kept on the launch list; not under graph capture, which then runs
-    the items in their own order (each item's result is the same anywhere)."""
+    three fifths of it for at most 32 rows: they fill a quarter of the matrix
+    tiles but read as much.  Ten players, 24 heads: 568 us in the list's order,
+    544 / 532 / 529 / 527 / 546 with 1, 4/5, 3/5, 2/5 and 1/5; six players, 16
+    heads: 279, then 264 / 244 / 244 / 256 / 257; one player's frame: 86, then
+    84 and 73 with any below 1.  Made on the current stream on first use and
+    kept on the launch list; not under graph capture, which then runs the items
+    in their own order (each item's result is the same anywhere)."""
     run = launch_list(tiles)
     hit = run.__dict__.get("_costly")
     if hit is not None:
@@ -1412,7 +1416,7 @@ def costly_first(tiles: TileList) -> TileList:
     if _ready.capturing(items.device):
         return dataclasses.replace(run, items=items, n_items=n, fwd_items=None)
     built = (tiles.fwd_items if fwd else tiles.items)[:n]
-    cost = built[:, 6] * torch.where(built[:, 4] <= 32, 2, 5)
+    cost = built[:, 6] * torch.where(built[:, 4] <= 32, 3, 5)
     order = torch.argsort(cost, descending=True, stable=True)
     piece = dataclasses.replace(run, items=items[:n].index_select(0, order), n_items=n, fwd_items=None)
     piece.__dict__["_is_launch"] = True
