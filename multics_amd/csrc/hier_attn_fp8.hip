@@ -13,10 +13,12 @@
 // significant bits and an e4m3 code 4, so a row of Q enters as two codes,
 // q = hi + lo, both over powers of two: the rest q - hi is at most half a step
 // of hi (8 of the 16 units that q resolves there), an integer below 16 units
-// and so a code itself.  The split is exact for every element down to 2^-14
-// of its row's largest; below that the error is at most 2^-22 of that
-// largest.  Two 8-bit products cost what one in bf16 does, and K needs no
-// conversion.
+// and so a code itself.  hi's power of two takes the row's largest to 224 .. 448,
+// lo's is 2^-4 of it, whose smallest step is 2^-13: the split is exact for every
+// element down to 2^-6, which is below 2^-13 of the row's largest; what is smaller
+// errs by at most 2^-14, below 2^-21 of the largest (a row whose largest is below
+// 448 * 2^-100 is held over 2^-100: by at most 2^-114).  Two 8-bit products cost
+// what one in bf16 does, and K needs no conversion.
 //
 // V is converted when its tile is staged (v_cvt_scalef32_pk_bf16_fp8, exact:
 // code and scale fit a bf16) and P V runs on v_mfma_f32_32x32x16_bf16 with P
@@ -29,9 +31,9 @@
 // 32 rows a wave leave room for S, P, O and the query's codes without spills
 // (three waves a SIMD spill: twice the time).  Full items are bound by the
 // matrix units and the softmax beside them at the card's power limit: 6,678
-// rows against their windows (24 heads of 128, 507 GFLOP) 530 us, 956 TFLOP/s
-// of what rows see, where the bf16 kernel takes 631 over the same lists; the
-// same instructions on queries of zeros, which draw less power, take 447.
+// rows against their windows (24 heads of 128, 507 GFLOP) 530 us, 957 TFLOP/s
+// of what rows see, where the bf16 kernel takes 626 over the same lists; the
+// same instructions on queries of zeros, which draw less power, take 455.
 // Few items are cut into parts (the caller's ``splits``; parts and their join
 // below), items of at most 32 rows shared by the four waves (few_rows).
 #include "hier_common.h"
@@ -634,9 +636,13 @@ __device__ __forceinline__ void last_tile(Ctx<D>& c, Rows<D>& R, const f32x16& s
 // block's loads are in flight while one is multiplied (two blocks ahead: the
 // same time).  The four states are joined through LDS.  Query heads that share
 // a key head are packed into the sub-block when they fit, so that its K and V
-// are read once.  Bound by the latency of a wave's loads: one token of 32 heads
-// of 128 over 8 key heads, 4,096 cached frames, 20.6 us with the join of its
-// eight parts (99 as an item whose waves share each tile).
+// are read once.  One token of 32 heads of 128 over 8 key heads, 4,096 cached
+// frames: 20.8 us (99 as an item whose waves share each tile), of it the join of
+// its eight parts 4.  A wave takes 12 blocks here, 0.6 us each by the latency of
+// its loads (25.9 us this kernel with four parts, 24 blocks a wave; 18.5 with
+// eight); about 11 do not depend on them (17.8 with sixteen parts): the loads of
+// item, query and first rows, the join in LDS, and the workgroups of packed
+// heads, which read their item and leave.
 
 template <int D>
 struct Block {               // what a wave loads of a 32-key block
@@ -847,8 +853,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fp8_kernel(HierFwdFp8Args a,
 // Joins the parts of one item and head, kJoinRows rows a workgroup, D / 4 lanes
 // a row: the parts' maxima and sums are read at once, one or two a lane (at
 // most 32 parts), and their O's eight at a time, so that a row costs a few
-// memory latencies and not one a part.  324 items of three parts: 12 of the
-// call's 130 us.
+// memory latencies and not one a part.  324 items of three parts: 13 of the
+// call's 133 us.
 constexpr int kMaxSplits = 32;
 template <int D>
 __global__ __launch_bounds__(kThreads) void join_fp8_kernel(HierFwdFp8Args a) {

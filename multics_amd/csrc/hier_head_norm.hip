@@ -13,8 +13,8 @@
 // Both are bound by HBM: every input is read once and every output written
 // once, a lane holding eight neighbouring channels (16 bytes, four rotated
 // pairs), a head 8 or 16 lanes, so that its sums are DPP adds and nothing goes
-// through LDS.  6,678 tokens of 24 + 24 heads of 128 (167 MB): 35.5 us,
-// 4.7 TB/s; the gradient of 18,816 such tokens (703 MB): 149 us, 4.7 TB/s; a
+// through LDS.  6,678 tokens of 24 + 24 heads of 128 (167 MB): 36.6 us,
+// 4.6 TB/s; the gradient of 18,816 such tokens (703 MB): 149 us, 4.7 TB/s; a
 // large copy reaches 4.8 to 5.0.
 #include "hier_common.h"
 
@@ -235,8 +235,8 @@ __global__ __launch_bounds__(kThreads) void gain_sum_kernel(HierHeadNormBwdArgs 
   (is_k ? a.dnorm_k : a.dnorm_q)[blockIdx.x * 16 + col] = v;
 }
 
-// Workgroups of the gradient for one tensor: eight tokens each at least, and
-// 1,024 over both tensors, four to a CU (18,816 tokens of 24 + 24 heads of 128:
+// Workgroups of the gradient for one tensor: at most eight tokens each until
+// there are 1,024 over both tensors, four to a CU (18,816 tokens of 24 + 24 heads of 128:
 // 149.7 us; 150.7 with 512, 155.1 with 2,048, whose rows of sums take longer to
 // add up).
 constexpr int kRowsAll = 1024;

@@ -810,8 +810,8 @@ def qk_head_prologue_backward(dq: torch.Tensor, dk: torch.Tensor, qx: torch.Tens
     dqx, dkx = qx.new_empty((S, Hq * D)), qx.new_empty((S, Hk * D))
     if S == 0:
         return dqx, dkx, *torch.zeros((2, D), device=qx.device).unbind(0)
-    # a row of sums for each workgroup: of eight tokens at least, 1,024 in all
-    # (checked by the entry)
+    # a row of sums for each workgroup: at most eight tokens each until there are
+    # 1,024 (checked by the entry)
     rows = min(2 * -(-S // 8), 1026)
     part = qx.new_empty((rows, D), dtype=torch.float32)
     dwq, dwk = qx.new_empty((2, D), dtype=torch.float32).unbind(0)
@@ -864,10 +864,14 @@ def _fp8_splits(workgroups: int, max_tiles: int) -> int:
     """Parts that every item's key list is cut into: one where the items fill
     the 512 workgroups that run at once (two a CU), else enough for 768 of
     them, of eight 64-key tiles at least (a part costs a second launch, and
-    its rows of O written and read in fp32), at most 32.  324 items of 163
-    tiles: 151 us in one part, 153 in two, 129 in three, 135 in four; 96 items
-    of 228 tiles: 248 in one, 74 in six, 71 in eight, 83 in ten, 94 in 24;
-    1,560 items: 511 in one, 577 in two."""
+    its rows of O written and read in fp32), at most 32.  Every item and head
+    counts alike, those of few rows too and those that packing leaves without
+    work.  324 items of 163 tiles: 153 us in one part, 152 in two, 132 in
+    three, 135 in four; 96 items of 228 tiles: 248 in one, 77 in six, 73 in
+    eight, 87 in ten, 101 in 24; 96 items of 192 tiles (24 that work): 77 in one,
+    47 in two, 29 in four, 20.9 in eight, 20.2 in ten, 20.8 in sixteen; 60 items
+    of 16 tiles: 14.3 in one to four, 15.7 in eight; 1,560 items: 531 in one,
+    592 in two."""
     if workgroups >= 512:
         return 1
     return max(1, min(32, -(-768 // workgroups), max_tiles // 8))

@@ -24,7 +24,8 @@ With ``dtype=torch.float8_e4m3fn`` the pools hold 8-bit codes and, for every 16
 rows and head, a power-of-two scale (``k_scale`` / ``v_scale``, e8m0
 ``[rows / 16, batch * H]``); a value is its code times its scale.  Pages are
 padded to whole blocks of 16 rows, so that a block belongs to one page and is
-always written as a whole (220 tokens: 224 rows).  ``append`` quantises
+always written as a whole (220 tokens: 224 rows; one token: 16, eight times
+its bytes in bf16).  ``append`` quantises
 (``hier_kv_append_fp8``), ``kernels.hier_cached_attention_fp8`` reads the codes.
 """
 
@@ -60,7 +61,10 @@ class HierPagedKVCache:
     kernel launch per block, which sees ``batch * H`` heads.
 
     ``dtype`` is bf16, or ``torch.float8_e4m3fn`` for a cache held in 8 bits
-    (half the memory; head dim 64 or 128).
+    (head dim 64 or 128).  Its pages are whole blocks of 16 rows of a byte a
+    channel and the scales: half of bf16's memory for frames of many tokens
+    (220: 0.51), as much for pages of eight, more for smaller ones (six tokens:
+    1.3 times, five: 1.6, one: 8).
     """
 
     def __init__(self, *, num_players: int, num_groups: int, num_patches: int,
