@@ -702,6 +702,104 @@ typedef struct HierFwdFp8Args {
 
 int hier_attn_fwd_fp8(const HierFwdFp8Args* args, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* The rest of a transformer block: norm, products, cross attention.  Rows   */
+/* are bf16 or fp16 (`type`), strides in elements; no counterpart in the     */
+/* reference, which composes them of torch operations.                       */
+/* ------------------------------------------------------------------------ */
+enum { HIER_BF16 = 0, HIER_FP16 = 1, HIER_FP32 = 2 };
+enum { HIER_ACT_NONE = 0, HIER_ACT_GELU_TANH = 1, HIER_ACT_GELU = 2, HIER_ACT_SILU = 3 };
+
+/* h = x + r, y = h / sqrt(mean(h^2) + eps) * w over C channels; without r,  */
+/* h = x and is not written.  Channels are contiguous; C <= 16384.           */
+typedef struct HierRmsNormArgs {
+  int64_t M;                       /* rows                                     */
+  int32_t C;
+  float eps;                       /* at least 0                               */
+  int32_t type, gain_type;         /* gain_type: HIER_BF16 / FP16 / FP32       */
+  const void* x;
+  const void* r;                   /* residual or NULL                         */
+  const void* w;                   /* [C]                                      */
+  void* y;
+  void* h;                         /* the sum (with r)                         */
+  int64_t x_ss, r_ss, y_ss, h_ss;
+} HierRmsNormArgs;
+
+int hier_rms_norm(const HierRmsNormArgs* args, void* stream);
+
+/* Its gradient: dx (the gradient of x and of r alike) and dw, fp32 [C], from */
+/* dy and, with r, dh (NULL: none).  `partial` is fp32 [partial_rows][C] of   */
+/* hier_rms_norm_bwd_rows(args) rows.  Deterministic.                        */
+typedef struct HierRmsNormBwdArgs {
+  int64_t M;
+  int32_t C;
+  float eps;
+  int32_t type, gain_type;
+  const void* x;
+  const void* r;
+  const void* w;
+  const void* dy;
+  const void* dh;
+  void* dx;
+  float* dw;
+  float* partial;
+  int64_t x_ss, r_ss, dy_ss, dh_ss, dx_ss, partial_rows;
+} HierRmsNormBwdArgs;
+
+int64_t hier_rms_norm_bwd_rows(const HierRmsNormBwdArgs* args);
+int hier_rms_norm_bwd(const HierRmsNormBwdArgs* args, void* stream);
+
+/* z = x w^T + bias, out = residual + gate * act(z); bias, residual, gate and */
+/* preact (receives z) may be NULL.  Gate row i scales rows i * rows_per_gate */
+/* .. of out.  x and w: 16-byte aligned rows of K contiguous elements, K a    */
+/* multiple of 8, at most 2^21 - 1 elements apart.  `workspace` of            */
+/* hier_linear_workspace(args) bytes (16-byte aligned) belongs to one call at */
+/* a time.  out may be residual.                                             */
+typedef struct HierLinearArgs {
+  int64_t M;
+  int32_t N, K;
+  int32_t type, act;
+  const void* x;                   /* [M][K]                                   */
+  const void* w;                   /* [N][K]                                   */
+  const void* bias;                /* [N]                                      */
+  const void* residual;            /* [M][N]                                   */
+  const void* gate;                /* [M / rows_per_gate][N]                   */
+  void* out;                       /* [M][N]                                   */
+  void* preact;                    /* [M][N]                                   */
+  int64_t x_ss, w_ss, residual_ss, gate_ss, out_ss, preact_ss;
+  int64_t rows_per_gate;
+  void* workspace;
+  int64_t workspace_bytes;
+} HierLinearArgs;
+
+int64_t hier_linear_workspace(const HierLinearArgs* args);   /* -1: invalid    */
+int hier_linear(const HierLinearArgs* args, void* stream);
+
+/* Gradients of hier_linear from dy and preact: each of dx, dw, db, dgate    */
+/* that is not NULL.  preact may be NULL without an activation and dgate.    */
+/* Deterministic.                                                            */
+typedef struct HierLinearBwdArgs {
+  int64_t M;
+  int32_t N, K;
+  int32_t type, act;
+  const void* x;
+  const void* w;
+  const void* gate;
+  const void* dy;                  /* [M][N]                                   */
+  const void* preact;              /* [M][N]                                   */
+  void* dx;                        /* [M][K]                                   */
+  void* dw;                        /* [N][K]                                   */
+  void* db;                        /* [N]                                      */
+  void* dgate;                     /* [M / rows_per_gate][N]                   */
+  int64_t x_ss, w_ss, gate_ss, dy_ss, preact_ss, dx_ss, dw_ss;
+  int64_t rows_per_gate;
+  void* workspace;                 /* hier_linear_bwd_workspace(args) bytes    */
+  int64_t workspace_bytes;
+} HierLinearBwdArgs;
+
+int64_t hier_linear_bwd_workspace(const HierLinearBwdArgs* args);
+int hier_linear_bwd(const HierLinearBwdArgs* args, void* stream);
+
 /* Last error message of the calling thread ("" if none).                    */
 const char* hier_last_error(void);
 

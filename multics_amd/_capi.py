@@ -199,6 +199,34 @@ class HierFwdFp8Args(C.Structure):
                                   "row_table", "part_o", "part_ml")]
 
 
+class HierRmsNormArgs(C.Structure):
+    _fields_ = [("M", i64), ("C", i32), ("eps", f32), ("type", i32), ("gain_type", i32)] + \
+               [(n, vp) for n in ("x", "r", "w", "y", "h")] + \
+               [(n, i64) for n in ("x_ss", "r_ss", "y_ss", "h_ss")]
+
+
+class HierRmsNormBwdArgs(C.Structure):
+    _fields_ = [("M", i64), ("C", i32), ("eps", f32), ("type", i32), ("gain_type", i32)] + \
+               [(n, vp) for n in ("x", "r", "w", "dy", "dh", "dx", "dw", "partial")] + \
+               [(n, i64) for n in ("x_ss", "r_ss", "dy_ss", "dh_ss", "dx_ss", "partial_rows")]
+
+
+class HierLinearArgs(C.Structure):
+    _fields_ = [("M", i64)] + [(n, i32) for n in ("N", "K", "type", "act")] + \
+               [(n, vp) for n in ("x", "w", "bias", "residual", "gate", "out", "preact")] + \
+               [(n, i64) for n in ("x_ss", "w_ss", "residual_ss", "gate_ss", "out_ss", "preact_ss",
+                                   "rows_per_gate")] + \
+               [("workspace", vp), ("workspace_bytes", i64)]
+
+
+class HierLinearBwdArgs(C.Structure):
+    _fields_ = [("M", i64)] + [(n, i32) for n in ("N", "K", "type", "act")] + \
+               [(n, vp) for n in ("x", "w", "gate", "dy", "preact", "dx", "dw", "db", "dgate")] + \
+               [(n, i64) for n in ("x_ss", "w_ss", "gate_ss", "dy_ss", "preact_ss", "dx_ss", "dw_ss",
+                                   "rows_per_gate")] + \
+               [("workspace", vp), ("workspace_bytes", i64)]
+
+
 def packer(cls):
     """A function from the fields' values, in order, to the structure's bytes
     (pointers as addresses, 0 for NULL): a quarter of the time that filling
@@ -238,9 +266,19 @@ EXPORTS = {
     "hier_head_prologue_bwd": [vp, vp],
     "hier_kv_append_fp8": [vp, vp],
     "hier_attn_fwd_fp8": [vp, vp],
+    "hier_rms_norm": [vp, vp],
+    "hier_rms_norm_bwd_rows": [vp],
+    "hier_rms_norm_bwd": [vp, vp],
+    "hier_linear_workspace": [vp],
+    "hier_linear": [vp, vp],
+    "hier_linear_bwd_workspace": [vp],
+    "hier_linear_bwd": [vp, vp],
     "hier_last_error": [],
     "hier_version": [],
 }
+
+_SIZES = ("hier_derive_workspace", "hier_rms_norm_bwd_rows", "hier_linear_workspace",
+          "hier_linear_bwd_workspace")        # entries that return a size
 
 _lock = threading.Lock()
 _lib = None
@@ -262,7 +300,7 @@ def lib() -> C.CDLL:
                 fn = getattr(handle, name)
                 fn.argtypes = argtypes
                 fn.restype = C.c_char_p if name in ("hier_last_error", "hier_version") else \
-                    (C.c_int64 if name == "hier_derive_workspace" else C.c_int)
+                    (C.c_int64 if name in _SIZES else C.c_int)
             _lib = handle
     return _lib
 

@@ -1,0 +1,360 @@
+"""The rest of a transformer block around the hierarchical attention, on HIP
+kernels: a root-mean-square norm with the residual's addition, the matrix
+product with bias, activation, gate and residual in its epilogue, and attention
+to an encoder's states of another length.  Each comes as a call without
+gradient, its gradient, and the two under autograd (``_train``).  Reached as
+``multics_amd.kernels.rms_norm`` and so on; ``module.CrossAttention`` and
+``module.FeedForward`` run on them.  No counterpart in the reference, which
+composes them of torch operations.
+
+Rows are bf16 or fp16, sums fp32.  A backward pass is captured into a graph only
+when no eager pass over the same leaves is held any more (outputs or a loss of
+it): autograd would join the two passes' streams, which ends the process.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+
+from . import _capi
+
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+ACTIVATIONS = {None: 0, "gelu_tanh": 1, "gelu": 2, "silu": 3}
+
+_pack_norm = _capi.packer(_capi.HierRmsNormArgs)
+_pack_norm_bwd = _capi.packer(_capi.HierRmsNormBwdArgs)
+_pack_linear = _capi.packer(_capi.HierLinearArgs)
+_pack_linear_bwd = _capi.packer(_capi.HierLinearBwdArgs)
+
+
+def _no_grad_call(name: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} gives no gradient: use {name}_train")
+
+
+def _gpu_type(name: str, t: torch.Tensor) -> int:
+    """The type code of the rows of ``t``, a GPU tensor."""
+    if t.dtype is not torch.bfloat16 and t.dtype is not torch.float16:
+        raise NotImplementedError(f"{name} must be bf16 or fp16, got {t.dtype}")
+    if not t.is_cuda:
+        raise NotImplementedError(f"{name} must be a GPU tensor")
+    return _TYPES[t.dtype]
+
+
+def _like(name: str, t: torch.Tensor, x: torch.Tensor, shape) -> None:
+    if t.shape != tuple(shape) or t.dtype != x.dtype or t.device != x.device:
+        raise ValueError(f"{name} must be {x.dtype} {tuple(shape)} on {x.device}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+
+
+def _rows(t: torch.Tensor):
+    """``t`` [..., C] as rows with contiguous channels (copied if no view of it
+    is), and their stride."""
+    C = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(-1, C)
+    if t.stride(1) != 1 and C > 1:
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else C)
+
+
+def _rows16(t: torch.Tensor):
+    """``_rows`` of 16-byte rows: copied, and padded to a multiple of eight
+    channels with zeros, where they are not."""
+    t, ss = _rows(t)
+    C = t.shape[1]
+    if C % 8:
+        t = torch.nn.functional.pad(t, (0, -C % 8))
+        return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if ss % 8 or t.data_ptr() % 16 or ss < C:
+        t = _capi.aligned(t)
+        ss = C
+    return t, ss
+
+
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _outs(name: str, out: Optional[torch.Tensor], like: torch.Tensor, shape) -> torch.Tensor:
+    """``out`` as given, checked, or a new one."""
+    if out is None:
+        return torch.empty(shape, dtype=like.dtype, device=like.device)
+    _like(name, out, like, shape)
+    if not out.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return out
+
+
+# --------------------------------------------------------------------------
+# root-mean-square norm with the residual's addition
+# --------------------------------------------------------------------------
+
+def _norm_args(name, x, weight, eps, residual):
+    kind = _gpu_type("x", x)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x must have channels, got {tuple(x.shape)}")
+    C = x.shape[-1]
+    if weight.shape != (C,) or weight.device != x.device or weight.dtype not in _TYPES:
+        raise ValueError(f"weight must be [{C}] bf16, fp16 or fp32 on {x.device}, got "
+                         f"{tuple(weight.shape)} {weight.dtype} on {weight.device}")
+    eps = float(eps)
+    if not 0.0 <= eps <= 3.4e38:
+        raise ValueError(f"eps must be a number of at least 0, got {eps}")
+    if residual is not None:
+        _like("residual", residual, x, x.shape)
+    return kind, C, eps
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float,
+             residual: Optional[torch.Tensor] = None):
+    """``y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension of
+    ``h = x + residual`` (``hier_rms_norm``); fp32 inside, rounded once.
+
+    ``x`` [..., C] is bf16 or fp16 (C up to 16384), ``weight`` [C] bf16, fp16 or
+    fp32.  Returns ``y``, and with ``residual`` (shaped like x) ``(y, h)``; the
+    norm is that of the sum before its rounding to ``h``.  No gradient:
+    ``rms_norm_train``."""
+    _no_grad_call("rms_norm", x, weight, residual)
+    return _rms_norm(x, weight, eps, residual)
+
+
+def _rms_norm(x, weight, eps, residual):
+    kind, C, eps = _norm_args("rms_norm", x, weight, eps, residual)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    h = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    xr, x_ss = _rows(x)
+    r, r_ss = (None, 0) if residual is None else _rows(residual)
+    w = weight.contiguous()
+    if xr.shape[0]:
+        _capi.call_on(x.device, "hier_rms_norm", _pack_norm(
+            xr.shape[0], C, eps, kind, _TYPES[w.dtype], xr.data_ptr(), _ptr(r), w.data_ptr(),
+            y.data_ptr(), _ptr(h), x_ss, r_ss, C, C))
+    return y if h is None else (y, h)
+
+
+def rms_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, *, eps: float,
+                      residual: Optional[torch.Tensor] = None, dh: Optional[torch.Tensor] = None):
+    """Gradient of ``rms_norm`` (``hier_rms_norm_bwd``) from its inputs and the
+    gradients ``dy`` of y and ``dh`` (optional) of h: ``(dx, dweight)``, dx the
+    gradient of ``x`` and of ``residual`` alike, dweight fp32 [C], summed in a
+    fixed order."""
+    kind, C, eps = _norm_args("rms_norm_backward", x, weight, eps, residual)
+    _like("dy", dy, x, x.shape)
+    if dh is not None:
+        _like("dh", dh, x, x.shape)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dw = torch.empty(C, dtype=torch.float32, device=x.device)
+    (xr, x_ss), (g, g_ss) = _rows(x), _rows(dy)
+    r, r_ss = (None, 0) if residual is None else _rows(residual)
+    d, d_ss = (None, 0) if dh is None else _rows(dh)
+    w = weight.contiguous()
+    M = xr.shape[0]
+    if M == 0:
+        return dx, dw.zero_()
+    # a row of sums for each workgroup (checked by the entry)
+    rows = min((M + 3) // 4 if C <= 2048 else M, 512)
+    part = torch.empty((rows, C), dtype=torch.float32, device=x.device)
+    _capi.call_on(x.device, "hier_rms_norm_bwd", _pack_norm_bwd(
+        M, C, eps, kind, _TYPES[w.dtype], xr.data_ptr(), _ptr(r), w.data_ptr(), g.data_ptr(), _ptr(d),
+        dx.data_ptr(), dw.data_ptr(), part.data_ptr(), x_ss, r_ss, g_ss, d_ss, C, rows))
+    return dx, dw
+
+
+class RMSNormFunction(torch.autograd.Function):
+    """Differentiable ``rms_norm``."""
+
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, weight, residual)
+        ctx.eps = eps
+        return _rms_norm(x, weight, eps, residual)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh=None):
+        x, weight, residual = ctx.saved_tensors
+        if dy is None and dh is None:
+            return None, None, None, None
+        if dy is None:                  # h alone was used
+            dx, dw = dh, torch.zeros_like(weight)
+        else:
+            dx, dw = rms_norm_backward(dy, x, weight, eps=ctx.eps, residual=residual, dh=dh)
+            dw = dw.to(weight.dtype)
+        return dx, dw, None if residual is None else dx, None
+
+
+def rms_norm_train(x: torch.Tensor, weight: torch.Tensor, *, eps: float,
+                   residual: Optional[torch.Tensor] = None):
+    """``rms_norm`` under autograd: differentiable in x, weight and residual.
+    The same arguments and results."""
+    return RMSNormFunction.apply(x, weight, residual, eps)
+
+
+# --------------------------------------------------------------------------
+# matrix product with bias, activation, gate and residual
+# --------------------------------------------------------------------------
+
+def _linear_args(x, weight, bias, activation, residual, gate):
+    """(type, activation code, M, N, K, rows per gate) of checked arguments."""
+    kind = _gpu_type("x", x)
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError(f"x must be [..., K] and weight [N, K], got {tuple(x.shape)}, {tuple(weight.shape)}")
+    N, K = weight.shape
+    _like("weight", weight, x, (N, K))
+    if bias is not None:
+        _like("bias", bias, x, (N,))
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r}: one of {', '.join(map(repr, ACTIVATIONS))}")
+    M = x.numel() // K
+    if residual is not None:
+        _like("residual", residual, x, (*x.shape[:-1], N))
+    per = 1
+    if gate is not None:
+        if gate.dim() != x.dim() and gate.dim() != 1:
+            raise ValueError(f"gate must be [..., F, N] or [N], got {tuple(gate.shape)}")
+        lead, rows = (x.shape[:-2], x.shape[-2]) if x.dim() > 1 else ((), 1)
+        if gate.dim() == 1:
+            _like("gate", gate, x, (N,))
+            per = max(M, 1)
+        else:
+            F = gate.shape[-2]
+            _like("gate", gate, x, (*lead, F, N))
+            if F < 1 or rows % F:
+                raise ValueError(f"{rows} rows do not divide into {F} gate rows")
+            per = max(rows // F, 1)
+    return kind, ACTIVATIONS[activation], M, N, K, per
+
+
+def _workspace(name: str, args: bytes) -> int:
+    size = getattr(_capi.lib(), name)(args)
+    if size < 0:
+        _capi.check(_capi.HIER_EINVAL, name)
+    return size
+
+
+def _linear(x, weight, bias, activation, residual, gate, out, preact):
+    kind, act, M, N, K, per = _linear_args(x, weight, bias, activation, residual, gate)
+    shape = (*x.shape[:-1], N)
+    out = _outs("out", out, x, shape)
+    if M == 0:
+        return out
+    (xr, x_ss), (w, w_ss) = _rows16(x), _rows16(weight)
+    K = xr.shape[1]
+    b = None if bias is None else bias.contiguous()
+    r, r_ss = (None, 0) if residual is None else _rows(residual)
+    g, g_ss = (None, 0) if gate is None else _rows(gate)
+    fields = (M, N, K, kind, act, xr.data_ptr(), w.data_ptr(), _ptr(b), _ptr(r), _ptr(g), out.data_ptr(),
+              _ptr(preact), x_ss, w_ss, r_ss, g_ss, N, N, per)
+    size = 0 if M <= 64 else _workspace("hier_linear_workspace", _pack_linear(*fields, 0, 0))
+    ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    _capi.call_on(x.device, "hier_linear", _pack_linear(*fields, _ptr(ws), size))
+    return out
+
+
+def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+               activation: Optional[str] = None, residual: Optional[torch.Tensor] = None,
+               gate: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``residual + gate * act(x @ weight.T + bias)`` in one pass
+    (``hier_linear``); fp32 inside, rounded once.
+
+    ``x`` [..., K] and ``weight`` [N, K] are bf16 or fp16; ``activation`` is None,
+    ``"gelu_tanh"``, ``"gelu"`` or ``"silu"``.  ``residual`` is [..., N]; ``gate`` is
+    [N], or [..., F, N] whose rows scale S / F rows of x's S each (a frame's tokens
+    share their frame's gate, as in ``gated_residual``).  ``out`` (optional, contiguous)
+    may be ``residual``.  Rows of a multiple of eight channels are read in place,
+    others are copied with zeros behind.  No gradient: ``linear_act_train``."""
+    _no_grad_call("linear_act", x, weight, bias, residual, gate)
+    return _linear(x, weight, bias, activation, residual, gate, out, None)
+
+
+def linear_act_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, *,
+                        preact: Optional[torch.Tensor] = None, activation: Optional[str] = None,
+                        gate: Optional[torch.Tensor] = None, need=("x", "weight", "bias", "gate")) -> dict:
+    """Gradients of ``linear_act`` (``hier_linear_bwd``) from the gradient ``dy``
+    [..., N] of its output and ``preact`` [..., N], the values before the activation
+    (not needed without an activation and the gate's gradient): those of ``need``,
+    by name, in x's type.  The residual's gradient is ``dy``.  Sums are taken in a
+    fixed order: equal inputs give equal bits."""
+    kind, act, M, N, K, per = _linear_args(x, weight, None, activation, None, gate)
+    shape = (*x.shape[:-1], N)
+    _like("dy", dy, x, shape)
+    need = [n for n in need if n != "gate" or gate is not None]
+    if preact is None and (act or "gate" in need):
+        raise ValueError("linear_act_backward needs preact, the values before the activation")
+    if preact is not None:
+        _like("preact", preact, x, shape)
+    new = lambda *s: torch.empty(s, dtype=x.dtype, device=x.device)  # noqa: E731
+    if M == 0:
+        made = {"x": lambda: torch.zeros_like(x), "weight": lambda: torch.zeros_like(weight),
+                "bias": lambda: new(N).zero_(), "gate": lambda: torch.zeros_like(gate)}
+        return {n: made[n]() for n in need}
+    (xr, x_ss), (w, w_ss) = _rows16(x), _rows16(weight)
+    Kp = xr.shape[1]
+    # dy is an operand of the products where dz is dy itself
+    Np, b_dy = N, dy
+    if not act and gate is None and ("x" in need or "weight" in need):
+        if N % 8:                   # channels of zeros behind: rows of zeros in dw
+            Np = N + -N % 8
+            if "x" in need:
+                w = torch.nn.functional.pad(w, (0, 0, 0, Np - N))
+                w_ss = Kp
+        g_dy, dy_ss = _rows16(b_dy)
+        preact = None
+    else:
+        g_dy, dy_ss = _rows(b_dy)
+    z, z_ss = (None, 0) if preact is None else _rows(preact)
+    g, g_ss = (None, 0) if gate is None else _rows(gate)
+    dx = new(M, Kp) if "x" in need else None
+    dw = new(Np, Kp) if "weight" in need else None
+    db = new(Np) if "bias" in need else None
+    dg = new(M // per, N) if "gate" in need else None
+    fields = (M, Np, Kp, kind, act, xr.data_ptr(), w.data_ptr(), _ptr(g), g_dy.data_ptr(), _ptr(z), _ptr(dx),
+              _ptr(dw), _ptr(db), _ptr(dg), x_ss, w_ss, g_ss, dy_ss, z_ss, Kp, Kp, per)
+    size = _workspace("hier_linear_bwd_workspace", _pack_linear_bwd(*fields, 0, 0))
+    ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    _capi.call_on(x.device, "hier_linear_bwd", _pack_linear_bwd(*fields, _ptr(ws), size))
+    made = {"x": lambda: (dx if Kp == K else dx[:, :K]).reshape(x.shape),
+            "weight": lambda: dw if (Np, Kp) == (N, K) else dw[:N, :K].contiguous(),
+            "bias": lambda: db if Np == N else db[:N].contiguous(),
+            "gate": lambda: dg.reshape(gate.shape)}
+    return {n: made[n]() for n in need}
+
+
+class LinearActFunction(torch.autograd.Function):
+    """Differentiable ``linear_act``: keeps x, the weights, the gate and, with an
+    activation or a gate, the values before the activation in x's type."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, gate, activation):
+        keep = activation is not None or gate is not None and ctx.needs_input_grad[4]
+        z = torch.empty((*x.shape[:-1], weight.shape[0]), dtype=x.dtype, device=x.device) if keep else None
+        y = _linear(x, weight, bias, activation, residual, gate, None, z)
+        ctx.save_for_backward(x, weight, gate, z)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, gate, z = ctx.saved_tensors
+        names = ("x", "weight", "bias", "residual", "gate")
+        want = [n for n, w in zip(names, ctx.needs_input_grad) if w]
+        need = [n for n in want if n != "residual"]
+        got = linear_act_backward(dy, x, weight, preact=z, activation=ctx.activation, gate=gate,
+                                  need=need) if need else {}
+        if "residual" in want:
+            got["residual"] = dy
+        return *(got.get(n) for n in names), None
+
+
+def linear_act_train(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+                     activation: Optional[str] = None, residual: Optional[torch.Tensor] = None,
+                     gate: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``linear_act`` under autograd: differentiable in every tensor.  The same
+    arguments and results."""
+    return LinearActFunction.apply(x, weight, bias, residual, gate, activation)

@@ -1,0 +1,764 @@
+// Matrix product with bias, activation, gate and residual in its epilogue, and
+// the gradients of it:
+//   z = x W^T + b,   y = r + g * act(z)
+//   dz = dy * g * act'(z),   dx = dz W,   dW = dz^T x,   db = sum of dz's rows,
+//   dg = sum over a gate's rows of dy * act(z)
+// (x [M][K], W [N][K], g one row for rows_per_gate rows of y.)  Everything is
+// summed in fp32 and y rounded once.  A training step also writes z rounded to
+// 16 bits (act' and dg are taken at it: an error of half a step of z, as y's own
+// rounding is one of y), and dz is rounded to 16 bits as the two products'
+// operand; db is summed from dz before that rounding.
+//
+// The products run on the tiles of hier_gemm.h; at most 64 rows of x on a kernel
+// that streams the weights past them.
+#include "hier_gemm.h"
+
+#include <algorithm>
+
+namespace hier {
+namespace {
+
+using gemm::f32x16;
+using gemm::u32x4;
+
+// ---- epilogue ------------------------------------------------------------------
+
+struct Epilogue {
+  const void* bias;
+  const void* residual;
+  const void* gate;
+  void* out;
+  void* preact;
+  float* partial;          // fp32 [splits][M][ld_part]: sums alone, no epilogue
+  int64_t residual_ss, gate_ss, out_ss, preact_ss, ld_part, part_stride;
+  uint32_t rows_per_gate;
+  int32_t act;
+  bool vec;                // 16-byte accesses of every row
+};
+
+__device__ __forceinline__ float sigmoid(float x) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
+}
+
+// tanh GELU as z sigmoid(2u), u = sqrt(2/pi) (z + 0.044715 z^3): no cancellation
+// where z is far below 0.
+constexpr float kGeluA = 1.5957691216057308f, kGeluB = 0.044715f;   // 2 sqrt(2/pi)
+
+__device__ __forceinline__ void activate8(float* v, int act) {
+  if (act == HIER_ACT_GELU_TANH) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= sigmoid(kGeluA * v[i] * fmaf(kGeluB, v[i] * v[i], 1.f));
+  } else if (act == HIER_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= sigmoid(v[i]);
+  } else if (act == HIER_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= 0.5f * erfcf(-0.7071067811865476f * v[i]);
+  }
+}
+
+// act(z) and act'(z).  Past |z| = 30 the slopes are 0 or 1 to fp32: z is kept
+// there, so no square of it overflows into inf * 0.
+__device__ __forceinline__ void activate2(float z, int act, float& a, float& slope) {
+  const float c = fminf(fmaxf(z, -30.f), 30.f);
+  switch (act) {
+    case HIER_ACT_GELU_TANH: {
+      const float s = sigmoid(kGeluA * c * fmaf(kGeluB, c * c, 1.f));
+      a = z * s;
+      slope = s + c * s * (1.f - s) * kGeluA * fmaf(3.f * kGeluB, c * c, 1.f);
+      return;
+    }
+    case HIER_ACT_GELU: {
+      const float half = 0.5f * erfcf(-0.7071067811865476f * z);
+      a = z * half;
+      slope = half + c * 0.3989422804014327f * __builtin_amdgcn_exp2f(-0.7213475204444817f * c * c);
+      return;
+    }
+    case HIER_ACT_SILU: {
+      const float w = fminf(fmaxf(z, -100.f), 100.f), s = sigmoid(w);
+      a = z * s;
+      slope = s + w * s * (1.f - s);
+      return;
+    }
+    default: a = z; slope = 1.f;
+  }
+}
+
+// Eight neighbouring channels n .. n + 8 of 16 bits; those past N read as 0.
+template <typename T>
+__device__ __forceinline__ void row8(const void* p, int64_t at, int n, int N, bool vec, float* f) {
+  const T* q = static_cast<const T*>(p) + at + n;
+  if (vec) {
+    widen<T>(*reinterpret_cast<const w32x4*>(q), f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = n + i < N ? (float)q[i] : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void put8(void* p, int64_t at, int n, int N, bool vec, const float* f) {
+  T* q = static_cast<T*>(p) + at + n;
+  if (vec) {
+    *reinterpret_cast<w32x4*>(q) = narrow<T>(f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (n + i < N) q[i] = (T)f[i];
+  }
+}
+
+// What the epilogue of eight channels of a row reads besides the sums.
+struct Extras {
+  float gate[8], residual[8];
+};
+
+template <typename T>
+__device__ __forceinline__ void load_extras(const Epilogue& e, bool vec, Extras& x, int64_t m, uint32_t grow,
+                                            int n, int N) {
+  if (e.gate) row8<T>(e.gate, (int64_t)grow * e.gate_ss, n, N, vec, x.gate);
+  if (e.residual) row8<T>(e.residual, m * e.residual_ss, n, N, vec, x.residual);
+}
+
+template <typename T>
+__device__ __forceinline__ void epilogue8(const Epilogue& e, bool vec, float* v, const float* bias,
+                                          const Extras& x, int64_t m, int n, int N) {
+  if (e.bias)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += bias[i];
+  if (e.preact) put8<T>(e.preact, m * e.preact_ss, n, N, vec, v);
+  activate8(v, e.act);
+  if (e.gate)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= x.gate[i];
+  if (e.residual)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += x.residual[i];
+  put8<T>(e.out, m * e.out_ss, n, N, vec, v);
+}
+
+// The whole epilogue of eight channels of one row.
+template <typename T>
+__device__ __forceinline__ void finish8(const Epilogue& e, float* v, int64_t m, int n, int N) {
+  Extras x;
+  float bias[8];
+  if (e.bias) row8<T>(e.bias, 0, n, N, e.vec, bias);
+  load_extras<T>(e, e.vec, x, m, e.gate ? (uint32_t)m / e.rows_per_gate : 0u, n, N);
+  epilogue8<T>(e, e.vec, v, bias, x, m, n, N);
+}
+
+// ---- products over LDS tiles -----------------------------------------------------
+
+struct GemmArgs {
+  const void* a;
+  const void* b;
+  int64_t lda, ldb, M, N, K;
+  int64_t kchunk;              // K of a split, a multiple of the tile's
+  int32_t tm, tn, splits, total;
+  Epilogue e;
+};
+
+template <typename T, bool ATR, bool BTR, int BM, int BN, int BK, int S, int WG>
+__global__ __launch_bounds__(256, WG) void gemm_kernel(GemmArgs g) {
+  typedef gemm::Product<T, ATR, BTR, BM, BN, BK, S> P;
+  __shared__ __align__(1024) char lds[P::LDS];
+  const int logical = xcd_logical(blockIdx.x, gridDim.x);
+  if (logical >= g.total) return;
+  const int split = logical / (g.tm * g.tn);
+  int tm, tn;
+  gemm::tile_of(logical - split * g.tm * g.tn, g.tm, g.tn, tm, tn);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave & 1, wn = wave >> 1;
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+  const int64_t k0 = split * g.kchunk, k1 = min(k0 + g.kchunk, g.K);
+  typename P::A a;
+  typename P::B b;
+  a.init(g.a, g.lda, g.M, m0, k0, k1, wave, wm, lane);
+  b.init(g.b, g.ldb, g.N, n0, k0, k1, wave, wn, lane);
+  f32x16 acc[P::NI][P::MI];
+  P::run(acc, a, b, lds, k1 - k0, wave, wm, wn);
+
+  // The sums of MIP x 32 rows at a time through the wave's part of LDS (its
+  // stages are idle now), so that a row's channels are neighbours again: the
+  // loads and stores below are whole rows of the wave's part.  16-byte chunk
+  // c of row r sits at c ^ (r % 16) ^ (c / 16): neither side meets in a bank.
+  constexpr int NI = P::NI, MIP = P::LDS / 4 / (NI * 128) / 32, PITCH = NI * 128;
+  static_assert(P::MI % MIP == 0, "");
+  constexpr int LPR = NI * 4, RPI = 64 / LPR, ITS = MIP * 32 / RPI, BATCH = 4;
+  char* const mine = lds + wave * (P::LDS / 4);
+  const int N = (int)g.N, j = lane % LPR;
+  const int n = (int)n0 + wn * NI * 32 + 8 * j;
+  const bool vec = g.e.vec;
+  float bias[8];
+  if (g.splits == 1 && g.e.bias && n < N) row8<T>(g.e.bias, 0, n, N, vec, bias);
+#pragma unroll
+  for (int pass = 0; pass < P::MI / MIP; ++pass) {
+#pragma unroll
+    for (int mi = 0; mi < MIP; ++mi)
+#pragma unroll
+      for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int r = mi * 32 + (lane & 31), c = 8 * ni + 2 * q + (lane >> 5);
+          const f32x16& s = acc[ni][pass * MIP + mi];
+          *reinterpret_cast<f32x4*>(mine + r * PITCH + 16 * (c ^ (r & 15) ^ (c >> 4))) =
+              f32x4{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
+        }
+    const int64_t mp = m0 + (wm * P::MI + pass * MIP) * 32 + lane / LPR;
+    if (n < N)
+#pragma unroll 1
+    for (int it = 0; it < ITS; it += BATCH) {
+      Extras x[BATCH];
+      if (g.splits == 1)
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+          const int64_t m = min(mp + (it + k) * RPI, g.M - 1);
+          load_extras<T>(g.e, vec, x[k], m, g.e.gate ? (uint32_t)m / g.e.rows_per_gate : 0u, n, N);
+        }
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const int r = (it + k) * RPI + lane / LPR;
+        const int64_t m = mp + (it + k) * RPI;
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(
+            mine + r * PITCH + 16 * ((2 * j) ^ (r & 15) ^ (2 * j >> 4)));
+        const f32x4 hi = *reinterpret_cast<const f32x4*>(
+            mine + r * PITCH + 16 * ((2 * j + 1) ^ (r & 15) ^ (2 * j >> 4)));
+        if (m >= g.M) continue;
+        if (g.splits > 1) {
+          float* q = g.e.partial + split * g.e.part_stride + m * g.e.ld_part + n;
+          *reinterpret_cast<f32x4*>(q) = lo;
+          *reinterpret_cast<f32x4*>(q + 4) = hi;
+        } else {
+          float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          epilogue8<T>(g.e, vec, v, bias, x[k], m, n, N);
+        }
+      }
+    }
+  }
+}
+
+// The splits' sums in their order, and the epilogue.
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(GemmArgs g) {
+  const int cpr = (int)((g.N + 7) / 8);
+  const int64_t n8 = g.M * cpr;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n8; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / cpr;
+    const int n = 8 * (int)(i - m * cpr);
+    const float* p = g.e.partial + m * g.e.ld_part + n;
+    float v[8] = {};
+    for (int s = 0; s < g.splits; ++s) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(p + s * g.e.part_stride);
+      const f32x4 y = *reinterpret_cast<const f32x4*>(p + s * g.e.part_stride + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[j] += x[j];
+        v[4 + j] += y[j];
+      }
+    }
+    finish8<T>(g.e, v, m, n, (int)g.N);
+  }
+}
+
+// ---- few rows --------------------------------------------------------------------
+//
+// At most 64 rows of x: the weights are what is read, each once.  A workgroup of
+// eight waves takes 16 output channels, a wave every eighth 64-wide piece of K, with
+// its weights straight from memory into the MFMA's registers (16 rows x 32 k:
+// 16 bytes a lane), several pieces ahead; the eight sums meet in LDS.
+// v_mfma_f32_16x16x32: lane l holds row l % 16, k 8 (l / 16) .. + 8 of both operands,
+// and of the result row (channel) 4 (l / 16) + i, column (row of x) l % 16.
+
+typedef float acc4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+__device__ __forceinline__ acc4 mfma16(const u32x4& a, const u32x4& b, const acc4& c) {
+  const vec8<T> x = __builtin_bit_cast(vec8<T>, a), y = __builtin_bit_cast(vec8<T>, b);
+  if constexpr (__is_same(T, __bf16))
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0);
+}
+
+constexpr int kFewWaves = 8;
+constexpr int kFewAhead = 4;       // 32-wide pieces of K in flight
+
+template <typename T, int MT>      // MT groups of 16 rows of x
+__global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(GemmArgs g) {
+  __shared__ float sums[kFewWaves][MT][64 * 4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = lane & 15, kg = 8 * (lane >> 4);
+  const int64_t n0 = 16 * (int64_t)blockIdx.x;
+  const T* wp = static_cast<const T*>(g.b) + min(n0 + r, g.N - 1) * g.ldb + kg;
+  const T* xp[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+    xp[m] = static_cast<const T*>(g.a) + min((int64_t)(16 * m + r), g.M - 1) * g.lda + kg;
+  acc4 acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m] = acc4{0.f, 0.f, 0.f, 0.f};
+  // pieces of kFewAhead x 32 k, in turn over the waves
+  constexpr int PIECE = 32 * kFewAhead;
+  for (int64_t k0 = (int64_t)wave * PIECE; k0 < g.K; k0 += kFewWaves * PIECE) {
+    u32x4 w[kFewAhead], x[MT][kFewAhead];
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < kFewAhead; ++j) {
+      const int64_t k = k0 + 32 * j;
+      const bool in = k + kg < g.K;      // (K is a multiple of 8)
+      w[j] = in ? __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wp + k)) : zero;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) x[m][j] = in ? *reinterpret_cast<const u32x4*>(xp[m] + k) : zero;
+    }
+#pragma unroll
+    for (int j = 0; j < kFewAhead; ++j)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[m] = mfma16<T>(w[j], x[m][j], acc[m]);
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sums[wave][m][(lane & 15) * 16 + 4 * (lane >> 4) + i] = acc[m][i];
+  __syncthreads();
+  // thread: row t / 2 of x, eight channels
+  const int t = threadIdx.x;
+  if (t >= 32 * MT) return;
+  const int64_t m = t / 2;
+  const int n = (int)n0 + 8 * (t & 1);
+  if (m >= g.M || n >= g.N) return;
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) s += sums[w][m / 16][(m % 16) * 16 + 8 * (t & 1) + i];
+    v[i] = s;
+  }
+  finish8<T>(g.e, v, m, n, (int)g.N);
+}
+
+// ---- dz, db and dg ---------------------------------------------------------------
+//
+// One pass over dy and z, eight channels a thread.  A workgroup row takes `rows`
+// rows; where a gate's rows are more than that it takes `rows` rows of one gate
+// at most (dg's sums then meet in sum_rows), else whole gates.
+
+struct DzArgs {
+  const void* dy;
+  const void* z;
+  const void* gate;
+  void* dz;
+  void* dgate;
+  float* db_part;
+  float* dg_part;
+  int64_t dy_ss, z_ss, gate_ss, dz_ss;
+  int64_t M, rpg;              // rows of a gate (M without gates)
+  int64_t rows, segs;          // rows of a workgroup; its rows of a gate's, if split
+  int32_t N, act;
+  bool vec, split;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void dz_kernel(DzArgs d) {
+  const int n = 8 * (blockIdx.y * 256 + threadIdx.x);
+  if (n >= d.N) return;
+  const int64_t seg = blockIdx.x;
+  int64_t r0, r1;
+  if (d.split) {
+    const int64_t gr = seg / d.segs, s = seg - gr * d.segs;
+    r0 = gr * d.rpg + s * d.rows;
+    r1 = min(r0 + d.rows, min((gr + 1) * d.rpg, d.M));
+  } else {
+    r0 = seg * d.rows;
+    r1 = min(r0 + d.rows, d.M);
+  }
+  float db[8] = {}, dg[8] = {}, gate[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) gate[i] = 1.f;
+  int64_t g = r0 / d.rpg, gend = (g + 1) * d.rpg;
+  if (d.gate) row8<T>(d.gate, g * d.gate_ss, n, d.N, d.vec, gate);
+  constexpr int AHEAD = 4;
+  for (int64_t r = r0; r < r1; r += AHEAD) {
+    float y[AHEAD][8], z[AHEAD][8];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int64_t row = min(r + j, r1 - 1);
+      row8<T>(d.dy, row * d.dy_ss, n, d.N, d.vec, y[j]);
+      if (d.z) row8<T>(d.z, row * d.z_ss, n, d.N, d.vec, z[j]);
+      else
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[j][i] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (r + j >= r1) break;
+      if (r + j == gend) {          // the next gate's rows begin (whole gates only)
+        if (d.dgate) put8<T>(d.dgate, g * (int64_t)d.N, n, d.N, d.vec, dg);
+        ++g;
+        gend += d.rpg;
+        row8<T>(d.gate, g * d.gate_ss, n, d.N, d.vec, gate);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dg[i] = 0.f;
+      }
+      float dz[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float a, slope;
+        activate2(z[j][i], d.act, a, slope);
+        dg[i] = fmaf(y[j][i], a, dg[i]);
+        dz[i] = y[j][i] * gate[i] * slope;
+        db[i] += dz[i];
+      }
+      if (d.dz) put8<T>(d.dz, (r + j) * d.dz_ss, n, (int)d.dz_ss, true, dz);
+    }
+  }
+  if (d.db_part) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (n + i < d.N) d.db_part[seg * d.N + n + i] = db[i];
+  }
+  if (d.dgate) {
+    if (d.split) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (n + i < d.N) d.dg_part[seg * d.N + n + i] = dg[i];
+    } else {
+      put8<T>(d.dgate, g * (int64_t)d.N, n, d.N, d.vec, dg);
+    }
+  }
+}
+
+// ---- plans -----------------------------------------------------------------------
+
+// How a product is cut: tiles of 256 or 128, and K into `splits` parts.
+struct Plan {
+  int tile;
+  int splits;
+  int64_t kchunk;
+  int64_t bytes;      // fp32 parts
+};
+
+constexpr int kBK = 64;
+
+Plan plan_of(int64_t M, int64_t N, int64_t K) {
+  Plan best = {};
+  double least = 1e30;
+  const int64_t kt = (K + kBK - 1) / kBK;
+  for (int tile : {256, 128}) {
+    const int64_t tiles = ((M + tile - 1) / tile) * ((N + tile - 1) / tile);
+    const int64_t slots = tile == 256 ? 256 : 512;
+    for (int64_t splits = 1; splits <= 32 && splits <= kt; ++splits) {
+      const int64_t per = (kt + splits - 1) / splits;
+      if ((kt + per - 1) / per != splits) continue;
+      // time in units of a 256-tile's 64 k: rounds of workgroups, each with a
+      // start and an end worth four of them; parts written and read again
+      const double rounds = (double)((tiles * splits + slots - 1) / slots);
+      const double step = tile == 256 ? 1.0 : 0.6;
+      double t = rounds * (per * step + 4);
+      if (splits > 1) t += 4 + 1e-6 * (double)(splits * M * N) * 2.0;
+      if (t < least) {
+        least = t;
+        best.tile = tile;
+        best.splits = (int)splits;
+        best.kchunk = per * kBK;
+        best.bytes = splits > 1 ? splits * M * ((N + 7) / 8 * 8) * 4 : 0;
+      }
+    }
+  }
+  return best;
+}
+
+template <typename T, bool ATR, bool BTR>
+int launch_gemm(GemmArgs g, const Plan& p, float* ws, hipStream_t st) {
+  g.tm = (int)((g.M + p.tile - 1) / p.tile);
+  g.tn = (int)((g.N + p.tile - 1) / p.tile);
+  g.splits = p.splits;
+  g.kchunk = p.kchunk;
+  const int64_t total = (int64_t)g.tm * g.tn * g.splits;
+  HIER_REQUIRE(total <= (1ll << 23), HIER_EUNSUPPORTED, "product: too many tiles");
+  g.total = (int)total;
+  g.e.partial = ws;
+  g.e.ld_part = (g.N + 7) / 8 * 8;
+  g.e.part_stride = g.M * g.e.ld_part;
+  const dim3 grid((unsigned)xcd_grid(total));
+  if (p.tile == 256)
+    hipLaunchKernelGGL((gemm_kernel<T, ATR, BTR, 256, 256, kBK, 2, 1>), grid, dim3(256), 0, st, g);
+  else
+    hipLaunchKernelGGL((gemm_kernel<T, ATR, BTR, 128, 128, kBK, 2, 2>), grid, dim3(256), 0, st, g);
+  if (int rc = check_launch("gemm_kernel")) return rc;
+  if (p.splits > 1) {
+    const int64_t n8 = g.M * ((g.N + 7) / 8);
+    hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)std::min<int64_t>((n8 + 255) / 256, 8192)),
+                       dim3(256), 0, st, g);
+    return check_launch("join_kernel");
+  }
+  return HIER_OK;
+}
+
+template <typename T>
+int launch_few(const GemmArgs& g, hipStream_t st) {
+  const dim3 grid((unsigned)((g.N + 15) / 16)), block(64 * kFewWaves);
+  if (g.M <= 16) hipLaunchKernelGGL((few_rows_kernel<T, 1>), grid, block, 0, st, g);
+  else if (g.M <= 32) hipLaunchKernelGGL((few_rows_kernel<T, 2>), grid, block, 0, st, g);
+  else hipLaunchKernelGGL((few_rows_kernel<T, 4>), grid, block, 0, st, g);
+  return check_launch("few_rows_kernel");
+}
+
+bool few_rows(int64_t M) { return M <= 64; }
+
+// Views that the copies address: 16-byte rows, a tile's rows (256) within 31
+// bits of bytes.
+int check_view(const char* who, const void* p, int64_t ld, int64_t cols) {
+  HIER_REQUIRE(p != nullptr && aligned16(p), HIER_EINVAL, "linear: %s must be a 16-byte aligned pointer", who);
+  HIER_REQUIRE(ld % 8 == 0 && (ld >= cols || ld == 0), HIER_EINVAL,
+               "linear: %s needs a row stride of a multiple of 8, at least its columns", who);
+  HIER_REQUIRE(ld < (1ll << 21), HIER_EUNSUPPORTED, "linear: %s: row stride of 2M elements or more", who);
+  return HIER_OK;
+}
+
+int check_sizes(int64_t M, int64_t N, int64_t K, int type, int act) {
+  HIER_REQUIRE(M >= 0 && N >= 1 && K >= 1, HIER_EINVAL, "linear: invalid M=%lld N=%lld K=%lld", (long long)M,
+               (long long)N, (long long)K);
+  HIER_REQUIRE(M < (1ll << 31) && N < (1 << 21) && K < (1 << 21), HIER_EUNSUPPORTED, "linear: too large");
+  HIER_REQUIRE(type == HIER_BF16 || type == HIER_FP16, HIER_EUNSUPPORTED, "linear: bf16 or fp16");
+  HIER_REQUIRE(act >= HIER_ACT_NONE && act <= HIER_ACT_SILU, HIER_EINVAL, "linear: unknown activation %d", act);
+  return HIER_OK;
+}
+
+int check_gate(const void* gate, int64_t rows_per_gate) {
+  HIER_REQUIRE(!gate || (rows_per_gate >= 1 && rows_per_gate < (1ll << 31)), HIER_EINVAL,
+               "linear: invalid rows_per_gate=%lld", (long long)rows_per_gate);
+  return HIER_OK;
+}
+
+// The rows of a workgroup of dz_kernel: enough of them to fill the card eight
+// waves a SIMD pair, at most 128 rows.
+struct DzPlan {
+  int64_t rows, segs, total;
+  bool split;
+};
+DzPlan dz_plan(int64_t M, int64_t N, int64_t rpg, bool gated) {
+  const int64_t lanes = (N + 7) / 8;
+  int64_t rows = std::max<int64_t>(4, std::min<int64_t>(128, M * lanes / 131072));
+  DzPlan p;
+  p.split = gated && rpg > rows;
+  if (p.split) {
+    p.segs = (rpg + rows - 1) / rows;
+    p.rows = (rpg + p.segs - 1) / p.segs;
+    p.total = (M / rpg) * p.segs;
+  } else {
+    if (gated) rows = rows / rpg * rpg;
+    p.rows = rows;
+    p.segs = 1;
+    p.total = (M + rows - 1) / rows;
+  }
+  return p;
+}
+
+int64_t round16(int64_t b) { return (b + 255) / 256 * 256; }
+
+struct BwdPlan {
+  Plan dx, dw;
+  DzPlan dz;
+  int64_t off_dz, off_db, off_dg, off_part, bytes;
+};
+// dz is dy itself where there is neither an activation nor a gate.
+bool dz_is_dy(const HierLinearBwdArgs& a) { return a.act == HIER_ACT_NONE && !a.gate; }
+
+BwdPlan bwd_plan(const HierLinearBwdArgs& a) {
+  BwdPlan p = {};
+  const int64_t Np = (a.N + 7) / 8 * 8;
+  p.dz = dz_plan(a.M, a.N, a.gate ? a.rows_per_gate : std::max<int64_t>(a.M, 1), a.gate != nullptr);
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += round16(bytes);
+    return o;
+  };
+  p.off_dz = dz_is_dy(a) ? 0 : take(a.M * Np * 2);
+  p.off_db = a.db ? take(p.dz.total * a.N * 4) : 0;
+  p.off_dg = a.dgate && p.dz.split ? take(p.dz.total * a.N * 4) : 0;
+  int64_t parts = 0;
+  if (a.dx) {
+    p.dx = plan_of(a.M, a.K, a.N);
+    parts = std::max(parts, p.dx.bytes);
+  }
+  if (a.dw) {
+    p.dw = plan_of(a.N, a.K, a.M);
+    parts = std::max(parts, p.dw.bytes);
+  }
+  p.off_part = take(parts);
+  p.bytes = at;
+  return p;
+}
+
+}  // namespace
+}  // namespace hier
+
+using namespace hier;
+
+static int check_linear(const HierLinearArgs& a) {
+  if (int rc = check_sizes(a.M, a.N, a.K, a.type, a.act)) return rc;
+  HIER_REQUIRE(a.K % 8 == 0, HIER_EINVAL, "linear: K must be a multiple of 8, got %d", a.K);
+  return check_gate(a.gate, a.rows_per_gate);
+}
+
+extern "C" int64_t hier_linear_workspace(const HierLinearArgs* a) {
+  clear_error();
+  if (!a || check_linear(*a)) return -1;
+  return a->M == 0 || few_rows(a->M) ? 0 : plan_of(a->M, a->N, a->K).bytes;
+}
+
+extern "C" int hier_linear(const HierLinearArgs* args, void* stream) {
+  clear_error();
+  HIER_REQUIRE(args != nullptr, HIER_EINVAL, "args is NULL");
+  const HierLinearArgs& a = *args;
+  if (int rc = check_linear(a)) return rc;
+  if (a.M == 0) return HIER_OK;
+  if (int rc = check_view("x", a.x, a.x_ss, a.K)) return rc;
+  if (int rc = check_view("weight", a.w, a.w_ss, a.K)) return rc;
+  HIER_REQUIRE(a.out != nullptr, HIER_EINVAL, "linear: NULL output");
+  HIER_REQUIRE(a.out_ss >= a.N && (!a.preact || a.preact_ss >= a.N) && (!a.residual || a.residual_ss >= 0) &&
+                   (!a.gate || a.gate_ss >= 0),
+               HIER_EINVAL, "linear: invalid row stride");
+  GemmArgs g = {};
+  g.a = a.x;
+  g.b = a.w;
+  g.lda = a.x_ss;
+  g.ldb = a.w_ss;
+  g.M = a.M;
+  g.N = a.N;
+  g.K = a.K;
+  Epilogue& e = g.e;
+  e.bias = a.bias;
+  e.residual = a.residual;
+  e.gate = a.gate;
+  e.out = a.out;
+  e.preact = a.preact;
+  e.residual_ss = a.residual_ss;
+  e.gate_ss = a.gate_ss;
+  e.out_ss = a.out_ss;
+  e.preact_ss = a.preact_ss;
+  e.rows_per_gate = a.gate ? (uint32_t)a.rows_per_gate : 1u;
+  e.act = a.act;
+  auto ok = [](const void* p, int64_t ss) { return !p || (aligned16(p) && ss % 8 == 0); };
+  e.vec = a.N % 8 == 0 && ok(a.bias, 0) && ok(a.residual, a.residual_ss) && ok(a.gate, a.gate_ss) &&
+          ok(a.out, a.out_ss) && ok(a.preact, a.preact_ss);
+  const hipStream_t st = (hipStream_t)stream;
+  if (few_rows(a.M)) return a.type == HIER_BF16 ? launch_few<__bf16>(g, st) : launch_few<_Float16>(g, st);
+  const Plan p = plan_of(a.M, a.N, a.K);
+  HIER_REQUIRE(p.bytes == 0 || (a.workspace && aligned16(a.workspace) && a.workspace_bytes >= p.bytes),
+               HIER_EINVAL, "linear: workspace of %lld bytes needed", (long long)p.bytes);
+  float* ws = static_cast<float*>(a.workspace);
+  return a.type == HIER_BF16 ? launch_gemm<__bf16, false, false>(g, p, ws, st)
+                             : launch_gemm<_Float16, false, false>(g, p, ws, st);
+}
+
+static int check_linear_bwd(const HierLinearBwdArgs& a) {
+  if (int rc = check_sizes(a.M, a.N, a.K, a.type, a.act)) return rc;
+  HIER_REQUIRE(a.M >= 1, HIER_EINVAL, "linear_bwd: no rows");
+  HIER_REQUIRE(a.K % 8 == 0, HIER_EINVAL, "linear_bwd: K must be a multiple of 8, got %d", a.K);
+  HIER_REQUIRE(!a.dgate || a.gate, HIER_EINVAL, "linear_bwd: dgate without a gate");
+  HIER_REQUIRE(!a.gate || (a.rows_per_gate >= 1 && a.M % a.rows_per_gate == 0), HIER_EINVAL,
+               "linear_bwd: %lld rows are not a multiple of rows_per_gate=%lld", (long long)a.M,
+               (long long)a.rows_per_gate);
+  return HIER_OK;
+}
+
+extern "C" int64_t hier_linear_bwd_workspace(const HierLinearBwdArgs* a) {
+  clear_error();
+  if (!a || check_linear_bwd(*a)) return -1;
+  return bwd_plan(*a).bytes;
+}
+
+template <typename T>
+static int linear_bwd(const HierLinearBwdArgs& a, const BwdPlan& p, hipStream_t st) {
+  char* ws = static_cast<char*>(a.workspace);
+  const int64_t Np = (a.N + 7) / 8 * 8;
+  const bool plain = dz_is_dy(a), products = a.dx || a.dw;
+  const void* dz = plain ? a.dy : ws + p.off_dz;
+  const int64_t dz_ss = plain ? a.dy_ss : Np;
+  if ((!plain && products) || a.db || a.dgate) {
+    DzArgs d = {};
+    d.dy = a.dy;
+    d.z = a.preact;
+    d.gate = a.gate;
+    d.dz = plain || !products ? nullptr : ws + p.off_dz;
+    d.dgate = a.dgate;
+    d.db_part = a.db ? reinterpret_cast<float*>(ws + p.off_db) : nullptr;
+    d.dg_part = reinterpret_cast<float*>(ws + p.off_dg);
+    d.dy_ss = a.dy_ss;
+    d.z_ss = a.preact_ss;
+    d.gate_ss = a.gate_ss;
+    d.dz_ss = Np;
+    d.M = a.M;
+    d.rpg = a.gate ? a.rows_per_gate : a.M;
+    d.rows = p.dz.rows;
+    d.segs = p.dz.segs;
+    d.N = a.N;
+    d.act = a.act;
+    d.split = p.dz.split;
+    auto ok = [](const void* q, int64_t ss) { return !q || (aligned16(q) && ss % 8 == 0); };
+    d.vec = a.N % 8 == 0 && ok(a.dy, a.dy_ss) && ok(a.preact, a.preact_ss) && ok(a.gate, a.gate_ss) &&
+            ok(a.dgate, 0);
+    const int64_t gy = (Np / 8 + 255) / 256;
+    HIER_REQUIRE(gy <= 65535 && p.dz.total < (1ll << 24), HIER_EUNSUPPORTED, "linear_bwd: too many rows");
+    hipLaunchKernelGGL(dz_kernel<T>, dim3((unsigned)p.dz.total, (unsigned)gy), dim3(256), 0, st, d);
+    if (int rc = check_launch("dz_kernel")) return rc;
+    if (a.db)
+      if (int rc = sum_rows(d.db_part, p.dz.total, 1, a.N, a.db, a.type, st)) return rc;
+    if (a.dgate && p.dz.split)
+      if (int rc = sum_rows(d.dg_part, p.dz.segs, a.M / a.rows_per_gate, a.N, a.dgate, a.type, st)) return rc;
+  }
+  float* parts = reinterpret_cast<float*>(ws + p.off_part);
+  auto product = [&](int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, const void* B, int64_t ldb,
+                     void* out, int64_t out_ss) {
+    GemmArgs g = {};
+    g.a = A;
+    g.b = B;
+    g.lda = lda;
+    g.ldb = ldb;
+    g.M = M;
+    g.N = N;
+    g.K = K;
+    g.e.out = out;
+    g.e.out_ss = out_ss;
+    g.e.rows_per_gate = 1;
+    g.e.vec = N % 8 == 0 && aligned16(out) && out_ss % 8 == 0;
+    return g;
+  };
+  if (a.dx)
+    if (int rc = launch_gemm<T, false, true>(
+            product(a.M, a.K, a.N, dz, dz_ss, a.w, a.w_ss, a.dx, a.dx_ss), p.dx, parts, st))
+      return rc;
+  if (a.dw)
+    return launch_gemm<T, true, true>(product(a.N, a.K, a.M, dz, dz_ss, a.x, a.x_ss, a.dw, a.dw_ss), p.dw,
+                                      parts, st);
+  return HIER_OK;
+}
+
+extern "C" int hier_linear_bwd(const HierLinearBwdArgs* args, void* stream) {
+  clear_error();
+  HIER_REQUIRE(args != nullptr, HIER_EINVAL, "args is NULL");
+  const HierLinearBwdArgs& a = *args;
+  if (int rc = check_linear_bwd(a)) return rc;
+  HIER_REQUIRE(a.dy != nullptr && a.dy_ss >= 0, HIER_EINVAL, "linear_bwd: invalid dy");
+  HIER_REQUIRE(a.preact || (a.act == HIER_ACT_NONE && !a.dgate), HIER_EINVAL,
+               "linear_bwd: needs the values before the activation");
+  HIER_REQUIRE(!a.preact || a.preact_ss >= a.N, HIER_EINVAL, "linear_bwd: invalid row stride");
+  if (a.dx)
+    if (int rc = check_view("weight", a.w, a.w_ss, a.K)) return rc;
+  if (a.dw)
+    if (int rc = check_view("x", a.x, a.x_ss, a.K)) return rc;
+  if (dz_is_dy(a) && (a.dx || a.dw)) {
+    if (int rc = check_view("dy", a.dy, a.dy_ss, a.N)) return rc;
+    HIER_REQUIRE(a.N % 8 == 0, HIER_EINVAL, "linear_bwd: dy needs a multiple of 8 columns");
+  }
+  HIER_REQUIRE((!a.dx || a.dx_ss >= a.K) && (!a.dw || a.dw_ss >= a.K), HIER_EINVAL,
+               "linear_bwd: invalid output stride");
+  const BwdPlan p = bwd_plan(a);
+  HIER_REQUIRE(p.bytes == 0 || (a.workspace && aligned16(a.workspace) && a.workspace_bytes >= p.bytes),
+               HIER_EINVAL, "linear_bwd: workspace of %lld bytes needed", (long long)p.bytes);
+  return a.type == HIER_BF16 ? linear_bwd<__bf16>(a, p, (hipStream_t)stream)
+                             : linear_bwd<_Float16>(a, p, (hipStream_t)stream);
+}

@@ -17,6 +17,8 @@ import torch
 
 from . import _capi
 from . import metadata as M
+from .block import (linear_act, linear_act_backward, linear_act_train, rms_norm,  # noqa: F401
+                    rms_norm_backward, rms_norm_train)
 from .metadata import HierTiledBlockLayout, TileList, backward_lists, folded_key_list
 
 
