@@ -800,6 +800,50 @@ typedef struct HierLinearBwdArgs {
 int64_t hier_linear_bwd_workspace(const HierLinearBwdArgs* args);
 int hier_linear_bwd(const HierLinearBwdArgs* args, void* stream);
 
+/* Attention of Sq queries to Sk keys of another sequence, D 64 or 128:      */
+/*   o = softmax(scale q k^T over the seen keys) v, 0 for a row that sees none */
+/* Query heads i * Hq/Hk .. share key head i.  kv_lens (int32 [B], NULL: all  */
+/* Sk; taken within [0, Sk]) counts a stream's keys, key_mask (bytes, NULL: */
+/* all) says which are seen; the rest of k and v is not read.  16-byte rows, */
+/* k_ss and v_ss at least D.  lse: fp32 [B][Hq][Sq] or NULL, -inf where no key */
+/* is seen.  `workspace` (hier_cross_workspace(args) bytes, 16-byte aligned)  */
+/* belongs to one call at a time.                                            */
+typedef struct HierCrossArgs {
+  int32_t B, Hq, Hk, D;
+  int32_t type;
+  float scale;
+  int64_t Sq, Sk;
+  const void* q;                   /* [B][Sq][Hq][D] by strides                */
+  const void* k;                   /* [B][Sk][Hk][D]                           */
+  const void* v;
+  void* o;                         /* [B][Sq][Hq][D]                           */
+  float* lse;
+  const int32_t* kv_lens;
+  const uint8_t* key_mask;         /* [B][Sk]                                  */
+  int64_t q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, o_sb, o_ss, o_sh;
+  int64_t mask_sb;
+  void* workspace;
+  int64_t workspace_bytes;
+} HierCrossArgs;
+
+int64_t hier_cross_workspace(const HierCrossArgs* args);     /* -1: invalid    */
+int hier_cross_attn(const HierCrossArgs* args, void* stream);
+
+/* Its gradients dq, dk, dv (bf16) from the forward's arguments, o and lse and */
+/* the gradient of o.  Every row of them is written (0 for a key that is not  */
+/* seen).  Deterministic.                                                    */
+typedef struct HierCrossBwdArgs {
+  HierCrossArgs f;                 /* f.o is read; f.workspace is used         */
+  const void* dout;                /* [B][Sq][Hq][D] by strides                */
+  void* dq;
+  void* dk;
+  void* dv;
+  int64_t do_sb, do_ss, do_sh, dq_sb, dq_ss, dq_sh, dk_sb, dk_ss, dk_sh, dv_sb, dv_ss, dv_sh;
+} HierCrossBwdArgs;
+
+int64_t hier_cross_bwd_workspace(const HierCrossArgs* args); /* -1: invalid    */
+int hier_cross_attn_bwd(const HierCrossBwdArgs* args, void* stream);
+
 /* Last error message of the calling thread ("" if none).                    */
 const char* hier_last_error(void);
 

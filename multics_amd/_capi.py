@@ -227,13 +227,32 @@ class HierLinearBwdArgs(C.Structure):
                [("workspace", vp), ("workspace_bytes", i64)]
 
 
+class HierCrossArgs(C.Structure):
+    _fields_ = [(n, i32) for n in ("B", "Hq", "Hk", "D", "type")] + \
+               [("scale", f32), ("Sq", i64), ("Sk", i64)] + \
+               [(n, vp) for n in ("q", "k", "v", "o", "lse", "kv_lens", "key_mask")] + \
+               [(n, i64) for n in ("q_sb", "q_ss", "q_sh", "k_sb", "k_ss", "k_sh", "v_sb", "v_ss", "v_sh",
+                                   "o_sb", "o_ss", "o_sh", "mask_sb")] + \
+               [("workspace", vp), ("workspace_bytes", i64)]
+
+
+class HierCrossBwdArgs(C.Structure):
+    _fields_ = [("f", HierCrossArgs)] + [(n, vp) for n in ("dout", "dq", "dk", "dv")] + \
+               [(n, i64) for n in ("do_sb", "do_ss", "do_sh", "dq_sb", "dq_ss", "dq_sh", "dk_sb", "dk_ss",
+                                   "dk_sh", "dv_sb", "dv_ss", "dv_sh")]
+
+
+def _formats(cls) -> str:
+    codes = {i32: "i", i64: "q", f32: "f", vp: "Q"}
+    return "".join(codes.get(t) or _formats(t) for _, t in cls._fields_)
+
+
 def packer(cls):
     """A function from the fields' values, in order, to the structure's bytes
     (pointers as addresses, 0 for NULL): a quarter of the time that filling
     the ctypes structure takes.  The entries that take it declare their
     argument ``c_void_p``, which reads a ``bytes`` object in place."""
-    fmt = struct.Struct("@" + "".join({i32: "i", i64: "q", f32: "f", vp: "Q"}[t]
-                                      for _, t in cls._fields_))
+    fmt = struct.Struct("@" + _formats(cls))
     if fmt.size != C.sizeof(cls):
         raise AssertionError(f"{cls.__name__}: packed {fmt.size} bytes, C {C.sizeof(cls)}")
     return fmt.pack
@@ -273,12 +292,16 @@ EXPORTS = {
     "hier_linear": [vp, vp],
     "hier_linear_bwd_workspace": [vp],
     "hier_linear_bwd": [vp, vp],
+    "hier_cross_workspace": [vp],
+    "hier_cross_attn": [vp, vp],
+    "hier_cross_bwd_workspace": [vp],
+    "hier_cross_attn_bwd": [vp, vp],
     "hier_last_error": [],
     "hier_version": [],
 }
 
 _SIZES = ("hier_derive_workspace", "hier_rms_norm_bwd_rows", "hier_linear_workspace",
-          "hier_linear_bwd_workspace")        # entries that return a size
+          "hier_linear_bwd_workspace", "hier_cross_workspace", "hier_cross_bwd_workspace")        # entries that return a size
 
 _lock = threading.Lock()
 _lib = None

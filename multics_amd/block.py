@@ -358,3 +358,171 @@ def linear_act_train(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     """``linear_act`` under autograd: differentiable in every tensor.  The same
     arguments and results."""
     return LinearActFunction.apply(x, weight, bias, residual, gate, activation)
+
+
+# --------------------------------------------------------------------------
+# attention to an encoder's states
+# --------------------------------------------------------------------------
+
+_pack_cross = _capi.packer(_capi.HierCrossArgs)
+_pack_cross_bwd = _capi.packer(_capi.HierCrossBwdArgs)
+
+
+def _heads(t: torch.Tensor):
+    """``t`` [B, S, H, D] readable in 16-byte rows (copied if it is not), and its
+    strides over streams, tokens and heads (0 over one alone)."""
+    B, S, H, D = t.shape
+    for _ in range(2):
+        sb, ss, sh, unit = t.stride()
+        sb, ss, sh = sb if B > 1 else 0, ss if S > 1 else 0, sh if H > 1 else 0
+        if unit == 1 and sb % 8 == 0 and ss % 8 == 0 and sh % 8 == 0 and t.data_ptr() % 16 == 0 and \
+                (ss >= D or S < 2) and 65 * ss + H * sh < 1 << 30:
+            break
+        t = _capi.aligned(t)
+    return t, (sb, ss, sh)
+
+
+def _cross_args(q, k, v, kv_lens, key_mask, scale):
+    """Checked arguments of the cross attention: (sizes and scale, q, k, v with their strides, lens,
+    mask)."""
+    kind = _gpu_type("q", q)
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be [B, S, H, D], got {tuple(t.shape)}")
+    B, Sq, Hq, D = q.shape
+    Sk, Hk = k.shape[1], k.shape[2]
+    _like("k", k, q, (B, Sk, Hk, D))
+    _like("v", v, q, (B, Sk, Hk, D))
+    if D not in (64, 128):
+        raise NotImplementedError(f"cross attention supports head_dim 64/128, got {D}")
+    if Hk < 1 or Hq < 1 or Hq % Hk:
+        raise ValueError(f"{Hq} query heads are not a multiple of {Hk} key heads")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError(f"the softmax scale must be positive, got {scale}")
+    if kv_lens is not None:
+        if kv_lens.shape != (B,) or kv_lens.dtype not in (torch.int32, torch.int64) or kv_lens.device != q.device:
+            raise ValueError(f"kv_lens must be int32 [{B}] on {q.device}, got {kv_lens.dtype} "
+                             f"{tuple(kv_lens.shape)} on {kv_lens.device}")
+        if kv_lens.dtype == torch.int64:
+            kv_lens = kv_lens.clamp(0, Sk).to(torch.int32)
+        kv_lens = kv_lens.contiguous()
+    if key_mask is not None:
+        if key_mask.shape != (B, Sk) or key_mask.dtype != torch.bool or key_mask.device != q.device:
+            raise ValueError(f"key_mask must be bool {(B, Sk)} on {q.device}, got {key_mask.dtype} "
+                             f"{tuple(key_mask.shape)} on {key_mask.device}")
+        if key_mask.stride(1) != 1 and Sk > 1:
+            key_mask = key_mask.contiguous()
+    return (B, Hq, Hk, D, kind, scale, Sq, Sk), _heads(q), _heads(k), _heads(v), kv_lens, key_mask
+
+
+def _cross_fields(sizes, q, k, v, o, lse, lens, mask):
+    (qt, qs), (kt, ks), (vt, vs), (ot, os) = q, k, v, o
+    return (*sizes, qt.data_ptr(), kt.data_ptr(), vt.data_ptr(), ot.data_ptr(), _ptr(lse), _ptr(lens), _ptr(mask),
+            *qs, *ks, *vs, *os, 0 if mask is None else mask.stride(0))
+
+
+def _check_lse(lse, sizes, device):
+    B, Hq, _, _, _, _, Sq, _ = sizes
+    if lse.shape != (B, Hq, Sq) or lse.dtype != torch.float32 or lse.device != device or not lse.is_contiguous():
+        raise ValueError(f"lse must be contiguous fp32 {(B, Hq, Sq)} on {device}, got {lse.dtype} "
+                         f"{tuple(lse.shape)} on {lse.device}")
+
+
+def _cross(q, k, v, kv_lens, key_mask, scale, out, lse):
+    sizes, qh, kh, vh, lens, mask = _cross_args(q, k, v, kv_lens, key_mask, scale)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _like("out", out, q, q.shape)
+    oh = _heads(out)
+    B, Hq, _, D, _, _, Sq, _ = sizes
+    if oh[0] is not out or any(n > 1 and s < D for n, s in zip((B, Sq, Hq), oh[1])):
+        raise ValueError("out must have rows of its own, a unit-stride head dimension and 16-byte rows")
+    if lse is not None:
+        _check_lse(lse, sizes, q.device)
+    if B == 0 or Sq == 0:
+        return out
+    fields = _cross_fields(sizes, qh, kh, vh, oh, lse, lens, mask)
+    size = _workspace("hier_cross_workspace", _pack_cross(*fields, 0, 0))
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    _capi.call_on(q.device, "hier_cross_attn", _pack_cross(*fields, _ptr(ws), size))
+    return out
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_lens: Optional[torch.Tensor] = None,
+                    key_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``softmax(scale * q k^T) v`` over another sequence's keys (``hier_cross_attn``).
+
+    ``q`` [B, Sq, H, D] and ``k`` / ``v`` [B, Sk, Hk, D] are bf16 or fp16 views
+    (unit-stride channels, D 64 or 128; others are copied), H a multiple of Hk:
+    query heads i * H/Hk .. share key head i.  A stream's keys are the first
+    ``kv_lens[b]`` (int32 [B] on the GPU, taken within [0, Sk]) whose ``key_mask``
+    [B, Sk] (bool) is true; what else k and v hold is not read.  Returns [B, Sq, H, D]
+    (``out`` where given); a row that sees no key is 0.  ``lse`` (optional, contiguous
+    fp32 [B, H, Sq]) receives the natural-log softmax normaliser, -inf for such a
+    row.  Sq may be one token: the keys are then cut into parts that fill the GPU.
+    No gradient: ``cross_attention_train``."""
+    _no_grad_call("cross_attention", q, k, v)
+    return _cross(q, k, v, kv_lens, key_mask, scale, out, lse)
+
+
+def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                             out: torch.Tensor, lse: torch.Tensor, *, kv_lens: Optional[torch.Tensor] = None,
+                             key_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None):
+    """Gradients ``(dq, dk, dv)`` of ``cross_attention`` (``hier_cross_attn_bwd``) from its
+    inputs, its ``out`` and ``lse`` and the gradient ``dout`` of out; bf16.  dk and dv are
+    summed over the query heads that share a head and 0 for keys that are not seen.
+    Sums are taken in a fixed order: equal inputs give equal bits."""
+    sizes, qh, kh, vh, lens, mask = _cross_args(q, k, v, kv_lens, key_mask, scale)
+    if q.dtype != torch.bfloat16:
+        raise NotImplementedError(f"cross attention's gradients are bf16 only, got {q.dtype}")
+    _like("out", out, q, q.shape)
+    _like("dout", dout, q, q.shape)
+    _check_lse(lse, sizes, q.device)
+    B, _, _, _, _, _, Sq, Sk = sizes
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    if B == 0 or Sq == 0 or Sk == 0:
+        return dq.zero_(), dk.zero_(), dv.zero_()
+    oh, (dot, dos) = _heads(out), _heads(dout)
+    fields = _cross_fields(sizes, qh, kh, vh, oh, lse, lens, mask)
+    size = _workspace("hier_cross_bwd_workspace", _pack_cross(*fields, 0, 0))
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+    strides = lambda t: t.stride()[:3]  # noqa: E731
+    _capi.call_on(q.device, "hier_cross_attn_bwd", _pack_cross_bwd(
+        *fields, ws.data_ptr(), size, dot.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *dos,
+        *strides(dq), *strides(dk), *strides(dv)))
+    return dq, dk, dv
+
+
+class CrossAttentionFunction(torch.autograd.Function):
+    """Differentiable ``cross_attention``."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, kv_lens, key_mask, scale):
+        if q.dtype != torch.bfloat16 and any(ctx.needs_input_grad):
+            raise NotImplementedError(f"cross attention's gradients are bf16 only, got {q.dtype}")
+        if q.dim() != 4:
+            raise ValueError(f"q must be [B, S, H, D], got {tuple(q.shape)}")
+        B, Sq, H, _ = q.shape
+        lse = torch.empty((B, H, Sq), dtype=torch.float32, device=q.device)
+        out = _cross(q, k, v, kv_lens, key_mask, scale, None, lse)
+        ctx.save_for_backward(q, k, v, out, lse, kv_lens, key_mask)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, kv_lens, key_mask = ctx.saved_tensors
+        grads = cross_attention_backward(dout, q, k, v, out, lse, kv_lens=kv_lens, key_mask=key_mask,
+                                         scale=ctx.scale)
+        return *grads, None, None, None
+
+
+def cross_attention_train(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
+                          kv_lens: Optional[torch.Tensor] = None, key_mask: Optional[torch.Tensor] = None,
+                          scale: Optional[float] = None) -> torch.Tensor:
+    """``cross_attention`` under autograd: differentiable in q, k and v (bf16)."""
+    return CrossAttentionFunction.apply(q, k, v, kv_lens, key_mask, scale)

@@ -17,8 +17,9 @@ import torch
 
 from . import _capi
 from . import metadata as M
-from .block import (linear_act, linear_act_backward, linear_act_train, rms_norm,  # noqa: F401
-                    rms_norm_backward, rms_norm_train)
+from .block import (cross_attention, cross_attention_backward,  # noqa: F401
+                    cross_attention_train, linear_act, linear_act_backward, linear_act_train,
+                    rms_norm, rms_norm_backward, rms_norm_train)
 from .metadata import HierTiledBlockLayout, TileList, backward_lists, folded_key_list
 
 
