@@ -331,7 +331,8 @@ class LinearActFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, gate, activation):
-        keep = activation is not None or gate is not None and ctx.needs_input_grad[4]
+        keep = any(ctx.needs_input_grad) and (activation is not None or
+                                              gate is not None and ctx.needs_input_grad[4])
         z = torch.empty((*x.shape[:-1], weight.shape[0]), dtype=x.dtype, device=x.device) if keep else None
         y = _linear(x, weight, bias, activation, residual, gate, None, z)
         ctx.save_for_backward(x, weight, gate, z)

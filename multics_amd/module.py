@@ -37,9 +37,10 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import metadata as M
-from .kernels import (_attn_out, gated_residual, hier_attention, hier_attention_forward,
-                      hier_cached_attention_fp8, qk_head_prologue, qk_head_prologue_train,
-                      qk_prologue_train, qkv_prologue)
+from .kernels import (_attn_out, cross_attention, cross_attention_train, gated_residual,
+                      hier_attention, hier_attention_forward, hier_cached_attention_fp8, linear_act,
+                      linear_act_train, qk_head_prologue, qk_head_prologue_train,
+                      qk_prologue_train, qkv_prologue, rms_norm, rms_norm_train)
 from .hier_masks import HierBlockMask
 from .kv_cache import stream_pool
 from .paged_cache import HierPagedKVCache
@@ -85,6 +86,103 @@ class CompatibleLinear(nn.Linear):
         super().__init__(in_features, out_features, bias=bias, device=device, dtype=dtype)
         self.output_chunk_size = output_chunk_size
         self.input_alignment = input_alignment
+
+
+class FeedForward(nn.Sequential):
+    """The block's feed-forward: ``Linear(dim, hidden), GELU(tanh), Linear(hidden, dim)``
+    with a sequential's state-dict keys (``0.weight`` .. ``2.bias``).  ``residual`` and
+    ``gate`` (``[..., dim]``; ``[dim]`` or per frame ``[..., F, dim]``, as for
+    ``GateModule``) join in the second product: ``residual + gate * ffn(x)``.  bf16 and
+    fp16 GPU tensors run on ``kernels.linear_act``, with and without autograd."""
+
+    def __init__(self, dim: int, hidden_dim: int, bias: bool = True):
+        super().__init__(nn.Linear(dim, hidden_dim, bias=bias), nn.GELU(approximate="tanh"),
+                         nn.Linear(hidden_dim, dim, bias=bias))
+
+    def forward(self, x, *, residual=None, gate=None):
+        up, down = self[0], self[2]
+        if _block_ok(x, up.weight):
+            linear = linear_act_train if torch.is_grad_enabled() else linear_act
+            h = linear(x, up.weight, up.bias, activation="gelu_tanh")
+            return linear(h, down.weight, down.bias, residual=residual, gate=gate)
+        return _gated(super().forward(x), residual, gate)
+
+
+def _block_ok(x, weight) -> bool:
+    """Whether the block's kernels take ``x`` and the module's weights."""
+    return x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and weight.dtype == x.dtype
+
+
+def _gated(y, residual, gate):
+    if gate is not None:
+        if gate.dim() > 1 and gate.shape[-2] != y.shape[-2]:
+            gate = gate.repeat_interleave(y.shape[-2] // gate.shape[-2], dim=-2)
+        y = gate * y
+    return y if residual is None else residual + y
+
+
+class CrossAttention(nn.Module):
+    """Attention of the block's tokens to an encoder's states (the text's), with the
+    reference's parameters (``q, k, v, o, norm_q, norm_k``; multics/models/attention.py:1046-1088).
+
+    ``forward(x, context)``: x [B, S, dim], context [B, Sc, dim].  ``kv_lens`` (int32 [B]) or
+    ``key_mask`` (bool [B, Sc]) leave out padded states; ``residual`` and ``gate`` join in the
+    o-projection, ``residual + gate * attention``.  A rollout projects its context once,
+    ``kv = attn.project_context(context)``, and passes ``kv=kv`` in its place.  bf16 and fp16
+    GPU tensors with head_dim 64 or 128 run on ``kernels.rms_norm``,
+    ``kernels.cross_attention`` and ``kernels.linear_act`` (fp16 without gradient), others on
+    torch operations."""
+
+    def __init__(self, dim: int, num_heads: int, eps: float = 1e-6):
+        super().__init__()
+        if dim % num_heads:
+            raise ValueError(f"{dim} channels do not divide into {num_heads} heads")
+        self.dim, self.num_heads, self.head_dim = dim, num_heads, dim // num_heads
+        self.q = nn.Linear(dim, dim)
+        self.k = nn.Linear(dim, dim)
+        self.v = nn.Linear(dim, dim)
+        self.o = nn.Linear(dim, dim)
+        self.norm_q = RMSNorm(dim, eps=eps)
+        self.norm_k = RMSNorm(dim, eps=eps)
+
+    def _fused(self, x) -> bool:
+        return _block_ok(x, self.q.weight) and self.head_dim in (64, 128) and \
+            not (x.dtype == torch.float16 and torch.is_grad_enabled())
+
+    def _heads(self, t):
+        return t.unflatten(-1, (self.num_heads, self.head_dim))
+
+    def _norm(self, norm, t):
+        if not self._fused(t):
+            return norm(t)
+        call = rms_norm_train if torch.is_grad_enabled() else rms_norm
+        return call(t, norm.weight, eps=norm.eps)
+
+    def project_context(self, context):
+        """(k, v) [B, Sc, H, D] of a context, for ``forward(kv=)``."""
+        return self._heads(self._norm(self.norm_k, self.k(context))), self._heads(self.v(context))
+
+    def forward(self, x, context=None, *, kv=None, kv_lens=None, key_mask=None, residual=None, gate=None):
+        if (context is None) == (kv is None):
+            raise ValueError("pass context or kv (from project_context)")
+        k, v = self.project_context(context) if kv is None else kv
+        q = self._heads(self._norm(self.norm_q, self.q(x)))
+        if self._fused(x):
+            grad = torch.is_grad_enabled()
+            attend = cross_attention_train if grad else cross_attention
+            y = attend(q, k, v, kv_lens=kv_lens, key_mask=key_mask).flatten(-2)
+            if residual is None and gate is None:
+                return self.o(y)
+            return (linear_act_train if grad else linear_act)(y, self.o.weight, self.o.bias, residual=residual,
+                                                              gate=gate)
+        seen = None if key_mask is None else key_mask[:, None, None]
+        if kv_lens is not None:
+            within = (torch.arange(k.shape[1], device=x.device) < kv_lens[:, None])[:, None, None]
+            seen = within if seen is None else seen & within
+        y = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), attn_mask=seen)
+        if seen is not None:            # a row that sees no key is 0
+            y = torch.where(seen.any(-1, keepdim=True), y, torch.zeros((), dtype=y.dtype, device=y.device))
+        return _gated(self.o(y.transpose(1, 2).flatten(-2)), residual, gate)
 
 
 def rope_apply(x: torch.Tensor, freqs: torch.Tensor, num_heads: int) -> torch.Tensor:

@@ -1,0 +1,160 @@
+"""The block's operators without a GPU: what their C entries and Python calls refuse, and the
+modules' torch path."""
+
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from multics_amd import _capi, kernels
+from multics_amd.module import CrossAttention, FeedForward
+
+AT = 1 << 20             # an aligned address that nothing reads: the calls refuse before a launch
+
+
+def _norm(**kw):
+    f = dict(M=4, C=64, eps=1e-6, type=0, gain_type=2, x=AT, w=AT, y=AT, x_ss=64, y_ss=64)
+    return _capi.HierRmsNormArgs(**{**f, **kw})
+
+
+def _linear(**kw):
+    f = dict(M=100, N=48, K=64, type=0, act=0, x=AT, w=AT, out=AT, x_ss=64, w_ss=64, out_ss=48, rows_per_gate=1)
+    return _capi.HierLinearArgs(**{**f, **kw})
+
+
+def _linear_bwd(**kw):
+    f = dict(M=100, N=48, K=64, type=0, act=0, x=AT, w=AT, dy=AT, dx=AT, dw=AT, x_ss=64, w_ss=64, dy_ss=48,
+             dx_ss=64, dw_ss=64, rows_per_gate=1)
+    return _capi.HierLinearBwdArgs(**{**f, **kw})
+
+
+def _cross(**kw):
+    f = dict(B=2, Hq=4, Hk=2, D=64, type=0, scale=0.125, Sq=1000, Sk=9, q=AT, k=AT, v=AT, o=AT, lse=AT,
+             q_sb=256000, q_ss=256, q_sh=64, k_sb=1152, k_ss=128, k_sh=64, v_sb=1152, v_ss=128, v_sh=64,
+             o_sb=256000, o_ss=256, o_sh=64)
+    return _capi.HierCrossArgs(**{**f, **kw})
+
+
+REFUSED = [
+    ("hier_rms_norm", _norm, dict(C=0), "invalid"),
+    ("hier_rms_norm", _norm, dict(C=16385, x_ss=16385, y_ss=16385), "16384"),
+    ("hier_rms_norm", _norm, dict(type=2), "bf16 or fp16"),
+    ("hier_rms_norm", _norm, dict(gain_type=7), "gain"),
+    ("hier_rms_norm", _norm, dict(eps=float("nan")), "eps"),
+    ("hier_rms_norm", _norm, dict(eps=-1.0), "eps"),
+    ("hier_rms_norm", _norm, dict(x=None), "NULL"),
+    ("hier_rms_norm", _norm, dict(r=AT), "NULL"),
+    ("hier_rms_norm", _norm, dict(y_ss=8), "stride"),
+    ("hier_linear", _linear, dict(K=60), "multiple of 8"),
+    ("hier_linear", _linear, dict(N=0), "invalid"),
+    ("hier_linear", _linear, dict(act=9), "activation"),
+    ("hier_linear", _linear, dict(type=2), "bf16 or fp16"),
+    ("hier_linear", _linear, dict(x=AT + 2), "aligned"),
+    ("hier_linear", _linear, dict(w_ss=60), "stride"),
+    ("hier_linear", _linear, dict(x_ss=1 << 21), "stride"),
+    ("hier_linear", _linear, dict(out=None), "NULL"),
+    ("hier_linear", _linear, dict(out_ss=40), "stride"),
+    ("hier_linear", _linear, dict(gate=AT, rows_per_gate=0), "rows_per_gate"),
+    ("hier_linear", _linear, dict(M=200, N=64, K=1 << 16, x_ss=1 << 16, w_ss=1 << 16, out_ss=64), "workspace"),
+    ("hier_linear_bwd", _linear_bwd, dict(act=1), "before the activation"),
+    ("hier_linear_bwd", _linear_bwd, dict(N=44, dy_ss=48), "multiple of 8"),
+    ("hier_linear_bwd", _linear_bwd, dict(dgate=AT), "without a gate"),
+    ("hier_linear_bwd", _linear_bwd, dict(gate=AT, rows_per_gate=33, preact=AT, preact_ss=48), "rows_per_gate"),
+    ("hier_linear_bwd", _linear_bwd, dict(dy=None), "dy"),
+    ("hier_linear_bwd", _linear_bwd, dict(dx_ss=8), "stride"),
+    ("hier_linear_bwd", _linear_bwd, dict(db=AT), "workspace"),
+    ("hier_cross_attn", _cross, dict(D=32), "head_dim"),
+    ("hier_cross_attn", _cross, dict(Hq=5), "invalid"),
+    ("hier_cross_attn", _cross, dict(type=2), "bf16 or fp16"),
+    ("hier_cross_attn", _cross, dict(scale=0.0), "scale"),
+    ("hier_cross_attn", _cross, dict(scale=float("nan")), "scale"),
+    ("hier_cross_attn", _cross, dict(q=AT + 8), "aligned"),
+    ("hier_cross_attn", _cross, dict(k_ss=60), "16-byte rows"),
+    ("hier_cross_attn", _cross, dict(k_ss=32), "overlap"),
+    ("hier_cross_attn", _cross, dict(k_ss=1 << 23), "stride"),
+    ("hier_cross_attn", _cross, dict(o_ss=0), "rows of its own"),
+    ("hier_cross_attn", _cross, dict(v=None), "NULL"),
+    ("hier_cross_attn", _cross, dict(Sk=512), "workspace"),
+    ("hier_cross_attn", _cross, dict(Sq=1 << 30), "too many"),
+]
+
+
+@pytest.mark.parametrize("name,make,change,says", REFUSED)
+def test_entries_refuse(name, make, change, says):
+    args = make(**change)
+    rc = getattr(_capi.lib(), name)(C.addressof(args), None)
+    assert rc < 0
+    assert says in _capi.lib().hier_last_error().decode()
+
+
+@pytest.mark.parametrize("change,says", [
+    (dict(type=1), "bf16 only"), (dict(lse=None), "NULL"), (dict(q_sh=1 << 29), "too large"),
+    (dict(), "workspace")])
+def test_cross_gradient_entry_refuses(change, says):
+    args = _capi.HierCrossBwdArgs(f=_cross(**change), dout=AT, dq=AT, dk=AT, dv=AT, do_sb=256000, do_ss=256, do_sh=64,
+                                  dq_sb=256000, dq_ss=256, dq_sh=64, dk_sb=1152, dk_ss=128, dk_sh=64, dv_sb=1152,
+                                  dv_ss=128, dv_sh=64)
+    assert _capi.lib().hier_cross_attn_bwd(C.addressof(args), None) < 0
+    assert says in _capi.lib().hier_last_error().decode()
+
+
+def test_entries_refuse_null():
+    for name in ("hier_rms_norm", "hier_rms_norm_bwd", "hier_linear", "hier_linear_bwd", "hier_cross_attn",
+                 "hier_cross_attn_bwd"):
+        assert getattr(_capi.lib(), name)(None, None) == (_capi.HIER_EINVAL)
+    for name in ("hier_rms_norm_bwd_rows", "hier_linear_workspace", "hier_linear_bwd_workspace",
+                 "hier_cross_workspace", "hier_cross_bwd_workspace"):
+        assert getattr(_capi.lib(), name)(None) == -1
+
+
+def test_nothing_to_do_is_done():
+    for name, args in (("hier_rms_norm", _norm(M=0)), ("hier_linear", _linear(M=0)), ("hier_cross_attn", _cross(B=0)),
+                       ("hier_cross_attn", _cross(Sq=0))):
+        assert getattr(_capi.lib(), name)(C.addressof(args), None) == 0
+
+
+def test_host_tensors_are_refused():
+    x, w = torch.zeros(2, 64, dtype=torch.bfloat16), torch.zeros(32, 64, dtype=torch.bfloat16)
+    q = torch.zeros(1, 2, 1, 64, dtype=torch.bfloat16)
+    for call in (lambda: kernels.rms_norm(x, w[0], eps=1e-6), lambda: kernels.linear_act(x, w),
+                 lambda: kernels.cross_attention(q, q, q)):
+        with pytest.raises(NotImplementedError):
+            call()
+    with pytest.raises(RuntimeError):
+        kernels.linear_act(x.requires_grad_(), w)
+
+
+def test_division_of_rows():
+    """The magic numbers of a row's query, r / G, for every group of heads up to 300."""
+    for g in range(2, 301):
+        shift = max(0, math.ceil(math.log2(g)) - 1)
+        mul = (1 << (32 + shift)) // g + 1
+        assert mul < 1 << 32
+        for r in [*range(0, 5 * g), (1 << 30) - 1, (1 << 30) - g, (1 << 30) // g * g, (1 << 30) // g * g - 1]:
+            assert (r * mul >> 32) >> shift == r // g, (g, r)
+
+
+def test_modules_on_the_host():
+    """The torch path: parameters, masks, a stream without keys, gates, a kept context."""
+    torch.manual_seed(0)
+    attn, ffn = CrossAttention(32, 2).double(), FeedForward(32, 64).double()
+    assert {k.split(".")[0] for k in attn.state_dict()} == {"q", "k", "v", "o", "norm_q", "norm_k"}
+    assert set(ffn.state_dict()) == {"0.weight", "0.bias", "2.weight", "2.bias"}
+    x, ctx = torch.randn(3, 6, 32).double(), torch.randn(3, 5, 32).double()
+    lens = torch.tensor([5, 2, 0], dtype=torch.int32)
+    y = attn(x, ctx, kv_lens=lens)
+    assert torch.allclose(y[1:2], attn(x[1:2], ctx[1:2, :2]), atol=1e-5)
+    assert torch.allclose(y[2], attn.o.bias.expand(6, 32))
+    mask = torch.arange(5) < lens[:, None]
+    assert torch.allclose(attn(x, ctx, key_mask=mask), y)
+    assert torch.allclose(attn(x, kv=attn.project_context(ctx), kv_lens=lens), y)
+    gate = torch.randn(3, 2, 32).double()
+    full = gate.repeat_interleave(3, 1)
+    assert torch.allclose(attn(x, ctx, kv_lens=lens, residual=x, gate=gate), x + full * y)
+    assert torch.allclose(ffn(x, residual=x, gate=gate),
+                          x + full * ffn[2](torch.nn.functional.gelu(ffn[0](x), approximate="tanh")))
+    with pytest.raises(ValueError):
+        attn(x)
+    with pytest.raises(ValueError):
+        CrossAttention(30, 4)
