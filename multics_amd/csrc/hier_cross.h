@@ -27,23 +27,6 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRows = 128;           // rows of a work item (forward, dQ), keys of one (dK, dV)
 
-// Division of row numbers below 2^31 by the heads of a group, g >= 1:
-// r / g = (r * mul) >> (32 + shift), mul = floor(2^(32 + shift) / g) + 1 with
-// shift = ceil(log2 g) - 1; g = 1 needs none.
-struct Div {
-  uint32_t g, mul, shift;
-};
-inline Div make_div(uint32_t g) {
-  Div d = {g, 0u, 0u};
-  if (g == 1) return d;
-  while ((1ull << (d.shift + 1)) < g) ++d.shift;
-  d.mul = (uint32_t)((1ull << (32 + d.shift)) / g + 1);
-  return d;
-}
-__device__ __forceinline__ uint32_t quotient(uint32_t r, const Div& d) {
-  return d.g == 1 ? r : __umulhi(r, d.mul) >> d.shift;
-}
-
 // Rows of 64 to a tile of LDS, S the read pattern's swizzle: the lane's offsets
 // from the tile's first row.
 template <int D, int S>

@@ -127,6 +127,11 @@ struct Operand {
     base += step;
     left -= step;
   }
+  // No more tiles: the copies write zeros.
+  __device__ __forceinline__ void end() {
+    left = 0;
+    step = 0;
+  }
 
   // Operand of block b and step k from the tile at `t`: lane l holds row
   // 32 b + l % 32, k = 16 k + 8 (l / 32) .. + 8.
@@ -144,6 +149,10 @@ struct Operand {
 
 // acc[ni][mi]: 32 x 32 blocks, lane l holds row m = 32 mi + l % 32 and
 // n = 32 ni + 8 (r / 4) + 4 (l / 32) + r % 4 of the wave's part.
+//
+// The K tiles of a workgroup's work items are one stream: while an item is
+// multiplied, and while its results go out, the copies run ahead into the next
+// (`Next` sets the operands to it), so only the first one waits for memory.
 template <typename T, bool ATR, bool BTR, int BM, int BN, int BK, int S>
 struct Product {
   typedef Operand<ATR, BM, BK> A;
@@ -152,53 +161,69 @@ struct Product {
   static constexpr int STAGE = A::BYTES + B::BYTES;
   static constexpr int LDS = S * STAGE;
   static constexpr int COPIES = A::COPIES + B::COPIES;
-  static constexpr int READS = MI + NI;
+  static constexpr int READS = MI + NI, NM = NI * MI;
+  // A tile's copies are made in the first SPREAD steps after its stage is free
+  // (the last step of one tile, the first of the next ..): the workgroup's copies
+  // leave at about the rate that the CU's address unit takes them (one 1 KiB copy in
+  // 16 cycles), and land before the tile after next needs them.  8192^3: in one
+  // step 1,184 TFLOP/s, in two 1,234, in three 1,189, in all four 1,118.
+  static constexpr int SPREAD = 2;
+  static constexpr int FIRST = (COPIES + SPREAD - 1) / SPREAD;
   static_assert(KK % 2 == 0 && S >= 2, "");
 
-  static __device__ __forceinline__ void run(f32x16 (&acc)[NI][MI], A& a, B& b, char* lds, int64_t K,
-                                             int wave, int wm, int wn) {
-    (void)wm;
-    (void)wn;
-    const uint32_t l0 = (uint32_t)(uintptr_t)lds;
-    const int nt = (int)((K + BK - 1) / BK);
-#pragma unroll
-    for (int n = 0; n < NI; ++n)
-#pragma unroll
-      for (int m = 0; m < MI; ++m)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[n][m][i] = 0.f;
-    int kleft = (int)(K < (1 << 30) ? K : (1 << 30));   // (only its being less than a tile matters)
-    int64_t kall = K;
-    uint32_t fill = 0;      // stage that the next tile is copied to
-    auto copy_one = [&](int j) {
-      if (j < A::COPIES) a.copy(j, kleft, l0 + fill, wave);
-      else b.copy(j - A::COPIES, kleft, l0 + fill + A::BYTES, wave);
-    };
-    auto copied = [&]() {
-      a.next();
-      b.next();
-      kall -= BK;
-      kleft = (int)(kall < (1 << 30) ? (kall > 0 ? kall : 0) : (1 << 30));
-      fill = fill + STAGE == LDS ? 0 : fill + STAGE;
-    };
+  A a;
+  B b;
+  int64_t kall;           // K left of the item that is being copied
+  int kleft;              // the same, at most 2^30
+  uint32_t l0, fill;      // LDS address, stage that the next tile goes to
+  const char* lds;
+  const char* cur;        // stage of the present tile
+  int wave;
+  u32x4 fa[2][MI], fb[2][NI];
+
+  __device__ __forceinline__ void item(int64_t K) {
+    kall = K;
+    kleft = (int)(K < (1 << 30) ? K : (1 << 30));
+  }
+  __device__ __forceinline__ void copy_one(int j) {
+    if (j < A::COPIES) a.copy(j, kleft, l0 + fill, wave);
+    else b.copy(j - A::COPIES, kleft, l0 + fill + A::BYTES, wave);
+  }
+  template <typename Next>
+  __device__ __forceinline__ void copied(Next& next) {
+    a.next();
+    b.next();
+    fill = fill + STAGE == LDS ? 0 : fill + STAGE;
+    item(kall - BK);
+    if (kall <= 0) next();
+  }
+  __device__ __forceinline__ void read_one(const char* t, int k, int par, int i) {
+    if (i < NI) fb[par][i] = b.read(t + A::BYTES, i, k);
+    else fa[par][i - NI] = a.read(t, i - NI, k);
+  }
+
+  // a, b and the first item set: the first tiles on their way, the first one's
+  // first operands read.
+  template <typename Next>
+  __device__ __forceinline__ void start(char* base, int w, Next& next) {
+    lds = cur = base;
+    l0 = (uint32_t)(uintptr_t)base;
+    fill = 0;
+    wave = w;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
 #pragma unroll
-      for (int j = 0; j < COPIES; ++j) copy_one(j);
-      copied();
+      for (int j = 0; j < (s < S - 1 ? COPIES : FIRST); ++j) copy_one(j);
+      if (SPREAD == 1 || s < S - 1) copied(next);
     }
-    wait_barrier<(S - 1) * COPIES>();
-    u32x4 fa[2][MI], fb[2][NI];
-    auto read_one = [&](const char* t, int k, int par, int i) {
-      // A and B in turn, in the order that the MFMAs take them
-      if (i < NI) fb[par][i] = b.read(t + A::BYTES, i, k);
-      else fa[par][i - NI] = a.read(t, i - NI, k);
-    };
-    const char* cur = lds;
+    wait_barrier<(S - 2) * COPIES + FIRST>();
 #pragma unroll
     for (int i = 0; i < READS; ++i) read_one(cur, 0, 0, i);
+  }
 
-    constexpr int NM = NI * MI;                       // MFMAs of a step
+  // acc += the item's product, nt tiles of K.
+  template <typename Next>
+  __device__ __forceinline__ void run(f32x16 (&acc)[NI][MI], int nt, Next& next) {
     for (int t = 0; t < nt; ++t) {
 #pragma unroll
       for (int k = 0; k < KK; ++k) {
@@ -209,17 +234,16 @@ struct Product {
           cur = cur + STAGE == lds + LDS ? lds : cur + STAGE;
           from = cur;
         }
-        const int kn = last ? 0 : k + 1;
-        int reads = 0, copies = 0;
+        const int kn = last ? 0 : k + 1, part = last ? 0 : k + 1;
+        int reads = 0, copies = min(part * FIRST, COPIES);
 #pragma unroll
         for (int i = 0; i < NM; ++i) {
-          // spread the next step's reads and, in the last step, the copies
-          // between the MFMAs
+          // the next step's reads and the copies spread between the MFMAs
           const int want_r = ((i + 1) * READS + NM - 1) / NM;
 #pragma unroll
           for (; reads < want_r; ++reads) read_one(from, kn, (k + 1) & 1, reads);
-          if (last) {
-            const int want_c = ((i + 1) * COPIES + NM - 1) / NM;
+          if (part < SPREAD) {
+            const int want_c = min(COPIES, part * FIRST + ((i + 1) * FIRST + NM - 1) / NM);
 #pragma unroll
             for (; copies < want_c; ++copies) copy_one(copies);
           }
@@ -227,11 +251,9 @@ struct Product {
           acc[n][m] = mfma<T>(fb[k & 1][n], fa[k & 1][m], acc[n][m]);
           __builtin_amdgcn_sched_barrier(0);
         }
-        if (last) copied();
+        if (part == SPREAD - 1) copied(next);
       }
     }
-    // nothing of this tile's may land in LDS after it is used again
-    wait_barrier<0>();
   }
 };
 

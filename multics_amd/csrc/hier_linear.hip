@@ -14,6 +14,8 @@
 #include "hier_gemm.h"
 
 #include <algorithm>
+#include <type_traits>
+#include <utility>
 
 namespace hier {
 namespace {
@@ -31,9 +33,8 @@ struct Epilogue {
   void* preact;
   float* partial;          // fp32 [splits][M][ld_part]: sums alone, no epilogue
   int64_t residual_ss, gate_ss, out_ss, preact_ss, ld_part, part_stride;
-  uint32_t rows_per_gate;
+  Div rows_per_gate;
   int32_t act;
-  bool vec;                // 16-byte accesses of every row
 };
 
 __device__ __forceinline__ float sigmoid(float x) {
@@ -84,66 +85,66 @@ __device__ __forceinline__ void activate2(float z, int act, float& a, float& slo
   }
 }
 
-// Eight neighbouring channels n .. n + 8 of 16 bits; those past N read as 0.
+// Eight neighbouring channels of 16 bits, at any even address (the hardware takes
+// 16-byte accesses there).
 template <typename T>
-__device__ __forceinline__ void row8(const void* p, int64_t at, int n, int N, bool vec, float* f) {
-  const T* q = static_cast<const T*>(p) + at + n;
-  if (vec) {
-    widen<T>(*reinterpret_cast<const w32x4*>(q), f);
+__device__ __forceinline__ w32x4 raw8(const void* p, int64_t at) {
+  w32x4 w;
+  __builtin_memcpy(&w, static_cast<const T*>(p) + at, 16);
+  return w;
+}
+template <typename T>
+__device__ __forceinline__ void put8(void* p, int64_t at, const float* f) {
+  const w32x4 w = narrow<T>(f);
+  __builtin_memcpy(static_cast<T*>(p) + at, &w, 16);
+}
+// The same where fewer than eight are left: zeros behind, which are not written.
+template <typename T>
+__device__ __forceinline__ void row8(const void* p, int64_t at, int n, int N, float* f) {
+  if (n + 8 <= N) {
+    widen<T>(raw8<T>(p, at + n), f);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = n + i < N ? (float)q[i] : 0.f;
+    for (int i = 0; i < 8; ++i) f[i] = n + i < N ? (float)static_cast<const T*>(p)[at + n + i] : 0.f;
   }
 }
 template <typename T>
-__device__ __forceinline__ void put8(void* p, int64_t at, int n, int N, bool vec, const float* f) {
-  T* q = static_cast<T*>(p) + at + n;
-  if (vec) {
-    *reinterpret_cast<w32x4*>(q) = narrow<T>(f);
+__device__ __forceinline__ void put_row8(void* p, int64_t at, int n, int N, const float* f) {
+  if (n + 8 <= N) {
+    put8<T>(p, at + n, f);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (n + i < N) q[i] = (T)f[i];
+      if (n + i < N) static_cast<T*>(p)[at + n + i] = (T)f[i];
   }
 }
 
-// What the epilogue of eight channels of a row reads besides the sums.
-struct Extras {
-  float gate[8], residual[8];
-};
-
-template <typename T>
-__device__ __forceinline__ void load_extras(const Epilogue& e, bool vec, Extras& x, int64_t m, uint32_t grow,
-                                            int n, int N) {
-  if (e.gate) row8<T>(e.gate, (int64_t)grow * e.gate_ss, n, N, vec, x.gate);
-  if (e.residual) row8<T>(e.residual, m * e.residual_ss, n, N, vec, x.residual);
-}
-
-template <typename T>
-__device__ __forceinline__ void epilogue8(const Epilogue& e, bool vec, float* v, const float* bias,
-                                          const Extras& x, int64_t m, int n, int N) {
-  if (e.bias)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += bias[i];
-  if (e.preact) put8<T>(e.preact, m * e.preact_ss, n, N, vec, v);
-  activate8(v, e.act);
-  if (e.gate)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= x.gate[i];
-  if (e.residual)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += x.residual[i];
-  put8<T>(e.out, m * e.out_ss, n, N, vec, v);
+__device__ __forceinline__ uint32_t gate_row(const Epilogue& e, int64_t m) {
+  return e.gate ? quotient((uint32_t)m, e.rows_per_gate) : 0u;
 }
 
 // The whole epilogue of eight channels of one row.
 template <typename T>
 __device__ __forceinline__ void finish8(const Epilogue& e, float* v, int64_t m, int n, int N) {
-  Extras x;
-  float bias[8];
-  if (e.bias) row8<T>(e.bias, 0, n, N, e.vec, bias);
-  load_extras<T>(e, e.vec, x, m, e.gate ? (uint32_t)m / e.rows_per_gate : 0u, n, N);
-  epilogue8<T>(e, e.vec, v, bias, x, m, n, N);
+  float t[8];
+  if (e.bias) {
+    row8<T>(e.bias, 0, n, N, t);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += t[i];
+  }
+  if (e.preact) put_row8<T>(e.preact, m * e.preact_ss, n, N, v);
+  activate8(v, e.act);
+  if (e.gate) {
+    row8<T>(e.gate, (int64_t)gate_row(e, m) * e.gate_ss, n, N, t);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= t[i];
+  }
+  if (e.residual) {
+    row8<T>(e.residual, m * e.residual_ss, n, N, t);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += t[i];
+  }
+  put_row8<T>(e.out, m * e.out_ss, n, N, v);
 }
 
 // ---- products over LDS tiles -----------------------------------------------------
@@ -157,84 +158,256 @@ struct GemmArgs {
   Epilogue e;
 };
 
-template <typename T, bool ATR, bool BTR, int BM, int BN, int BK, int S, int WG>
+// What a launch's epilogue needs: kPlain has neither gate nor residual, kExtra may
+// have them; both take 16-byte rows.  kAny takes any.
+enum { kPlain, kExtra, kAny };
+
+// Rows of a tile in one of the epilogue's tensors.  Buffer accesses: one out of
+// range is a row or column that is not there, with no branch around it, so the
+// compiler knows how many accesses are on their way and a load is not waited for
+// with the stores behind it.
+struct View {
+  __amdgpu_buffer_rsrc_t rsrc;
+  __device__ __forceinline__ void init(const void* p, int64_t at) {
+    rsrc = __builtin_amdgcn_make_buffer_rsrc((char*)p + at, 0, 0x7fffffff, 0x00020000);
+  }
+  __device__ __forceinline__ u32x4 load(uint32_t off) const {
+    return __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, 0);
+  }
+  __device__ __forceinline__ void store(const u32x4& v, uint32_t off) const {
+    __builtin_amdgcn_raw_buffer_store_b128(v, rsrc, off, 0, 0);
+  }
+};
+
+// Pass K's sums (32 rows, COLS x 32 channels) into the wave's part of LDS.
+template <int K, int NI, int MI, int COLS>
+__device__ __forceinline__ void put_sums_of(const f32x16 (&acc)[NI][MI], char* mine, int lane) {
+  constexpr int HALVES = NI / COLS, mi = K / HALVES, ni = K % HALVES * COLS;
+  const int r = lane & 31;
+#pragma unroll
+  for (int c = 0; c < COLS; ++c)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x16& s = acc[ni + c][mi];
+      *reinterpret_cast<f32x4*>(mine + r * (COLS * 128) +
+                                16 * ((8 * c + 2 * q + (lane >> 5)) ^ (r % (8 * COLS)))) =
+          f32x4{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
+    }
+  // (unlike in every pass: with their ends merged, the passes would choose their sums by address)
+  asm volatile("; pass %0" :: "i"(K) : "memory");
+}
+// The pass by number: registers cannot be chosen by one, hence a test for each.  (The
+// passes are a loop: unrolled they would not fit the instruction cache.)
+template <int NI, int MI, int COLS, int... K>
+__device__ __forceinline__ void put_sums(const f32x16 (&acc)[NI][MI], char* mine, int lane, int pass,
+                                         std::integer_sequence<int, K...>) {
+  ((pass == K ? put_sums_of<K, NI, MI, COLS>(acc, mine, lane) : (void)0), ...);
+}
+
+// Workgroups in flight: one a CU (WG of them); each takes its XCD's items in
+// turn, the XCD's workgroups neighbouring ones.
+constexpr int kSlots = 256;
+
+template <typename T, bool ATR, bool BTR, int BM, int BN, int BK, int S, int WG, int KIND>
 __global__ __launch_bounds__(256, WG) void gemm_kernel(GemmArgs g) {
   typedef gemm::Product<T, ATR, BTR, BM, BN, BK, S> P;
-  __shared__ __align__(1024) char lds[P::LDS];
-  const int logical = xcd_logical(blockIdx.x, gridDim.x);
-  if (logical >= g.total) return;
-  const int split = logical / (g.tm * g.tn);
-  int tm, tn;
-  gemm::tile_of(logical - split * g.tm * g.tn, g.tm, g.tn, tm, tn);
+  // The sums leave through LDS, 32 rows x 32 COLS channels of a wave at a time, so
+  // that a row's channels are neighbours again and the accesses whole lines.
+  // 16-byte chunk c of row r sits at c ^ (r % (8 COLS)): neither side meets in a bank.
+  constexpr int NI = P::NI, MI = P::MI, COLS = WG == 1 ? 2 : 1, PITCH = COLS * 128;
+  constexpr int LPR = COLS * 4, RPI = 64 / LPR, ITS = 32 / RPI;    // lanes a row, rows an access
+  constexpr int PASSES = MI * NI / COLS, HALVES = NI / COLS;
+  static_assert(PASSES % 2 == 0, "");
+  __shared__ __align__(1024) char lds[P::LDS + 4 * 32 * PITCH];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave & 1, wn = wave >> 1;
-  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-  const int64_t k0 = split * g.kchunk, k1 = min(k0 + g.kchunk, g.K);
-  typename P::A a;
-  typename P::B b;
-  a.init(g.a, g.lda, g.M, m0, k0, k1, wave, wm, lane);
-  b.init(g.b, g.ldb, g.N, n0, k0, k1, wave, wn, lane);
-  f32x16 acc[P::NI][P::MI];
-  P::run(acc, a, b, lds, k1 - k0, wave, wm, wn);
+  const int per = (int)gridDim.x / kXcds;           // workgroups of an XCD
+  const int chunk = (g.total + kXcds - 1) / kXcds;  // items of an XCD
+  const int xcd = blockIdx.x % kXcds;
+  const int end = min((xcd + 1) * chunk, g.total);
+  const int first = xcd * chunk + blockIdx.x / kXcds;
+  if (first >= end) return;
 
-  // The sums of MIP x 32 rows at a time through the wave's part of LDS (its
-  // stages are idle now), so that a row's channels are neighbours again: the
-  // loads and stores below are whole rows of the wave's part.  16-byte chunk
-  // c of row r sits at c ^ (r % 16) ^ (c / 16): neither side meets in a bank.
-  constexpr int NI = P::NI, MIP = P::LDS / 4 / (NI * 128) / 32, PITCH = NI * 128;
-  static_assert(P::MI % MIP == 0, "");
-  constexpr int LPR = NI * 4, RPI = 64 / LPR, ITS = MIP * 32 / RPI, BATCH = 4;
-  char* const mine = lds + wave * (P::LDS / 4);
-  const int N = (int)g.N, j = lane % LPR;
-  const int n = (int)n0 + wn * NI * 32 + 8 * j;
-  const bool vec = g.e.vec;
-  float bias[8];
-  if (g.splits == 1 && g.e.bias && n < N) row8<T>(g.e.bias, 0, n, N, vec, bias);
+  P p;
+  int copying = first;        // the item that is being copied
+  auto set = [&](int item) {
+    const int split = item / (g.tm * g.tn);
+    int tm, tn;
+    gemm::tile_of(item - split * g.tm * g.tn, g.tm, g.tn, tm, tn);
+    const int64_t k0 = split * g.kchunk, k1 = min(k0 + g.kchunk, g.K);
+    p.a.init(g.a, g.lda, g.M, (int64_t)tm * BM, k0, k1, wave, wm, lane);
+    p.b.init(g.b, g.ldb, g.N, (int64_t)tn * BN, k0, k1, wave, wn, lane);
+    p.item(k1 - k0);
+  };
+  auto next = [&]() {
+    copying += per;
+    if (copying < end) {
+      set(copying);
+    } else {
+      p.a.end();
+      p.b.end();
+    }
+  };
+  set(first);
+  p.start(lds, wave, next);
+  char* const mine = lds + P::LDS + wave * 32 * PITCH;
+  const int N = (int)g.N;
+  auto chunk_at = [&](int r, int c) { return mine + r * PITCH + 16 * (c ^ (r % (8 * COLS))); };
+
+  for (int item = first; item < end; item += per) {
+    const int split = item / (g.tm * g.tn);
+    int tm, tn;
+    gemm::tile_of(item - split * g.tm * g.tn, g.tm, g.tn, tm, tn);
+    const int64_t k0 = split * g.kchunk;
+    const int nt = (int)((min(k0 + g.kchunk, g.K) - k0 + BK - 1) / BK);
+    const int64_t m0 = (int64_t)tm * BM + wm * MI * 32;
+    const int n0 = tn * BN + wn * NI * 32;
+    const int rows = (int)min(g.M - m0, (int64_t)(32 * MI));     // (may be none)
+    f32x16 acc[NI][MI];
 #pragma unroll
-  for (int pass = 0; pass < P::MI / MIP; ++pass) {
+    for (int n = 0; n < NI; ++n)
 #pragma unroll
-    for (int mi = 0; mi < MIP; ++mi)
+      for (int m = 0; m < MI; ++m)
 #pragma unroll
-      for (int ni = 0; ni < NI; ++ni)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int r = mi * 32 + (lane & 31), c = 8 * ni + 2 * q + (lane >> 5);
-          const f32x16& s = acc[ni][pass * MIP + mi];
-          *reinterpret_cast<f32x4*>(mine + r * PITCH + 16 * (c ^ (r & 15) ^ (c >> 4))) =
-              f32x4{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
-        }
-    const int64_t mp = m0 + (wm * P::MI + pass * MIP) * 32 + lane / LPR;
-    if (n < N)
+        for (int i = 0; i < 16; ++i) acc[n][m][i] = 0.f;
+
+    // The lane as the epilogue sees it: opaque, so that what it computes of it is not
+    // kept in registers through the product.
+    int el = lane;
+    if constexpr (KIND == kAny) {
+      p.run(acc, nt, next);
+      asm volatile("" : "+v"(el));
+      const int j = el % LPR, row = el / LPR;
 #pragma unroll 1
-    for (int it = 0; it < ITS; it += BATCH) {
-      Extras x[BATCH];
-      if (g.splits == 1)
-#pragma unroll
-        for (int k = 0; k < BATCH; ++k) {
-          const int64_t m = min(mp + (it + k) * RPI, g.M - 1);
-          load_extras<T>(g.e, vec, x[k], m, g.e.gate ? (uint32_t)m / g.e.rows_per_gate : 0u, n, N);
-        }
-#pragma unroll
-      for (int k = 0; k < BATCH; ++k) {
-        const int r = (it + k) * RPI + lane / LPR;
-        const int64_t m = mp + (it + k) * RPI;
-        const f32x4 lo = *reinterpret_cast<const f32x4*>(
-            mine + r * PITCH + 16 * ((2 * j) ^ (r & 15) ^ (2 * j >> 4)));
-        const f32x4 hi = *reinterpret_cast<const f32x4*>(
-            mine + r * PITCH + 16 * ((2 * j + 1) ^ (r & 15) ^ (2 * j >> 4)));
-        if (m >= g.M) continue;
-        if (g.splits > 1) {
-          float* q = g.e.partial + split * g.e.part_stride + m * g.e.ld_part + n;
-          *reinterpret_cast<f32x4*>(q) = lo;
-          *reinterpret_cast<f32x4*>(q + 4) = hi;
-        } else {
+      for (int pass = 0; pass < PASSES; ++pass) {
+        put_sums<NI, MI, COLS>(acc, mine, el, pass, std::make_integer_sequence<int, PASSES>{});
+        const int n = n0 + 32 * COLS * (pass % HALVES) + 8 * j;
+        if (n >= N) continue;
+#pragma unroll 1
+        for (int it = 0; it < ITS; ++it) {
+          const int r = it * RPI + row, mr = pass / HALVES * 32 + r;
+          if (mr >= rows) continue;
+          const f32x4 lo = *reinterpret_cast<const f32x4*>(chunk_at(r, 2 * j));
+          const f32x4 hi = *reinterpret_cast<const f32x4*>(chunk_at(r, 2 * j + 1));
           float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-          epilogue8<T>(g.e, vec, v, bias, x[k], m, n, N);
+          finish8<T>(g.e, v, m0 + mr, n, N);
         }
       }
+    } else {
+      // offset of row r (of the wave's part) at channel n in a tensor of row stride ss
+      auto off = [&](int r, int n, int64_t ss) {
+        return r < rows && n < N ? (uint32_t)(r * (int)(2 * ss) + 2 * n) : gemm::kOut;
+      };
+      View vb;
+      u32x4 bias[HALVES], res[ITS], gate[ITS], held[ITS];
+      if (g.e.bias && g.splits == 1) {
+        vb.init(g.e.bias, 0);
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          const int n = n0 + 32 * COLS * h + 8 * (lane % LPR);
+          bias[h] = vb.load(n < N ? 2 * n : gemm::kOut);
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) bias[h] = u32x4{0u, 0u, 0u, 0u};
+      }
+      p.run(acc, nt, next);
+      asm volatile("" : "+v"(el));
+      const int j = el % LPR, row = el / LPR;
+      View vo, vz, vr, vg;
+      vo.init(g.e.out, 2 * m0 * g.e.out_ss);
+      vz.init(g.e.preact, 2 * m0 * g.e.preact_ss);
+      const uint32_t gate0 = gate_row(g.e, min(m0, g.M - 1));
+      if constexpr (KIND == kExtra) {
+        vr.init(g.e.residual, 2 * m0 * g.e.residual_ss);
+        vg.init(g.e.gate, 2 * (int64_t)gate0 * g.e.gate_ss);
+#pragma unroll
+        for (int it = 0; it < ITS; ++it) held[it] = u32x4{0u, 0u, 0u, 0u};
+      }
+      // (here, so that no pass waits for it and with it for the stores of the one before)
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) asm volatile("" : "+v"(bias[h]));
+      uint32_t to[ITS];
+#pragma unroll
+      for (int it = 0; it < ITS; ++it) to[it] = gemm::kOut;
+#pragma unroll 1
+      for (int pass = 0; pass < PASSES; ++pass) {
+        const int h = pass % HALVES, n = n0 + 32 * COLS * h + 8 * j, r0 = pass / HALVES * 32 + row;
+        if constexpr (KIND == kExtra) {
+          // this pass's residual and gate are asked for before the results of the pass
+          // before go out: the wait for them is not one for those stores
+          if (g.e.gate) {
+#pragma unroll
+            for (int it = 0; it < ITS; ++it) {
+              const int r = r0 + it * RPI;
+              const uint32_t gr = gate_row(g.e, min(m0 + r, g.M - 1)) - gate0;
+              gate[it] = vg.load(r < rows && n < N ? gr * (uint32_t)(2 * g.e.gate_ss) + 2 * n : gemm::kOut);
+            }
+          }
+          // (without a residual its view takes zeros: out of range)
+#pragma unroll
+          for (int it = 0; it < ITS; ++it)
+            res[it] = vr.load(g.e.residual ? off(r0 + it * RPI, n, g.e.residual_ss) : gemm::kOut);
+#pragma unroll
+          for (int it = 0; it < ITS; ++it) vo.store(held[it], to[it]);
+        }
+        put_sums<NI, MI, COLS>(acc, mine, el, pass, std::make_integer_sequence<int, PASSES>{});
+        f32x4 lo[ITS], hi[ITS];
+#pragma unroll
+        for (int it = 0; it < ITS; ++it) {
+          lo[it] = *reinterpret_cast<const f32x4*>(chunk_at(it * RPI + row, 2 * j));
+          hi[it] = *reinterpret_cast<const f32x4*>(chunk_at(it * RPI + row, 2 * j + 1));
+        }
+        if (KIND == kPlain && g.splits > 1) {
+          View vp;
+          vp.init(g.e.partial, 4 * (split * g.e.part_stride + m0 * g.e.ld_part));
+#pragma unroll
+          for (int it = 0; it < ITS; ++it) {
+            const int r = r0 + it * RPI;
+            const bool there = r < rows && n < N;
+            const uint32_t at = there ? (uint32_t)(r * (int)(4 * g.e.ld_part) + 4 * n) : gemm::kOut;
+            vp.store(__builtin_bit_cast(u32x4, lo[it]), at);
+            vp.store(__builtin_bit_cast(u32x4, hi[it]), there ? at + 16 : gemm::kOut);
+          }
+          continue;
+        }
+        float b[8];
+        u32x4 braw = bias[0];
+#pragma unroll
+        for (int i = 1; i < HALVES; ++i) braw = h == i ? bias[i] : braw;
+        widen<T>(braw, b);
+#pragma unroll
+        for (int it = 0; it < ITS; ++it) {
+          float v[8] = {lo[it][0], lo[it][1], lo[it][2], lo[it][3], hi[it][0], hi[it][1], hi[it][2], hi[it][3]}, t[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] += b[i];
+          if (g.e.preact) vz.store(narrow<T>(v), off(r0 + it * RPI, n, g.e.preact_ss));
+          activate8(v, g.e.act);
+          const uint32_t at = off(r0 + it * RPI, n, g.e.out_ss);
+          if constexpr (KIND == kExtra) {
+            if (g.e.gate) {
+              widen<T>(gate[it], t);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] *= t[i];
+            }
+            widen<T>(res[it], t);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += t[i];
+            held[it] = narrow<T>(v);
+            to[it] = at;
+          } else {
+            vo.store(narrow<T>(v), at);
+          }
+        }
+      }
+      if constexpr (KIND == kExtra)
+#pragma unroll
+        for (int it = 0; it < ITS; ++it) vo.store(held[it], to[it]);
     }
   }
+  // no copy may be on its way when the workgroup ends
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 // The splits' sums in their order, and the epilogue.
@@ -355,7 +528,7 @@ struct DzArgs {
   int64_t M, rpg;              // rows of a gate (M without gates)
   int64_t rows, segs;          // rows of a workgroup; its rows of a gate's, if split
   int32_t N, act;
-  bool vec, split;
+  bool split;
 };
 
 template <typename T>
@@ -376,15 +549,15 @@ __global__ __launch_bounds__(256) void dz_kernel(DzArgs d) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) gate[i] = 1.f;
   int64_t g = r0 / d.rpg, gend = (g + 1) * d.rpg;
-  if (d.gate) row8<T>(d.gate, g * d.gate_ss, n, d.N, d.vec, gate);
+  if (d.gate) row8<T>(d.gate, g * d.gate_ss, n, d.N, gate);
   constexpr int AHEAD = 4;
   for (int64_t r = r0; r < r1; r += AHEAD) {
     float y[AHEAD][8], z[AHEAD][8];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       const int64_t row = min(r + j, r1 - 1);
-      row8<T>(d.dy, row * d.dy_ss, n, d.N, d.vec, y[j]);
-      if (d.z) row8<T>(d.z, row * d.z_ss, n, d.N, d.vec, z[j]);
+      row8<T>(d.dy, row * d.dy_ss, n, d.N, y[j]);
+      if (d.z) row8<T>(d.z, row * d.z_ss, n, d.N, z[j]);
       else
 #pragma unroll
         for (int i = 0; i < 8; ++i) z[j][i] = 0.f;
@@ -393,10 +566,10 @@ __global__ __launch_bounds__(256) void dz_kernel(DzArgs d) {
     for (int j = 0; j < AHEAD; ++j) {
       if (r + j >= r1) break;
       if (r + j == gend) {          // the next gate's rows begin (whole gates only)
-        if (d.dgate) put8<T>(d.dgate, g * (int64_t)d.N, n, d.N, d.vec, dg);
+        if (d.dgate) put_row8<T>(d.dgate, g * (int64_t)d.N, n, d.N, dg);
         ++g;
         gend += d.rpg;
-        row8<T>(d.gate, g * d.gate_ss, n, d.N, d.vec, gate);
+        row8<T>(d.gate, g * d.gate_ss, n, d.N, gate);
 #pragma unroll
         for (int i = 0; i < 8; ++i) dg[i] = 0.f;
       }
@@ -409,7 +582,7 @@ __global__ __launch_bounds__(256) void dz_kernel(DzArgs d) {
         dz[i] = y[j][i] * gate[i] * slope;
         db[i] += dz[i];
       }
-      if (d.dz) put8<T>(d.dz, (r + j) * d.dz_ss, n, (int)d.dz_ss, true, dz);
+      if (d.dz) put8<T>(d.dz, (r + j) * d.dz_ss + n, dz);
     }
   }
   if (d.db_part) {
@@ -423,7 +596,7 @@ __global__ __launch_bounds__(256) void dz_kernel(DzArgs d) {
       for (int i = 0; i < 8; ++i)
         if (n + i < d.N) d.dg_part[seg * d.N + n + i] = dg[i];
     } else {
-      put8<T>(d.dgate, g * (int64_t)d.N, n, d.N, d.vec, dg);
+      put_row8<T>(d.dgate, g * (int64_t)d.N, n, d.N, dg);
     }
   }
 }
@@ -469,7 +642,7 @@ Plan plan_of(int64_t M, int64_t N, int64_t K) {
 }
 
 template <typename T, bool ATR, bool BTR>
-int launch_gemm(GemmArgs g, const Plan& p, float* ws, hipStream_t st) {
+int launch_gemm(GemmArgs g, const Plan& p, float* ws, bool rows16, hipStream_t st) {
   g.tm = (int)((g.M + p.tile - 1) / p.tile);
   g.tn = (int)((g.N + p.tile - 1) / p.tile);
   g.splits = p.splits;
@@ -480,11 +653,23 @@ int launch_gemm(GemmArgs g, const Plan& p, float* ws, hipStream_t st) {
   g.e.partial = ws;
   g.e.ld_part = (g.N + 7) / 8 * 8;
   g.e.part_stride = g.M * g.e.ld_part;
-  const dim3 grid((unsigned)xcd_grid(total));
-  if (p.tile == 256)
-    hipLaunchKernelGGL((gemm_kernel<T, ATR, BTR, 256, 256, kBK, 2, 1>), grid, dim3(256), 0, st, g);
-  else
-    hipLaunchKernelGGL((gemm_kernel<T, ATR, BTR, 128, 128, kBK, 2, 2>), grid, dim3(256), 0, st, g);
+  auto run = [&](auto kind) {
+    constexpr int KIND = decltype(kind)::value;
+    if (p.tile == 256)
+      hipLaunchKernelGGL((gemm_kernel<T, ATR, BTR, 256, 256, kBK, 2, 1, KIND>),
+                         dim3((unsigned)xcd_grid(std::min<int64_t>(total, kSlots))), dim3(256), 0, st, g);
+    else
+      hipLaunchKernelGGL((gemm_kernel<T, ATR, BTR, 128, 128, kBK, 2, 2, KIND>),
+                         dim3((unsigned)xcd_grid(std::min<int64_t>(total, 2 * kSlots))), dim3(256), 0, st, g);
+  };
+  // (the parts' launch writes whole rows of its own)
+  if constexpr (ATR || BTR) {
+    run(std::integral_constant<int, kPlain>{});
+  } else {
+    if (p.splits > 1 || (rows16 && !g.e.gate && !g.e.residual)) run(std::integral_constant<int, kPlain>{});
+    else if (rows16) run(std::integral_constant<int, kExtra>{});
+    else run(std::integral_constant<int, kAny>{});
+  }
   if (int rc = check_launch("gemm_kernel")) return rc;
   if (p.splits > 1) {
     const int64_t n8 = g.M * ((g.N + 7) / 8);
@@ -639,19 +824,19 @@ extern "C" int hier_linear(const HierLinearArgs* args, void* stream) {
   e.gate_ss = a.gate_ss;
   e.out_ss = a.out_ss;
   e.preact_ss = a.preact_ss;
-  e.rows_per_gate = a.gate ? (uint32_t)a.rows_per_gate : 1u;
+  e.rows_per_gate = make_div(a.gate ? (uint32_t)a.rows_per_gate : 1u);
   e.act = a.act;
-  auto ok = [](const void* p, int64_t ss) { return !p || (aligned16(p) && ss % 8 == 0); };
-  e.vec = a.N % 8 == 0 && ok(a.bias, 0) && ok(a.residual, a.residual_ss) && ok(a.gate, a.gate_ss) &&
-          ok(a.out, a.out_ss) && ok(a.preact, a.preact_ss);
   const hipStream_t st = (hipStream_t)stream;
   if (few_rows(a.M)) return a.type == HIER_BF16 ? launch_few<__bf16>(g, st) : launch_few<_Float16>(g, st);
   const Plan p = plan_of(a.M, a.N, a.K);
   HIER_REQUIRE(p.bytes == 0 || (a.workspace && aligned16(a.workspace) && a.workspace_bytes >= p.bytes),
                HIER_EINVAL, "linear: workspace of %lld bytes needed", (long long)p.bytes);
   float* ws = static_cast<float*>(a.workspace);
-  return a.type == HIER_BF16 ? launch_gemm<__bf16, false, false>(g, p, ws, st)
-                             : launch_gemm<_Float16, false, false>(g, p, ws, st);
+  auto ok = [](const void* q, int64_t ss) { return !q || (aligned16(q) && ss % 8 == 0 && ss < (1ll << 21)); };
+  const bool rows16 = a.N % 8 == 0 && ok(a.bias, 0) && ok(a.residual, a.residual_ss) && ok(a.gate, a.gate_ss) &&
+                      ok(a.out, a.out_ss) && ok(a.preact, a.preact_ss);
+  return a.type == HIER_BF16 ? launch_gemm<__bf16, false, false>(g, p, ws, rows16, st)
+                             : launch_gemm<_Float16, false, false>(g, p, ws, rows16, st);
 }
 
 static int check_linear_bwd(const HierLinearBwdArgs& a) {
@@ -698,9 +883,6 @@ static int linear_bwd(const HierLinearBwdArgs& a, const BwdPlan& p, hipStream_t 
     d.N = a.N;
     d.act = a.act;
     d.split = p.dz.split;
-    auto ok = [](const void* q, int64_t ss) { return !q || (aligned16(q) && ss % 8 == 0); };
-    d.vec = a.N % 8 == 0 && ok(a.dy, a.dy_ss) && ok(a.preact, a.preact_ss) && ok(a.gate, a.gate_ss) &&
-            ok(a.dgate, 0);
     const int64_t gy = (Np / 8 + 255) / 256;
     HIER_REQUIRE(gy <= 65535 && p.dz.total < (1ll << 24), HIER_EUNSUPPORTED, "linear_bwd: too many rows");
     hipLaunchKernelGGL(dz_kernel<T>, dim3((unsigned)p.dz.total, (unsigned)gy), dim3(256), 0, st, d);
@@ -723,17 +905,16 @@ static int linear_bwd(const HierLinearBwdArgs& a, const BwdPlan& p, hipStream_t 
     g.K = K;
     g.e.out = out;
     g.e.out_ss = out_ss;
-    g.e.rows_per_gate = 1;
-    g.e.vec = N % 8 == 0 && aligned16(out) && out_ss % 8 == 0;
+    g.e.rows_per_gate = make_div(1u);
     return g;
   };
   if (a.dx)
     if (int rc = launch_gemm<T, false, true>(
-            product(a.M, a.K, a.N, dz, dz_ss, a.w, a.w_ss, a.dx, a.dx_ss), p.dx, parts, st))
+            product(a.M, a.K, a.N, dz, dz_ss, a.w, a.w_ss, a.dx, a.dx_ss), p.dx, parts, true, st))
       return rc;
   if (a.dw)
     return launch_gemm<T, true, true>(product(a.N, a.K, a.M, dz, dz_ss, a.x, a.x_ss, a.dw, a.dw_ss), p.dw,
-                                      parts, st);
+                                      parts, true, st);
   return HIER_OK;
 }
 
@@ -754,8 +935,9 @@ extern "C" int hier_linear_bwd(const HierLinearBwdArgs* args, void* stream) {
     if (int rc = check_view("dy", a.dy, a.dy_ss, a.N)) return rc;
     HIER_REQUIRE(a.N % 8 == 0, HIER_EINVAL, "linear_bwd: dy needs a multiple of 8 columns");
   }
-  HIER_REQUIRE((!a.dx || a.dx_ss >= a.K) && (!a.dw || a.dw_ss >= a.K), HIER_EINVAL,
-               "linear_bwd: invalid output stride");
+  auto ok = [](const void* q, int64_t ss) { return !q || (aligned16(q) && ss % 8 == 0 && ss < (1ll << 21)); };
+  HIER_REQUIRE((!a.dx || a.dx_ss >= a.K) && (!a.dw || a.dw_ss >= a.K) && ok(a.dx, a.dx_ss) && ok(a.dw, a.dw_ss),
+               HIER_EINVAL, "linear_bwd: dx and dw need 16-byte rows and an output stride of at least K");
   const BwdPlan p = bwd_plan(a);
   HIER_REQUIRE(p.bytes == 0 || (a.workspace && aligned16(a.workspace) && a.workspace_bytes >= p.bytes),
                HIER_EINVAL, "linear_bwd: workspace of %lld bytes needed", (long long)p.bytes);

@@ -32,6 +32,23 @@ __device__ __forceinline__ w32x4 narrow(const float* f) {
   return __builtin_bit_cast(w32x4, v);
 }
 
+// Division of row numbers below 2^31 by g, 1 <= g < 2^31:
+// r / g = (r * mul) >> (32 + shift), mul = floor(2^(32 + shift) / g) + 1 with
+// shift = ceil(log2 g) - 1; g = 1 needs none.
+struct Div {
+  uint32_t g, mul, shift;
+};
+inline Div make_div(uint32_t g) {
+  Div d = {g, 0u, 0u};
+  if (g == 1) return d;
+  while ((1ull << (d.shift + 1)) < g) ++d.shift;
+  d.mul = (uint32_t)((1ull << (32 + d.shift)) / g + 1);
+  return d;
+}
+__device__ __forceinline__ uint32_t quotient(uint32_t r, const Div& d) {
+  return d.g == 1 ? r : __umulhi(r, d.mul) >> d.shift;
+}
+
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 // out[g][c] = sum of the rows g * rows .. + rows of partial [groups * rows][C], in
