@@ -10,13 +10,13 @@
 // reads from LDS feed (BM/64)(BN/64) MFMAs, so the larger the wave's part the
 // fewer bytes LDS has to deliver for an MFMA.
 //
-// K tiles of BK go HBM/L2 -> LDS with buffer_load_dwordx4 ... lds, S stages.
+// K tiles of 64 go HBM/L2 -> LDS with buffer_load_dwordx4 ... lds.
 // A buffer load out of its range writes zeros: rows past the end, the ragged
 // last K tile and tiles past the end need no other handling, and nothing past a
 // view's last element is read.  The operands of step k+1 are read while the
 // MFMAs of step k run.  One barrier a tile, before its last step: by then every
 // wave has read the tile to its end, and the next tile has landed, so the last
-// step starts on the next tile and its stage is filled anew.
+// step starts on the next tile and its slots are filled anew.
 //
 // LDS layouts (16-byte chunks, XOR-swizzled so that no 16 lanes of a read meet
 // in a bank; a global read of a wave is whole lines all the same):
@@ -35,6 +35,15 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
+// 16 x 16 x 32: lane l holds row l % 16, k 8 (l / 16) .. + 8 of both operands.
+template <typename T>
+__device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+  const vec8<T> x = __builtin_bit_cast(vec8<T>, a), y = __builtin_bit_cast(vec8<T>, b);
+  if constexpr (__is_same(T, __bf16)) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0);
+}
+
+// 32 x 32 x 16: lane l holds row l % 32, k 8 (l / 32) .. + 8.
 template <typename T>
 __device__ __forceinline__ f32x16 mfma(const u32x4& a, const u32x4& b, const f32x16& c) {
   const vec8<T> x = __builtin_bit_cast(vec8<T>, a), y = __builtin_bit_cast(vec8<T>, b);
@@ -70,9 +79,10 @@ struct Operand {
   static constexpr int LPC = 64 / CPR;                            // LDS rows per copy
   static constexpr int KK = BK / 16;
   static constexpr int MI = R / 64;                               // 32-row blocks of a wave
-  uint64_t base;       // first byte of the present tile to copy
-  int64_t left;        // bytes of the view from there
-  int64_t step;        // bytes to the next tile
+  uint64_t base;       // first byte of the tile to copy next
+  uint32_t range;      // bytes from there that the copies may read
+  uint32_t step;       // bytes to the next tile
+  int kall;            // K left of the item, from `base` on
   uint32_t voff, sstep;
   int k8;              // rows: the lane's first k of a tile
   int rd[TR ? MI : KK];
@@ -82,15 +92,16 @@ struct Operand {
   __device__ __forceinline__ void init(const void* p, int64_t ld, int64_t rows, int64_t first, int64_t k0,
                                        int64_t kend, int wave, int part, int lane) {
     const int line = lane / CPR, pos = lane % CPR;
+    int64_t bytes;
     if constexpr (TR) {
       rows = (rows + 7) / 8 * 8;         // (a view's rows of k are whole chunks)
       const int chunk = pos ^ (4 * ((LPC * wave + line) & 3));
       base = (uint64_t)p + 2 * (k0 * ld + first);
-      left = 2 * ((kend - k0 - 1) * ld + rows - first);
-      step = 2 * BK * ld;
+      bytes = 0x7fffffff;                // (the end of K: see edge)
+      step = (uint32_t)(2 * BK * ld);
       voff = (uint32_t)((LPC * wave + line) * (int)(2 * ld) + 16 * chunk);
       if (first + 8 * chunk >= rows) voff = kOut;
-      k8 = 0;
+      k8 = (int)(2 * (rows - first));    // bytes of a row of k
 #pragma unroll
       for (int b = 0; b < MI; ++b) {
         const int i = lane & 15, r = 8 * (lane >> 5) + (i >> 2);
@@ -98,11 +109,12 @@ struct Operand {
         rd[b] = r * (2 * R) + 16 * (q ^ (4 * (r & 3))) + 8 * (i & 1);
       }
     } else {
-      kend = (kend + 7) / 8 * 8;
       const int row = LPC * wave + line;
       const int chunk = pos ^ (row / (128 / BK) % CPR);
       base = (uint64_t)p + 2 * (first * ld + k0);
-      left = 2 * ((rows - first - 1) * ld + kend - k0);
+      // up to the last row's end, seen from the item's first tile: a row past it starts
+      // behind that from any tile (the view's rows do not overlap)
+      bytes = 2 * ((rows - first - 1) * ld + (kend - k0 + 7) / 8 * 8);   // (whole chunks)
       step = 2 * BK;
       voff = (uint32_t)(row * (int)(2 * ld) + 16 * chunk);
       k8 = 8 * chunk;
@@ -112,25 +124,37 @@ struct Operand {
         rd[k] = (part * 32 * MI + r) * (2 * BK) + 16 * ((2 * k + (lane >> 5)) ^ (r / (128 / BK) % CPR));
     }
     sstep = (uint32_t)(4 * LPC * (2 * ld));
+    range = (uint32_t)(bytes < 0x7fffffff ? bytes : 0x7fffffff);
+    kall = (int)(kend - k0);
+    if (kall < BK) edge();
+  }
+  // The item's last tile is not a whole one: chunks (rows of k) past its end are out of
+  // range.
+  __device__ __forceinline__ void edge() {
+    if constexpr (TR) range = (uint32_t)((kall - 1) * (int)(step / BK) + k8);
+    else if (k8 >= kall) voff = kOut;
   }
 
-  // Copy j of the wave's for the tile that `base` is at; kleft = its K.
-  __device__ __forceinline__ void copy(int j, int kleft, uint32_t lds, int wave) const {
-    const uint32_t n = left <= 0 ? 0u : (left < 0x7fffffff ? (uint32_t)left : 0x7fffffffu);
-    const u32x4 srd = {(uint32_t)base, (uint32_t)(base >> 32) & 0xffffu, n, 0x00020000u};
-    const uint32_t v = TR ? voff : (k8 < kleft ? voff : kOut);
-    // (the whole offset in the lane's register: it is what the range check sees;
-    // kOut plus the copies' rows, under 2^30, stays past every range)
-    dma(srd, v + j * sstep, lds + 1024 * (wave + 4 * j));
+  // Copy j of the wave's for the tile that `base` is at.  (The whole offset is in the
+  // lane's register: that is what the range check sees.  kOut plus the copies' rows,
+  // under 2^30, stays past every range.)
+  __device__ __forceinline__ void copy(int j, uint32_t lds, int wave) const {
+    const u32x4 srd = {(uint32_t)base, (uint32_t)(base >> 32), range, 0x00020000u};
+    dma(srd, voff + j * sstep, lds + 1024 * (wave + 4 * j));
   }
-  __device__ __forceinline__ void next() {
+  // The next tile; true past the item's last.
+  __device__ __forceinline__ bool next() {
     base += step;
-    left -= step;
+    kall -= BK;
+    if (kall >= BK) return false;
+    if (kall <= 0) return true;
+    edge();
+    return false;
   }
   // No more tiles: the copies write zeros.
   __device__ __forceinline__ void end() {
-    left = 0;
-    step = 0;
+    range = 0;
+    kall = 0x7fffffff;
   }
 
   // Operand of block b and step k from the tile at `t`: lane l holds row
@@ -150,108 +174,119 @@ struct Operand {
 // acc[ni][mi]: 32 x 32 blocks, lane l holds row m = 32 mi + l % 32 and
 // n = 32 ni + 8 (r / 4) + 4 (l / 32) + r % 4 of the wave's part.
 //
+// LDS is a ring of five slots of one operand's tile each, filled in the order A0 B0
+// A1 B1 A2 ..: with two tiles of both in use or on their way there is room for a
+// third of A, so the copies leave evenly over the four steps of a tile -- the second
+// half of B(t+1), A(t+2) in two steps, the first half of B(t+2) -- at the rate at which
+// the caches deliver them (42 bytes a cycle and CU, three quarters of what the MFMAs
+// leave time for), and each has two steps at least to land.  (Two stages of both,
+// copies in one step of four: 8192^3 at 1,184 TFLOP/s, in two 1,234, in three 1,189.)
+//
 // The K tiles of a workgroup's work items are one stream: while an item is
 // multiplied, and while its results go out, the copies run ahead into the next
-// (`Next` sets the operands to it), so only the first one waits for memory.
-template <typename T, bool ATR, bool BTR, int BM, int BN, int BK, int S>
+// (`next_a`, `next_b` set the operands to it), so only the first one waits for memory.
+template <typename T, bool ATR, bool BTR, int BM, int BN, int BK>
 struct Product {
   typedef Operand<ATR, BM, BK> A;
   typedef Operand<BTR, BN, BK> B;
-  static constexpr int MI = A::MI, NI = B::MI, KK = BK / 16;
-  static constexpr int STAGE = A::BYTES + B::BYTES;
-  static constexpr int LDS = S * STAGE;
-  static constexpr int COPIES = A::COPIES + B::COPIES;
+  static constexpr int MI = A::MI, NI = B::MI, KK = A::KK;
+  static constexpr int SLOT = A::BYTES;
+  static constexpr int LDS = 5 * SLOT;
+  static constexpr int COPIES = A::COPIES, HALF = COPIES / 2;    // of one operand
   static constexpr int READS = MI + NI, NM = NI * MI;
-  // A tile's copies are made in the first SPREAD steps after its stage is free
-  // (the last step of one tile, the first of the next ..): the workgroup's copies
-  // leave at about the rate that the CU's address unit takes them (one 1 KiB copy in
-  // 16 cycles), and land before the tile after next needs them.  8192^3: in one
-  // step 1,184 TFLOP/s, in two 1,234, in three 1,189, in all four 1,118.
-  static constexpr int SPREAD = 2;
-  static constexpr int FIRST = (COPIES + SPREAD - 1) / SPREAD;
-  static_assert(KK % 2 == 0 && S >= 2, "");
+  static_assert(KK == 4 && A::BYTES == B::BYTES && NM % READS == 0 && NM % HALF == 0, "");
 
   A a;
   B b;
-  int64_t kall;           // K left of the item that is being copied
-  int kleft;              // the same, at most 2^30
-  uint32_t l0, fill;      // LDS address, stage that the next tile goes to
+  uint32_t l0;            // LDS address of the ring
+  uint32_t fill;          // slot that is being filled, in bytes; in use: A and B of the
+  uint32_t at_a, at_b;    // present tile
   const char* lds;
-  const char* cur;        // stage of the present tile
   int wave;
   u32x4 fa[2][MI], fb[2][NI];
 
-  __device__ __forceinline__ void item(int64_t K) {
-    kall = K;
-    kleft = (int)(K < (1 << 30) ? K : (1 << 30));
+  static __device__ __forceinline__ uint32_t after(uint32_t slot, int n) {
+    slot += n * SLOT;
+    return slot >= LDS ? slot - LDS : slot;
   }
-  __device__ __forceinline__ void copy_one(int j) {
-    if (j < A::COPIES) a.copy(j, kleft, l0 + fill, wave);
-    else b.copy(j - A::COPIES, kleft, l0 + fill + A::BYTES, wave);
+  __device__ __forceinline__ void copy_a(int j) { a.copy(j, l0 + fill, wave); }
+  __device__ __forceinline__ void copy_b(int j) { b.copy(j, l0 + fill, wave); }
+  template <typename Next>
+  __device__ __forceinline__ void done_a(Next& next) {
+    fill = after(fill, 1);
+    if (a.next()) next();
   }
   template <typename Next>
-  __device__ __forceinline__ void copied(Next& next) {
-    a.next();
-    b.next();
-    fill = fill + STAGE == LDS ? 0 : fill + STAGE;
-    item(kall - BK);
-    if (kall <= 0) next();
+  __device__ __forceinline__ void done_b(Next& next) {
+    fill = after(fill, 1);
+    if (b.next()) next();
   }
-  __device__ __forceinline__ void read_one(const char* t, int k, int par, int i) {
-    if (i < NI) fb[par][i] = b.read(t + A::BYTES, i, k);
-    else fa[par][i - NI] = a.read(t, i - NI, k);
+  __device__ __forceinline__ void read_one(uint32_t from_a, uint32_t from_b, int k, int par, int i) {
+    if (i < NI) fb[par][i] = b.read(lds + from_b, i, k);
+    else fa[par][i - NI] = a.read(lds + from_a, i - NI, k);
   }
+  // The slot that nothing uses between two items.
+  __device__ __forceinline__ uint32_t spare() const { return after(fill, 1); }
 
-  // a, b and the first item set: the first tiles on their way, the first one's
+  // a and b set to the first item: the first tiles on their way, the first one's
   // first operands read.
-  template <typename Next>
-  __device__ __forceinline__ void start(char* base, int w, Next& next) {
-    lds = cur = base;
+  template <typename NextA, typename NextB>
+  __device__ __forceinline__ void start(char* base, int w, NextA& next_a, NextB& next_b) {
+    lds = base;
     l0 = (uint32_t)(uintptr_t)base;
-    fill = 0;
+    fill = at_a = 0;
+    at_b = SLOT;
     wave = w;
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
+    for (int t = 0; t < 2; ++t) {
 #pragma unroll
-      for (int j = 0; j < (s < S - 1 ? COPIES : FIRST); ++j) copy_one(j);
-      if (SPREAD == 1 || s < S - 1) copied(next);
+      for (int j = 0; j < COPIES; ++j) copy_a(j);
+      done_a(next_a);
+#pragma unroll
+      for (int j = 0; j < (t ? HALF : COPIES); ++j) copy_b(j);
+      if (!t) done_b(next_b);
     }
-    wait_barrier<(S - 2) * COPIES + FIRST>();
+    wait_barrier<COPIES + HALF>();
 #pragma unroll
-    for (int i = 0; i < READS; ++i) read_one(cur, 0, 0, i);
+    for (int i = 0; i < READS; ++i) read_one(at_a, at_b, 0, 0, i);
   }
 
   // acc += the item's product, nt tiles of K.
-  template <typename Next>
-  __device__ __forceinline__ void run(f32x16 (&acc)[NI][MI], int nt, Next& next) {
+  template <typename NextA, typename NextB>
+  __device__ __forceinline__ void run(f32x16 (&acc)[NI][MI], int nt, NextA& next_a, NextB& next_b) {
     for (int t = 0; t < nt; ++t) {
 #pragma unroll
       for (int k = 0; k < KK; ++k) {
         const bool last = k == KK - 1;
-        const char* from = cur;
         if (last) {
-          wait_barrier<(S - 2) * COPIES>();
-          cur = cur + STAGE == lds + LDS ? lds : cur + STAGE;
-          from = cur;
+          // every wave has read this tile to its end, and the next one is here: all
+          // copies but those of A(t+2)
+          wait_barrier<COPIES>();
+          at_a = after(at_a, 2);
+          at_b = after(at_b, 2);
         }
-        const int kn = last ? 0 : k + 1, part = last ? 0 : k + 1;
-        int reads = 0, copies = min(part * FIRST, COPIES);
+        const int kn = last ? 0 : k + 1;
+        // the next step's reads between the MFMAs of the first half of this one, the
+        // copies between all
+        int reads = 0;
+        constexpr int PER_COPY = NM / HALF;
 #pragma unroll
         for (int i = 0; i < NM; ++i) {
-          // the next step's reads and the copies spread between the MFMAs
-          const int want_r = ((i + 1) * READS + NM - 1) / NM;
+          const int want_r = min(READS, (2 * (i + 1) * READS + NM - 1) / NM);
 #pragma unroll
-          for (; reads < want_r; ++reads) read_one(from, kn, (k + 1) & 1, reads);
-          if (part < SPREAD) {
-            const int want_c = min(COPIES, part * FIRST + ((i + 1) * FIRST + NM - 1) / NM);
-#pragma unroll
-            for (; copies < want_c; ++copies) copy_one(copies);
+          for (; reads < want_r; ++reads) read_one(at_a, at_b, kn, (k + 1) & 1, reads);
+          if (i % PER_COPY == 0) {
+            const int c = i / PER_COPY;
+            if (k == 0) copy_b(HALF + c);
+            else if (last) copy_b(c);
+            else copy_a((k - 1) * HALF + c);
           }
           const int n = i / MI, m = i % MI;
           acc[n][m] = mfma<T>(fb[k & 1][n], fa[k & 1][m], acc[n][m]);
           __builtin_amdgcn_sched_barrier(0);
         }
-        if (part == SPREAD - 1) copied(next);
+        if (k == 0) done_b(next_b);
+        if (k == 2) done_a(next_a);
       }
     }
   }

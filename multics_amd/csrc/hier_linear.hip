@@ -208,17 +208,17 @@ __device__ __forceinline__ void put_sums(const f32x16 (&acc)[NI][MI], char* mine
 // turn, the XCD's workgroups neighbouring ones.
 constexpr int kSlots = 256;
 
-template <typename T, bool ATR, bool BTR, int BM, int BN, int BK, int S, int WG, int KIND>
+template <typename T, bool ATR, bool BTR, int BM, int BN, int BK, int WG, int KIND>
 __global__ __launch_bounds__(256, WG) void gemm_kernel(GemmArgs g) {
-  typedef gemm::Product<T, ATR, BTR, BM, BN, BK, S> P;
+  typedef gemm::Product<T, ATR, BTR, BM, BN, BK> P;
   // The sums leave through LDS, 32 rows x 32 COLS channels of a wave at a time, so
   // that a row's channels are neighbours again and the accesses whole lines.
   // 16-byte chunk c of row r sits at c ^ (r % (8 COLS)): neither side meets in a bank.
   constexpr int NI = P::NI, MI = P::MI, COLS = WG == 1 ? 2 : 1, PITCH = COLS * 128;
   constexpr int LPR = COLS * 4, RPI = 64 / LPR, ITS = 32 / RPI;    // lanes a row, rows an access
-  constexpr int PASSES = MI * NI / COLS, HALVES = NI / COLS;
-  static_assert(PASSES % 2 == 0, "");
-  __shared__ __align__(1024) char lds[P::LDS + 4 * 32 * PITCH];
+  constexpr int HALVES = NI / COLS, PASSES = MI * HALVES;
+  static_assert(4 * 32 * PITCH == P::SLOT, "the sums leave through the spare slot");
+  __shared__ __align__(1024) char lds[P::LDS];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave & 1, wn = wave >> 1;
@@ -230,29 +230,31 @@ __global__ __launch_bounds__(256, WG) void gemm_kernel(GemmArgs g) {
   if (first >= end) return;
 
   P p;
-  int copying = first;        // the item that is being copied
-  auto set = [&](int item) {
+  // operand A or B at an item's first tile
+  int item_a = first, item_b = first;
+  auto set = [&](int item, bool of_a) {
     const int split = item / (g.tm * g.tn);
     int tm, tn;
     gemm::tile_of(item - split * g.tm * g.tn, g.tm, g.tn, tm, tn);
     const int64_t k0 = split * g.kchunk, k1 = min(k0 + g.kchunk, g.K);
-    p.a.init(g.a, g.lda, g.M, (int64_t)tm * BM, k0, k1, wave, wm, lane);
-    p.b.init(g.b, g.ldb, g.N, (int64_t)tn * BN, k0, k1, wave, wn, lane);
-    p.item(k1 - k0);
+    if (of_a) p.a.init(g.a, g.lda, g.M, (int64_t)tm * BM, k0, k1, wave, wm, lane);
+    else p.b.init(g.b, g.ldb, g.N, (int64_t)tn * BN, k0, k1, wave, wn, lane);
   };
-  auto next = [&]() {
-    copying += per;
-    if (copying < end) {
-      set(copying);
-    } else {
-      p.a.end();
-      p.b.end();
-    }
+  auto next_a = [&]() {
+    item_a += per;
+    if (item_a < end) set(item_a, true);
+    else p.a.end();
   };
-  set(first);
-  p.start(lds, wave, next);
-  char* const mine = lds + P::LDS + wave * 32 * PITCH;
+  auto next_b = [&]() {
+    item_b += per;
+    if (item_b < end) set(item_b, false);
+    else p.b.end();
+  };
+  set(first, true);
+  set(first, false);
+  p.start(lds, wave, next_a, next_b);
   const int N = (int)g.N;
+  char* mine = nullptr;           // the wave's part of the spare slot
   auto chunk_at = [&](int r, int c) { return mine + r * PITCH + 16 * (c ^ (r % (8 * COLS))); };
 
   for (int item = first; item < end; item += per) {
@@ -276,7 +278,8 @@ __global__ __launch_bounds__(256, WG) void gemm_kernel(GemmArgs g) {
     // kept in registers through the product.
     int el = lane;
     if constexpr (KIND == kAny) {
-      p.run(acc, nt, next);
+      p.run(acc, nt, next_a, next_b);
+      mine = lds + p.spare() + wave * 32 * PITCH;
       asm volatile("" : "+v"(el));
       const int j = el % LPR, row = el / LPR;
 #pragma unroll 1
@@ -312,7 +315,8 @@ __global__ __launch_bounds__(256, WG) void gemm_kernel(GemmArgs g) {
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) bias[h] = u32x4{0u, 0u, 0u, 0u};
       }
-      p.run(acc, nt, next);
+      p.run(acc, nt, next_a, next_b);
+      mine = lds + p.spare() + wave * 32 * PITCH;
       asm volatile("" : "+v"(el));
       const int j = el % LPR, row = el / LPR;
       View vo, vz, vr, vg;
@@ -405,6 +409,8 @@ __global__ __launch_bounds__(256, WG) void gemm_kernel(GemmArgs g) {
 #pragma unroll
         for (int it = 0; it < ITS; ++it) vo.store(held[it], to[it]);
     }
+    // every wave is done with the spare slot before it is filled
+    barrier_lds();
   }
   // no copy may be on its way when the workgroup ends
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -442,17 +448,6 @@ __global__ __launch_bounds__(256) void join_kernel(GemmArgs g) {
 // v_mfma_f32_16x16x32: lane l holds row l % 16, k 8 (l / 16) .. + 8 of both operands,
 // and of the result row (channel) 4 (l / 16) + i, column (row of x) l % 16.
 
-typedef float acc4 __attribute__((ext_vector_type(4)));
-
-template <typename T>
-__device__ __forceinline__ acc4 mfma16(const u32x4& a, const u32x4& b, const acc4& c) {
-  const vec8<T> x = __builtin_bit_cast(vec8<T>, a), y = __builtin_bit_cast(vec8<T>, b);
-  if constexpr (__is_same(T, __bf16))
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0);
-}
-
 constexpr int kFewWaves = 8;
 constexpr int kFewAhead = 4;       // 32-wide pieces of K in flight
 
@@ -467,9 +462,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(GemmArgs g) {
 #pragma unroll
   for (int m = 0; m < MT; ++m)
     xp[m] = static_cast<const T*>(g.a) + min((int64_t)(16 * m + r), g.M - 1) * g.lda + kg;
-  acc4 acc[MT];
+  f32x4 acc[MT];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) acc[m] = acc4{0.f, 0.f, 0.f, 0.f};
+  for (int m = 0; m < MT; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
   // pieces of kFewAhead x 32 k, in turn over the waves
   constexpr int PIECE = 32 * kFewAhead;
   for (int64_t k0 = (int64_t)wave * PIECE; k0 < g.K; k0 += kFewWaves * PIECE) {
@@ -486,7 +481,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(GemmArgs g) {
 #pragma unroll
     for (int j = 0; j < kFewAhead; ++j)
 #pragma unroll
-      for (int m = 0; m < MT; ++m) acc[m] = mfma16<T>(w[j], x[m][j], acc[m]);
+      for (int m = 0; m < MT; ++m) acc[m] = gemm::mfma16<T>(w[j], x[m][j], acc[m]);
   }
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -656,10 +651,10 @@ int launch_gemm(GemmArgs g, const Plan& p, float* ws, bool rows16, hipStream_t s
   auto run = [&](auto kind) {
     constexpr int KIND = decltype(kind)::value;
     if (p.tile == 256)
-      hipLaunchKernelGGL((gemm_kernel<T, ATR, BTR, 256, 256, kBK, 2, 1, KIND>),
+      hipLaunchKernelGGL((gemm_kernel<T, ATR, BTR, 256, 256, kBK, 1, KIND>),
                          dim3((unsigned)xcd_grid(std::min<int64_t>(total, kSlots))), dim3(256), 0, st, g);
     else
-      hipLaunchKernelGGL((gemm_kernel<T, ATR, BTR, 128, 128, kBK, 2, 2, KIND>),
+      hipLaunchKernelGGL((gemm_kernel<T, ATR, BTR, 128, 128, kBK, 2, KIND>),
                          dim3((unsigned)xcd_grid(std::min<int64_t>(total, 2 * kSlots))), dim3(256), 0, st, g);
   };
   // (the parts' launch writes whole rows of its own)
