@@ -44,11 +44,15 @@ __device__ __forceinline__ float sigmoid(float x) {
 // tanh GELU as z sigmoid(2u), u = sqrt(2/pi) (z + 0.044715 z^3): no cancellation
 // where z is far below 0.
 constexpr float kGeluA = 1.5957691216057308f, kGeluB = 0.044715f;   // 2 sqrt(2/pi)
+__device__ __forceinline__ float gelu_gate(float z) {                // sigmoid(2u)
+  constexpr float L = -1.4426950408889634f;
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * fmaf(L * kGeluA * kGeluB, z * z, L * kGeluA)));
+}
 
 __device__ __forceinline__ void activate8(float* v, int act) {
   if (act == HIER_ACT_GELU_TANH) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= sigmoid(kGeluA * v[i] * fmaf(kGeluB, v[i] * v[i], 1.f));
+    for (int i = 0; i < 8; ++i) v[i] *= gelu_gate(v[i]);
   } else if (act == HIER_ACT_SILU) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] *= sigmoid(v[i]);
@@ -58,30 +62,25 @@ __device__ __forceinline__ void activate8(float* v, int act) {
   }
 }
 
-// act(z) and act'(z).  Past |z| = 30 the slopes are 0 or 1 to fp32: z is kept
+// act(z) and act'(z).  Past |z| = 30 (SiLU: 100) the slopes are 0 or 1 to fp32: z is kept
 // there, so no square of it overflows into inf * 0.
-__device__ __forceinline__ void activate2(float z, int act, float& a, float& slope) {
-  const float c = fminf(fmaxf(z, -30.f), 30.f);
-  switch (act) {
-    case HIER_ACT_GELU_TANH: {
-      const float s = sigmoid(kGeluA * c * fmaf(kGeluB, c * c, 1.f));
-      a = z * s;
-      slope = s + c * s * (1.f - s) * kGeluA * fmaf(3.f * kGeluB, c * c, 1.f);
-      return;
-    }
-    case HIER_ACT_GELU: {
-      const float half = 0.5f * erfcf(-0.7071067811865476f * z);
-      a = z * half;
-      slope = half + c * 0.3989422804014327f * __builtin_amdgcn_exp2f(-0.7213475204444817f * c * c);
-      return;
-    }
-    case HIER_ACT_SILU: {
-      const float w = fminf(fmaxf(z, -100.f), 100.f), s = sigmoid(w);
-      a = z * s;
-      slope = s + w * s * (1.f - s);
-      return;
-    }
-    default: a = z; slope = 1.f;
+template <int ACT>
+__device__ __forceinline__ void activate2(float z, float& a, float& slope) {
+  if constexpr (ACT == HIER_ACT_GELU_TANH) {
+    const float c = __builtin_amdgcn_fmed3f(z, -30.f, 30.f), s = gelu_gate(c);
+    a = z * s;
+    slope = fmaf(c * fmaf(3.f * kGeluA * kGeluB, c * c, kGeluA), fmaf(-s, s, s), s);
+  } else if constexpr (ACT == HIER_ACT_GELU) {
+    const float c = __builtin_amdgcn_fmed3f(z, -30.f, 30.f), half = 0.5f * erfcf(-0.7071067811865476f * z);
+    a = z * half;
+    slope = half + c * 0.3989422804014327f * __builtin_amdgcn_exp2f(-0.7213475204444817f * c * c);
+  } else if constexpr (ACT == HIER_ACT_SILU) {
+    const float c = __builtin_amdgcn_fmed3f(z, -100.f, 100.f), s = sigmoid(c);
+    a = z * s;
+    slope = fmaf(c, fmaf(-s, s, s), s);
+  } else {
+    a = z;
+    slope = 1.f;
   }
 }
 
@@ -522,11 +521,11 @@ struct DzArgs {
   int64_t dy_ss, z_ss, gate_ss, dz_ss;
   int64_t M, rpg;              // rows of a gate (M without gates)
   int64_t rows, segs;          // rows of a workgroup; its rows of a gate's, if split
-  int32_t N, act;
+  int32_t N;
   bool split;
 };
 
-template <typename T>
+template <typename T, int ACT, bool VEC>
 __global__ __launch_bounds__(256) void dz_kernel(DzArgs d) {
   const int n = 8 * (blockIdx.y * 256 + threadIdx.x);
   if (n >= d.N) return;
@@ -545,21 +544,31 @@ __global__ __launch_bounds__(256) void dz_kernel(DzArgs d) {
   for (int i = 0; i < 8; ++i) gate[i] = 1.f;
   int64_t g = r0 / d.rpg, gend = (g + 1) * d.rpg;
   if (d.gate) row8<T>(d.gate, g * d.gate_ss, n, d.N, gate);
-  constexpr int AHEAD = 4;
+  // AHEAD rows' loads leave together (VEC: no branch is between them)
+  constexpr int AHEAD = VEC ? 4 : 1;
   for (int64_t r = r0; r < r1; r += AHEAD) {
-    float y[AHEAD][8], z[AHEAD][8];
+    w32x4 yw[AHEAD], zw[AHEAD];
+    float y[8], z[8];
+    if constexpr (VEC) {
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      const int64_t row = min(r + j, r1 - 1);
-      row8<T>(d.dy, row * d.dy_ss, n, d.N, y[j]);
-      if (d.z) row8<T>(d.z, row * d.z_ss, n, d.N, z[j]);
-      else
+      for (int j = 0; j < AHEAD; ++j) yw[j] = raw8<T>(d.dy, min(r + j, r1 - 1) * d.dy_ss + n);
+      if (d.z)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) z[j][i] = 0.f;
+        for (int j = 0; j < AHEAD; ++j) zw[j] = raw8<T>(d.z, min(r + j, r1 - 1) * d.z_ss + n);
     }
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       if (r + j >= r1) break;
+      if constexpr (VEC) {
+        widen<T>(yw[j], y);
+        if (d.z) widen<T>(zw[j], z);
+      } else {
+        row8<T>(d.dy, r * d.dy_ss, n, d.N, y);
+        if (d.z) row8<T>(d.z, r * d.z_ss, n, d.N, z);
+      }
+      if (!d.z)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = 0.f;
       if (r + j == gend) {          // the next gate's rows begin (whole gates only)
         if (d.dgate) put_row8<T>(d.dgate, g * (int64_t)d.N, n, d.N, dg);
         ++g;
@@ -572,9 +581,9 @@ __global__ __launch_bounds__(256) void dz_kernel(DzArgs d) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         float a, slope;
-        activate2(z[j][i], d.act, a, slope);
-        dg[i] = fmaf(y[j][i], a, dg[i]);
-        dz[i] = y[j][i] * gate[i] * slope;
+        activate2<ACT>(z[i], a, slope);
+        dg[i] = fmaf(y[i], a, dg[i]);
+        dz[i] = y[i] * gate[i] * slope;
         db[i] += dz[i];
       }
       if (d.dz) put8<T>(d.dz, (r + j) * d.dz_ss + n, dz);
@@ -876,11 +885,21 @@ static int linear_bwd(const HierLinearBwdArgs& a, const BwdPlan& p, hipStream_t 
     d.rows = p.dz.rows;
     d.segs = p.dz.segs;
     d.N = a.N;
-    d.act = a.act;
     d.split = p.dz.split;
     const int64_t gy = (Np / 8 + 255) / 256;
     HIER_REQUIRE(gy <= 65535 && p.dz.total < (1ll << 24), HIER_EUNSUPPORTED, "linear_bwd: too many rows");
-    hipLaunchKernelGGL(dz_kernel<T>, dim3((unsigned)p.dz.total, (unsigned)gy), dim3(256), 0, st, d);
+    const dim3 grid((unsigned)p.dz.total, (unsigned)gy);
+    auto run = [&](auto kind) {
+      constexpr int ACT = decltype(kind)::value;
+      if (a.N % 8 == 0) hipLaunchKernelGGL((dz_kernel<T, ACT, true>), grid, dim3(256), 0, st, d);
+      else hipLaunchKernelGGL((dz_kernel<T, ACT, false>), grid, dim3(256), 0, st, d);
+    };
+    switch (a.act) {
+      case HIER_ACT_GELU_TANH: run(std::integral_constant<int, HIER_ACT_GELU_TANH>{}); break;
+      case HIER_ACT_GELU: run(std::integral_constant<int, HIER_ACT_GELU>{}); break;
+      case HIER_ACT_SILU: run(std::integral_constant<int, HIER_ACT_SILU>{}); break;
+      default: run(std::integral_constant<int, HIER_ACT_NONE>{});
+    }
     if (int rc = check_launch("dz_kernel")) return rc;
     if (a.db)
       if (int rc = sum_rows(d.db_part, p.dz.total, 1, a.N, a.db, a.type, st)) return rc;

@@ -67,21 +67,43 @@ __device__ __forceinline__ int channel(int i, int j, int t) {
   return VEC == 8 ? 8 * (i * 64 * WPR + t) + j : (8 * i + j) * 64 * WPR + t;
 }
 
+// Chunk i of a row as it lies in memory.  Lanes past the last channel read the
+// row's end and get zeros in `values`: without a branch around them all of a
+// row's loads leave together.
+template <typename T, int VEC>
+struct Raw {
+  w32x4 w;
+};
+template <typename T>
+struct Raw<T, 1> {
+  T v[8];
+};
 template <typename T, int VEC, int WPR>
-__device__ __forceinline__ void load8(const T* row, int i, int t, int C, float* f) {
+__device__ __forceinline__ Raw<T, VEC> fetch(const T* row, int i, int t, int C) {
+  Raw<T, VEC> r;
   if constexpr (VEC == 8) {
-    const int c = channel<8, WPR>(i, 0, t);
-    if (c < C) widen<T>(*reinterpret_cast<const w32x4*>(row + c), f);
-    else
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = 0.f;
+    r.w = *reinterpret_cast<const w32x4*>(row + min(channel<8, WPR>(i, 0, t), C - 8));
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = channel<1, WPR>(i, j, t);
-      f[j] = c < C ? (float)row[c] : 0.f;
-    }
+    for (int j = 0; j < 8; ++j) r.v[j] = row[min(channel<1, WPR>(i, j, t), C - 1)];
   }
+  return r;
+}
+template <typename T, int VEC, int WPR>
+__device__ __forceinline__ void values(const Raw<T, VEC>& r, int i, int t, int C, float* f) {
+  if constexpr (VEC == 8) {
+    widen<T>(r.w, f);
+    const bool in = channel<8, WPR>(i, 0, t) < C;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = in ? f[j] : 0.f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = channel<1, WPR>(i, j, t) < C ? (float)r.v[j] : 0.f;
+  }
+}
+template <typename T, int VEC, int WPR>
+__device__ __forceinline__ void load8(const T* row, int i, int t, int C, float* f) {
+  values<T, VEC, WPR>(fetch<T, VEC, WPR>(row, i, t, C), i, t, C, f);
 }
 
 template <typename T, int VEC, int WPR>
@@ -103,10 +125,20 @@ template <int VEC, int WPR>
 __device__ __forceinline__ void load_gain(const void* w, int type, int i, int t, int C, float* f) {
   if (type == HIER_FP32) {
     const float* p = static_cast<const float*>(w);
+    if constexpr (VEC == 8) {
+      const int c = channel<8, WPR>(i, 0, t), at = min(c, C - 8);
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(p + at), hi = *reinterpret_cast<const f32x4*>(p + at + 4);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = channel<VEC, WPR>(i, j, t);
-      f[j] = c < C ? p[c] : 0.f;
+      for (int j = 0; j < 4; ++j) {
+        f[j] = c < C ? lo[j] : 0.f;
+        f[4 + j] = c < C ? hi[j] : 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int c = channel<1, WPR>(i, j, t);
+        f[j] = c < C ? p[min(c, C - 1)] : 0.f;
+      }
     }
   } else if (type == HIER_BF16) {
     load8<__bf16, VEC, WPR>(static_cast<const __bf16*>(w), i, t, C, f);
@@ -141,16 +173,23 @@ __global__ __launch_bounds__(threads_of<WPR>()) void norm_kernel(HierRmsNormArgs
   const int t = threadIdx.x % (64 * WPR);
   const int64_t row = WPR == 1 ? (int64_t)blockIdx.x * 4 + threadIdx.x / 64 : blockIdx.x;
   if (row >= a.M) return;                // (WPR > 1: the whole workgroup or none of it)
-  float h[NCH][8];
+  float h[NCH][8], w[NCH][8];
   float sq = 0.f;
+  Raw<T, VEC> xr[NCH], rr[NCH];
 #pragma unroll
-  for (int i = 0; i < NCH; ++i)
-    load8<T, VEC, WPR>(static_cast<const T*>(a.x) + row * a.x_ss, i, t, a.C, h[i]);
+  for (int i = 0; i < NCH; ++i) xr[i] = fetch<T, VEC, WPR>(static_cast<const T*>(a.x) + row * a.x_ss, i, t, a.C);
+  if (a.r)
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) rr[i] = fetch<T, VEC, WPR>(static_cast<const T*>(a.r) + row * a.r_ss, i, t, a.C);
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) load_gain<VEC, WPR>(a.w, a.gain_type, i, t, a.C, w[i]);
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) values<T, VEC, WPR>(xr[i], i, t, a.C, h[i]);
   if (a.r) {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       float r[8];
-      load8<T, VEC, WPR>(static_cast<const T*>(a.r) + row * a.r_ss, i, t, a.C, r);
+      values<T, VEC, WPR>(rr[i], i, t, a.C, r);
 #pragma unroll
       for (int j = 0; j < 8; ++j) h[i][j] += r[j];
       store8<T, VEC, WPR>(static_cast<T*>(a.h) + row * a.h_ss, i, t, a.C, h[i]);
@@ -163,10 +202,9 @@ __global__ __launch_bounds__(threads_of<WPR>()) void norm_kernel(HierRmsNormArgs
   const float s = 1.f / sqrtf(row_sum<WPR>(sq, lds) / (float)a.C + a.eps);
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    float w[8], y[8];
-    load_gain<VEC, WPR>(a.w, a.gain_type, i, t, a.C, w);
+    float y[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = h[i][j] * s * w[j];
+    for (int j = 0; j < 8; ++j) y[j] = h[i][j] * s * w[i][j];
     store8<T, VEC, WPR>(static_cast<T*>(a.y) + row * a.y_ss, i, t, a.C, y);
   }
 }
@@ -188,16 +226,29 @@ __global__ __launch_bounds__(threads_of<WPR>()) void norm_bwd_kernel(HierRmsNorm
   for (int64_t row = first; row < a.M; row += (int64_t)gridDim.x * ROWS) {
     float h[NCH][8], g[NCH][8];
     float sq = 0.f, dot = 0.f;
+    Raw<T, VEC> xr[NCH], rr[NCH], gr[NCH], dr[NCH];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      load8<T, VEC, WPR>(static_cast<const T*>(a.x) + row * a.x_ss, i, t, a.C, h[i]);
-      load8<T, VEC, WPR>(static_cast<const T*>(a.dy) + row * a.dy_ss, i, t, a.C, g[i]);
+      xr[i] = fetch<T, VEC, WPR>(static_cast<const T*>(a.x) + row * a.x_ss, i, t, a.C);
+      gr[i] = fetch<T, VEC, WPR>(static_cast<const T*>(a.dy) + row * a.dy_ss, i, t, a.C);
+    }
+    if (a.r)
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) rr[i] = fetch<T, VEC, WPR>(static_cast<const T*>(a.r) + row * a.r_ss, i, t, a.C);
+    if (a.dh)
+#pragma unroll
+      for (int i = 0; i < NCH; ++i)
+        dr[i] = fetch<T, VEC, WPR>(static_cast<const T*>(a.dh) + row * a.dh_ss, i, t, a.C);
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      values<T, VEC, WPR>(xr[i], i, t, a.C, h[i]);
+      values<T, VEC, WPR>(gr[i], i, t, a.C, g[i]);
     }
     if (a.r)
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
         float r[8];
-        load8<T, VEC, WPR>(static_cast<const T*>(a.r) + row * a.r_ss, i, t, a.C, r);
+        values<T, VEC, WPR>(rr[i], i, t, a.C, r);
 #pragma unroll
         for (int j = 0; j < 8; ++j) h[i][j] += r[j];
       }
@@ -219,7 +270,7 @@ __global__ __launch_bounds__(threads_of<WPR>()) void norm_bwd_kernel(HierRmsNorm
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       float d[8] = {};
-      if (a.dh) load8<T, VEC, WPR>(static_cast<const T*>(a.dh) + row * a.dh_ss, i, t, a.C, d);
+      if (a.dh) values<T, VEC, WPR>(dr[i], i, t, a.C, d);
 #pragma unroll
       for (int j = 0; j < 8; ++j) d[j] = fmaf(s, fmaf(-h[i][j], mean, g[i][j]), d[j]);
       store8<T, VEC, WPR>(static_cast<T*>(a.dx) + row * a.dx_ss, i, t, a.C, d);
