@@ -179,8 +179,8 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(Launch p) {
   const int logical = xcd_logical(blockIdx.x, gridDim.x);
   const HierCrossArgs& a = p.a.f;
   if (logical >= a.B * a.Hk * p.row_tiles) return;
-  const int bh = logical / p.row_tiles, rt = logical - bh * p.row_tiles;
-  const int b = bh / a.Hk, hk = bh - b * a.Hk;
+  const int hb = logical / p.row_tiles, rt = logical - hb * p.row_tiles;
+  const int hk = hb / a.B, b = hb - hk * a.B, bh = b * a.Hk + hk;      // (as the forward's)
   QWork<D> w;
   w.lane = threadIdx.x & 63;
   w.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -302,9 +302,9 @@ __global__ __launch_bounds__(512, 1) void cross_dkv_kernel(Launch p) {
   if (logical >= p.total) return;
   const HierCrossArgs& a = p.a.f;
   const int per = p.key_tiles * p.splits;
-  const int bh = logical / per, in = logical - bh * per;
+  const int hb = logical / per, in = logical - hb * per;
   const int split = in / p.key_tiles, kt = in - split * p.key_tiles;
-  const int b = bh / a.Hk, hk = bh - b * a.Hk;
+  const int hk = hb / a.B, b = hb - hk * a.B, bh = b * a.Hk + hk;
   KWork<D> w;
   w.lane = threadIdx.x & 63;
   const int wave8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

@@ -267,11 +267,13 @@ __global__ __launch_bounds__(kThreads, 2) void cross_fwd_kernel(Launch p) {
   const int logical = xcd_logical(blockIdx.x, gridDim.x);
   if (logical >= p.total) return;
   const HierCrossArgs& a = p.a;
-  // items of one (stream, key head) are neighbours: they share its keys in one L2
+  // items of one (stream, key head) are neighbours: they share its keys in one L2.
+  // Streams take turns, so that one of few keys leaves no XCD without work (ten
+  // streams of 660 queries, of 512 keys or fewer: 43 -> 36 us)
   const int per = p.row_tiles * p.splits;
-  const int bh = logical / per, in = logical - bh * per;
+  const int hb = logical / per, in = logical - hb * per;
   const int split = in / p.row_tiles, rt = in - split * p.row_tiles;
-  const int b = bh / a.Hk, hk = bh - b * a.Hk;
+  const int hk = hb / a.B, b = hb - hk * a.B, bh = b * a.Hk + hk;
   Work<T, D> w;
   w.lane = threadIdx.x & 63;
   w.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
