@@ -250,7 +250,7 @@ def _linear(x, weight, bias, activation, residual, gate, out, preact):
     g, g_ss = (None, 0) if gate is None else _rows(gate)
     fields = (M, N, K, kind, act, xr.data_ptr(), w.data_ptr(), _ptr(b), _ptr(r), _ptr(g), out.data_ptr(),
               _ptr(preact), x_ss, w_ss, r_ss, g_ss, N, N, per)
-    size = 0 if M <= 64 else _workspace("hier_linear_workspace", _pack_linear(*fields, 0, 0))
+    size = 0 if M <= 8 else _workspace("hier_linear_workspace", _pack_linear(*fields, 0, 0))
     ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
     _capi.call_on(x.device, "hier_linear", _pack_linear(*fields, _ptr(ws), size))
     return out

@@ -103,8 +103,11 @@ __device__ __forceinline__ void row8(const void* p, int64_t at, int n, int N, fl
   if (n + 8 <= N) {
     widen<T>(raw8<T>(p, at + n), f);
   } else {
+    T t[8];                    // (the last one's again past the end: no branch is between the loads)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = n + i < N ? (float)static_cast<const T*>(p)[at + n + i] : 0.f;
+    for (int i = 0; i < 8; ++i) t[i] = static_cast<const T*>(p)[at + min(n + i, N - 1)];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = n + i < N ? (float)t[i] : 0.f;
   }
 }
 template <typename T>
@@ -172,6 +175,9 @@ struct View {
   }
   __device__ __forceinline__ u32x4 load(uint32_t off) const {
     return __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, 0);
+  }
+  __device__ __forceinline__ u32x4 load_once(uint32_t off) const {      // not kept in the caches
+    return __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, 2);
   }
   __device__ __forceinline__ void store(const u32x4& v, uint32_t off) const {
     __builtin_amdgcn_raw_buffer_store_b128(v, rsrc, off, 0, 0);
@@ -421,17 +427,23 @@ __global__ __launch_bounds__(256) void join_kernel(GemmArgs g) {
   const int cpr = (int)((g.N + 7) / 8);
   const int64_t n8 = g.M * cpr;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n8; i += (int64_t)gridDim.x * 256) {
-    const int64_t m = i / cpr;
+    const int64_t m = n8 >> 32 ? i / cpr : (uint32_t)i / (uint32_t)cpr;
     const int n = 8 * (int)(i - m * cpr);
     const float* p = g.e.partial + m * g.e.ld_part + n;
     float v[8] = {};
-    for (int s = 0; s < g.splits; ++s) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(p + s * g.e.part_stride);
-      const f32x4 y = *reinterpret_cast<const f32x4*>(p + s * g.e.part_stride + 4);
+    // (four splits' loads leave together, the last split's again past the end)
+    for (int s = 0; s < g.splits; s += 4) {
+      f32x4 x[4][2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[j] += x[j];
-        v[4 + j] += y[j];
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          x[i][h] = *reinterpret_cast<const f32x4*>(p + min(s + i, g.splits - 1) * g.e.part_stride + 4 * h);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (s + i >= g.splits) break;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += x[i][j / 4][j % 4];
       }
     }
     finish8<T>(g.e, v, m, n, (int)g.N);
@@ -440,10 +452,11 @@ __global__ __launch_bounds__(256) void join_kernel(GemmArgs g) {
 
 // ---- few rows --------------------------------------------------------------------
 //
-// At most 64 rows of x: the weights are what is read, each once.  A workgroup of
-// eight waves takes 16 output channels, a wave every eighth 64-wide piece of K, with
-// its weights straight from memory into the MFMA's registers (16 rows x 32 k:
-// 16 bytes a lane), several pieces ahead; the eight sums meet in LDS.
+// Up to 64 rows of x, of weights that are not many (few_rows).  A workgroup of eight
+// waves takes 16 output channels, a wave every eighth 128-wide piece of K, with its
+// weights straight from memory into the MFMA's registers (16 rows x 32 k: 16 bytes a
+// lane); the eight sums meet in LDS.  Bound by a wait for memory a piece and by x,
+// read again for every 16 channels: 9 / 64 rows of 1536 x 1536 5.2 / 10.2 us.
 // v_mfma_f32_16x16x32: lane l holds row l % 16, k 8 (l / 16) .. + 8 of both operands,
 // and of the result row (channel) 4 (l / 16) + i, column (row of x) l % 16.
 
@@ -502,6 +515,93 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(GemmArgs g) {
     v[i] = s;
   }
   finish8<T>(g.e, v, m, n, (int)g.N);
+}
+
+// ---- fewer rows still ------------------------------------------------------------
+//
+// At most eight rows of x: one product a weight and row, on the vector units, with
+// the weights in the order of memory (a wave's load is 1 KB of one channel, where
+// few_rows_kernel's takes 64 bytes of 16).  A workgroup of four waves takes CH
+// channels, a wave every fourth 512-wide piece of K of all of them, x's piece read
+// once for them; the sums meet in LDS.  Measured for 1 row of K 1536 x N 8960 /
+// 8960 x 1536 / 4096 x 16384 (weights of 27.5, 27.5 and 134 MB): 6.2 / 6.4 / 21 us
+// (6.3 TB/s), of few_rows_kernel 9.0 / 14.8 / 27; 8 rows 10.5 / 11.6 / 26 for 10.7 /
+// 18 / 32.  More channels a workgroup read x less often, fewer make more workgroups:
+// two up to two rows, else as many as the rows (1 row with 8: 6.4 / 7.2 / 22; 8 rows
+// with 2: 10.7 / 11.6 / 43).
+
+template <typename T>
+__device__ __forceinline__ float dot8(const u32x4& a, const u32x4& b, float c) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t x = a[e], y = b[e];     // (a bit cast of an element reads the first)
+    if constexpr (__is_same(T, __bf16)) {
+      typedef __bf16 pair __attribute__((ext_vector_type(2)));
+      c = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair, x), __builtin_bit_cast(pair, y), c, false);
+    } else {
+      typedef _Float16 pair __attribute__((ext_vector_type(2)));
+      c = __builtin_amdgcn_fdot2(__builtin_bit_cast(pair, x), __builtin_bit_cast(pair, y), c, false);
+    }
+  }
+  return c;
+}
+
+// Sums of N lanes' values over the wave: lane l returns that of value l % N.  Each step
+// hands half of the values to the lanes that keep the other half.
+template <int N>
+__device__ __forceinline__ float wave_sums(float* v, int lane) {
+#pragma unroll
+  for (int n = N / 2, d = 1; d < 64; n /= 2, d *= 2) {
+    if (n > 0) {
+      const bool odd = lane & d;
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        const float keep = odd ? v[2 * i + 1] : v[2 * i], give = odd ? v[2 * i] : v[2 * i + 1];
+        v[i] = keep + __shfl_xor(give, d, 64);
+      }
+    } else {
+      v[0] += __shfl_xor(v[0], d, 64);
+    }
+  }
+  return v[0];
+}
+
+constexpr int kDotRows = 8;
+
+template <typename T, int M>       // M rows of x at most: 1, 2, 4 or 8
+__global__ __launch_bounds__(256) void dot_kernel(GemmArgs g) {
+  constexpr int CH = M < 2 ? 2 : M;
+  __shared__ float sums[4][M * CH];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t n0 = (int64_t)CH * blockIdx.x;
+  View wv[CH], xv[M];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) wv[c].init(g.b, 2 * min(n0 + c, g.N - 1) * g.ldb);
+#pragma unroll
+  for (int m = 0; m < M; ++m) xv[m].init(g.a, 2 * min((int64_t)m, g.M - 1) * g.lda);
+  float acc[M * CH] = {};
+  const int K = (int)g.K;
+  for (int k0 = 512 * wave; k0 < K; k0 += 2048) {
+    const int k = k0 + 8 * lane;
+    const uint32_t at = k < K ? 2u * k : gemm::kOut;       // (K is a multiple of 8; out of range gives zeros)
+    u32x4 w[CH], x[M];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) w[c] = wv[c].load_once(at);
+#pragma unroll
+    for (int m = 0; m < M; ++m) x[m] = xv[m].load(at);
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int c = 0; c < CH; ++c) acc[m * CH + c] = dot8<T>(w[c], x[m], acc[m * CH + c]);
+  }
+  const float s = wave_sums<M * CH>(acc, lane);
+  if (lane < M * CH) sums[wave][lane] = s;
+  __syncthreads();
+  // thread: a channel of a row
+  const int t = threadIdx.x, m = t / CH, n = (int)n0 + t % CH;
+  if (t >= M * CH || m >= g.M || n >= g.N) return;
+  float v[8] = {sums[0][t] + sums[1][t] + sums[2][t] + sums[3][t]};
+  finish8<T>(g.e, v, m, n, n + 1);
 }
 
 // ---- dz, db and dg ---------------------------------------------------------------
@@ -686,6 +786,15 @@ int launch_gemm(GemmArgs g, const Plan& p, float* ws, bool rows16, hipStream_t s
 
 template <typename T>
 int launch_few(const GemmArgs& g, hipStream_t st) {
+  auto dots = [&](auto rows) {
+    constexpr int M = decltype(rows)::value, CH = M < 2 ? 2 : M;
+    hipLaunchKernelGGL((dot_kernel<T, M>), dim3((unsigned)((g.N + CH - 1) / CH)), dim3(256), 0, st, g);
+    return check_launch("dot_kernel");
+  };
+  if (g.M == 1) return dots(std::integral_constant<int, 1>{});
+  if (g.M == 2) return dots(std::integral_constant<int, 2>{});
+  if (g.M <= 4) return dots(std::integral_constant<int, 4>{});
+  if (g.M <= kDotRows) return dots(std::integral_constant<int, 8>{});
   const dim3 grid((unsigned)((g.N + 15) / 16)), block(64 * kFewWaves);
   if (g.M <= 16) hipLaunchKernelGGL((few_rows_kernel<T, 1>), grid, block, 0, st, g);
   else if (g.M <= 32) hipLaunchKernelGGL((few_rows_kernel<T, 2>), grid, block, 0, st, g);
@@ -693,7 +802,11 @@ int launch_few(const GemmArgs& g, hipStream_t st) {
   return check_launch("few_rows_kernel");
 }
 
-bool few_rows(int64_t M) { return M <= 64; }
+// Whether dot_kernel or few_rows_kernel takes a product.  The second reads x again for
+// every 16 channels: past some 200 million products the tiles win (64 rows of 1536 x 1536 10.1
+// us for 11.1; 17 of 1536 x 8960 13.5 for 15.7, 32 of them 17.8 for 15.7; 16 of 8960 x
+// 1536 22 for 18.4, of 4096 x 16384 38 for 34.7).
+bool few_rows(int64_t M, int64_t N, int64_t K) { return M <= kDotRows || (M <= 64 && M * N * K <= 200000000); }
 
 // Views that the copies address: 16-byte rows, a tile's rows (256) within 31
 // bits of bytes.
@@ -795,7 +908,7 @@ static int check_linear(const HierLinearArgs& a) {
 extern "C" int64_t hier_linear_workspace(const HierLinearArgs* a) {
   clear_error();
   if (!a || check_linear(*a)) return -1;
-  return a->M == 0 || few_rows(a->M) ? 0 : plan_of(a->M, a->N, a->K).bytes;
+  return a->M == 0 || few_rows(a->M, a->N, a->K) ? 0 : plan_of(a->M, a->N, a->K).bytes;
 }
 
 extern "C" int hier_linear(const HierLinearArgs* args, void* stream) {
@@ -831,7 +944,7 @@ extern "C" int hier_linear(const HierLinearArgs* args, void* stream) {
   e.rows_per_gate = make_div(a.gate ? (uint32_t)a.rows_per_gate : 1u);
   e.act = a.act;
   const hipStream_t st = (hipStream_t)stream;
-  if (few_rows(a.M)) return a.type == HIER_BF16 ? launch_few<__bf16>(g, st) : launch_few<_Float16>(g, st);
+  if (few_rows(a.M, a.N, a.K)) return a.type == HIER_BF16 ? launch_few<__bf16>(g, st) : launch_few<_Float16>(g, st);
   const Plan p = plan_of(a.M, a.N, a.K);
   HIER_REQUIRE(p.bytes == 0 || (a.workspace && aligned16(a.workspace) && a.workspace_bytes >= p.bytes),
                HIER_EINVAL, "linear: workspace of %lld bytes needed", (long long)p.bytes);

@@ -161,6 +161,14 @@ LINEARS = [
     (1000, 136, 1032, "gelu_tanh", 5, True, BF16),
     (1, 70, 4099, None, 0, False, FP16),
     (600, 8, 8, "silu", 0, False, BF16),
+    (2, 2500, 33, "silu", 2, True, BF16),          # eight rows or fewer: every count of rows, K past
+    (3, 4104, 10, "gelu_tanh", 1, True, FP16),     # a pass of the waves, channels past the last group
+    (4, 2049, 3, None, 0, True, BF16),
+    (5, 512, 1, "gelu", 5, True, FP16),
+    (7, 520, 63, "silu", 0, False, BF16),
+    (8, 6000, 72, "gelu_tanh", 2, True, BF16),
+    (9, 2056, 100, None, 3, True, FP16),
+    (16, 4000, 4000, "silu", 4, True, BF16),       # few rows of many weights: over tiles
 ]
 LIPSCHITZ = 1.2          # bounds every activation's slope; their second derivatives are under 1
 
@@ -464,6 +472,30 @@ def test_large_scores_keep_their_softmax():
             got = kernels.cross_attention(q, k, v)
             want = (p[:, None, None] * v[0].double()).sum(0)
             assert bool(((got[0].double() - want).abs() <= 2.0 ** -7 * (want.abs() + 1e-3)).all()), (big, sign)
+
+
+def test_small_weights_count_in_the_sum():
+    """One key whose score is far above thousands of equal others: their weights, subnormal in
+    fp16, are in the sum as they are in the product."""
+    need_gpu()
+    S, D, R = 4096, 64, 66000            # rows enough that no split has a maximum of its own
+    for t, gap in ((FP16, 11.0), (FP16, 14.0), (BF16, 14.0)):
+        q, k = torch.zeros(1, R, 1, D, dtype=t, device="cuda"), torch.zeros(1, S, 1, D, dtype=t, device="cuda")
+        q[..., 0], k[:, 1:, :, 0] = 8.0, -gap            # scores -gap at a scale of 1/8
+        v = (1 + _rnd(5)(1, S, 1, D)).to(t)
+        lse = torch.empty(1, 1, R, device="cuda")
+        say("small weights", t, gap)
+        out = kernels.cross_attention(q, k, v, lse=lse)
+        w = torch.full((S,), -gap, dtype=torch.float64, device="cuda").exp()
+        w[0] = 1.0
+        want = (w[:, None] * v[0, :, 0].double()).sum(0) / w.sum()
+        # weights: each off by half a step of the type, for fp16 below 2^-14 by at most 2^-25; both
+        # enter O's numerator (|v| <= 6) and its sum, which is that of the rounded weights
+        half = torch.finfo(t).eps / 2
+        wobble = (half * w.sum() + S * (2.0 ** -25 if t == FP16 else 0.0)) / w.sum() * 2 * 6 + 2.0 ** -12
+        err = (out[0, :, 0].double() - want).abs()
+        assert bool((err <= half * want.abs() + wobble).all())
+        assert bool((lse - w.sum().log()).abs().max() <= half + S * 2.0 ** -25 + 2.0 ** -12)
 
 
 def test_growing_scores_refresh_the_maximum():
