@@ -40,12 +40,12 @@ struct Rows64 {
 #pragma unroll
     for (int e = 0; e < Geo<D>::NI; ++e) voff[e] = (uint32_t)((first + e) * (int)(2 * ss)) + c.add(e);
   }
-  // Rows of the tile at byte address `base`, `rows` of them (or fewer) in range;
-  // with MASK only those whose bit of `seen` is set.
-  template <bool MASK>
+  // Rows of the tile (of SPAN) at byte address `base`, `rows` of them (or fewer) in
+  // range; with MASK only those whose bit of `seen` is set.
+  template <bool MASK, int SPAN = kSlab>
   __device__ __forceinline__ void copy(uint64_t base, int64_t rows, int64_t ss, uint64_t seen, const char* slot,
                                        int wave) const {
-    const int64_t left = rows <= 0 ? 0 : rows >= kSlab ? 0x7fffffff : 2 * ((rows - 1) * ss + D);
+    const int64_t left = rows <= 0 ? 0 : rows >= SPAN ? 0x7fffffff : 2 * ((rows - 1) * ss + D);
     const u32x4 srd = {(uint32_t)base, (uint32_t)(base >> 32) & 0xffffu, (uint32_t)left, 0x00020000u};
     const uint32_t bits = MASK ? (uint32_t)(seen >> first) : 0u;
 #pragma unroll

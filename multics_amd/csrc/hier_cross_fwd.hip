@@ -20,6 +20,7 @@
 #include "hier_cross.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace hier {
 namespace {
@@ -361,9 +362,177 @@ __global__ __launch_bounds__(kThreads, 2) void cross_fwd_kernel(Launch p) {
   store_row<T, D>(p, w, valid, q, head, b, prow, split);
 }
 
+// ---- few rows --------------------------------------------------------------------
+//
+// At most 32 rows of a key head (a token of a few query heads): the keys are what is
+// read, each once, and nothing is shared by the waves.  Each takes every fourth 64-key
+// tile of the item through an LDS tile of its own, with its own waits and no barrier:
+// K's next tile leaves as soon as the scores are made, V's after PV.  The four waves'
+// O, maximum and sum meet in LDS.  Bound by memory, and by the start and the join where
+// the keys are few: four streams of 8 heads and 4,096 keys (67 MB) 17.3 us with the join
+// (3.9 TB/s; the 128-row kernel, whose waves wait for one another's tiles, 27.8), one of
+// 8 and 8,192 keys 14.6 (29.3), 64 of 12 and 512 keys (201 MB) 42 (44; 4.8 TB/s).
+
+constexpr int kFewRows = 32;
+
+template <int N>
+__device__ __forceinline__ void wait_own() {     // at most N of the wave's copies in flight, its LDS reads done
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "i"(N) : "memory");
+}
+
+template <typename T, int D, int WAVES, bool MASK>
+__global__ __launch_bounds__(64 * WAVES, 1) void cross_few_kernel(Launch p) {
+  constexpr int COPIES = 4 * Geo<D>::NI;         // instructions of a tile
+  constexpr int Q4 = D / 4;                      // 16-byte pieces of a row of O
+  __shared__ __align__(16) char lds[WAVES][2][Geo<D>::TILEB];
+  __shared__ float stat[WAVES][2][kFewRows];
+  static_assert(kFewRows * D * 4 <= 2 * Geo<D>::TILEB, "a wave's O fits its tiles");
+  const int logical = xcd_logical(blockIdx.x, gridDim.x);
+  if (logical >= p.total) return;
+  const HierCrossArgs& a = p.a;
+  const int hb = logical / p.splits, split = logical - hb * p.splits;
+  const int hk = hb / a.B, b = hb - hk * a.B, bh = b * a.Hk + hk;       // (as above)
+  Work<T, D> w;
+  w.lane = threadIdx.x & 63;
+  w.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int64_t len = a.Sk;
+  if (a.kv_lens) len = min(max((int64_t)a.kv_lens[b], (int64_t)0), a.Sk);
+  const int tiles = (int)((len + kSlab - 1) / kSlab);
+  const int each = (tiles + p.splits - 1) / p.splits;
+  const int first = min(split * each, tiles) + w.wave, end = min((split + 1) * each, tiles);
+  const uint64_t kbase = (uint64_t)a.k + 2 * (b * a.k_sb + hk * a.k_sh);
+  const uint64_t vbase = (uint64_t)a.v + 2 * (b * a.v_sb + hk * a.v_sh);
+  const uint8_t* mask = MASK ? a.key_mask + b * a.mask_sb + w.lane : nullptr;
+  w.ck.init(0, w.lane, a.k_ss);
+  w.cv.init(0, w.lane, a.v_ss);
+#pragma unroll
+  for (int c = 0; c < Geo<D>::NC; ++c) w.krd[c] = tile::row_read_off<D, kRowRead>(w.lane, c);
+#pragma unroll
+  for (int d = 0; d < Geo<D>::NDB; ++d) w.vrd[d] = tile::tr_read_off<D, kTrRead>(w.lane, d, 0);
+  const uint32_t R = (uint32_t)(a.Sq * p.div.g);
+  {
+    const uint32_t r = min((uint32_t)w.lane & 31, R - 1), q = quotient(r, p.div);
+    const int head = hk * (int)p.div.g + (int)(r - q * p.div.g);
+    load_row<D>(w.q, static_cast<const uint16_t*>(a.q) + b * a.q_sb + (int64_t)q * a.q_ss + head * a.q_sh, w.lane);
+  }
+  w.m = 0.f;
+  w.l = 0.f;
+  w.c2 = a.scale * kLog2e;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w.negm[i] = 0.f;
+#pragma unroll
+  for (int d = 0; d < Geo<D>::NDB; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w.o[d][i] = 0.f;
+  char* const ks = lds[w.wave][0];
+  char* const vs = lds[w.wave][1];
+  auto byte_of = [&](int t) -> uint32_t {
+    if constexpr (MASK) return (int64_t)t * kSlab + w.lane < len ? mask[(int64_t)t * kSlab] : 0u;
+    else return 0u;
+  };
+  // rows 16 i .. + 16 of a tile are the copies of a workgroup's wave i
+  auto copy = [&](const auto& c, uint64_t base, int64_t ss, int t, uint64_t seen, char* slot) {
+    const int64_t key0 = (int64_t)t * kSlab;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      c.template copy<MASK, 16>(base + (uint64_t)((key0 + 16 * i) * 2 * ss), len - key0 - 16 * i, ss, seen >> (16 * i),
+                                slot, i);
+  };
+  if (first < end) {
+    uint64_t seen = seen_keys<MASK>(len, first, byte_of(first));
+    copy(w.ck, kbase, a.k_ss, first, seen, ks);
+    copy(w.cv, vbase, a.v_ss, first, seen, vs);
+    // Q too, here: the compiler, which does not see the copies, would wait for all of them in the loop
+#pragma unroll
+    for (int c = 0; c < Geo<D>::NC; ++c) asm volatile("" : "+v"(w.q[c]));
+    for (int t = first; t < end; t += WAVES) {
+      const bool more = t + WAVES < end;
+      const uint32_t mb = more ? byte_of(t + WAVES) : 0u;
+      wait_own<COPIES>();                        // K is there
+      f32x16 sa = scores<T, D>(w, ks, 0), sb = scores<T, D>(w, ks, 1);
+      const uint64_t now = seen;
+      seen = seen_keys<MASK>(len, t + WAVES, mb);
+      wait_own<COPIES>();                        // (its LDS reads)
+      if (more) copy(w.ck, kbase, a.k_ss, t + WAVES, seen, ks);
+      if (now != ~0ull) {
+        mask_scores(sa, (uint32_t)now, w.lane);
+        mask_scores(sb, (uint32_t)(now >> 32), w.lane);
+      }
+      u32x4 pa[2], pb[2];
+      float alpha = 1.f;
+      bool resc = settle<T, D>(w, sa, sb, pa, weights<T>(sa, pa, w.c2), alpha);
+      if (resc) rescale<T, D>(w, alpha);
+      resc = settle<T, D>(w, sb, sa, pb, weights<T>(sb, pb, w.c2), alpha);
+      if (more) wait_own<COPIES>();              // V is there
+      else wait_own<0>();
+      weigh<T, D>(w, pa, vs, 0);
+      if (resc) rescale<T, D>(w, alpha);
+      weigh<T, D>(w, pb, vs, 1);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (more) copy(w.cv, vbase, a.v_ss, t + WAVES, seen, vs);
+    }
+  }
+  // the waves' results, 16-byte pieces of a row swizzled by the row
+  const int row = w.lane & 31, half = w.lane >> 5;
+  {
+    const float l = tile::pair_sum(w.l);
+    if (half == 0) {
+      stat[w.wave][0][row] = w.m;
+      stat[w.wave][1][row] = l;
+    }
+    f32x4* const mine = reinterpret_cast<f32x4*>(ks) + row * Q4;
+#pragma unroll
+    for (int d = 0; d < Geo<D>::NDB; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        mine[(8 * d + 2 * g + half) ^ (row & (Q4 - 1))] =
+            f32x4{w.o[d][4 * g], w.o[d][4 * g + 1], w.o[d][4 * g + 2], w.o[d][4 * g + 3]};
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < (int)R * Q4; i += 64 * WAVES) {
+    const uint32_t r = i / Q4, c = i % Q4;
+    float top = -INFINITY, l = 0.f, wt[WAVES];
+#pragma unroll
+    for (int j = 0; j < WAVES; ++j) {
+      wt[j] = stat[j][1][r] == 0.f ? -INFINITY : stat[j][0][r];
+      top = fmaxf(top, wt[j]);
+    }
+    f32x4 o = {};
+#pragma unroll
+    for (int j = 0; j < WAVES; ++j) {
+      const float lj = stat[j][1][r];
+      wt[j] = lj == 0.f ? 0.f : __builtin_amdgcn_exp2f((wt[j] - top) * w.c2);
+      l += lj * wt[j];
+      const f32x4 x = reinterpret_cast<const f32x4*>(lds[j][0])[r * Q4 + (c ^ (r & (Q4 - 1)))];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], wt[j], o[e]);
+    }
+    if (p.splits > 1) {
+      const int64_t at = ((int64_t)split * a.B * a.Hk + bh) * R + r;
+      *reinterpret_cast<f32x4*>(p.part_o + at * D + 4 * c) = o;
+      if (c == 0) {
+        p.part_ml[2 * at] = top;
+        p.part_ml[2 * at + 1] = l;
+      }
+      continue;
+    }
+    const uint32_t q = quotient(r, p.div);
+    const int head = hk * (int)p.div.g + (int)(r - q * p.div.g);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    typedef T quad __attribute__((ext_vector_type(4)));
+    quad v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (T)(o[e] * inv);
+    *reinterpret_cast<u32x2*>(static_cast<T*>(a.o) + b * a.o_sb + (int64_t)q * a.o_ss + head * a.o_sh + 4 * c) =
+        __builtin_bit_cast(u32x2, v);
+    if (a.lse && c == 0)
+      a.lse[((int64_t)b * a.Hq + head) * a.Sq + q] = l == 0.f ? -INFINITY : top * a.scale + __logf(l);
+  }
+}
+
 // ---- the splits' join ------------------------------------------------------------
 
-constexpr int kMaxSplits = 64;
+constexpr int kMaxSplits = 64;      // a lane of the join each
 
 // A wave a row: lane s holds split s's maximum and sum.
 template <typename T, int D>
@@ -389,11 +558,21 @@ __global__ __launch_bounds__(256) void cross_join_kernel(Launch p) {
   for (int d = 32; d > 0; d /= 2) total += __shfl_xor(total, d, 64);
   constexpr int E = D / 64;
   float o[E] = {};
-  for (int s = 0; s < p.splits; ++s) {
-    const float ws = __shfl(weight, s, 64);
-    const float* src = p.part_o + ((int64_t)s * rows + row) * D + E * lane;
+  // (eight splits' loads leave together, the last split's again past the end)
+  for (int s0 = 0; s0 < p.splits; s0 += 8) {
+    float x[8][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(src[e], ws, o[e]);
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        x[i][e] = p.part_o[((int64_t)min(s0 + i, p.splits - 1) * rows + row) * D + E * lane + e];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float ws = __shfl(weight, (s0 + i) & 63, 64);
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (s0 + i < p.splits) o[e] = fmaf(x[i][e], ws, o[e]);
+    }
   }
   const int R = (int)(a.Sq * p.div.g);
   const int bh = (int)(row / R);
@@ -409,9 +588,23 @@ __global__ __launch_bounds__(256) void cross_join_kernel(Launch p) {
 
 // Parts of every key list: one where the items fill the 512 workgroups that run at
 // once, else enough for 768 of them, of two tiles at least.
+// (few rows: workgroups for the 256 CUs, of a tile a wave at least.)
+bool few_rows(const HierCrossArgs& a) { return a.Sq * (a.Hq / a.Hk) <= kFewRows; }
+
+// Waves of a few-row workgroup: two (and two workgroups a CU) where the items need no
+// splits, so that streams of unlike lengths and of two tiles leave fewer waves without
+// work, else four (less to join).  64 streams of 8 heads and 77 keys 8.4 us with two,
+// 11.9 with four; 64 of 12 and 512 keys or fewer 27 / 31; 16 of 12 and 512 15 / 11.7;
+// one of 8 and 8,192 17 / 14.6.
+int few_waves(const HierCrossArgs& a) { return (int64_t)a.B * a.Hk >= 512 ? 2 : 4; }
+
 int splits_of(const HierCrossArgs& a) {
   const int64_t items = (int64_t)a.B * a.Hk * row_tiles(a.Sq * (a.Hq / a.Hk));
   const int64_t tiles = (a.Sk + kSlab - 1) / kSlab;
+  if (few_rows(a) && items > 0) {
+    const int waves = few_waves(a);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({1024 / waves / items, (tiles + waves - 1) / waves, kMaxSplits}));
+  }
   if (items >= 512 || items == 0) return 1;
   return (int)std::max<int64_t>(1, std::min<int64_t>({(768 + items - 1) / items, tiles / 2, kMaxSplits}));
 }
@@ -423,7 +616,18 @@ int64_t part_bytes(const HierCrossArgs& a, int splits, int D) {
 template <typename T, int D>
 int launch(const Launch& p, hipStream_t st) {
   const dim3 grid((unsigned)xcd_grid(p.total));
-  if (p.a.key_mask)
+  if (few_rows(p.a)) {
+    auto few = [&](auto waves, auto mask) {
+      constexpr int W = decltype(waves)::value;
+      hipLaunchKernelGGL((cross_few_kernel<T, D, W, decltype(mask)::value>), grid, dim3(64 * W), 0, st, p);
+    };
+    const bool two = few_waves(p.a) == 2;
+    typedef std::integral_constant<int, 2> Two;
+    typedef std::integral_constant<int, 4> Four;
+    if (p.a.key_mask) two ? few(Two{}, std::true_type{}) : few(Four{}, std::true_type{});
+    else two ? few(Two{}, std::false_type{}) : few(Four{}, std::false_type{});
+  }
+  else if (p.a.key_mask)
     hipLaunchKernelGGL((cross_fwd_kernel<T, D, true>), grid, dim3(kThreads), 0, st, p);
   else
     hipLaunchKernelGGL((cross_fwd_kernel<T, D, false>), grid, dim3(kThreads), 0, st, p);
