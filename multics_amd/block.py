@@ -89,6 +89,16 @@ def _outs(name: str, out: Optional[torch.Tensor], like: torch.Tensor, shape) -> 
     return out
 
 
+def _apart(out: torch.Tensor, **inputs: torch.Tensor) -> None:
+    """Refuses an ``out`` in the memory of an input that is still read while it is
+    written (views that interleave with it, in a larger tensor, pass)."""
+    first, last = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
+    for name, t in inputs.items():
+        at = t.data_ptr()
+        if t.is_contiguous() and out.is_contiguous() and at < last and first < at + t.numel() * t.element_size():
+            raise ValueError(f"out must not share memory with {name}")
+
+
 # --------------------------------------------------------------------------
 # root-mean-square norm with the residual's addition
 # --------------------------------------------------------------------------
@@ -240,6 +250,8 @@ def _workspace(name: str, args: bytes) -> int:
 def _linear(x, weight, bias, activation, residual, gate, out, preact):
     kind, act, M, N, K, per = _linear_args(x, weight, bias, activation, residual, gate)
     shape = (*x.shape[:-1], N)
+    if out is not None:
+        _apart(out, x=x, weight=weight)
     out = _outs("out", out, x, shape)
     if M == 0:
         return out
@@ -266,7 +278,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     ``"gelu_tanh"``, ``"gelu"`` or ``"silu"``.  ``residual`` is [..., N]; ``gate`` is
     [N], or [..., F, N] whose rows scale S / F rows of x's S each (a frame's tokens
     share their frame's gate, as in ``gated_residual``).  ``out`` (optional, contiguous)
-    may be ``residual``.  Rows of a multiple of eight channels are read in place,
+    may be ``residual``, not ``x`` or ``weight``.  Rows of a multiple of eight channels are read in place,
     others are copied with zeros behind.  No gradient: ``linear_act_train``."""
     _no_grad_call("linear_act", x, weight, bias, residual, gate)
     return _linear(x, weight, bias, activation, residual, gate, out, None)
@@ -436,6 +448,7 @@ def _cross(q, k, v, kv_lens, key_mask, scale, out, lse):
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     else:
         _like("out", out, q, q.shape)
+        _apart(out, q=q, k=k, v=v)
     oh = _heads(out)
     B, Hq, _, D, _, _, Sq, _ = sizes
     if oh[0] is not out or any(n > 1 and s < D for n, s in zip((B, Sq, Hq), oh[1])):
@@ -461,7 +474,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     query heads i * H/Hk .. share key head i.  A stream's keys are the first
     ``kv_lens[b]`` (int32 [B] on the GPU, taken within [0, Sk]) whose ``key_mask``
     [B, Sk] (bool) is true; what else k and v hold is not read.  Returns [B, Sq, H, D]
-    (``out`` where given); a row that sees no key is 0.  ``lse`` (optional, contiguous
+    (``out`` where given, which is none of them); a row that sees no key is 0.  ``lse`` (optional, contiguous
     fp32 [B, H, Sq]) receives the natural-log softmax normaliser, -inf for such a
     row.  Sq may be one token: the keys are then cut into parts that fill the GPU.
     No gradient: ``cross_attention_train``."""

@@ -24,37 +24,39 @@ namespace {
 
 constexpr int kCols = 32, kLines = 32;
 
-__global__ __launch_bounds__(kCols * kLines) void sum_rows_kernel(const float* partial, int64_t rows,
+__global__ __launch_bounds__(kCols * kLines) void sum_rows_kernel(const float* partial, int64_t rows, int64_t groups,
                                                                   int64_t C, void* out, int type) {
   __shared__ float part[kLines][kCols + 1];
   const int col = threadIdx.x % kCols, line = threadIdx.x / kCols;
   const int64_t c = (int64_t)blockIdx.x * kCols + col;
-  const float* p = partial + (int64_t)blockIdx.y * rows * C + c;
-  float s = 0.f;
-  if (c < C) {
-    int64_t r = line;
-    for (; r + 7 * kLines < rows; r += 8 * kLines) {   // eight loads in flight
-      float v[8];
+  for (int64_t g = blockIdx.y; g < groups; g += gridDim.y) {
+    const float* p = partial + g * rows * C + c;
+    float s = 0.f;
+    if (c < C) {
+      int64_t r = line;
+      for (; r + 7 * kLines < rows; r += 8 * kLines) {   // eight loads in flight
+        float v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = p[(r + i * kLines) * C];
+        for (int i = 0; i < 8; ++i) v[i] = p[(r + i * kLines) * C];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += v[i];
+        for (int i = 0; i < 8; ++i) s += v[i];
+      }
+      for (; r < rows; r += kLines) s += p[r * C];
     }
-    for (; r < rows; r += kLines) s += p[r * C];
-  }
-  part[line][col] = s;
-  __syncthreads();
-#pragma unroll
-  for (int n = kLines / 2; n > 0; n /= 2) {
-    if (line < n) part[line][col] += part[line + n][col];
+    part[line][col] = s;
     __syncthreads();
-  }
-  if (line == 0 && c < C) {
-    const int64_t at = (int64_t)blockIdx.y * C + c;
-    const float v = part[0][col];
-    if (type == HIER_FP32) static_cast<float*>(out)[at] = v;
-    else if (type == HIER_BF16) static_cast<__bf16*>(out)[at] = (__bf16)v;
-    else static_cast<_Float16*>(out)[at] = (_Float16)v;
+#pragma unroll
+    for (int n = kLines / 2; n > 0; n /= 2) {
+      if (line < n) part[line][col] += part[line + n][col];
+      __syncthreads();
+    }
+    if (line == 0 && c < C) {
+      const int64_t at = g * C + c;
+      const float v = part[0][col];
+      if (type == HIER_FP32) static_cast<float*>(out)[at] = v;
+      else if (type == HIER_BF16) static_cast<__bf16*>(out)[at] = (__bf16)v;
+      else static_cast<_Float16*>(out)[at] = (_Float16)v;
+    }
   }
 }
 
@@ -358,9 +360,9 @@ bool rows16(const void* p, int64_t ss) { return aligned16(p) && ss % 8 == 0; }
 
 int sum_rows(const float* partial, int64_t rows, int64_t groups, int64_t C, void* out, int type,
              hipStream_t stream) {
-  HIER_REQUIRE(groups >= 1 && groups <= 65535, HIER_EUNSUPPORTED, "sum of rows: too many groups");
-  hipLaunchKernelGGL(sum_rows_kernel, dim3((unsigned)((C + kCols - 1) / kCols), (unsigned)groups),
-                     dim3(kCols * kLines), 0, stream, partial, rows, C, out, type);
+  hipLaunchKernelGGL(sum_rows_kernel,
+                     dim3((unsigned)((C + kCols - 1) / kCols), (unsigned)std::min<int64_t>(groups, 65535)),
+                     dim3(kCols * kLines), 0, stream, partial, rows, groups, C, out, type);
   return check_launch("sum_rows_kernel");
 }
 

@@ -325,6 +325,73 @@ def test_values_that_are_not_numbers_stay_in_their_rows():
         assert torch.equal(got[keep], clean[keep]) and not bool(torch.isfinite(got[77]).all())
 
 
+def test_product_of_many_gates():
+    """More gates than a launch has rows of workgroups, each of more rows than one workgroup takes."""
+    need_gpu()
+    F, per = 65600, 5
+    x, w, _, _, gate, dy = _linear_case(F * per, 8, 8, None, F, False, BF16, seed=3)
+    z = kernels.linear_act(x, w)
+    got = kernels.linear_act_backward(dy, x, w, preact=z, gate=gate, need=("gate",))["gate"]
+    ref = (dy.double() * z.double()).view(F, per, 8)
+    _within(got, ref.sum(1), (per + 8) * U * ref.abs().sum(1))
+    assert torch.equal(kernels.linear_act(x, w, gate=gate)[-per:], kernels.linear_act(x[-per:], w, gate=gate[-1:]))
+
+
+def test_offsets_past_32_bits():
+    """Rows and sums over rows that lie behind the first 4 GiB of their tensors."""
+    need_gpu()
+    r = _rnd(23)
+    tail = 300
+    M, C = 1_500_000, 1536
+    x = torch.zeros(M, C, dtype=BF16, device="cuda")
+    w = 1 + 0.1 * r(C)
+    x[-tail:] = r(tail, C).to(BF16)
+    assert torch.equal(kernels.rms_norm(x, w, eps=1e-6)[-tail:], kernels.rms_norm(x[-tail:], w, eps=1e-6))
+    say("norm past 4 GiB")
+    # a product over those rows: x [M, C] as operand, dw a sum over M whose terms lie at its end
+    wt, dy = r(72, C).to(BF16), torch.zeros(M, 72, dtype=BF16, device="cuda")
+    dy[-tail:] = r(tail, 72).to(BF16)
+    y = kernels.linear_act(x, wt)
+    say("product past 4 GiB")
+    ref = x[-tail:].double() @ wt.double().t()
+    _within(y[-tail:], ref, (C + 8) * U * (x[-tail:].double().abs() @ wt.double().abs().t()))
+    assert not y[:-tail].any()
+    got = kernels.linear_act_backward(dy, x, wt, need=("x", "weight", "bias"))
+    say("its gradients past 4 GiB")
+    a, b = dy[-tail:].double(), x[-tail:].double()
+    _within(got["weight"], a.t() @ b, (M + 8) * U * (a.abs().t() @ b.abs()))
+    _within(got["x"][-tail:], a @ wt.double(), (72 + 8) * U * (a.abs() @ wt.double().abs()))
+    _within(got["bias"], a.sum(0), (M + 8) * U * a.abs().sum(0))
+    assert not got["x"][:-tail].any()
+
+
+def test_long_caches_of_keys():
+    """Keys whose tokens lie 16 KB apart, 4.9 GB of them; the seen ones are the last."""
+    need_gpu()
+    r = _rnd(29)
+    S, D, last = 300_000, 64, 200
+    buf = torch.zeros(S, 2, 64, D, dtype=BF16, device="cuda")
+    buf[-last:, :, 5] = r(last, 2, D).to(BF16)
+    k, v = (buf[None, :, i, 5:6] for i in (0, 1))
+    mask = torch.zeros(1, S, dtype=torch.bool, device="cuda")
+    mask[:, -last:] = True
+    for Sq in (1, 140):
+        say("long cache", Sq)
+        q, dout = r(1, Sq, 1, D).to(BF16), r(1, Sq, 1, D).to(BF16)
+        lse = torch.empty(1, 1, Sq, device="cuda")
+        out = kernels.cross_attention(q, k, v, key_mask=mask, lse=lse)
+        short = [t[:, -last:] for t in (k, v)]
+        seen = torch.ones(1, last, dtype=torch.bool, device="cuda")
+        O, slack, _, grads = _cross_formula(q, *short, seen, D ** -0.5, dout)  # noqa: E741
+        _within(out, O, slack)
+        for name, g in zip(("dq", "dk", "dv"),
+                           kernels.cross_attention_backward(dout, q, k, v, out, lse, key_mask=mask)):
+            if name != "dq":
+                assert not g[:, :-last].any()
+                g = g[:, -last:]
+            _within(g, grads[name][0], grads[name][1] + 1e-30)
+
+
 # ---- cross attention -----------------------------------------------------------------------
 
 CROSS = [
@@ -339,6 +406,11 @@ CROSS = [
     (1, 700, 3, 2, 1, 128, "all", BF16),
     (2, 3, 2500, 3, 1, 64, "mask", BF16),
     (5, 2, 66, 1, 7, 128, "both", BF16),
+    (2, 4, 4000, 1, 8, 128, "mask", BF16),       # 32 rows: the last size of a wave a tile, in parts
+    (1, 33, 1500, 1, 1, 64, "lens", BF16),       # the first over tiles of 128 rows
+    (64, 1, 2100, 5, 1, 128, "mask", FP16),      # nine tiles a wave
+    (130, 1, 300, 4, 2, 64, "both", BF16),       # two waves a workgroup
+    (260, 2, 200, 2, 1, 128, "lens", FP16),
 ]
 
 
@@ -704,6 +776,8 @@ def test_refusals():
         (ValueError, lambda: kernels.linear_act(x, w, residual=x)),
         (ValueError, lambda: kernels.linear_act(x, w, out=torch.empty(8, 32, dtype=BF16, device="cuda")[::2])),
         (ValueError, lambda: kernels.linear_act(x, w.cpu())),
+        (ValueError, lambda: kernels.linear_act(x, r(64, 64).to(BF16), out=x)),
+        (ValueError, lambda: kernels.linear_act(x[1:], r(64, 64).to(BF16), out=x[:3])),
         (ValueError, lambda: kernels.linear_act_backward(r(4, 32).to(BF16), x, w, activation="silu")),
         (NotImplementedError, lambda: kernels.linear_act(x.float(), w.float())),
         (RuntimeError, lambda: kernels.linear_act(x, w.clone().requires_grad_())),
@@ -730,6 +804,8 @@ def test_refusals():
         (ValueError, lambda: kernels.cross_attention(q, k, k, scale=-1.0)),
         (ValueError, lambda: kernels.cross_attention(q, k, k, scale=float("nan"))),
         (ValueError, lambda: kernels.cross_attention(q, k, k, out=q[:1].expand(2, -1, -1, -1))),
+        (ValueError, lambda: kernels.cross_attention(q, k, k, out=q)),
+        (ValueError, lambda: kernels.cross_attention(k, k, k, out=k)),
         (ValueError, lambda: kernels.cross_attention(q, k, k, lse=torch.empty(2, 4, 6, device="cuda"))),
         (RuntimeError, lambda: kernels.cross_attention(q.clone().requires_grad_(), k, k)),
         (NotImplementedError, lambda: kernels.cross_attention_train(q.half().requires_grad_(), k.half(), k.half())),
