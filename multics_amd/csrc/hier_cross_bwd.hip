@@ -11,7 +11,7 @@
 // dkv     128 keys an item, eight waves: wave w makes S, P and dV of its 32 keys,
 //         wave w + 4 of the same keys dP, dS and dK, P handed over through LDS as
 //         fp16 (10 bits of a value of at most 1).  Items are few where the keys are
-//         (an encoder's 512 are four a head): the rows are then cut into splits, whose
+//         (an encoder's 512 are four a head): the rows may then be cut into splits, whose
 //         fp32 sums a third kernel adds in their order.
 // dP starts from -delta, as S does from -m in the forward: the subtraction is the
 // matrix product's.
@@ -537,13 +537,30 @@ __global__ __launch_bounds__(256) void cross_dkv_join_kernel(Launch p) {
   *reinterpret_cast<u32x2*>(out + d) = __builtin_bit_cast(u32x2, v);
 }
 
-// Parts of the rows of every key item: one where the items fill the card (one
-// workgroup a CU), else enough for three rounds of them, of eight tiles at least.
+// Parts of the rows of every key item, by a model of the time in us: a workgroup takes
+// 2.4 a tile of D 128 where all 256 CUs work, 1.8 at best (the power bounds both: three
+// quarters of the CUs make as many tiles as all of them), three tiles' time to start
+// and end, and the parts' fp32 sums are written and read at 5 TB/s.  192 items of 73 tiles
+// 262 us in one part with dq, 282 in four (three whole rounds of workgroups); 32 items
+// of 128 tiles, D 64, 147 us in one, 54 in eight, 58 in sixteen.
 int splits_of(const HierCrossArgs& a) {
   const int64_t items = (int64_t)a.B * a.Hk * row_tiles(a.Sk);
   const int64_t tiles = (a.Sq * (a.Hq / a.Hk) + kSlab - 1) / kSlab;
-  if (items >= 768 || items == 0) return 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({(768 + items - 1) / items, tiles / 8, 64}));
+  if (items == 0) return 1;
+  int best = 1;
+  double least = 1e30;
+  for (int64_t s = 1; s <= 64 && (s == 1 || s * 8 <= tiles); ++s) {
+    const double scale = a.D == 128 ? 1.0 : 0.6, each = (double)((tiles + s - 1) / s + 3);
+    const int64_t whole = items * s / 256;
+    const double rest = (double)(items * s % 256) / 256;
+    double t = scale * each * (2.4 * (double)whole + (rest > 0 ? std::max(1.8, 2.4 * rest) : 0.0));
+    if (s > 1) t += 4 + (double)(s * items * kRows * a.D) * 16 / 5e6;
+    if (t < least) {
+      least = t;
+      best = (int)s;
+    }
+  }
+  return best;
 }
 
 int64_t rows_bytes(const HierCrossArgs& a) {
