@@ -90,6 +90,32 @@ __device__ __forceinline__ bool key_bit(uint32_t bits, int i, int lane) {
 // HIER_OK, or what is wrong with the sizes, types and views (hier_cross_fwd.hip).
 int check(const HierCrossArgs& a);
 
+// Parts of the tiles that an item goes over, by a model of the time in us: of the `slots`
+// workgroups that run at once each takes `full` a tile where all of them work, `least` at
+// best, `start` tiles' time to start and end, and the parts' fp32 sums (`bytes` of
+// one part of all items) are written and read at 5 TB/s by a launch more.
+struct SplitModel {
+  int slots;
+  double full, least, start;
+  int tiles;                         // of a part, at least
+};
+inline int best_splits(const SplitModel& m, int64_t items, int64_t tiles, double bytes, int most) {
+  int best = 1;
+  double time = 1e30;
+  for (int64_t n = 1; n <= most && (n == 1 || n * m.tiles <= tiles); ++n) {
+    const double each = (double)((tiles + n - 1) / n) + m.start;
+    const int64_t whole = items * n / m.slots;
+    const double rest = (double)(items * n % m.slots) / m.slots;
+    double t = each * (m.full * (double)whole + (rest > 0 ? (m.least > m.full * rest ? m.least : m.full * rest) : 0.0));
+    if (n > 1) t += 4 + 2 * (double)n * bytes / 5e6;
+    if (t < time) {
+      time = t;
+      best = (int)n;
+    }
+  }
+  return best;
+}
+
 inline int64_t row_tiles(int64_t rows) { return (rows + kRows - 1) / kRows; }
 
 }  // namespace cross

@@ -30,10 +30,10 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 struct Launch {
   HierCrossBwdArgs a;
   Div div;
-  int32_t row_tiles, key_tiles, splits, total;
+  int32_t row_tiles, key_tiles, splits, total, dq_splits;
   float* lse2;         // [B * Hk][row_tiles * 128]
   float* delta;        // minus it
-  float* part;         // [splits][dk, dv][B * Hk][Sk][D]
+  float* part;         // [splits][dk, dv][B * Hk][Sk][D]; before that dQ's [dq_splits][B * Hk][rows][D]
 };
 
 template <int N, int R, int V>
@@ -80,6 +80,17 @@ __device__ __forceinline__ void store_acc(uint16_t* row, const f32x16* acc, floa
       for (int e = 0; e < 4; ++e) v[e] = (T)(acc[d][4 * g + e] * mul);
       *reinterpret_cast<u32x2*>(row + d * 32 + 8 * g + 4 * half) = __builtin_bit_cast(u32x2, v);
     }
+}
+
+template <int D>
+__device__ __forceinline__ void store_part(float* row, const f32x16* acc, int lane) {
+  const int half = lane >> 5;
+#pragma unroll
+  for (int d = 0; d < Geo<D>::NDB; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<f32x4*>(row + d * 32 + 8 * g + 4 * half) =
+          f32x4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
 }
 
 // ---- dQ ----------------------------------------------------------------------------
@@ -178,20 +189,27 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(Launch p) {
   const Stages st = {{k0, k1}, {v0, v1}};
   const int logical = xcd_logical(blockIdx.x, gridDim.x);
   const HierCrossArgs& a = p.a.f;
-  if (logical >= a.B * a.Hk * p.row_tiles) return;
-  const int hb = logical / p.row_tiles, rt = logical - hb * p.row_tiles;
+  const int per = p.row_tiles * p.dq_splits;
+  if (logical >= a.B * a.Hk * per) return;
+  const int hb = logical / per, in = logical - hb * per;
+  const int split = in / p.row_tiles, rt = in - split * p.row_tiles;
   const int hk = hb / a.B, b = hb - hk * a.B, bh = b * a.Hk + hk;      // (as the forward's)
   QWork<D> w;
   w.lane = threadIdx.x & 63;
   w.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   w.len = a.Sk;
   if (a.kv_lens) w.len = min(max((int64_t)a.kv_lens[b], (int64_t)0), a.Sk);
-  w.nt = (int)((w.len + kSlab - 1) / kSlab);
+  const int tiles = (int)((w.len + kSlab - 1) / kSlab);
+  const int each = (tiles + p.dq_splits - 1) / p.dq_splits;
+  const int t0 = min(split * each, tiles);
+  w.nt = min(each, tiles - t0);
+  const int64_t key0 = (int64_t)t0 * kSlab;
+  w.len = min(w.len - key0, (int64_t)w.nt * kSlab);
   w.k_ss = a.k_ss;
   w.v_ss = a.v_ss;
-  w.kbase = (uint64_t)a.k + 2 * (b * a.k_sb + hk * a.k_sh);
-  w.vbase = (uint64_t)a.v + 2 * (b * a.v_sb + hk * a.v_sh);
-  w.mask = MASK ? a.key_mask + b * a.mask_sb + w.lane : nullptr;
+  w.kbase = (uint64_t)a.k + 2 * (b * a.k_sb + hk * a.k_sh + key0 * a.k_ss);
+  w.vbase = (uint64_t)a.v + 2 * (b * a.v_sb + hk * a.v_sh + key0 * a.v_ss);
+  w.mask = MASK ? a.key_mask + b * a.mask_sb + key0 + w.lane : nullptr;
   w.ck.init(w.wave, w.lane, a.k_ss);
   w.cv.init(w.wave, w.lane, a.v_ss);
 #pragma unroll
@@ -233,7 +251,7 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(Launch p) {
   const float lse = a.lse[((int64_t)b * a.Hq + head) * a.Sq + q];
   w.lse2 = lse == -INFINITY ? INFINITY : lse * kLog2e;
   w.c2 = a.scale * kLog2e;
-  if (w.lane < 32) {       // rows past the last: P = 0, whatever dkv reads there
+  if (split == 0 && w.lane < 32) {       // rows past the last: P = 0, whatever dkv reads there
     const int64_t at = (int64_t)bh * p.row_tiles * kRows + r0 + w.lane;
     p.lse2[at] = valid ? w.lse2 : INFINITY;
     p.delta[at] = valid ? w.ndelta : 0.f;
@@ -272,7 +290,10 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(Launch p) {
     }
     if (t < w.nt) dq_tile<D, MASK, true, 0>(w, t, seen, next, st);
   }
-  if (w.active && valid)
+  if (!w.active || !valid) return;
+  if (p.dq_splits > 1)
+    store_part<D>(p.part + ((int64_t)(split * a.B * a.Hk + bh) * R + r) * D, w.dq, w.lane);
+  else
     store_acc<D>(static_cast<uint16_t*>(p.a.dq) + b * p.a.dq_sb + (int64_t)q * p.a.dq_ss + head * p.a.dq_sh, w.dq,
                  a.scale, w.lane);
 }
@@ -497,13 +518,7 @@ __global__ __launch_bounds__(512, 1) void cross_dkv_kernel(Launch p) {
       for (int i = 0; i < 16; ++i) w.acc[d][i] = 0.f;
   }
   if (p.splits > 1) {
-    float* out = p.part + ((((int64_t)split * 2 + (role_b ? 0 : 1)) * a.B * a.Hk + bh) * a.Sk + key) * D;
-#pragma unroll
-    for (int d = 0; d < Geo<D>::NDB; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4*>(out + d * 32 + 8 * g + 4 * (w.lane >> 5)) =
-            f32x4{w.acc[d][4 * g], w.acc[d][4 * g + 1], w.acc[d][4 * g + 2], w.acc[d][4 * g + 3]};
+    store_part<D>(p.part + ((((int64_t)split * 2 + (role_b ? 0 : 1)) * a.B * a.Hk + bh) * a.Sk + key) * D, w.acc, w.lane);
   } else if (role_b) {
     store_acc<D>(static_cast<uint16_t*>(p.a.dk) + b * p.a.dk_sb + key * p.a.dk_ss + hk * p.a.dk_sh, w.acc, a.scale,
                  w.lane);
@@ -513,23 +528,39 @@ __global__ __launch_bounds__(512, 1) void cross_dkv_kernel(Launch p) {
   }
 }
 
-// The splits' sums, in their order.
-template <int D>
-__global__ __launch_bounds__(256) void cross_dkv_join_kernel(Launch p) {
+// The splits' sums, in their order: four channels a thread of dK and dV (DQ: of dQ).
+// Four splits' loads leave together, the last split's again past the end.
+template <int D, bool DQ>
+__global__ __launch_bounds__(256) void cross_grad_join_kernel(Launch p) {
   const HierCrossArgs& a = p.a.f;
-  const int64_t rows = (int64_t)a.B * a.Hk * a.Sk, n = 2 * rows * (D / 4);
+  const int64_t rows = DQ ? (int64_t)a.B * a.Hq * a.Sq : (int64_t)a.B * a.Hk * a.Sk, n = rows * (D / 4);
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const bool dv = i >= n / 2;
-  const int64_t j = dv ? i - n / 2 : i, row = j / (D / 4);
-  const int d = 4 * (int)(j - row * (D / 4));
+  if (i >= (DQ ? n : 2 * n)) return;
+  const bool dv = !DQ && i >= n;
+  const int64_t j = dv ? i - n : i, row = j / (D / 4);
+  const int d = 4 * (int)(j - row * (D / 4)), splits = DQ ? p.dq_splits : p.splits;
+  const int64_t step = (DQ ? rows : 2 * rows) * D;
+  const float* src = p.part + ((dv ? rows : 0) + row) * D + d;
   f32x4 s = {};
-  for (int k = 0; k < p.splits; ++k)
-    s += *reinterpret_cast<const f32x4*>(p.part + (((int64_t)k * 2 + dv) * rows + row) * D + d);
-  const int64_t bh = row / a.Sk, key = row - bh * a.Sk;
+  for (int k = 0; k < splits; k += 4) {
+    f32x4 x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = *reinterpret_cast<const f32x4*>(src + min(k + e, splits - 1) * step);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (k + e < splits) s += x[e];
+  }
+  const int64_t per = DQ ? (int64_t)a.Sq * p.div.g : a.Sk, bh = row / per, r = row - bh * per;
   const int b = (int)(bh / a.Hk), hk = (int)(bh - (int64_t)b * a.Hk);
-  uint16_t* out = dv ? static_cast<uint16_t*>(p.a.dv) + b * p.a.dv_sb + key * p.a.dv_ss + hk * p.a.dv_sh
-                     : static_cast<uint16_t*>(p.a.dk) + b * p.a.dk_sb + key * p.a.dk_ss + hk * p.a.dk_sh;
+  uint16_t* out;
+  if constexpr (DQ) {
+    const uint32_t q = quotient((uint32_t)r, p.div);
+    const int head = hk * (int)p.div.g + (int)((uint32_t)r - q * p.div.g);
+    out = static_cast<uint16_t*>(p.a.dq) + b * p.a.dq_sb + (int64_t)q * p.a.dq_ss + head * p.a.dq_sh;
+  } else {
+    out = dv ? static_cast<uint16_t*>(p.a.dv) + b * p.a.dv_sb + r * p.a.dv_ss + hk * p.a.dv_sh
+             : static_cast<uint16_t*>(p.a.dk) + b * p.a.dk_sb + r * p.a.dk_ss + hk * p.a.dk_sh;
+  }
   typedef T quad __attribute__((ext_vector_type(4)));
   quad v;
 #pragma unroll
@@ -537,30 +568,22 @@ __global__ __launch_bounds__(256) void cross_dkv_join_kernel(Launch p) {
   *reinterpret_cast<u32x2*>(out + d) = __builtin_bit_cast(u32x2, v);
 }
 
-// Parts of the rows of every key item, by a model of the time in us: a workgroup takes
-// 2.4 a tile of D 128 where all 256 CUs work, 1.8 at best (the power bounds both: three
-// quarters of the CUs make as many tiles as all of them), three tiles' time to start
-// and end, and the parts' fp32 sums are written and read at 5 TB/s.  192 items of 73 tiles
-// 262 us in one part with dq, 282 in four (three whole rounds of workgroups); 32 items
-// of 128 tiles, D 64, 147 us in one, 54 in eight, 58 in sixteen.
-int splits_of(const HierCrossArgs& a) {
+// Parts (SplitModel).  dK, dV, of the rows: 192 items of 73 tiles 132 us in one part, 152 in
+// four (three whole rounds of workgroups; the power bounds them: three quarters of the
+// CUs make as many tiles as all); 32 items of 128 tiles, D 64, 147 us with dq in one, 54
+// in eight, 58 in sixteen.  dQ, of the keys: 12 items of 128
+// tiles (one row each) 238 us with dK and dV in one part, 57 in 26.
+int dkv_splits(const HierCrossArgs& a) {
+  const double size = a.D == 128 ? 1.0 : 0.6;
   const int64_t items = (int64_t)a.B * a.Hk * row_tiles(a.Sk);
   const int64_t tiles = (a.Sq * (a.Hq / a.Hk) + kSlab - 1) / kSlab;
-  if (items == 0) return 1;
-  int best = 1;
-  double least = 1e30;
-  for (int64_t s = 1; s <= 64 && (s == 1 || s * 8 <= tiles); ++s) {
-    const double scale = a.D == 128 ? 1.0 : 0.6, each = (double)((tiles + s - 1) / s + 3);
-    const int64_t whole = items * s / 256;
-    const double rest = (double)(items * s % 256) / 256;
-    double t = scale * each * (2.4 * (double)whole + (rest > 0 ? std::max(1.8, 2.4 * rest) : 0.0));
-    if (s > 1) t += 4 + (double)(s * items * kRows * a.D) * 16 / 5e6;
-    if (t < least) {
-      least = t;
-      best = (int)s;
-    }
-  }
-  return best;
+  return best_splits({256, 2.4 * size, 1.8 * size, 3, 8}, items, tiles, 8.0 * a.B * a.Hk * (double)a.Sk * a.D, 64);
+}
+int dq_splits(const HierCrossArgs& a) {
+  const double size = a.D == 128 ? 1.0 : 0.6;
+  const int64_t items = (int64_t)a.B * a.Hk * row_tiles(a.Sq * (a.Hq / a.Hk));
+  return best_splits({512, 3.0 * size, 1.8 * size, 3.5, 2}, items, (a.Sk + kSlab - 1) / kSlab,
+                     4.0 * a.B * a.Hq * (double)a.Sq * a.D, 64);
 }
 
 int64_t rows_bytes(const HierCrossArgs& a) {
@@ -568,27 +591,33 @@ int64_t rows_bytes(const HierCrossArgs& a) {
 }
 
 int64_t work_bytes(const HierCrossArgs& a) {
-  const int s = splits_of(a);
-  return 2 * rows_bytes(a) + (s > 1 ? (int64_t)s * 2 * a.B * a.Hk * a.Sk * a.D * 4 : 0);
+  const int sk = dkv_splits(a), sq = dq_splits(a);     // (dQ's parts are joined before the others are made)
+  return 2 * rows_bytes(a) + std::max(sk > 1 ? (int64_t)sk * 2 * a.B * a.Hk * a.Sk * a.D * 4 : 0,
+                                      sq > 1 ? (int64_t)sq * a.B * a.Hq * a.Sq * a.D * 4 : 0);
 }
 
 template <int D>
 int launch(const Launch& p, hipStream_t st) {
   const HierCrossArgs& a = p.a.f;
-  const int64_t items = (int64_t)a.B * a.Hk * p.row_tiles;
+  const int64_t items = (int64_t)a.B * a.Hk * p.row_tiles * p.dq_splits;
+  auto join = [&](auto dq, int64_t rows) {
+    const int64_t n = rows * (D / 4);
+    hipLaunchKernelGGL((cross_grad_join_kernel<D, decltype(dq)::value>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0,
+                       st, p);
+    return check_launch("cross_grad_join_kernel");
+  };
   if (items > 0) {
     const dim3 grid((unsigned)xcd_grid(items));
     if (a.key_mask) hipLaunchKernelGGL((cross_dq_kernel<D, true>), grid, dim3(256), 0, st, p);
     else hipLaunchKernelGGL((cross_dq_kernel<D, false>), grid, dim3(256), 0, st, p);
     if (int rc = check_launch("cross_dq_kernel")) return rc;
+    if (p.dq_splits > 1)
+      if (int rc = join(std::true_type{}, (int64_t)a.B * a.Hq * a.Sq)) return rc;
   }
   if (p.total == 0) return HIER_OK;
   hipLaunchKernelGGL(cross_dkv_kernel<D>, dim3((unsigned)xcd_grid(p.total)), dim3(512), 0, st, p);
   if (int rc = check_launch("cross_dkv_kernel")) return rc;
-  if (p.splits == 1) return HIER_OK;
-  const int64_t n = 2 * (int64_t)a.B * a.Hk * a.Sk * (D / 4);
-  hipLaunchKernelGGL(cross_dkv_join_kernel<D>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, p);
-  return check_launch("cross_dkv_join_kernel");
+  return p.splits == 1 ? HIER_OK : join(std::false_type{}, 2 * (int64_t)a.B * a.Hk * a.Sk);
 }
 
 }  // namespace
@@ -634,7 +663,8 @@ extern "C" int hier_cross_attn_bwd(const HierCrossBwdArgs* args, void* stream) {
   p.div = make_div((uint32_t)G);
   p.row_tiles = (int)row_tiles(a.Sq * G);
   p.key_tiles = (int)row_tiles(a.Sk);
-  p.splits = splits_of(a);
+  p.splits = dkv_splits(a);
+  p.dq_splits = dq_splits(a);
   p.total = a.B * a.Hk * p.key_tiles * p.splits;
   const int64_t need = work_bytes(a);
   HIER_REQUIRE(need == 0 || (a.workspace && aligned16(a.workspace) && a.workspace_bytes >= need), HIER_EINVAL,

@@ -586,10 +586,8 @@ __global__ __launch_bounds__(256) void cross_join_kernel(Launch p) {
     a.lse[((int64_t)b * a.Hq + head) * a.Sq + q] = total == 0.f ? -INFINITY : top * a.scale + __logf(total);
 }
 
-// Parts of every key list, by a model of the time in us: of the 512 workgroups that run
-// at once each takes 2.1 a tile of D 128 where all work, 1.4 at best, 3.5 tiles' time to
-// start and end, and the parts' fp32 sums are written and read at 5 TB/s.  444 items of
-// 8 tiles 27 us in one part, 58 in two; 16 items of 64 tiles 20.7 in 16, 25 in 32.
+// Parts of every key list (SplitModel).  444 items of 8 tiles 27 us in one part, 58 in
+// two; 16 items of 64 tiles 20.7 in 16, 25 in 32.
 // Few rows: workgroups for the 256 CUs, of a tile a wave at least.
 bool few_rows(const HierCrossArgs& a) { return a.Sq * (a.Hq / a.Hk) <= kFewRows; }
 
@@ -607,21 +605,8 @@ int splits_of(const HierCrossArgs& a) {
     const int waves = few_waves(a);
     return (int)std::max<int64_t>(1, std::min<int64_t>({1024 / waves / items, (tiles + waves - 1) / waves, kMaxSplits}));
   }
-  if (items == 0) return 1;
-  int best = 1;
-  double least = 1e30;
-  for (int64_t n = 1; n <= kMaxSplits && (n == 1 || 2 * n <= tiles); ++n) {
-    const double scale = a.D == 128 ? 1.0 : 0.6, each = (double)((tiles + n - 1) / n) + 3.5;
-    const int64_t whole = items * n / 512;
-    const double rest = (double)(items * n % 512) / 512;
-    double t = scale * each * (2.1 * (double)whole + (rest > 0 ? std::max(1.4, 2.1 * rest) : 0.0));
-    if (n > 1) t += 4 + (double)(n * items * kRows * a.D) * 8 / 5e6;
-    if (t < least) {
-      least = t;
-      best = (int)n;
-    }
-  }
-  return best;
+  const double size = a.D == 128 ? 1.0 : 0.6;
+  return best_splits({512, 2.1 * size, 1.4 * size, 3.5, 2}, items, tiles, 4.0 * a.B * a.Hq * (double)a.Sq * a.D, kMaxSplits);
 }
 
 int64_t part_bytes(const HierCrossArgs& a, int splits, int D) {
