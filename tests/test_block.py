@@ -75,7 +75,7 @@ REFUSED = [
     ("hier_cross_attn", _cross, dict(k_ss=1 << 23), "stride"),
     ("hier_cross_attn", _cross, dict(o_ss=0), "rows of its own"),
     ("hier_cross_attn", _cross, dict(v=None), "NULL"),
-    ("hier_cross_attn", _cross, dict(Sk=512), "workspace"),
+    ("hier_cross_attn", _cross, dict(Sq=1, Sk=8192), "workspace"),
     ("hier_cross_attn", _cross, dict(Sq=1 << 30), "too many"),
 ]
 
