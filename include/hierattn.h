@@ -775,6 +775,21 @@ typedef struct HierLinearArgs {
 int64_t hier_linear_workspace(const HierLinearArgs* args);   /* -1: invalid    */
 int hier_linear(const HierLinearArgs* args, void* stream);
 
+/* Rows of two matrices of C 16-bit elements, at any address and stride, as  */
+/* 16-byte rows of C rounded up to a multiple of 8, zeros behind: what the   */
+/* products read x and w from where they are not.  dst is contiguous and      */
+/* 16-byte aligned; a matrix of 0 rows is left out.                           */
+typedef struct HierPadRowsArgs {
+  int64_t rows[2];
+  int64_t ss[2];                   /* elements from row to row of src          */
+  const void* src[2];
+  void* dst[2];
+  int32_t C;
+  int32_t pad;
+} HierPadRowsArgs;
+
+int hier_pad_rows(const HierPadRowsArgs* args, void* stream);
+
 /* Gradients of hier_linear from dy and preact: each of dx, dw, db, dgate    */
 /* that is not NULL.  preact may be NULL without an activation and dgate.    */
 /* Deterministic.                                                            */

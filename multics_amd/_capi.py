@@ -219,6 +219,11 @@ class HierLinearArgs(C.Structure):
                [("workspace", vp), ("workspace_bytes", i64)]
 
 
+class HierPadRowsArgs(C.Structure):
+    _fields_ = [(n, i64) for n in ("rows0", "rows1", "ss0", "ss1")] + \
+               [(n, vp) for n in ("src0", "src1", "dst0", "dst1")] + [("C", i32), ("pad", i32)]   # the header's pairs
+
+
 class HierLinearBwdArgs(C.Structure):
     _fields_ = [("M", i64)] + [(n, i32) for n in ("N", "K", "type", "act")] + \
                [(n, vp) for n in ("x", "w", "gate", "dy", "preact", "dx", "dw", "db", "dgate")] + \
@@ -290,6 +295,7 @@ EXPORTS = {
     "hier_rms_norm_bwd": [vp, vp],
     "hier_linear_workspace": [vp],
     "hier_linear": [vp, vp],
+    "hier_pad_rows": [vp, vp],
     "hier_linear_bwd_workspace": [vp],
     "hier_linear_bwd": [vp, vp],
     "hier_cross_workspace": [vp],

@@ -28,6 +28,7 @@ _pack_norm = _capi.packer(_capi.HierRmsNormArgs)
 _pack_norm_bwd = _capi.packer(_capi.HierRmsNormBwdArgs)
 _pack_linear = _capi.packer(_capi.HierLinearArgs)
 _pack_linear_bwd = _capi.packer(_capi.HierLinearBwdArgs)
+_pack_pad = _capi.packer(_capi.HierPadRowsArgs)
 
 
 def _no_grad_call(name: str, *tensors) -> None:
@@ -61,20 +62,6 @@ def _rows(t: torch.Tensor):
     return t, (t.stride(0) if t.shape[0] > 1 else C)
 
 
-def _rows16(t: torch.Tensor):
-    """``_rows`` of 16-byte rows: copied, and padded to a multiple of eight
-    channels with zeros, where they are not."""
-    t, ss = _rows(t)
-    C = t.shape[1]
-    if C % 8:
-        t = torch.nn.functional.pad(t, (0, -C % 8))
-        return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    if ss % 8 or t.data_ptr() % 16 or ss < C:
-        t = _capi.aligned(t)
-        ss = C
-    return t, ss
-
-
 def _ptr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
@@ -87,6 +74,26 @@ def _outs(name: str, out: Optional[torch.Tensor], like: torch.Tensor, shape) -> 
     if not out.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return out
+
+
+def _operands(x: torch.Tensor, w: torch.Tensor):
+    """x [..., K] and w [N, K] as a product's operands, 16-byte rows of a multiple of
+    eight elements: their addresses and strides, that multiple, and what has to live as
+    long.  Others are copied, with zeros behind (``hier_pad_rows``)."""
+    (x, x_ss), (w, w_ss) = _rows(x), _rows(w)
+    K = x.shape[1]
+    at = [x.data_ptr(), w.data_ptr()]
+    ss = [x_ss, w_ss]
+    copy = [K % 8 or s % 8 or p % 16 or s < K for p, s in zip(at, ss)]
+    if not any(copy):
+        return at[0], x_ss, at[1], w_ss, K, (x, w)
+    Kp = K + -K % 8
+    rows = [t.shape[0] if c else 0 for t, c in zip((x, w), copy)]
+    buf = torch.empty((rows[0] + rows[1]) * Kp, dtype=x.dtype, device=x.device)
+    to = [buf.data_ptr(), buf.data_ptr() + 2 * rows[0] * Kp]
+    _capi.call_on(x.device, "hier_pad_rows", _pack_pad(*rows, *ss, *at, *to, K, 0))
+    at, ss = zip(*((to[i], Kp) if copy[i] else (at[i], ss[i]) for i in (0, 1)))
+    return at[0], ss[0], at[1], ss[1], Kp, (x, w, buf)
 
 
 def _apart(out: torch.Tensor, **inputs: torch.Tensor) -> None:
@@ -255,12 +262,11 @@ def _linear(x, weight, bias, activation, residual, gate, out, preact):
     out = _outs("out", out, x, shape)
     if M == 0:
         return out
-    (xr, x_ss), (w, w_ss) = _rows16(x), _rows16(weight)
-    K = xr.shape[1]
+    x_at, x_ss, w_at, w_ss, K, kept = _operands(x, weight)
     b = None if bias is None else bias.contiguous()
     r, r_ss = (None, 0) if residual is None else _rows(residual)
     g, g_ss = (None, 0) if gate is None else _rows(gate)
-    fields = (M, N, K, kind, act, xr.data_ptr(), w.data_ptr(), _ptr(b), _ptr(r), _ptr(g), out.data_ptr(),
+    fields = (M, N, K, kind, act, x_at, w_at, _ptr(b), _ptr(r), _ptr(g), out.data_ptr(),
               _ptr(preact), x_ss, w_ss, r_ss, g_ss, N, N, per)
     size = 0 if M <= 8 else _workspace("hier_linear_workspace", _pack_linear(*fields, 0, 0))
     ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
@@ -305,34 +311,24 @@ def linear_act_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
         made = {"x": lambda: torch.zeros_like(x), "weight": lambda: torch.zeros_like(weight),
                 "bias": lambda: new(N).zero_(), "gate": lambda: torch.zeros_like(gate)}
         return {n: made[n]() for n in need}
-    (xr, x_ss), (w, w_ss) = _rows16(x), _rows16(weight)
-    Kp = xr.shape[1]
-    # dy is an operand of the products where dz is dy itself
-    Np, b_dy = N, dy
-    if not act and gate is None and ("x" in need or "weight" in need):
-        if N % 8:                   # channels of zeros behind: rows of zeros in dw
-            Np = N + -N % 8
-            if "x" in need:
-                w = torch.nn.functional.pad(w, (0, 0, 0, Np - N))
-                w_ss = Kp
-        g_dy, dy_ss = _rows16(b_dy)
+    x_at, x_ss, w_at, w_ss, Kp, kept = _operands(x, weight)
+    g_dy, dy_ss = _rows(dy)
+    if not act and gate is None:
         preact = None
-    else:
-        g_dy, dy_ss = _rows(b_dy)
     z, z_ss = (None, 0) if preact is None else _rows(preact)
     g, g_ss = (None, 0) if gate is None else _rows(gate)
     dx = new(M, Kp) if "x" in need else None
-    dw = new(Np, Kp) if "weight" in need else None
-    db = new(Np) if "bias" in need else None
+    dw = new(N, Kp) if "weight" in need else None
+    db = new(N) if "bias" in need else None
     dg = new(M // per, N) if "gate" in need else None
-    fields = (M, Np, Kp, kind, act, xr.data_ptr(), w.data_ptr(), _ptr(g), g_dy.data_ptr(), _ptr(z), _ptr(dx),
+    fields = (M, N, Kp, kind, act, x_at, w_at, _ptr(g), g_dy.data_ptr(), _ptr(z), _ptr(dx),
               _ptr(dw), _ptr(db), _ptr(dg), x_ss, w_ss, g_ss, dy_ss, z_ss, Kp, Kp, per)
     size = _workspace("hier_linear_bwd_workspace", _pack_linear_bwd(*fields, 0, 0))
     ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
     _capi.call_on(x.device, "hier_linear_bwd", _pack_linear_bwd(*fields, _ptr(ws), size))
     made = {"x": lambda: (dx if Kp == K else dx[:, :K]).reshape(x.shape),
-            "weight": lambda: dw if (Np, Kp) == (N, K) else dw[:N, :K].contiguous(),
-            "bias": lambda: db if Np == N else db[:N].contiguous(),
+            "weight": lambda: dw if Kp == K else dw[:, :K],
+            "bias": lambda: db,
             "gate": lambda: dg.reshape(gate.shape)}
     return {n: made[n]() for n in need}
 

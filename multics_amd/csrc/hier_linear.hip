@@ -604,6 +604,39 @@ __global__ __launch_bounds__(256) void dot_kernel(GemmArgs g) {
   finish8<T>(g.e, v, m, n, n + 1);
 }
 
+// ---- rows at any address ---------------------------------------------------------
+
+struct PadArgs {
+  HierPadRowsArgs a;
+  int64_t first[2];            // chunks of eight elements of the first matrix, of both
+  int32_t cpr;
+};
+
+__global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs p) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.first[1]; i += (int64_t)gridDim.x * 256) {
+    const int which = i >= p.first[0];
+    const int64_t j = which ? i - p.first[0] : i;
+    const int64_t row = j >> 32 ? j / p.cpr : (uint32_t)j / (uint32_t)p.cpr;
+    const int n = 8 * (int)(j - row * p.cpr), C = p.a.C;
+    const uint16_t* src = static_cast<const uint16_t*>(which ? p.a.src[1] : p.a.src[0]) +
+                          row * (which ? p.a.ss[1] : p.a.ss[0]);
+    u32x4 w;
+    if (n + 8 <= C) {
+      __builtin_memcpy(&w, src + n, 16);
+    } else {
+      uint16_t t[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) t[e] = src[min(n + e, C - 1)];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t lo = n + 2 * e < C ? t[2 * e] : 0, hi = n + 2 * e + 1 < C ? t[2 * e + 1] : 0;
+        w[e] = lo | hi << 16;
+      }
+    }
+    reinterpret_cast<u32x4*>(which ? p.a.dst[1] : p.a.dst[0])[j] = w;
+  }
+}
+
 // ---- dz, db and dg ---------------------------------------------------------------
 //
 // One pass over dy and z, eight channels a thread.  A workgroup row takes `rows`
@@ -864,8 +897,12 @@ struct BwdPlan {
   DzPlan dz;
   int64_t off_dz, off_db, off_dg, off_part, bytes;
 };
-// dz is dy itself where there is neither an activation nor a gate.
-bool dz_is_dy(const HierLinearBwdArgs& a) { return a.act == HIER_ACT_NONE && !a.gate; }
+// dz is dy itself where there is neither an activation nor a gate, and dy has the
+// products' rows.
+bool dz_is_dy(const HierLinearBwdArgs& a) {
+  return a.act == HIER_ACT_NONE && !a.gate && a.N % 8 == 0 && aligned16(a.dy) && a.dy_ss % 8 == 0 && a.dy_ss >= a.N &&
+         a.dy_ss < (1 << 21);
+}
 
 BwdPlan bwd_plan(const HierLinearBwdArgs& a) {
   BwdPlan p = {};
@@ -954,6 +991,28 @@ extern "C" int hier_linear(const HierLinearArgs* args, void* stream) {
                       ok(a.out, a.out_ss) && ok(a.preact, a.preact_ss);
   return a.type == HIER_BF16 ? launch_gemm<__bf16, false, false>(g, p, ws, rows16, st)
                              : launch_gemm<_Float16, false, false>(g, p, ws, rows16, st);
+}
+
+extern "C" int hier_pad_rows(const HierPadRowsArgs* args, void* stream) {
+  clear_error();
+  HIER_REQUIRE(args != nullptr, HIER_EINVAL, "args is NULL");
+  PadArgs p = {};
+  p.a = *args;
+  const HierPadRowsArgs& a = p.a;
+  HIER_REQUIRE(a.C >= 1 && a.C < (1 << 21) && a.rows[0] >= 0 && a.rows[1] >= 0 && a.rows[0] < (1ll << 31) &&
+                   a.rows[1] < (1ll << 31),
+               HIER_EINVAL, "pad_rows: invalid sizes");
+  for (int i = 0; i < 2; ++i)
+    HIER_REQUIRE(a.rows[i] == 0 || (a.src[i] && a.dst[i] && aligned16(a.dst[i]) && (uintptr_t)a.src[i] % 2 == 0 &&
+                                    a.ss[i] >= 0),
+                 HIER_EINVAL, "pad_rows: needs rows, 16-byte aligned results and strides of at least 0");
+  p.cpr = (a.C + 7) / 8;
+  p.first[0] = a.rows[0] * p.cpr;
+  p.first[1] = p.first[0] + a.rows[1] * p.cpr;
+  if (p.first[1] == 0) return HIER_OK;
+  hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)std::min<int64_t>((p.first[1] + 255) / 256, 1 << 16)), dim3(256), 0,
+                     (hipStream_t)stream, p);
+  return check_launch("pad_rows_kernel");
 }
 
 static int check_linear_bwd(const HierLinearBwdArgs& a) {
@@ -1058,10 +1117,6 @@ extern "C" int hier_linear_bwd(const HierLinearBwdArgs* args, void* stream) {
     if (int rc = check_view("weight", a.w, a.w_ss, a.K)) return rc;
   if (a.dw)
     if (int rc = check_view("x", a.x, a.x_ss, a.K)) return rc;
-  if (dz_is_dy(a) && (a.dx || a.dw)) {
-    if (int rc = check_view("dy", a.dy, a.dy_ss, a.N)) return rc;
-    HIER_REQUIRE(a.N % 8 == 0, HIER_EINVAL, "linear_bwd: dy needs a multiple of 8 columns");
-  }
   auto ok = [](const void* q, int64_t ss) { return !q || (aligned16(q) && ss % 8 == 0 && ss < (1ll << 21)); };
   HIER_REQUIRE((!a.dx || a.dx_ss >= a.K) && (!a.dw || a.dw_ss >= a.K) && ok(a.dx, a.dx_ss) && ok(a.dw, a.dw_ss),
                HIER_EINVAL, "linear_bwd: dx and dw need 16-byte rows and an output stride of at least K");

@@ -36,6 +36,11 @@ def _cross(**kw):
     return _capi.HierCrossArgs(**{**f, **kw})
 
 
+def _pad(**kw):
+    f = dict(rows0=3, rows1=2, ss0=7, ss1=7, src0=AT, src1=AT, dst0=AT, dst1=AT, C=7)
+    return _capi.HierPadRowsArgs(**{**f, **kw})
+
+
 REFUSED = [
     ("hier_rms_norm", _norm, dict(C=0), "invalid"),
     ("hier_rms_norm", _norm, dict(C=16385, x_ss=16385, y_ss=16385), "16384"),
@@ -58,7 +63,12 @@ REFUSED = [
     ("hier_linear", _linear, dict(gate=AT, rows_per_gate=0), "rows_per_gate"),
     ("hier_linear", _linear, dict(M=200, N=64, K=1 << 16, x_ss=1 << 16, w_ss=1 << 16, out_ss=64), "workspace"),
     ("hier_linear_bwd", _linear_bwd, dict(act=1), "before the activation"),
-    ("hier_linear_bwd", _linear_bwd, dict(N=44, dy_ss=48), "multiple of 8"),
+    ("hier_linear_bwd", _linear_bwd, dict(N=44, dy_ss=45), "workspace"),     # dy's rows are copied
+    ("hier_pad_rows", _pad, dict(C=0), "invalid"),
+    ("hier_pad_rows", _pad, dict(rows0=-1), "invalid"),
+    ("hier_pad_rows", _pad, dict(dst0=AT + 2), "aligned"),
+    ("hier_pad_rows", _pad, dict(src0=None), "rows"),
+    ("hier_pad_rows", _pad, dict(ss1=-3), "strides"),
     ("hier_linear_bwd", _linear_bwd, dict(dgate=AT), "without a gate"),
     ("hier_linear_bwd", _linear_bwd, dict(gate=AT, rows_per_gate=33, preact=AT, preact_ss=48), "rows_per_gate"),
     ("hier_linear_bwd", _linear_bwd, dict(dy=None), "dy"),
@@ -100,7 +110,7 @@ def test_cross_gradient_entry_refuses(change, says):
 
 
 def test_entries_refuse_null():
-    for name in ("hier_rms_norm", "hier_rms_norm_bwd", "hier_linear", "hier_linear_bwd", "hier_cross_attn",
+    for name in ("hier_rms_norm", "hier_rms_norm_bwd", "hier_linear", "hier_linear_bwd", "hier_pad_rows", "hier_cross_attn",
                  "hier_cross_attn_bwd"):
         assert getattr(_capi.lib(), name)(None, None) == (_capi.HIER_EINVAL)
     for name in ("hier_rms_norm_bwd_rows", "hier_linear_workspace", "hier_linear_bwd_workspace",
