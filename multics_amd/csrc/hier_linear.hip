@@ -155,6 +155,7 @@ struct GemmArgs {
   const void* a;
   const void* b;
   int64_t lda, ldb, M, N, K;
+  int64_t m_first;             // row of the launch's first tile
   int64_t kchunk;              // K of a split, a multiple of the tile's
   int32_t tm, tn, splits, total;
   Epilogue e;
@@ -242,7 +243,7 @@ __global__ __launch_bounds__(256, WG) void gemm_kernel(GemmArgs g) {
     int tm, tn;
     gemm::tile_of(item - split * g.tm * g.tn, g.tm, g.tn, tm, tn);
     const int64_t k0 = split * g.kchunk, k1 = min(k0 + g.kchunk, g.K);
-    if (of_a) p.a.init(g.a, g.lda, g.M, (int64_t)tm * BM, k0, k1, wave, wm, lane);
+    if (of_a) p.a.init(g.a, g.lda, g.M, g.m_first + (int64_t)tm * BM, k0, k1, wave, wm, lane);
     else p.b.init(g.b, g.ldb, g.N, (int64_t)tn * BN, k0, k1, wave, wn, lane);
   };
   auto next_a = [&]() {
@@ -268,7 +269,7 @@ __global__ __launch_bounds__(256, WG) void gemm_kernel(GemmArgs g) {
     gemm::tile_of(item - split * g.tm * g.tn, g.tm, g.tn, tm, tn);
     const int64_t k0 = split * g.kchunk;
     const int nt = (int)((min(k0 + g.kchunk, g.K) - k0 + BK - 1) / BK);
-    const int64_t m0 = (int64_t)tm * BM + wm * MI * 32;
+    const int64_t m0 = g.m_first + (int64_t)tm * BM + wm * MI * 32;
     const int n0 = tn * BN + wn * NI * 32;
     const int rows = (int)min(g.M - m0, (int64_t)(32 * MI));     // (may be none)
     f32x16 acc[NI][MI];
@@ -746,6 +747,7 @@ struct Plan {
   int splits;
   int64_t kchunk;
   int64_t bytes;      // fp32 parts
+  int64_t rows;       // by these tiles; the rest by tiles of 128 in a launch of their own
 };
 
 constexpr int kBK = 64;
@@ -775,39 +777,59 @@ Plan plan_of(int64_t M, int64_t N, int64_t K) {
       }
     }
   }
+  best.rows = M;
+  if (best.tile == 256 && best.splits == 1) {
+    // a last round of few tiles: the rows past the whole rounds in small tiles, where those
+    // and a launch more take less than the round
+    const int64_t tn = (N + 255) / 256, rounds = ((M + 255) / 256 * tn + kSlots - 1) / kSlots;
+    const int64_t rows = (rounds - 1) * kSlots / tn * 256;
+    if (rows > 0 && rows < M) {
+      const int64_t small = ((M - rows + 127) / 128) * ((N + 127) / 128);
+      if (kt + 8 > 5 + (double)((small + 2 * kSlots - 1) / (2 * kSlots)) * (0.6 * (double)kt + 4)) best.rows = rows;
+    }
+  }
   return best;
 }
 
 template <typename T, bool ATR, bool BTR>
 int launch_gemm(GemmArgs g, const Plan& p, float* ws, bool rows16, hipStream_t st) {
-  g.tm = (int)((g.M + p.tile - 1) / p.tile);
-  g.tn = (int)((g.N + p.tile - 1) / p.tile);
   g.splits = p.splits;
   g.kchunk = p.kchunk;
-  const int64_t total = (int64_t)g.tm * g.tn * g.splits;
-  HIER_REQUIRE(total <= (1ll << 23), HIER_EUNSUPPORTED, "product: too many tiles");
-  g.total = (int)total;
   g.e.partial = ws;
   g.e.ld_part = (g.N + 7) / 8 * 8;
   g.e.part_stride = g.M * g.e.ld_part;
-  auto run = [&](auto kind) {
-    constexpr int KIND = decltype(kind)::value;
-    if (p.tile == 256)
-      hipLaunchKernelGGL((gemm_kernel<T, ATR, BTR, 256, 256, kBK, 1, KIND>),
-                         dim3((unsigned)xcd_grid(std::min<int64_t>(total, kSlots))), dim3(256), 0, st, g);
-    else
-      hipLaunchKernelGGL((gemm_kernel<T, ATR, BTR, 128, 128, kBK, 2, KIND>),
-                         dim3((unsigned)xcd_grid(std::min<int64_t>(total, 2 * kSlots))), dim3(256), 0, st, g);
+  // rows from g.m_first to `end` in tiles of `tile`
+  auto rows = [&](int tile, int64_t end) {
+    g.tm = (int)((end - g.m_first + tile - 1) / tile);
+    g.tn = (int)((g.N + tile - 1) / tile);
+    const int64_t total = (int64_t)g.tm * g.tn * g.splits;
+    HIER_REQUIRE(total <= (1ll << 23), HIER_EUNSUPPORTED, "product: too many tiles");
+    g.total = (int)total;
+    auto run = [&](auto kind) {
+      constexpr int KIND = decltype(kind)::value;
+      if (tile == 256)
+        hipLaunchKernelGGL((gemm_kernel<T, ATR, BTR, 256, 256, kBK, 1, KIND>),
+                           dim3((unsigned)xcd_grid(std::min<int64_t>(total, kSlots))), dim3(256), 0, st, g);
+      else
+        hipLaunchKernelGGL((gemm_kernel<T, ATR, BTR, 128, 128, kBK, 2, KIND>),
+                           dim3((unsigned)xcd_grid(std::min<int64_t>(total, 2 * kSlots))), dim3(256), 0, st, g);
+    };
+    // (the parts' launch writes whole rows of its own)
+    if constexpr (ATR || BTR) {
+      run(std::integral_constant<int, kPlain>{});
+    } else {
+      if (p.splits > 1 || (rows16 && !g.e.gate && !g.e.residual)) run(std::integral_constant<int, kPlain>{});
+      else if (rows16) run(std::integral_constant<int, kExtra>{});
+      else run(std::integral_constant<int, kAny>{});
+    }
+    return check_launch("gemm_kernel");
   };
-  // (the parts' launch writes whole rows of its own)
-  if constexpr (ATR || BTR) {
-    run(std::integral_constant<int, kPlain>{});
-  } else {
-    if (p.splits > 1 || (rows16 && !g.e.gate && !g.e.residual)) run(std::integral_constant<int, kPlain>{});
-    else if (rows16) run(std::integral_constant<int, kExtra>{});
-    else run(std::integral_constant<int, kAny>{});
+  if (int rc = rows(p.tile, p.rows)) return rc;
+  if (p.rows < g.M) {
+    g.m_first = p.rows;
+    g.kchunk = (g.K + kBK - 1) / kBK * kBK;
+    if (int rc = rows(128, g.M)) return rc;
   }
-  if (int rc = check_launch("gemm_kernel")) return rc;
   if (p.splits > 1) {
     const int64_t n8 = g.M * ((g.N + 7) / 8);
     hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)std::min<int64_t>((n8 + 255) / 256, 8192)),

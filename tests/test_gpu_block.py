@@ -169,6 +169,8 @@ LINEARS = [
     (8, 6000, 72, "gelu_tanh", 2, True, BF16),
     (9, 2056, 100, None, 3, True, FP16),
     (16, 4000, 4000, "silu", 4, True, BF16),       # few rows of many weights: over tiles
+    (2305, 2400, 8000, "silu", 5, True, BF16),     # the rows of a last round in small tiles, dw's too
+    (2305, 520, 7999, "gelu_tanh", 461, True, FP16),
 ]
 LIPSCHITZ = 1.2          # bounds every activation's slope; their second derivatives are under 1
 
