@@ -183,6 +183,12 @@ struct View {
   __device__ __forceinline__ void store(const u32x4& v, uint32_t off) const {
     __builtin_amdgcn_raw_buffer_store_b128(v, rsrc, off, 0, 0);
   }
+  // Results: through the L2 as they come (scope of the GPU, non-temporal).  Left in it a
+  // round's (4 MB an XCD, all it holds) push the operands out: 18,816 x 8,960 x 1,536
+  // 438 -> 429 us, 4,300 x 4,096 x 512 35.4 -> 32.5.  (Parts are read again: left in it.)
+  __device__ __forceinline__ void stream(const u32x4& v, uint32_t off) const {
+    __builtin_amdgcn_raw_buffer_store_b128(v, rsrc, off, 0, 18);
+  }
 };
 
 // Pass K's sums (32 rows, COLS x 32 channels) into the wave's part of LDS.
@@ -360,7 +366,7 @@ __global__ __launch_bounds__(256, WG) void gemm_kernel(GemmArgs g) {
           for (int it = 0; it < ITS; ++it)
             res[it] = vr.load(g.e.residual ? off(r0 + it * RPI, n, g.e.residual_ss) : gemm::kOut);
 #pragma unroll
-          for (int it = 0; it < ITS; ++it) vo.store(held[it], to[it]);
+          for (int it = 0; it < ITS; ++it) vo.stream(held[it], to[it]);
         }
         put_sums<NI, MI, COLS>(acc, mine, el, pass, std::make_integer_sequence<int, PASSES>{});
         f32x4 lo[ITS], hi[ITS];
@@ -392,7 +398,7 @@ __global__ __launch_bounds__(256, WG) void gemm_kernel(GemmArgs g) {
           float v[8] = {lo[it][0], lo[it][1], lo[it][2], lo[it][3], hi[it][0], hi[it][1], hi[it][2], hi[it][3]}, t[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] += b[i];
-          if (g.e.preact) vz.store(narrow<T>(v), off(r0 + it * RPI, n, g.e.preact_ss));
+          if (g.e.preact) vz.stream(narrow<T>(v), off(r0 + it * RPI, n, g.e.preact_ss));
           activate8(v, g.e.act);
           const uint32_t at = off(r0 + it * RPI, n, g.e.out_ss);
           if constexpr (KIND == kExtra) {
@@ -407,13 +413,13 @@ __global__ __launch_bounds__(256, WG) void gemm_kernel(GemmArgs g) {
             held[it] = narrow<T>(v);
             to[it] = at;
           } else {
-            vo.store(narrow<T>(v), at);
+            vo.stream(narrow<T>(v), at);
           }
         }
       }
       if constexpr (KIND == kExtra)
 #pragma unroll
-        for (int it = 0; it < ITS; ++it) vo.store(held[it], to[it]);
+        for (int it = 0; it < ITS; ++it) vo.stream(held[it], to[it]);
     }
     // every wave is done with the spare slot before it is filled
     barrier_lds();
