@@ -572,11 +572,12 @@ def test_small_weights_count_in_the_sum():
         assert bool((lse - w.sum().log()).abs().max() <= half + S * 2.0 ** -25 + 2.0 ** -12)
 
 
-def test_growing_scores_refresh_the_maximum():
+@pytest.mark.parametrize("Sq", [70, 4])
+def test_growing_scores_refresh_the_maximum(Sq):
     """Every key block above the one before, the first keys masked."""
     need_gpu()
     r = _rnd(23)
-    q = torch.ones(1, 70, 1, 128, device="cuda", dtype=BF16)
+    q = torch.ones(1, Sq, 1, 128, device="cuda", dtype=BF16)
     k = 0.05 * r(1, 640, 1, 128)
     k = (k + torch.arange(640, device="cuda")[None, :, None, None] / 80).to(BF16)
     v = r(1, 640, 1, 128).to(BF16)
@@ -584,6 +585,29 @@ def test_growing_scores_refresh_the_maximum():
     got = kernels.cross_attention(q, k, v, key_mask=mask)
     O, slack, _, _ = _cross_formula(q, k, v, mask, 1 / math.sqrt(128), torch.zeros_like(q))  # noqa: E741
     _within(got, O, slack)
+
+
+@pytest.mark.parametrize("Sq", [1, 40, 200])
+def test_keys_that_are_not_numbers_stay_in_their_stream(Sq):
+    """A seen key or value that is NaN or infinite makes its stream's rows (that see it) so, no
+    others, in one part or several; hidden ones nothing (the other tests' masked keys are NaN)."""
+    need_gpu()
+    r = _rnd(31)
+    q, k, v = r(3, Sq, 2, 64).to(BF16), r(3, 3000, 2, 64).to(BF16), r(3, 3000, 2, 64).to(BF16)
+    clean = kernels.cross_attention(q, k, v)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        for which in (0, 1):
+            kk, vv = k.clone(), v.clone()
+            (kk, vv)[which][1, 2500, 1, 7] = bad
+            say("not a number", Sq, bad, which)
+            lse = torch.empty(3, 2, Sq, device="cuda")
+            got = kernels.cross_attention(q, kk, vv, lse=lse)
+            assert torch.equal(got[0], clean[0]) and torch.equal(got[2], clean[2])
+            assert torch.equal(got[1, :, 0], clean[1, :, 0])
+            P = torch.softmax((q[1, :, 1].float() @ kk[1, :, 1].float().t()) / 8, -1)
+            want = P @ vv[1, :, 1].float()
+            assert torch.equal(torch.isnan(got[1, :, 1]), torch.isnan(want))
+            assert torch.equal(torch.isinf(got[1, :, 1]), torch.isinf(want))
 
 
 def test_cross_attention_reads_views():
