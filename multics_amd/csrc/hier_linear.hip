@@ -130,28 +130,38 @@ __device__ __forceinline__ uint32_t gate_row(const Epilogue& e, int64_t m) {
   return e.gate ? quotient((uint32_t)m, e.rows_per_gate) : 0u;
 }
 
-// The whole epilogue of eight channels of one row.
+// The whole epilogue of eight channels of one row: what it reads, and the rest of it.
+template <typename T>
+struct Finish {
+  float bias[8], gate[8], residual[8];
+  __device__ __forceinline__ void read(const Epilogue& e, int64_t m, int n, int N) {
+    if (e.bias) row8<T>(e.bias, 0, n, N, bias);
+    if (e.gate) row8<T>(e.gate, (int64_t)gate_row(e, m) * e.gate_ss, n, N, gate);
+    if (e.residual) row8<T>(e.residual, m * e.residual_ss, n, N, residual);
+  }
+  __device__ __forceinline__ void write(const Epilogue& e, float* v, int64_t m, int n, int N) const {
+    if (e.bias) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += bias[i];
+    }
+    if (e.preact) put_row8<T>(e.preact, m * e.preact_ss, n, N, v);
+    activate8(v, e.act);
+    if (e.gate) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= gate[i];
+    }
+    if (e.residual) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += residual[i];
+    }
+    put_row8<T>(e.out, m * e.out_ss, n, N, v);
+  }
+};
 template <typename T>
 __device__ __forceinline__ void finish8(const Epilogue& e, float* v, int64_t m, int n, int N) {
-  float t[8];
-  if (e.bias) {
-    row8<T>(e.bias, 0, n, N, t);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += t[i];
-  }
-  if (e.preact) put_row8<T>(e.preact, m * e.preact_ss, n, N, v);
-  activate8(v, e.act);
-  if (e.gate) {
-    row8<T>(e.gate, (int64_t)gate_row(e, m) * e.gate_ss, n, N, t);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= t[i];
-  }
-  if (e.residual) {
-    row8<T>(e.residual, m * e.residual_ss, n, N, t);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += t[i];
-  }
-  put_row8<T>(e.out, m * e.out_ss, n, N, v);
+  Finish<T> f;
+  f.read(e, m, n, N);
+  f.write(e, v, m, n, N);
 }
 
 // ---- products over LDS tiles -----------------------------------------------------
@@ -435,7 +445,7 @@ __global__ __launch_bounds__(256, WG) void gemm_kernel(GemmArgs g) {
 
 // The splits' sums in their order, and the epilogue.
 template <typename T>
-__global__ __launch_bounds__(256) void join_kernel(GemmArgs g) {
+__global__ __launch_bounds__(256, 4) void join_kernel(GemmArgs g) {
   const int cpr = (int)((g.N + 7) / 8);
   const int64_t n8 = g.M * cpr;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n8; i += (int64_t)gridDim.x * 256) {
@@ -443,22 +453,27 @@ __global__ __launch_bounds__(256) void join_kernel(GemmArgs g) {
     const int n = 8 * (int)(i - m * cpr);
     const float* p = g.e.partial + m * g.e.ld_part + n;
     float v[8] = {};
-    // (four splits' loads leave together, the last split's again past the end)
-    for (int s = 0; s < g.splits; s += 4) {
-      f32x4 x[4][2];
+    Finish<T> f;
+    // (eight splits' loads leave together, the last split's again past the end, and with the
+    // first ones those of the epilogue)
+    for (int s = 0; s < g.splits; s += 8) {
+      f32x4 x[8][2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 8; ++i) {
+        if (i == 4 && s + 4 >= g.splits) break;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           x[i][h] = *reinterpret_cast<const f32x4*>(p + min(s + i, g.splits - 1) * g.e.part_stride + 4 * h);
+      }
+      if (s == 0) f.read(g.e, m, n, (int)g.N);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 8; ++i) {
         if (s + i >= g.splits) break;
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] += x[i][j / 4][j % 4];
       }
     }
-    finish8<T>(g.e, v, m, n, (int)g.N);
+    f.write(g.e, v, m, n, (int)g.N);
   }
 }
 
@@ -873,10 +888,13 @@ int launch_few(const GemmArgs& g, hipStream_t st) {
 }
 
 // Whether dot_kernel or few_rows_kernel takes a product.  The second reads x again for
-// every 16 channels: past some 200 million products the tiles win (64 rows of 1536 x 1536 10.1
-// us for 11.1; 17 of 1536 x 8960 13.5 for 15.7, 32 of them 17.8 for 15.7; 16 of 8960 x
-// 1536 22 for 18.4, of 4096 x 16384 38 for 34.7).
-bool few_rows(int64_t M, int64_t N, int64_t K) { return M <= kDotRows || (M <= 64 && M * N * K <= 200000000); }
+// every 16 channels and waits for memory a thousand of K at a time: past some 200
+// million products, or a long K, the tiles win (64 rows of 1536 x 1536 10.1 us for 11.1; 17
+// of 1536 x 8960 13.5 for 13.1, 32 of them 17.8 for 14.1; 9 of 8960 x 1536 18.6 for 15.6;
+// 16 of 4096 x 16384 38 for 30.7).
+bool few_rows(int64_t M, int64_t N, int64_t K) {
+  return M <= kDotRows || (M <= 64 && K <= 4096 && M * N * K <= 200000000);
+}
 
 // Views that the copies address: 16-byte rows, a tile's rows (256) within 31
 // bits of bytes.
