@@ -397,7 +397,7 @@ extern "C" int64_t hier_rms_norm_bwd_rows(const HierRmsNormBwdArgs* a) {
 extern "C" int hier_rms_norm_bwd(const HierRmsNormBwdArgs* args, void* stream) {
   clear_error();
   HIER_REQUIRE(args != nullptr, HIER_EINVAL, "args is NULL");
-  const HierRmsNormBwdArgs& a = *args;
+  HierRmsNormBwdArgs a = *args;
   if (int rc = check_common(a, "rms_norm_bwd")) return rc;
   HIER_REQUIRE(a.M >= 1, HIER_EINVAL, "rms_norm_bwd: no rows");
   HIER_REQUIRE(a.x && a.w && a.dy && a.dx && a.dw && a.partial, HIER_EINVAL, "rms_norm_bwd: NULL pointer");
@@ -410,7 +410,9 @@ extern "C" int hier_rms_norm_bwd(const HierRmsNormBwdArgs* args, void* stream) {
   const bool vec = a.C % 8 == 0 && aligned16(a.w) && rows16(a.x, a.x_ss) && rows16(a.dy, a.dy_ss) &&
                    rows16(a.dx, a.dx_ss) && (!a.r || rows16(a.r, a.r_ss)) &&
                    (!a.dh || rows16(a.dh, a.dh_ss));
+  const bool one = bwd_groups(a.M, a.C) == 1;        // its row of sums is dw
+  if (one) a.partial = a.dw;
   by_type(a, vec, (hipStream_t)stream);
   if (int rc = check_launch("norm_bwd_kernel")) return rc;
-  return sum_rows(a.partial, bwd_groups(a.M, a.C), 1, a.C, a.dw, HIER_FP32, (hipStream_t)stream);
+  return one ? HIER_OK : sum_rows(a.partial, bwd_groups(a.M, a.C), 1, a.C, a.dw, HIER_FP32, (hipStream_t)stream);
 }
