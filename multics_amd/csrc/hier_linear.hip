@@ -68,7 +68,8 @@ __device__ __forceinline__ void activate8(float* v, int act) {
 }
 
 // act(z) and act'(z).  Past |z| = 30 (SiLU: 100) the slopes are 0 or 1 to fp32: z is kept
-// there, so no square of it overflows into inf * 0.
+// there, so no square of it overflows into inf * 0.  (The clamp takes a NaN to one of its
+// bounds: its slope is set right by keep_nans.)
 template <int ACT>
 __device__ __forceinline__ void activate2(float z, float& a, float& slope) {
   if constexpr (ACT == HIER_ACT_GELU_TANH) {
@@ -87,6 +88,20 @@ __device__ __forceinline__ void activate2(float z, float& a, float& slope) {
     a = z;
     slope = 1.f;
   }
+}
+
+// dz is NaN where z is.  By the bits: the compiler takes it that there are no NaNs and drops
+// comparisons and classes of floats.  One test for eight values, as hardly any row has one
+// (a test a value: 118 -> 126 us for 9,408 x 8,960).
+__device__ __forceinline__ uint32_t magnitude(float z) { return __float_as_uint(z) << 1; }
+__device__ __forceinline__ void keep_nans(const float* z, float* dz) {
+  constexpr uint32_t INF = 0xff000000u;
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, magnitude(z[i]));
+  if (top <= INF) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) dz[i] = magnitude(z[i]) > INF ? z[i] : dz[i];
 }
 
 // Eight neighbouring channels of 16 bits, at any even address (the hardware takes
@@ -748,8 +763,10 @@ __global__ __launch_bounds__(256) void dz_kernel(DzArgs d) {
         activate2<ACT>(z[i], a, slope);
         dg[i] = fmaf(y[i], a, dg[i]);
         dz[i] = y[i] * gate[i] * slope;
-        db[i] += dz[i];
       }
+      if constexpr (ACT != HIER_ACT_NONE) keep_nans(z, dz);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) db[i] += dz[i];
       if (d.dz) put8<T>(d.dz, (r + j) * d.dz_ss + n, dz);
     }
   }
