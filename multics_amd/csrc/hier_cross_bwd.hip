@@ -6,11 +6,15 @@
 // backward's (hier_attn_bwd.hip), each gradient row written by one workgroup:
 //
 // dq      128 rows an item, four waves: K and V tiles through LDS, per 32-key block
-//         S, dP, dQ.  Also writes -delta and lse log2(e) of every row, in the order
-//         of the rows, for dkv.
+//         S, dP, dQ.  Also writes -delta and lse log2(e) - 15 of every row, in the
+//         order of the rows, for dkv.
 // dkv     128 keys an item, eight waves: wave w makes S, P and dV of its 32 keys,
 //         wave w + 4 of the same keys dP, dS and dK, P handed over through LDS as
-//         fp16 (10 bits of a value of at most 1).  Items are few where the keys are
+//         fp16.  P is 2^15 times the weight throughout (hence the 15 above; dK and dV
+//         are scaled back at the end): a weight is at most 1, and down to 2^-29 it keeps
+//         fp16's eleven bits, as many keys as a call may have.  (lse in fp32 leaves a weight's
+//         exponent off by 2^-23 of the score: past scores of 5 million one may come out
+//         as 2, which fp16 does not hold.)  Items are few where the keys are
 //         (an encoder's 512 are four a head): the rows may then be cut into splits, whose
 //         fp32 sums a third kernel adds in their order.
 // dP starts from -delta, as S does from -m in the forward: the subtraction is the
@@ -29,13 +33,14 @@ namespace {
 
 using namespace cross;
 typedef __bf16 T;
+constexpr float kUpLog2 = 15.f, kDown = 1.f / 32768.f;   // of dkv's P
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 struct Launch {
   HierCrossBwdArgs a;
   Div div;
   int32_t row_tiles, key_tiles, splits, total, dq_splits;
-  float* lse2;         // [B * Hk][row_tiles * 128]
+  float* lse2;         // [B * Hk][row_tiles * 128], less kUpLog2
   float* delta;        // minus it
   float* part;         // [splits][dk, dv][B * Hk][Sk][D]; before that dQ's [dq_splits][B * Hk][rows][D]
 };
@@ -257,7 +262,7 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(Launch p) {
   w.c2 = a.scale * kLog2e;
   if (split == 0 && w.lane < 32) {       // rows past the last: P = 0, whatever dkv reads there
     const int64_t at = (int64_t)bh * p.row_tiles * kRows + r0 + w.lane;
-    p.lse2[at] = valid ? w.lse2 : INFINITY;
+    p.lse2[at] = valid ? w.lse2 - kUpLog2 : INFINITY;
     p.delta[at] = valid ? w.ndelta : 0.f;
   }
 #pragma unroll
@@ -397,8 +402,8 @@ __global__ __launch_bounds__(512, 1) void cross_dkv_kernel(Launch p) {
   };
   f16x8* const pslot = lds_p + w.wave * 2 * 64 + w.lane;   // + parity * 1024 + block * 512 + half * 64
 
-  // waves 0-3: S and P of a block of the tile in stage sg, kept as dV's operand and
-  // handed over
+  // waves 0-3: S and P (2^15 times it) of a block of the tile in stage sg, kept as dV's
+  // operand and handed over
   auto a_block = [&](int sg, int par, int qb, u32x4* pb) {
     const float* l2 = reinterpret_cast<const float*>(lds_w[sg]);
     const f32x16 zero = {};
@@ -524,10 +529,10 @@ __global__ __launch_bounds__(512, 1) void cross_dkv_kernel(Launch p) {
   if (p.splits > 1) {
     store_part<D>(p.part + ((((int64_t)split * 2 + (role_b ? 0 : 1)) * a.B * a.Hk + bh) * a.Sk + key) * D, w.acc, w.lane);
   } else if (role_b) {
-    store_acc<D>(static_cast<uint16_t*>(p.a.dk) + b * p.a.dk_sb + key * p.a.dk_ss + hk * p.a.dk_sh, w.acc, a.scale,
-                 w.lane);
+    store_acc<D>(static_cast<uint16_t*>(p.a.dk) + b * p.a.dk_sb + key * p.a.dk_ss + hk * p.a.dk_sh, w.acc,
+                 a.scale * kDown, w.lane);
   } else {
-    store_acc<D>(static_cast<uint16_t*>(p.a.dv) + b * p.a.dv_sb + key * p.a.dv_ss + hk * p.a.dv_sh, w.acc, 1.f,
+    store_acc<D>(static_cast<uint16_t*>(p.a.dv) + b * p.a.dv_sb + key * p.a.dv_ss + hk * p.a.dv_sh, w.acc, kDown,
                  w.lane);
   }
 }
@@ -565,10 +570,11 @@ __global__ __launch_bounds__(256) void cross_grad_join_kernel(Launch p) {
     out = dv ? static_cast<uint16_t*>(p.a.dv) + b * p.a.dv_sb + r * p.a.dv_ss + hk * p.a.dv_sh
              : static_cast<uint16_t*>(p.a.dk) + b * p.a.dk_sb + r * p.a.dk_ss + hk * p.a.dk_sh;
   }
+  const float mul = DQ ? a.scale : dv ? kDown : a.scale * kDown;
   typedef T quad __attribute__((ext_vector_type(4)));
   quad v;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = (T)(dv ? s[e] : s[e] * a.scale);
+  for (int e = 0; e < 4; ++e) v[e] = (T)(s[e] * mul);
   *reinterpret_cast<u32x2*>(out + d) = __builtin_bit_cast(u32x2, v);
 }
 

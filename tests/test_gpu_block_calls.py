@@ -1,12 +1,14 @@
 """Calls of the block's operators that their documentation allows and the formulas' cases
 do not make, against the formulas in 64 bits.  Bounds as in ``test_gpu_block``."""
 
+import math
+
 import pytest
 import torch
 
 from multics_amd import kernels
 from tests.gpu_util import need_gpu, say
-from tests.test_gpu_block import BF16, FP16, _linear_case
+from tests.test_gpu_block import BF16, FP16, U, _linear_case, _rnd, _step, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +35,53 @@ def test_gradient_of_a_nan_before_the_activation(act, t, N):
     assert torch.isnan(got["gate"][1, 5])                    # (50 rows a gate)
     got["gate"][1, 5] = clean["gate"][1, 5]
     assert torch.equal(got["gate"], clean["gate"])
+
+
+# ---- small weights of the attention's gradient ----------------------------------------------
+
+@pytest.mark.parametrize("Sq,Sk,peak,D", [(40, 4096, 14.0, 64), (40, 4096, 20.0, 128), (2000, 300, 18.0, 128),
+                                          (200, 65536, None, 64)])
+def test_gradient_of_keys_of_small_weight(Sq, Sk, peak, D):
+    """Thousands of keys beside one that takes most of the weight, or of even weight: their
+    gradients to the precision of bf16, however small the weights."""
+    need_gpu()
+    r = _rnd(19)
+    scale = D ** -0.5
+    q, k = r(1, Sq, 1, D), 0.25 * r(1, Sk, 1, D)
+    if peak is not None:
+        q[..., 0], k[..., 0] = 4.0, 0.0
+        k[:, 3] = 0.0
+        k[:, 3, :, 0] = peak / (4.0 * scale)
+    q, k, v, dout = q.to(BF16), k.to(BF16), r(1, Sk, 1, D).to(BF16), r(1, Sq, 1, D).to(BF16)
+    say("keys of small weight", Sq, Sk, peak, D)
+    lse = torch.empty(1, 1, Sq, device="cuda")
+    out = kernels.cross_attention(q, k, v, lse=lse)
+    dq, dk, dv = kernels.cross_attention_backward(dout, q, k, v, out, lse)
+    Q, K, V, dO = (t[0, :, 0].double() for t in (q, k, v, dout))
+    S = Q @ K.t() * scale
+    P = torch.softmax(S, -1)
+    step = _step(BF16)
+    size = Q.abs() @ K.abs().t() * scale
+    e_S = (D + 8) * U * 4 * (size + size.amax(-1, keepdim=True)) + 2.0 ** -20
+    O = P @ V  # noqa: E741
+    e_O = (P * (step + e_S)) @ V.abs() + (P * (step + e_S)).sum(-1, keepdim=True) * O.abs() + (Sk + 8) * U * (P @ V.abs())
+    e_O = e_O + step * (O.abs() + e_O)
+    # P: of scores in fp32 and a sum of rounded weights; handed over in eleven bits, down to 2^-29
+    e_P = P * (e_S + step + (P * (step + e_S)).sum(-1, keepdim=True) + 2.0 ** -11) + 2.0 ** -40
+    dP, delta = dO @ V.t(), (dO * O).sum(-1, keepdim=True)
+    e_dP = (D + 8) * U * (dO.abs() @ V.abs().t() + (dO * O).abs().sum(-1, keepdim=True)) + \
+        (dO.abs() * e_O).sum(-1, keepdim=True)
+    dS = P * (dP - delta)
+    e_dS = e_P * ((dP - delta).abs() + e_dP) + P * e_dP
+    e_dS = e_dS + step * (dS.abs() + e_dS)
+    n = (Sq + 8) * U
+    _within(dk[0, :, 0], dS.t() @ Q * scale, (e_dS + n * dS.abs()).t() @ Q.abs() * scale + 1e-30)
+    _within(dv[0, :, 0], P.t() @ dO, (e_P + n * P).t() @ dO.abs() + 1e-30)
+    _within(dq[0, :, 0], dS @ K * scale, (e_dS + (Sk + 8) * U * dS.abs()) @ K.abs() * scale + 1e-30)
+    if peak is not None:                       # and no key's gradient is lost
+        ref = dS.t() @ Q * scale
+        err = (dk[0, :, 0].double() - ref).norm(dim=-1) / ref.norm(dim=-1)
+        err[3] = 0.0
+        # three roundings (O, dS, the result) of at most a step of the terms, at random over rows and
+        # channels: the terms' root of squares is within 1.5 of the sum's norm
+        assert float(err.max()) <= 1.5 * math.sqrt(3) * step, float(err.max())
