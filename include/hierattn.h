@@ -754,7 +754,8 @@ int hier_rms_norm_bwd(const HierRmsNormBwdArgs* args, void* stream);
 /* .. of out.  x and w: 16-byte aligned rows of K contiguous elements, K a    */
 /* multiple of 8, at most 2^21 - 1 elements apart.  `workspace` of            */
 /* hier_linear_workspace(args) bytes (16-byte aligned) belongs to one call at */
-/* a time.  out may be residual.                                             */
+/* a time.  out may be residual itself; what is written shares no memory with */
+/* what is read otherwise.                                                    */
 typedef struct HierLinearArgs {
   int64_t M;
   int32_t N, K;
@@ -821,7 +822,7 @@ int hier_linear_bwd(const HierLinearBwdArgs* args, void* stream);
 /* Sk; taken within [0, Sk]) counts a stream's keys, key_mask (bytes, NULL: */
 /* all) says which are seen; the rest of k and v is not read.  16-byte rows, */
 /* k_ss and v_ss at least D.  lse: fp32 [B][Hq][Sq] or NULL, -inf where no key */
-/* is seen.  `workspace` (hier_cross_workspace(args) bytes, 16-byte aligned)  */
+/* is seen.  o and lse share no memory with what is read.  `workspace` (hier_cross_workspace(args) bytes, 16-byte aligned)  */
 /* belongs to one call at a time.                                            */
 typedef struct HierCrossArgs {
   int32_t B, Hq, Hk, D;

@@ -99,14 +99,34 @@ def _operands(x: torch.Tensor, w: torch.Tensor):
     return at[0], ss[0], at[1], ss[1], Kp, (x, w, buf)
 
 
-def _apart(out: torch.Tensor, **inputs: torch.Tensor) -> None:
-    """Refuses an ``out`` in the memory of an input that is still read while it is
-    written (views that interleave with it, in a larger tensor, pass)."""
-    first, last = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
-    for name, t in inputs.items():
-        at = t.data_ptr()
-        if t.is_contiguous() and out.is_contiguous() and at < last and first < at + t.numel() * t.element_size():
-            raise ValueError(f"out must not share memory with {name}")
+def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors may have a byte in common: not where one ends before the other
+    begins, nor where both are rows (of whatever inner dimensions) of one pitch that lie
+    side by side, as a projection's slices do."""
+    if not a.numel() or not b.numel():
+        return False
+    (pa, da, ia), (pb, db, ib) = (
+        (t.data_ptr(), [(n, s * t.element_size()) for n, s in zip(t.shape, t.stride()) if n > 1 and s], t.element_size())
+        for t in (a, b))
+
+    def span(dims, item, below=math.inf):
+        return sum((n - 1) * s for n, s in dims if s < below) + item
+    if pa + span(da, ia) <= pb or pb + span(db, ib) <= pa:
+        return False
+    strides = {s for _, s in da + db}
+    for least in strides:
+        pitch = math.gcd(*(s for s in strides if s >= least))
+        at = (pb - pa) % pitch
+        if at >= span(da, ia, least) and at + span(db, ib, least) <= pitch:
+            return False
+    return True
+
+
+def _apart(name: str, written: torch.Tensor, /, **inputs: Optional[torch.Tensor]) -> None:
+    """Refuses an output in the memory of a tensor that is read while it is written."""
+    for other, t in inputs.items():
+        if t is not None and _share(written, t):
+            raise ValueError(f"{name} must not share memory with {other}")
 
 
 # --------------------------------------------------------------------------
@@ -260,9 +280,11 @@ def _workspace(name: str, args: bytes) -> int:
 def _linear(x, weight, bias, activation, residual, gate, out, preact):
     kind, act, M, N, K, per = _linear_args(x, weight, bias, activation, residual, gate)
     shape = (*x.shape[:-1], N)
-    if out is not None:
-        _apart(out, x=x, weight=weight)
+    given = out is not None
     out = _outs("out", out, x, shape)
+    if given:
+        same = residual is not None and residual.data_ptr() == out.data_ptr() and residual.is_contiguous()
+        _apart("out", out, x=x, weight=weight, bias=bias, gate=gate, residual=None if same else residual)
     if M == 0:
         return out
     x_at, x_ss, w_at, w_ss, K, kept = _operands(x, weight)
@@ -287,7 +309,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     ``"gelu_tanh"``, ``"gelu"`` or ``"silu"``.  ``residual`` is [..., N]; ``gate`` is
     [N], or [..., F, N] whose rows scale S / F rows of x's S each (a frame's tokens
     share their frame's gate, as in ``gated_residual``).  ``out`` (optional, contiguous)
-    may be ``residual``, not ``x`` or ``weight``.  Rows of a multiple of eight channels are read in place,
+    may be ``residual`` itself and shares no memory with the inputs otherwise.  Rows of a multiple of eight channels are read in place,
     others are copied with zeros behind.  No gradient: ``linear_act_train``."""
     _no_grad_call("linear_act", x, weight, bias, residual, gate)
     return _linear(x, weight, bias, activation, residual, gate, out, None)
@@ -447,13 +469,14 @@ def _cross(q, k, v, kv_lens, key_mask, scale, out, lse):
         out = torch.empty_like(q, memory_format=_ROWS)
     else:
         _like("out", out, q, q.shape)
-        _apart(out, q=q, k=k, v=v)
+        _apart("out", out, q=q, k=k, v=v, kv_lens=kv_lens, key_mask=key_mask)
     oh = _heads(out)
     B, Hq, _, D, _, _, Sq, _ = sizes
     if oh[0] is not out or any(n > 1 and s < D for n, s in zip((B, Sq, Hq), oh[1])):
         raise ValueError("out must have rows of its own, a unit-stride head dimension and 16-byte rows")
     if lse is not None:
         _check_lse(lse, sizes, q.device)
+        _apart("lse", lse, q=q, k=k, v=v, kv_lens=kv_lens, key_mask=key_mask, out=out)
     if B == 0 or Sq == 0:
         return out
     fields = _cross_fields(sizes, qh, kh, vh, oh, lse, lens, mask)
@@ -473,9 +496,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     query heads i * H/Hk .. share key head i.  A stream's keys are the first
     ``kv_lens[b]`` (int32 [B] on the GPU, taken within [0, Sk]) whose ``key_mask``
     [B, Sk] (bool) is true; what else k and v hold is not read.  Returns [B, Sq, H, D]
-    (``out`` where given, which is none of them); a row that sees no key is 0.  ``lse`` (optional, contiguous
+    (``out`` where given); a row that sees no key is 0.  ``lse`` (optional, contiguous
     fp32 [B, H, Sq]) receives the natural-log softmax normaliser, -inf for such a
-    row.  Sq may be one token: the keys are then cut into parts that fill the GPU.
+    row.  ``out`` and ``lse`` share no memory with the inputs or one another.  Sq may be one token: the keys are then cut into parts that fill the GPU.
     No gradient: ``cross_attention_train``."""
     _no_grad_call("cross_attention", q, k, v)
     return _cross(q, k, v, kv_lens, key_mask, scale, out, lse)

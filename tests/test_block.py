@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from multics_amd import _capi, kernels
+from multics_amd import _capi, block, kernels
 from multics_amd.module import CrossAttention, FeedForward
 
 AT = 1 << 20             # an aligned address that nothing reads: the calls refuse before a launch
@@ -133,6 +133,45 @@ def test_host_tensors_are_refused():
             call()
     with pytest.raises(RuntimeError):
         kernels.linear_act(x.requires_grad_(), w)
+
+
+def _addresses(t):
+    at = torch.zeros((), dtype=torch.int64)
+    for n, s in zip(t.shape, t.stride()):
+        at = at[..., None] + torch.arange(n) * s
+    return {t.data_ptr() + t.element_size() * int(i) + b for i in at.flatten() for b in range(t.element_size())}
+
+
+def test_outputs_over_inputs_are_told():
+    """``_share`` against the sets of addresses: a shifted view, a projection's slices, heads
+    between heads, gaps, expanded and single rows, other types, and views at random."""
+    buf = torch.zeros(3000, dtype=torch.bfloat16)
+    rows = buf[:240].view(10, 24)
+    qkv = buf[:960].view(2, 10, 3, 2, 8)
+    heads = buf[:480].view(10, 2, 3, 8)
+    told = [
+        (rows[1:], rows[:-1], True), (rows, rows, True), (rows[:5], rows[5:], False),
+        (rows[:, :8], rows[:, 8:], False), (rows[:, :9], rows[:, 8:], True), (rows[::2], rows[1::2], False),
+        (qkv[:, :, 0], qkv[:, :, 1], False), (qkv[:, :, 1], qkv[:, 1:, 1], True), (qkv[:, :, 1], qkv[:, 1:, 0], False),
+        (heads[:, :, 0], heads[:, :, 2], False), (heads[:, 0], heads[:, 1, 1:], False),
+        (rows[0, 16:], rows[:, :16], False), (rows[0, 16:], rows[:, :17], True),
+        (rows[:1].expand(5, 24), rows[1:], False), (rows[:1].expand(5, 24), rows[:2], True),
+        (buf[:100], buf[100:200].view(torch.float32), False), (buf[:102], buf[100:200].view(torch.float32), True),
+        (rows[:0], rows, False),
+    ]
+    for i, (a, b, want) in enumerate(told):
+        assert bool(_addresses(a) & _addresses(b)) == want, i
+        assert block._share(a, b) == want and block._share(b, a) == want, i
+    g = torch.Generator().manual_seed(0)
+    pick = lambda *c: c[int(torch.randint(len(c), (), generator=g))]  # noqa: E731
+    missed = 0
+    for _ in range(3000):
+        a, b = (buf.as_strided((pick(1, 2, 3), pick(1, 4, 5), pick(1, 3, 8)), (pick(0, 48, 120), pick(8, 16, 24), 1),
+                               pick(0, 1, 3, 8, 16, 24, 40, 200)) for _ in range(2))
+        touch = bool(_addresses(a) & _addresses(b))
+        assert block._share(a, b) or not touch, (a.stride(), b.stride())
+        missed += block._share(a, b) != touch
+    assert missed < 600, missed      # (views of unlike pitch that interleave are refused too)
 
 
 def test_division_of_rows():

@@ -85,3 +85,41 @@ def test_gradient_of_keys_of_small_weight(Sq, Sk, peak, D):
         # three roundings (O, dS, the result) of at most a step of the terms, at random over rows and
         # channels: the terms' root of squares is within 1.5 of the sum's norm
         assert float(err.max()) <= 1.5 * math.sqrt(3) * step, float(err.max())
+
+
+# ---- outputs that are given --------------------------------------------------------------
+
+def test_outputs_in_the_memory_of_inputs():
+    """Refused wherever a row that is written may be read; slices of one projection pass."""
+    need_gpu()
+    r = _rnd(29)
+    x, w, buf = r(40, 64).to(BF16), r(72, 64).to(BF16), r(41, 72).to(BF16)
+    square = r(64, 64).to(BF16)
+    wide = r(40, 128).to(BF16)
+    for call in (lambda: kernels.linear_act(x, w, residual=buf[1:], out=buf[:-1]),
+                 lambda: kernels.linear_act(x, w, residual=buf[:1].expand(40, 72), out=buf[:-1]),
+                 lambda: kernels.linear_act(x, w, gate=buf[0], out=buf[:-1]),
+                 lambda: kernels.linear_act(x, w, buf[7], out=buf[:-1]),
+                 lambda: kernels.linear_act(wide[:, :64], square, out=wide.view(80, 64)[:40])):
+        with pytest.raises(ValueError, match="share memory"):
+            call()
+    qkv = r(2, 50, 3, 4, 64).to(BF16)
+    q, k, v = qkv.unbind(2)
+    lse = torch.empty(2, 4, 50, device="cuda")
+    floats = torch.empty(2 * 50 * 4 * 32, device="cuda")
+    cases = [dict(out=q), dict(out=k), dict(out=v), dict(out=q.flip(1).contiguous(), lse=qkv.view(-1).view(torch.float32)[:400].view(2, 4, 50)),
+             dict(out=floats.view(BF16).view(2, 50, 4, 64), lse=floats[:400].view(2, 4, 50))]
+    for kw in cases:
+        with pytest.raises(ValueError, match="share memory"):
+            kernels.cross_attention(q, k, v, **kw)
+    # a fourth slice beside the three
+    want = kernels.cross_attention(q, k, v)
+    four = torch.zeros(2, 50, 4, 4, 64, dtype=BF16, device="cuda")
+    four[:, :, :3] = qkv
+    q, k, v, out = four.unbind(2)
+    assert kernels.cross_attention(q, k, v, out=out, lse=lse) is out
+    assert torch.equal(out, want) and torch.equal(four[:, :, :3], qkv)
+    # the residual itself, also as rows of a larger tensor
+    res = buf[3:].clone()
+    got = kernels.linear_act(x[:38], w, residual=buf[3:], out=buf[3:])
+    assert torch.equal(got, kernels.linear_act(x[:38], w, residual=res))
