@@ -93,19 +93,38 @@ class FeedForward(nn.Sequential):
     with a sequential's state-dict keys (``0.weight`` .. ``2.bias``).  ``residual`` and
     ``gate`` (``[..., dim]``; ``[dim]`` or per frame ``[..., F, dim]``, as for
     ``GateModule``) join in the second product: ``residual + gate * ffn(x)``.  bf16 and
-    fp16 GPU tensors run on ``kernels.linear_act``, with and without autograd."""
+    fp16 GPU tensors run on ``kernels.linear_act``, with and without autograd, unless a
+    child was exchanged, wrapped or hooked: then the children are called."""
 
     def __init__(self, dim: int, hidden_dim: int, bias: bool = True):
         super().__init__(nn.Linear(dim, hidden_dim, bias=bias), nn.GELU(approximate="tanh"),
                          nn.Linear(hidden_dim, dim, bias=bias))
 
     def forward(self, x, *, residual=None, gate=None):
-        up, down = self[0], self[2]
-        if _block_ok(x, up.weight):
+        if self._fused(x):
+            up, _, down = self
             linear = linear_act_train if torch.is_grad_enabled() else linear_act
             h = linear(x, up.weight, up.bias, activation="gelu_tanh")
             return linear(h, down.weight, down.bias, residual=residual, gate=gate)
         return _gated(super().forward(x), residual, gate)
+
+    def _fused(self, x) -> bool:
+        """Whether the kernels do what the children would, called as modules."""
+        return len(self) == 3 and _product(self[0], x) and _plain(self[1], nn.GELU) and \
+            self[1].approximate == "tanh" and _product(self[2], x)
+
+
+def _plain(module, *classes) -> bool:
+    """Whether a call of ``module`` is its class's ``forward``, the class one of ``classes``
+    itself, and nothing else: no hooks, no adapter around it."""
+    return type(module) in classes and "forward" not in module.__dict__ and not (
+        module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or
+        module._backward_pre_hooks or nn.modules.module._has_any_global_hook())
+
+
+def _product(module, x) -> bool:
+    """Whether ``kernels.linear_act`` on the module's weights is a call of it on ``x``'s rows."""
+    return _plain(module, nn.Linear, CompatibleLinear) and _block_ok(x, module.weight)
 
 
 def _block_ok(x, weight) -> bool:
@@ -131,7 +150,7 @@ class CrossAttention(nn.Module):
     ``kv = attn.project_context(context)``, and passes ``kv=kv`` in its place.  bf16 and fp16
     GPU tensors with head_dim 64 or 128 run on ``kernels.rms_norm``,
     ``kernels.cross_attention`` and ``kernels.linear_act`` (fp16 without gradient), others on
-    torch operations."""
+    torch operations; a norm or an o-projection that was exchanged, wrapped or hooked is called."""
 
     def __init__(self, dim: int, num_heads: int, eps: float = 1e-6):
         super().__init__()
@@ -145,15 +164,15 @@ class CrossAttention(nn.Module):
         self.norm_q = RMSNorm(dim, eps=eps)
         self.norm_k = RMSNorm(dim, eps=eps)
 
-    def _fused(self, x) -> bool:
-        return _block_ok(x, self.q.weight) and self.head_dim in (64, 128) and \
-            not (x.dtype == torch.float16 and torch.is_grad_enabled())
+    def _fused(self, t) -> bool:
+        return t.is_cuda and t.dtype in (torch.bfloat16, torch.float16) and self.head_dim in (64, 128) and \
+            not (t.dtype == torch.float16 and torch.is_grad_enabled())
 
     def _heads(self, t):
         return t.unflatten(-1, (self.num_heads, self.head_dim))
 
     def _norm(self, norm, t):
-        if not self._fused(t):
+        if not (self._fused(t) and _plain(norm, RMSNorm)):
             return norm(t)
         call = rms_norm_train if torch.is_grad_enabled() else rms_norm
         return call(t, norm.weight, eps=norm.eps)
@@ -167,12 +186,12 @@ class CrossAttention(nn.Module):
             raise ValueError("pass context or kv (from project_context)")
         k, v = self.project_context(context) if kv is None else kv
         q = self._heads(self._norm(self.norm_q, self.q(x)))
-        if self._fused(x):
+        if self._fused(q) and q.dtype == k.dtype == v.dtype:
             grad = torch.is_grad_enabled()
             attend = cross_attention_train if grad else cross_attention
             y = attend(q, k, v, kv_lens=kv_lens, key_mask=key_mask).flatten(-2)
-            if residual is None and gate is None:
-                return self.o(y)
+            if residual is None and gate is None or not _product(self.o, y):
+                return _gated(self.o(y), residual, gate)
             return (linear_act_train if grad else linear_act)(y, self.o.weight, self.o.bias, residual=residual,
                                                               gate=gate)
         seen = None if key_mask is None else key_mask[:, None, None]

@@ -7,8 +7,8 @@ import math
 import pytest
 import torch
 
-from multics_amd import _capi, block, kernels
-from multics_amd.module import CrossAttention, FeedForward
+from multics_amd import _capi, block, kernels, module
+from multics_amd.module import CompatibleLinear, CrossAttention, FeedForward, RMSNorm
 
 AT = 1 << 20             # an aligned address that nothing reads: the calls refuse before a launch
 
@@ -207,3 +207,81 @@ def test_modules_on_the_host():
         attn(x)
     with pytest.raises(ValueError):
         CrossAttention(30, 4)
+
+
+class _Adapter(torch.nn.Module):
+    """A projection with a low-rank term, which shows the projection's weights."""
+
+    def __init__(self, base):
+        super().__init__()
+        self.base = base
+        self.a = torch.nn.Parameter(torch.randn(2, base.in_features))
+        self.b = torch.nn.Parameter(torch.randn(base.out_features, 2))
+
+    weight = property(lambda self: self.base.weight)
+    bias = property(lambda self: self.base.bias)
+
+    def forward(self, x):
+        return self.base(x) + (x @ self.a.to(x.dtype).t()) @ self.b.to(x.dtype).t()
+
+
+def change_ffn(ffn, how):
+    if how == "adapter":
+        ffn[0] = _Adapter(ffn[0])
+    elif how == "second adapter":
+        ffn[2] = _Adapter(ffn[2])
+    elif how == "activation":
+        ffn[1] = torch.nn.ReLU()
+    elif how == "exact gelu":
+        ffn[1] = torch.nn.GELU()
+    elif how == "appended":
+        ffn.append(torch.nn.Tanh())
+    elif how == "hook":
+        ffn[2].register_forward_hook(lambda m, i, o: 2 * o)
+    elif how == "pre-hook":
+        ffn[0].register_forward_pre_hook(lambda m, i: (i[0] + 1,))
+    elif how == "own forward":
+        ffn[0].forward = lambda x: torch.nn.functional.linear(x, ffn[0].weight) - 1
+
+
+CHANGES = ["adapter", "second adapter", "activation", "exact gelu", "appended", "hook", "pre-hook", "own forward", "none"]
+
+
+@pytest.mark.parametrize("how", CHANGES)
+def test_feed_forward_calls_changed_children(how, monkeypatch):
+    """With the kernels' branch open on the host: taken for plain children alone."""
+    torch.manual_seed(0)
+    ffn = FeedForward(8, 16)
+    change_ffn(ffn, how)
+    x, res = torch.randn(3, 8), torch.randn(3, 8)
+    want = res + torch.nn.Sequential.forward(ffn, x)
+    calls = []
+
+    def linear(x, w, b, *, activation=None, residual=None, gate=None):
+        calls.append(activation)
+        y = torch.nn.functional.linear(x, w, b)
+        y = torch.nn.functional.gelu(y, approximate="tanh") if activation else y
+        return y if residual is None else residual + y
+    monkeypatch.setattr(module, "_block_ok", lambda x, w: True)
+    monkeypatch.setattr(module, "linear_act_train", linear)
+    assert torch.allclose(ffn(x, residual=res), want, atol=1e-5)
+    assert calls == (["gelu_tanh", None] if how == "none" else [])
+
+
+def test_what_a_plain_child_is():
+    p = module._plain
+    assert p(torch.nn.Linear(2, 2), torch.nn.Linear) and p(CompatibleLinear(2, 2), torch.nn.Linear, CompatibleLinear)
+    assert not p(CompatibleLinear(2, 2), torch.nn.Linear) and not p(torch.nn.LayerNorm(4), RMSNorm)
+    hooked = RMSNorm(4)
+    assert p(hooked, RMSNorm)
+    handle = hooked.register_full_backward_hook(lambda m, i, o: None)
+    assert not p(hooked, RMSNorm)
+    handle.remove()
+    assert p(hooked, RMSNorm)
+    weighted = torch.nn.utils.parametrizations.weight_norm(torch.nn.Linear(2, 2))
+    assert not p(weighted, torch.nn.Linear)
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda m, i, o: None)
+    try:
+        assert not p(hooked, RMSNorm)
+    finally:
+        handle.remove()

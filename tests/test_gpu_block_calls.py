@@ -1,13 +1,16 @@
 """Calls of the block's operators that their documentation allows and the formulas' cases
 do not make, against the formulas in 64 bits.  Bounds as in ``test_gpu_block``."""
 
+import copy
 import math
 
 import pytest
 import torch
 
 from multics_amd import kernels
+from multics_amd.module import CrossAttention, FeedForward
 from tests.gpu_util import need_gpu, say
+from tests.test_block import CHANGES, _Adapter, change_ffn
 from tests.test_gpu_block import BF16, FP16, U, _linear_case, _rnd, _step, _within
 
 pytestmark = pytest.mark.gpu
@@ -123,3 +126,56 @@ def test_outputs_in_the_memory_of_inputs():
     res = buf[3:].clone()
     got = kernels.linear_act(x[:38], w, residual=buf[3:], out=buf[3:])
     assert torch.equal(got, kernels.linear_act(x[:38], w, residual=res))
+
+
+# ---- modules -------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("how", CHANGES)
+def test_feed_forward_with_changed_children(how):
+    need_gpu()
+    torch.manual_seed(1)
+    ffn = FeedForward(64, 128)
+    change_ffn(ffn, how)
+    ffn = ffn.cuda().to(BF16)
+    x, res = _rnd(1)(3, 20, 64).to(BF16), _rnd(2)(3, 20, 64).to(BF16)
+    y = ffn(x, residual=res)
+    want = res + torch.nn.Sequential.forward(ffn, x)
+    with torch.no_grad():
+        assert torch.equal(ffn(x, residual=res), y)
+    if how == "none":           # y rounds h and itself, the other h (twice), z and itself: three steps of it
+        size = want.double().abs() + res.double().abs() + 8
+        assert bool(((y.double() - want.double()).abs() <= 4 * 2.0 ** -8 * size).all())
+    else:
+        assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("how", ["o adapter", "o hook", "q adapter", "norm", "norm hook", "none"])
+def test_cross_attention_with_changed_children(how):
+    """Against the same module on the host in fp32."""
+    need_gpu()
+    torch.manual_seed(2)
+    host = CrossAttention(128, 2)
+    if how in ("o adapter", "q adapter"):
+        child = _Adapter(getattr(host, how[0]))
+        if how == "q adapter":
+            type(child).weight, kept = property(lambda self: 1 / 0), type(child).weight      # nobody looks at it
+        setattr(host, how[0], child)
+    elif how == "o hook":
+        host.o.register_forward_hook(lambda m, i, o: 2 * o)
+    elif how == "norm":
+        host.norm_q = torch.nn.LayerNorm(128)
+    elif how == "norm hook":
+        host.norm_k.register_forward_hook(lambda m, i, o: 3 * o)
+    try:
+        gpu = copy.deepcopy(host).cuda().to(BF16)
+        host.load_state_dict({k: v.float().cpu() for k, v in gpu.state_dict().items()})
+        x, ctx, gate = _rnd(1)(2, 20, 128).to(BF16), _rnd(2)(2, 9, 128).to(BF16), _rnd(3)(2, 4, 128).to(BF16)
+        with torch.no_grad():
+            for kw in (dict(), dict(residual=x, gate=gate)):
+                want = host(x.float().cpu(), ctx.float().cpu(), **{k: v.float().cpu() for k, v in kw.items()})
+                y = gpu(x, ctx, **kw)
+                # some ten roundings in a row of 2^-8 each, in the norm (a dropped child moves it by half)
+                assert float((y.double().cpu() - want).norm()) <= 10 * 2.0 ** -8 * float(want.norm())
+    finally:
+        if how == "q adapter":
+            type(child).weight = kept
