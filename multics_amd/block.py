@@ -81,13 +81,13 @@ def _outs(name: str, out: Optional[torch.Tensor], like: torch.Tensor, shape) -> 
 
 def _operands(x: torch.Tensor, w: torch.Tensor):
     """x [..., K] and w [N, K] as a product's operands, 16-byte rows of a multiple of
-    eight elements: their addresses and strides, that multiple, and what has to live as
-    long.  Others are copied, with zeros behind (``hier_pad_rows``)."""
+    eight elements, less than 2^21 apart: their addresses and strides, that multiple, and
+    what has to live as long.  Others are copied, with zeros behind (``hier_pad_rows``)."""
     (x, x_ss), (w, w_ss) = _rows(x), _rows(w)
     K = x.shape[1]
     at = [x.data_ptr(), w.data_ptr()]
     ss = [x_ss, w_ss]
-    copy = [K % 8 or s % 8 or p % 16 or s < K for p, s in zip(at, ss)]
+    copy = [K % 8 or s % 8 or p % 16 or not K <= s < 1 << 21 for p, s in zip(at, ss)]
     if not any(copy):
         return at[0], x_ss, at[1], w_ss, K, (x, w)
     Kp = K + -K % 8
@@ -310,7 +310,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     [N], or [..., F, N] whose rows scale S / F rows of x's S each (a frame's tokens
     share their frame's gate, as in ``gated_residual``).  ``out`` (optional, contiguous)
     may be ``residual`` itself and shares no memory with the inputs otherwise.  Rows of a multiple of eight channels are read in place,
-    others are copied with zeros behind.  No gradient: ``linear_act_train``."""
+    others, and rows 2^21 elements apart or more, are copied with zeros behind.  No gradient: ``linear_act_train``."""
     _no_grad_call("linear_act", x, weight, bias, residual, gate)
     return _linear(x, weight, bias, activation, residual, gate, out, None)
 

@@ -40,6 +40,31 @@ def test_gradient_of_a_nan_before_the_activation(act, t, N):
     assert torch.equal(got["gate"], clean["gate"])
 
 
+# ---- rows far apart ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("B,S,K,N,act", [(4, 4620, 1536, 200, "gelu_tanh"), (70, 1400, 1536, 136, "silu"),
+                                         (3, 2100, 1001, 33, None)])
+def test_product_of_rows_far_apart(B, S, K, N, act):
+    """The last token of every stream: rows two million elements apart and more."""
+    need_gpu()
+    r = _rnd(15)
+    buf = torch.zeros(B, S, K, dtype=BF16, device="cuda")
+    buf[:, -1] = r(B, K).to(BF16)
+    x = buf[:, -1]
+    assert x.stride(0) >= 1 << 21
+    w, b, dy = (r(N, K) / math.sqrt(K)).to(BF16), r(N).to(BF16), r(B, N).to(BF16)
+    far = torch.zeros(N, 1 << 21, dtype=BF16, device="cuda")[:, :K] if N == 33 else w    # weights too
+    far.copy_(w)
+    say("rows far apart", B, S, K, N, act)
+    assert torch.equal(kernels.linear_act(x, far, b, activation=act),
+                       kernels.linear_act(x.contiguous(), w, b, activation=act))
+    grads = []
+    for rows, weights in ((x, far), (x.contiguous(), w)):
+        leaves = [t.detach().requires_grad_() for t in (rows, weights, b)]
+        grads.append(torch.autograd.grad(kernels.linear_act_train(*leaves, activation=act), leaves, dy))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
 # ---- small weights of the attention's gradient ----------------------------------------------
 
 @pytest.mark.parametrize("Sq,Sk,peak,D", [(40, 4096, 14.0, 64), (40, 4096, 20.0, 128), (2000, 300, 18.0, 128),
