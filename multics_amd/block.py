@@ -79,18 +79,19 @@ def _outs(name: str, out: Optional[torch.Tensor], like: torch.Tensor, shape) -> 
     return out
 
 
-def _operands(x: torch.Tensor, w: torch.Tensor):
+def _operands(x: torch.Tensor, w: torch.Tensor, read=(True, True)):
     """x [..., K] and w [N, K] as a product's operands, 16-byte rows of a multiple of
     eight elements, less than 2^21 apart: their addresses and strides, that multiple, and
-    what has to live as long.  Others are copied, with zeros behind (``hier_pad_rows``)."""
-    (x, x_ss), (w, w_ss) = _rows(x), _rows(w)
-    K = x.shape[1]
+    what has to live as long.  Others are copied, with zeros behind (``hier_pad_rows``), if
+    the call reads them (``read``)."""
+    K = x.shape[-1]
+    (x, x_ss), (w, w_ss) = (_rows(t) if r else (t, K) for t, r in zip((x, w), read))
     at = [x.data_ptr(), w.data_ptr()]
     ss = [x_ss, w_ss]
-    copy = [K % 8 or s % 8 or p % 16 or not K <= s < 1 << 21 for p, s in zip(at, ss)]
-    if not any(copy):
-        return at[0], x_ss, at[1], w_ss, K, (x, w)
+    copy = [r and (K % 8 or s % 8 or p % 16 or not K <= s < 1 << 21) for p, s, r in zip(at, ss, read)]
     Kp = K + -K % 8
+    if not any(copy):
+        return at[0], x_ss, at[1], w_ss, Kp, (x, w)
     rows = [t.shape[0] if c else 0 for t, c in zip((x, w), copy)]
     buf = x.new_empty((rows[0] + rows[1]) * Kp)
     to = [buf.data_ptr(), buf.data_ptr() + 2 * rows[0] * Kp]
@@ -336,7 +337,7 @@ def linear_act_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
         made = {"x": lambda: torch.zeros_like(x), "weight": lambda: torch.zeros_like(weight),
                 "bias": lambda: new(N).zero_(), "gate": lambda: torch.zeros_like(gate)}
         return {n: made[n]() for n in need}
-    x_at, x_ss, w_at, w_ss, Kp, kept = _operands(x, weight)
+    x_at, x_ss, w_at, w_ss, Kp, kept = _operands(x, weight, ("weight" in need, "x" in need))
     g_dy, dy_ss = _rows(dy)
     if not act and gate is None:
         preact = None

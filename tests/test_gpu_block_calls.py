@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from multics_amd import kernels
+from multics_amd import block, kernels
 from multics_amd.module import CrossAttention, FeedForward
 from tests.gpu_util import need_gpu, say
 from tests.test_block import CHANGES, _Adapter, change_ffn
@@ -63,6 +63,28 @@ def test_product_of_rows_far_apart(B, S, K, N, act):
         leaves = [t.detach().requires_grad_() for t in (rows, weights, b)]
         grads.append(torch.autograd.grad(kernels.linear_act_train(*leaves, activation=act), leaves, dy))
     assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+# ---- what a gradient reads ----------------------------------------------------------------
+
+@pytest.mark.parametrize("need,rows", [(("bias", "gate"), None), (("x",), (0, 33)), (("weight",), (50, 0)),
+                                       (("x", "weight"), (50, 33))])
+def test_gradient_copies_what_it_reads(need, rows, monkeypatch):
+    """Odd channels: x is copied to whole rows for the weights' gradient alone, the weights for x's."""
+    need_gpu()
+    x, w, b, _, gate, dy = _linear_case(50, 77, 33, None, 2, False, BF16)
+    z = (x.float() @ w.float().t()).to(BF16)
+    want = kernels.linear_act_backward(dy, x, w, preact=z, gate=gate)
+    seen = []
+    pack = block._pack_pad
+
+    def spy(*fields):
+        seen.append(fields[:2])
+        return pack(*fields)
+    monkeypatch.setattr(block, "_pack_pad", spy)
+    got = kernels.linear_act_backward(dy, x, w, preact=z, gate=gate, need=need)
+    assert set(got) == set(need) and all(torch.equal(got[n], want[n]) for n in need)
+    assert seen == ([] if rows is None else [rows])
 
 
 # ---- small weights of the attention's gradient ----------------------------------------------
