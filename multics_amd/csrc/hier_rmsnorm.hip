@@ -18,6 +18,7 @@
 // much reaches 5.1), its gradient 59 + 4 of sum_rows (289 MB, 4.9 TB/s); with a row's
 // loads one after the other, each waited for by its conversion, 70 and 90.  2 x 1,536:
 // 2.6, a launch.  512 workgroups of the gradient: each sum is one row to read again.
+#include "hier_launch.h"
 #include "hier_types.h"
 
 #include <algorithm>
@@ -178,7 +179,8 @@ template <typename T, int VEC, int WPR, int NCH>
 __global__ __launch_bounds__(threads_of<WPR>()) void norm_kernel(HierRmsNormArgs a) {
   __shared__ float lds[16];
   const int t = threadIdx.x % (64 * WPR);
-  const int64_t row = WPR == 1 ? (int64_t)blockIdx.x * 4 + threadIdx.x / 64 : blockIdx.x;
+  const int64_t group = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;      // (launch_grid)
+  const int64_t row = WPR == 1 ? group * 4 + threadIdx.x / 64 : group;
   if (row >= a.M) return;                // (WPR > 1: the whole workgroup or none of it)
   float h[NCH][8], w[NCH][8];
   float sq = 0.f;
@@ -316,33 +318,35 @@ int64_t bwd_groups(int64_t M, int64_t C) {
 }
 
 template <typename T, int VEC, int WPR, int NCH>
-void launch(const HierRmsNormArgs& a, hipStream_t st) {
-  const int64_t groups = WPR == 1 ? (a.M + 3) / 4 : a.M;
-  hipLaunchKernelGGL((norm_kernel<T, VEC, WPR, NCH>), dim3((unsigned)groups),
-                     dim3(threads_of<WPR>()), 0, st, a);
+int launch(const HierRmsNormArgs& a, hipStream_t st) {
+  const Grid grid = launch_grid(WPR == 1 ? (a.M + 3) / 4 : a.M, threads_of<WPR>());
+  HIER_REQUIRE(grid.x > 0, HIER_EUNSUPPORTED, "rms_norm: too many rows");
+  hipLaunchKernelGGL((norm_kernel<T, VEC, WPR, NCH>), dim3(grid.x, grid.y), dim3(threads_of<WPR>()), 0, st, a);
+  return check_launch("norm_kernel");
 }
 template <typename T, int VEC, int WPR, int NCH>
-void launch(const HierRmsNormBwdArgs& a, hipStream_t st) {
+int launch(const HierRmsNormBwdArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, WPR, NCH>), dim3((unsigned)bwd_groups(a.M, a.C)),
                      dim3(threads_of<WPR>()), 0, st, a);
+  return check_launch("norm_bwd_kernel");
 }
 
 template <typename T, int VEC, typename A>
-void by_channels(const A& a, hipStream_t st) {
-  if (a.C <= 512) launch<T, VEC, 1, 1>(a, st);
-  else if (a.C <= 1024) launch<T, VEC, 1, 2>(a, st);
-  else if (a.C <= 1536) launch<T, VEC, 1, 3>(a, st);
-  else if (a.C <= 2048) launch<T, VEC, 1, 4>(a, st);
-  else if (a.C <= 4096) launch<T, VEC, 4, 2>(a, st);
-  else if (a.C <= 6144) launch<T, VEC, 4, 3>(a, st);
-  else if (a.C <= 8192) launch<T, VEC, 4, 4>(a, st);
-  else launch<T, VEC, 16, 2>(a, st);
+int by_channels(const A& a, hipStream_t st) {
+  if (a.C <= 512) return launch<T, VEC, 1, 1>(a, st);
+  if (a.C <= 1024) return launch<T, VEC, 1, 2>(a, st);
+  if (a.C <= 1536) return launch<T, VEC, 1, 3>(a, st);
+  if (a.C <= 2048) return launch<T, VEC, 1, 4>(a, st);
+  if (a.C <= 4096) return launch<T, VEC, 4, 2>(a, st);
+  if (a.C <= 6144) return launch<T, VEC, 4, 3>(a, st);
+  if (a.C <= 8192) return launch<T, VEC, 4, 4>(a, st);
+  return launch<T, VEC, 16, 2>(a, st);
 }
 
 template <typename A>
-void by_type(const A& a, bool vec, hipStream_t st) {
-  if (a.type == HIER_BF16) vec ? by_channels<__bf16, 8>(a, st) : by_channels<__bf16, 1>(a, st);
-  else vec ? by_channels<_Float16, 8>(a, st) : by_channels<_Float16, 1>(a, st);
+int by_type(const A& a, bool vec, hipStream_t st) {
+  if (a.type == HIER_BF16) return vec ? by_channels<__bf16, 8>(a, st) : by_channels<__bf16, 1>(a, st);
+  return vec ? by_channels<_Float16, 8>(a, st) : by_channels<_Float16, 1>(a, st);
 }
 
 template <typename A>
@@ -386,8 +390,7 @@ extern "C" int hier_rms_norm(const HierRmsNormArgs* args, void* stream) {
                "rms_norm: invalid row stride");
   const bool vec = a.C % 8 == 0 && aligned16(a.w) && rows16(a.x, a.x_ss) && rows16(a.y, a.y_ss) &&
                    (!a.r || (rows16(a.r, a.r_ss) && rows16(a.h, a.h_ss)));
-  by_type(a, vec, (hipStream_t)stream);
-  return check_launch("norm_kernel");
+  return by_type(a, vec, (hipStream_t)stream);
 }
 
 extern "C" int64_t hier_rms_norm_bwd_rows(const HierRmsNormBwdArgs* a) {
@@ -412,7 +415,6 @@ extern "C" int hier_rms_norm_bwd(const HierRmsNormBwdArgs* args, void* stream) {
                    (!a.dh || rows16(a.dh, a.dh_ss));
   const bool one = bwd_groups(a.M, a.C) == 1;        // its row of sums is dw
   if (one) a.partial = a.dw;
-  by_type(a, vec, (hipStream_t)stream);
-  if (int rc = check_launch("norm_bwd_kernel")) return rc;
+  if (int rc = by_type(a, vec, (hipStream_t)stream)) return rc;
   return one ? HIER_OK : sum_rows(a.partial, bwd_groups(a.M, a.C), 1, a.C, a.dw, HIER_FP32, (hipStream_t)stream);
 }

@@ -226,3 +226,19 @@ def test_cross_attention_with_changed_children(how):
     finally:
         if how == "q adapter":
             type(child).weight = kept
+
+
+# ---- many rows ---------------------------------------------------------------------------
+
+def test_norm_of_more_rows_than_a_line_of_threads():
+    """2^26 rows and a few: 2^32 threads, more than a launch takes side by side."""
+    need_gpu()
+    few, M = 1 << 16, (1 << 26) + 37
+    r = _rnd(33)
+    base, w = r(few, 8).to(BF16), 1 + 0.1 * r(8)
+    x = base.repeat(M // few + 1, 1)[:M]
+    say("norm of many rows", M)
+    want = kernels.rms_norm(base, w, eps=1e-6)
+    got = kernels.rms_norm(x, w, eps=1e-6)
+    assert torch.equal(got[:-37].view(-1, few, 8), want.expand(M // few, few, 8))
+    assert torch.equal(got[-37:], want[:37])
