@@ -676,6 +676,9 @@ extern "C" int hier_cross_attn_bwd(const HierCrossBwdArgs* args, void* stream) {
   p.splits = dkv_splits(a);
   p.dq_splits = dq_splits(a);
   p.total = a.B * a.Hk * p.key_tiles * p.splits;
+  // fewer than 2^32 threads a launch, of 256 and of 512
+  HIER_REQUIRE(xcd_grid((int64_t)a.B * a.Hk * p.row_tiles * p.dq_splits) < (1 << 24) && xcd_grid(p.total) < (1 << 23),
+               HIER_EUNSUPPORTED, "cross attention: too many work items");
   const int64_t need = work_bytes(a);
   HIER_REQUIRE(need == 0 || (a.workspace && aligned16(a.workspace) && a.workspace_bytes >= need), HIER_EINVAL,
                "cross attention: workspace of %lld bytes needed", (long long)need);

@@ -109,6 +109,17 @@ def test_cross_gradient_entry_refuses(change, says):
     assert says in _capi.lib().hier_last_error().decode()
 
 
+def test_cross_gradient_entry_refuses_as_many_items_as_a_launch_has_not():
+    """512 threads for each key head of 9 keys: 2^32 are refused, less are asked for their workspace."""
+    for heads, says in (((1 << 23) - 4, "too many"), ((1 << 23) - 8, "workspace")):
+        f = _cross(B=1, Hq=heads, Hk=heads, Sq=1, q_ss=0, k_ss=1 << 22, v_ss=1 << 22)
+        wide = {f"{n}_{s}": 64 if s == "sh" else 1 << 30 for n in ("do", "dq", "dk", "dv") for s in ("sb", "ss", "sh")}
+        wide.update(do_ss=0)
+        args = _capi.HierCrossBwdArgs(f=f, dout=AT, dq=AT, dk=AT, dv=AT, **wide)
+        assert _capi.lib().hier_cross_attn_bwd(C.addressof(args), None) < 0
+        assert says in _capi.lib().hier_last_error().decode()
+
+
 def test_entries_refuse_null():
     for name in ("hier_rms_norm", "hier_rms_norm_bwd", "hier_linear", "hier_linear_bwd", "hier_pad_rows", "hier_cross_attn",
                  "hier_cross_attn_bwd"):
