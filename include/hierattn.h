@@ -750,9 +750,10 @@ int64_t hier_rms_norm_bwd_rows(const HierRmsNormBwdArgs* args);
 int hier_rms_norm_bwd(const HierRmsNormBwdArgs* args, void* stream);
 
 /* z = x w^T + bias, out = residual + gate * act(z); bias, residual, gate and */
-/* preact (receives z) may be NULL.  Gate row i scales rows i * rows_per_gate */
-/* .. of out.  x and w: 16-byte aligned rows of K contiguous elements, K a    */
-/* multiple of 8, at most 2^21 - 1 elements apart.  `workspace` of            */
+/* preact (receives z; in fp16 with an activation -65504 for a finite z below */
+/* it) may be NULL.  Gate row i scales rows i * rows_per_gate .. of out.      */
+/* x and w: 16-byte aligned rows of K contiguous elements, K a multiple of 8, */
+/* at most 2^21 - 1 elements apart.  `workspace` of                           */
 /* hier_linear_workspace(args) bytes (16-byte aligned) belongs to one call at */
 /* a time.  out may be residual itself; what is written shares no memory with */
 /* what is read otherwise.                                                    */

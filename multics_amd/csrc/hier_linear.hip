@@ -5,7 +5,7 @@
 //   dg = sum over a gate's rows of dy * act(z)
 // (x [M][K], W [N][K], g one row for rows_per_gate rows of y.)  Everything is
 // summed in fp32 and y rounded once.  A training step also writes z rounded to
-// 16 bits (act' and dg are taken at it: an error of half a step of z, as y's own
+// 16 bits (fp16 with an activation: no lower than -65504; act' and dg are taken at it: an error of half a step of z, as y's own
 // rounding is one of y), and dz is rounded to 16 bits as the two products'
 // operand; db is summed from dz before that rounding.
 //
@@ -141,6 +141,21 @@ __device__ __forceinline__ void put_row8(void* p, int64_t at, int n, int N, cons
   }
 }
 
+// z as it is kept for the gradient.  Below fp16's range every activation and its slope are
+// 0, at -65504 as there, while -inf would make the gate's gradient -inf * 0.  (By the bits,
+// as NaNs pass; -inf itself stays, and so does overflow above, as y's own.)
+template <typename T>
+__device__ __forceinline__ void kept(const float* v, int act, float* z) {
+  constexpr uint32_t LOW = 0xc77fe000u, INF = 0xff800000u;      // -65504, -inf
+#pragma unroll
+  for (int i = 0; i < 8; ++i) z[i] = v[i];
+  if constexpr (__is_same(T, _Float16)) {
+    if (act == HIER_ACT_NONE) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] = __float_as_uint(v[i]) - LOW < INF - LOW ? -65504.f : v[i];
+  }
+}
+
 __device__ __forceinline__ uint32_t gate_row(const Epilogue& e, int64_t m) {
   return e.gate ? quotient((uint32_t)m, e.rows_per_gate) : 0u;
 }
@@ -159,7 +174,11 @@ struct Finish {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] += bias[i];
     }
-    if (e.preact) put_row8<T>(e.preact, m * e.preact_ss, n, N, v);
+    if (e.preact) {
+      float z[8];
+      kept<T>(v, e.act, z);
+      put_row8<T>(e.preact, m * e.preact_ss, n, N, z);
+    }
     activate8(v, e.act);
     if (e.gate) {
 #pragma unroll
@@ -428,7 +447,10 @@ __global__ __launch_bounds__(256, WG) void gemm_kernel(GemmArgs g) {
           float v[8] = {lo[it][0], lo[it][1], lo[it][2], lo[it][3], hi[it][0], hi[it][1], hi[it][2], hi[it][3]}, t[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] += b[i];
-          if (g.e.preact) vz.stream(narrow<T>(v), off(r0 + it * RPI, n, g.e.preact_ss));
+          if (g.e.preact) {
+            kept<T>(v, g.e.act, t);
+            vz.stream(narrow<T>(t), off(r0 + it * RPI, n, g.e.preact_ss));
+          }
           activate8(v, g.e.act);
           const uint32_t at = off(r0 + it * RPI, n, g.e.out_ss);
           if constexpr (KIND == kExtra) {

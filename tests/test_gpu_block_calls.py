@@ -11,7 +11,7 @@ from multics_amd import block, kernels
 from multics_amd.module import CrossAttention, FeedForward
 from tests.gpu_util import need_gpu, say
 from tests.test_block import CHANGES, _Adapter, change_ffn
-from tests.test_gpu_block import BF16, FP16, U, _linear_case, _rnd, _step, _within
+from tests.test_gpu_block import BF16, FP16, U, _act64, _linear_case, _rnd, _step, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -38,6 +38,28 @@ def test_gradient_of_a_nan_before_the_activation(act, t, N):
     assert torch.isnan(got["gate"][1, 5])                    # (50 rows a gate)
     got["gate"][1, 5] = clean["gate"][1, 5]
     assert torch.equal(got["gate"], clean["gate"])
+
+
+@pytest.mark.parametrize("M,N", [(6, 40), (33, 40), (140, 264), (140, 77)])
+@pytest.mark.parametrize("act", ["gelu_tanh", "gelu", "silu"])
+def test_gate_gradient_of_values_below_fp16(act, M, N):
+    """Far below what fp16 holds every activation is 0: the gate's gradient is that of
+    the other rows, not a NaN of -inf * 0."""
+    need_gpu()
+    r = _rnd(7)
+    x, w = torch.zeros(M, 8, dtype=FP16, device="cuda"), torch.zeros(N, 8, dtype=FP16, device="cuda")
+    x[:, 0], w[:, 0] = r(M).to(FP16), r(N).to(FP16)
+    x[2, 1], w[::3, 1] = 1000.0, -100.0                      # row 2: z about -10^5 in every third channel
+    gate, dy = r(N).to(FP16).requires_grad_(), r(M, N).to(FP16)
+    say("values below fp16", act, M, N)
+    y = kernels.linear_act_train(x, w, activation=act, gate=gate)
+    got, = torch.autograd.grad(y, gate, dy)
+    z = x.double() @ w.double().t()
+    a, size = _act64(z, act), z.abs() * (z > -1e4)           # (exactly 0 below)
+    step = _step(FP16)
+    # z as kept: one rounding; the sum over M rows
+    terms = dy.double().abs() * (1.2 * step * size + 2.0 ** -25 + 2.0 ** -19 * size + (M + 16) * U * a.abs())
+    _within(got, (dy.double() * a).sum(0), terms.sum(0))
 
 
 # ---- rows far apart ---------------------------------------------------------------------
