@@ -198,6 +198,9 @@ class CrossAttention(nn.Module):
         if kv_lens is not None:
             within = (torch.arange(k.shape[1], device=x.device) < kv_lens[:, None])[:, None, None]
             seen = within if seen is None else seen & within
+        if seen is not None:            # what a hidden key holds is not read: 0 * inf would be
+            hidden = ~seen[:, 0, 0, :, None, None]
+            k, v = k.masked_fill(hidden, 0), v.masked_fill(hidden, 0)
         y = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), attn_mask=seen)
         if seen is not None:            # a row that sees no key is 0
             y = torch.where(seen.any(-1, keepdim=True), y, torch.zeros((), dtype=y.dtype, device=y.device))

@@ -296,3 +296,26 @@ def test_what_a_plain_child_is():
         assert not p(hooked, RMSNorm)
     finally:
         handle.remove()
+
+
+@pytest.mark.parametrize("how", ["kv_lens", "key_mask", "both"])
+def test_hidden_states_stay_out_on_the_host(how):
+    """NaN and infinite padding changes neither values nor gradients, as on the kernels' path."""
+    torch.manual_seed(0)
+    attn = CrossAttention(32, 2).double()
+    x, ctx = torch.randn(3, 6, 32).double().requires_grad_(), torch.randn(3, 5, 32).double()
+    lens = torch.tensor([5, 2, 0])
+    mask = torch.arange(5) < lens[:, None]
+    kw = {"kv_lens": dict(kv_lens=lens), "key_mask": dict(key_mask=mask),
+          "both": dict(kv_lens=lens.clamp(min=1), key_mask=mask)}[how]
+    k, v = (t.detach() for t in attn.project_context(ctx))
+    results = []
+    for bad in (0.0, float("nan"), float("inf")):
+        kk, vv = k.clone(), v.clone()
+        kk[~mask], vv[~mask] = bad, -bad
+        kk.requires_grad_(), vv.requires_grad_()
+        y = attn(x, kv=(kk, vv), **kw)
+        results.append((y, *torch.autograd.grad(y.square().sum(), (x, kk, vv))))
+    for other in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(results[0], other))
+    assert not results[0][2][~mask].any() and not results[0][3][~mask].any()
