@@ -105,7 +105,7 @@ class FeedForward(nn.Sequential):
             up, _, down = self
             linear = linear_act_train if torch.is_grad_enabled() else linear_act
             h = linear(x, up.weight, up.bias, activation="gelu_tanh")
-            return linear(h, down.weight, down.bias, residual=residual, gate=gate)
+            return _gated_product(linear, h, down, residual, gate)
         return _gated(super().forward(x), residual, gate)
 
     def _fused(self, x) -> bool:
@@ -132,9 +132,24 @@ def _block_ok(x, weight) -> bool:
     return x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and weight.dtype == x.dtype
 
 
+def _gated_product(linear, x, child, residual, gate):
+    """``_gated(child(x), residual, gate)``, in the product's epilogue where it takes them: in
+    x's type, a row or a gate for each of x's."""
+    shape = (*x.shape[:-1], child.weight.shape[0])
+    fits = (residual is None or residual.dtype == x.dtype and residual.shape == shape) and \
+        (gate is None or gate.dtype == x.dtype and
+         (gate.shape == shape[-1:] or gate.dim() == x.dim() > 1 and gate.shape[-2] > 0 and
+          x.shape[-2] % gate.shape[-2] == 0 and gate.shape == (*shape[:-2], gate.shape[-2], shape[-1])))
+    if fits:
+        return linear(x, child.weight, child.bias, residual=residual, gate=gate)
+    return _gated(linear(x, child.weight, child.bias), residual, gate)
+
+
 def _gated(y, residual, gate):
     if gate is not None:
         if gate.dim() > 1 and gate.shape[-2] != y.shape[-2]:
+            if not gate.shape[-2] or y.shape[-2] % gate.shape[-2]:
+                raise ValueError(f"{y.shape[-2]} rows do not divide into {gate.shape[-2]} gate rows")
             gate = gate.repeat_interleave(y.shape[-2] // gate.shape[-2], dim=-2)
         y = gate * y
     return y if residual is None else residual + y
@@ -192,8 +207,7 @@ class CrossAttention(nn.Module):
             y = attend(q, k, v, kv_lens=kv_lens, key_mask=key_mask).flatten(-2)
             if residual is None and gate is None or not _product(self.o, y):
                 return _gated(self.o(y), residual, gate)
-            return (linear_act_train if grad else linear_act)(y, self.o.weight, self.o.bias, residual=residual,
-                                                              gate=gate)
+            return _gated_product(linear_act_train if grad else linear_act, y, self.o, residual, gate)
         seen = None if key_mask is None else key_mask[:, None, None]
         if kv_lens is not None:
             within = (torch.arange(k.shape[1], device=x.device) < kv_lens[:, None])[:, None, None]

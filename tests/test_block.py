@@ -319,3 +319,46 @@ def test_hidden_states_stay_out_on_the_host(how):
     for other in results[1:]:
         assert all(torch.equal(a, b) for a, b in zip(results[0], other))
     assert not results[0][2][~mask].any() and not results[0][3][~mask].any()
+
+
+EPILOGUES = [
+    # residual, gate (shape and type; None: none), whether the product's epilogue takes them
+    (None, None, True),
+    (((2, 6, 8), "same"), None, True),
+    (((2, 6, 8), "same"), ((8,), "same"), True),
+    (None, ((2, 3, 8), "same"), True),
+    (None, ((2, 1, 8), "same"), True),
+    (((2, 6, 8), "same"), ((2, 6, 8), "same"), True),
+    (((2, 6, 8), "wide"), None, False),
+    (((2, 6, 8), "same"), ((2, 3, 8), "wide"), False),
+    (((2, 6, 8), "wide"), ((8,), "wide"), False),
+    (((1, 6, 8), "same"), None, False),
+    (((8,), "same"), None, False),
+    (None, ((1, 3, 8), "same"), False),
+    (None, ((1, 1, 8), "same"), False),
+    (None, ((2, 3, 1), "same"), False),
+]
+
+
+@pytest.mark.parametrize("residual,gate,fits", EPILOGUES)
+def test_what_joins_in_the_products_epilogue(residual, gate, fits):
+    """What the kernel does not take is applied to its result, as the host's path does."""
+    torch.manual_seed(0)
+    same, wide = torch.float32, torch.float64
+    make = lambda what: None if what is None else torch.randn(what[0], dtype=same if what[1] == "same" else wide)  # noqa: E731
+    child, x, res, g = torch.nn.Linear(4, 8), torch.randn(2, 6, 4), make(residual), make(gate)
+    calls = []
+
+    def linear(x, w, b, *, residual=None, gate=None):
+        calls.append(residual is not None or gate is not None)
+        return module._gated(torch.nn.functional.linear(x, w, b), residual, gate)
+    got = module._gated_product(linear, x, child, res, g)
+    want = module._gated(child(x), res, g)
+    assert got.dtype == want.dtype and torch.equal(got, want)
+    assert calls == [fits and (res is not None or g is not None)]
+
+
+def test_gate_rows_have_to_divide():
+    for rows, gates in ((5, 2), (1, 3), (4, 0)):
+        with pytest.raises(ValueError, match="divide"):
+            module._gated(torch.zeros(2, rows, 8), None, torch.zeros(2, gates, 8))

@@ -8,9 +8,9 @@ import pytest
 import torch
 
 from multics_amd import block, kernels
-from multics_amd.module import CrossAttention, FeedForward
+from multics_amd.module import CrossAttention, FeedForward, _gated
 from tests.gpu_util import need_gpu, say
-from tests.test_block import CHANGES, _Adapter, change_ffn
+from tests.test_block import CHANGES, EPILOGUES, _Adapter, change_ffn
 from tests.test_gpu_block import BF16, FP16, U, _act64, _linear_case, _rnd, _step, _within
 
 pytestmark = pytest.mark.gpu
@@ -248,6 +248,28 @@ def test_cross_attention_with_changed_children(how):
     finally:
         if how == "q adapter":
             type(child).weight = kept
+
+
+@pytest.mark.parametrize("residual,gate,fits", EPILOGUES)
+def test_modules_with_residuals_and_gates_of_other_types_and_shapes(residual, gate, fits):
+    """An fp32 residual stream or gate, broadcast ones: as on the host, in the wider type."""
+    need_gpu()
+    torch.manual_seed(3)
+    ffn, attn = FeedForward(8, 32).cuda().to(BF16), CrossAttention(128, 2).cuda().to(BF16)
+    r = _rnd(4)
+    for module, dim in ((ffn, 8), (attn, 128)):
+        make = lambda what: None if what is None else r(*(dim if n == 8 else n for n in what[0])).to(  # noqa: E731, B023
+            torch.float32 if what[1] == "wide" else BF16)
+        res, g = make(residual), make(gate)
+        args = (r(2, 6, dim).to(BF16),) + ((r(2, 5, dim).to(BF16),) if module is attn else ())
+        say("residual and gate", residual, gate, dim)
+        y = module(*args, residual=res, gate=g)
+        want = _gated(module(*args), res, g)
+        assert y.dtype == want.dtype and y.shape == want.shape
+        # the bare product rounds to bf16 before the gate, the epilogue after it, and the sum
+        # again: a step of the product at most, and one of the sum
+        slack = (want.double() - (0 if res is None else res.double())).abs() + want.double().abs()
+        assert bool(((y.double() - want.double()).abs() <= 2.0 ** -7 * slack + 1e-6).all())
 
 
 # ---- many rows ---------------------------------------------------------------------------
