@@ -794,6 +794,7 @@ int hier_pad_rows(const HierPadRowsArgs* args, void* stream);
 
 /* Gradients of hier_linear from dy and preact: each of dx, dw, db, dgate    */
 /* that is not NULL.  preact may be NULL without an activation and dgate.    */
+/* Rows of x and w do not overlap (hier_linear takes a stride of 0).          */
 /* Deterministic.                                                            */
 typedef struct HierLinearBwdArgs {
   int64_t M;

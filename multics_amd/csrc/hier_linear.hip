@@ -1190,11 +1190,11 @@ static int linear_bwd(const HierLinearBwdArgs& a, const BwdPlan& p, hipStream_t 
   };
   if (a.dx)
     if (int rc = launch_gemm<T, false, true>(
-            product(a.M, a.K, a.N, dz, dz_ss, a.w, a.w_ss, a.dx, a.dx_ss), p.dx, parts, true, st))
+            product(a.M, a.K, a.N, dz, dz_ss, a.w, a.N == 1 ? a.K : a.w_ss, a.dx, a.dx_ss), p.dx, parts, true, st))
       return rc;
   if (a.dw)
-    return launch_gemm<T, true, true>(product(a.N, a.K, a.M, dz, dz_ss, a.x, a.x_ss, a.dw, a.dw_ss), p.dw,
-                                      parts, true, st);
+    return launch_gemm<T, true, true>(
+        product(a.N, a.K, a.M, dz, dz_ss, a.x, a.M == 1 ? a.K : a.x_ss, a.dw, a.dw_ss), p.dw, parts, true, st);
   return HIER_OK;
 }
 
@@ -1211,6 +1211,9 @@ extern "C" int hier_linear_bwd(const HierLinearBwdArgs* args, void* stream) {
     if (int rc = check_view("weight", a.w, a.w_ss, a.K)) return rc;
   if (a.dw)
     if (int rc = check_view("x", a.x, a.x_ss, a.K)) return rc;
+  // (a row read as several would be read past the last one too, and be inf * 0 there)
+  HIER_REQUIRE((!a.dx || a.w_ss > 0 || a.N == 1) && (!a.dw || a.x_ss > 0 || a.M == 1), HIER_EINVAL,
+               "linear_bwd: rows of x and weight must not overlap");
   auto ok = [](const void* q, int64_t ss) { return !q || (aligned16(q) && ss % 8 == 0 && ss < (1ll << 21)); };
   HIER_REQUIRE((!a.dx || a.dx_ss >= a.K) && (!a.dw || a.dw_ss >= a.K) && ok(a.dx, a.dx_ss) && ok(a.dw, a.dw_ss),
                HIER_EINVAL, "linear_bwd: dx and dw need 16-byte rows and an output stride of at least K");

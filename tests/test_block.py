@@ -74,6 +74,10 @@ REFUSED = [
     ("hier_linear_bwd", _linear_bwd, dict(dy=None), "dy"),
     ("hier_linear_bwd", _linear_bwd, dict(dx_ss=8), "stride"),
     ("hier_linear_bwd", _linear_bwd, dict(db=AT), "workspace"),
+    ("hier_linear_bwd", _linear_bwd, dict(x_ss=0, db=AT), "overlap"),
+    ("hier_linear_bwd", _linear_bwd, dict(w_ss=0, db=AT), "overlap"),
+    ("hier_linear_bwd", _linear_bwd, dict(w_ss=0, dx=None, db=AT), "workspace"),
+    ("hier_linear_bwd", _linear_bwd, dict(x_ss=0, M=1, db=AT), "workspace"),
     ("hier_cross_attn", _cross, dict(D=32), "head_dim"),
     ("hier_cross_attn", _cross, dict(Hq=5), "invalid"),
     ("hier_cross_attn", _cross, dict(type=2), "bf16 or fp16"),

@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from multics_amd import block, kernels
+from multics_amd import _capi, block, kernels
 from multics_amd.module import CrossAttention, FeedForward, _gated
 from tests.gpu_util import need_gpu, say
 from tests.test_block import CHANGES, EPILOGUES, _Adapter, change_ffn
@@ -85,6 +85,20 @@ def test_product_of_rows_far_apart(B, S, K, N, act):
         leaves = [t.detach().requires_grad_() for t in (rows, weights, b)]
         grads.append(torch.autograd.grad(kernels.linear_act_train(*leaves, activation=act), leaves, dy))
     assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_weights_gradient_of_one_row_at_a_stride_of_0():
+    """The C entry: an infinity of the only row is one in dw (the rows past it are not that row)."""
+    need_gpu()
+    x, w = torch.zeros(1, 64, dtype=BF16, device="cuda"), torch.ones(32, 64, dtype=BF16, device="cuda")
+    x[0, 3], x[0, 4] = float("inf"), 2.0
+    dy, dw = torch.ones(1, 32, dtype=BF16, device="cuda"), torch.empty(32, 64, dtype=BF16, device="cuda")
+    fields = (1, 32, 64, 0, 0, x.data_ptr(), w.data_ptr(), 0, dy.data_ptr(), 0, 0, dw.data_ptr(), 0, 0, 0, 64, 0, 32, 0,
+              64, 64, 1)
+    size = block._workspace("hier_linear_bwd_workspace", block._pack_linear_bwd(*fields, 0, 0))
+    ws = torch.empty(max(size, 1), dtype=torch.uint8, device="cuda")
+    _capi.call_on(x.device, "hier_linear_bwd", block._pack_linear_bwd(*fields, ws.data_ptr(), size))
+    assert torch.equal(dw, x.expand(32, 64))
 
 
 # ---- what a gradient reads ----------------------------------------------------------------
