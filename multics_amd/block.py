@@ -196,8 +196,8 @@ def rms_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, *
     M = xr.shape[0]
     if M == 0:
         return dx, dw.zero_()
-    # a row of sums for each workgroup (checked by the entry)
-    rows = min((M + 3) // 4 if C <= 2048 else M, 512)
+    # a row of sums for each workgroup
+    rows = _workspace("hier_rms_norm_bwd_rows", _pack_norm_bwd(M, C, eps, kind, 0, *(0,) * 14))
     part = x.new_empty((rows, C), dtype=torch.float32)
     _capi.call_on(x.device, "hier_rms_norm_bwd", _pack_norm_bwd(
         M, C, eps, kind, _TYPES[w.dtype], xr.data_ptr(), _ptr(r), w.data_ptr(), g.data_ptr(), _ptr(d),
