@@ -100,20 +100,27 @@ def _operands(x: torch.Tensor, w: torch.Tensor, read=(True, True)):
     return at[0], ss[0], at[1], ss[1], Kp, (x, w, buf)
 
 
+def _extent(t: torch.Tensor):
+    """The addresses that ``t`` lies within."""
+    first, size = t.data_ptr(), t.element_size()
+    if t.is_contiguous():
+        return first, first + t.numel() * size
+    return first, first + size * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
 def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two tensors may have a byte in common: not where one ends before the other
     begins, nor where both are rows (of whatever inner dimensions) of one pitch that lie
     side by side, as a projection's slices do."""
-    if not a.numel() or not b.numel():
+    (pa, ea), (pb, eb) = _extent(a), _extent(b)
+    if ea <= pb or eb <= pa or not a.numel() or not b.numel():
         return False
-    (pa, da, ia), (pb, db, ib) = (
-        (t.data_ptr(), [(n, s * t.element_size()) for n, s in zip(t.shape, t.stride()) if n > 1 and s], t.element_size())
+    (da, ia), (db, ib) = (
+        ([(n, s * t.element_size()) for n, s in zip(t.shape, t.stride()) if n > 1 and s], t.element_size())
         for t in (a, b))
 
-    def span(dims, item, below=math.inf):
+    def span(dims, item, below):
         return sum((n - 1) * s for n, s in dims if s < below) + item
-    if pa + span(da, ia) <= pb or pb + span(db, ib) <= pa:
-        return False
     strides = {s for _, s in da + db}
     for least in strides:
         pitch = math.gcd(*(s for s in strides if s >= least))
@@ -477,7 +484,6 @@ def _cross(q, k, v, kv_lens, key_mask, scale, out, lse):
         raise ValueError("out must have rows of its own, a unit-stride head dimension and 16-byte rows")
     if lse is not None:
         _check_lse(lse, sizes, q.device)
-        _apart("lse", lse, q=q, k=k, v=v, kv_lens=kv_lens, key_mask=key_mask, out=out)
     if B == 0 or Sq == 0:
         return out
     fields = _cross_fields(sizes, qh, kh, vh, oh, lse, lens, mask)
@@ -502,6 +508,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     row.  ``out`` and ``lse`` share no memory with the inputs or one another.  Sq may be one token: the keys are then cut into parts that fill the GPU.
     No gradient: ``cross_attention_train``."""
     _no_grad_call("cross_attention", q, k, v)
+    if lse is not None:
+        _apart("lse", lse, q=q, k=k, v=v, kv_lens=kv_lens, key_mask=key_mask, out=out)
     return _cross(q, k, v, kv_lens, key_mask, scale, out, lse)
 
 
