@@ -102,7 +102,7 @@ class FeedForward(nn.Sequential):
 
     def forward(self, x, *, residual=None, gate=None):
         if self._fused(x):
-            up, _, down = self
+            up, _, down = self._modules.values()
             linear = linear_act_train if torch.is_grad_enabled() else linear_act
             h = linear(x, up.weight, up.bias, activation="gelu_tanh")
             return _gated_product(linear, h, down, residual, gate)
@@ -110,8 +110,10 @@ class FeedForward(nn.Sequential):
 
     def _fused(self, x) -> bool:
         """Whether the kernels do what the children would, called as modules."""
-        return len(self) == 3 and _product(self[0], x) and _plain(self[1], nn.GELU) and \
-            self[1].approximate == "tanh" and _product(self[2], x)
+        if len(self._modules) != 3:
+            return False
+        up, act, down = self._modules.values()
+        return _product(up, x) and _plain(act, nn.GELU) and act.approximate == "tanh" and _product(down, x)
 
 
 def _plain(module, *classes) -> bool:
@@ -199,6 +201,8 @@ class CrossAttention(nn.Module):
     def forward(self, x, context=None, *, kv=None, kv_lens=None, key_mask=None, residual=None, gate=None):
         if (context is None) == (kv is None):
             raise ValueError("pass context or kv (from project_context)")
+        # (q, k, v and a bare o are calls of their modules: 18,816 rows of 1,536 x 1,536 take
+        # the library 73 us and linear_act 85, 4,620 rows 27 and 28, 660 rows 19 and 15)
         k, v = self.project_context(context) if kv is None else kv
         q = self._heads(self._norm(self.norm_q, self.q(x)))
         if self._fused(q) and q.dtype == k.dtype == v.dtype:
