@@ -20,8 +20,13 @@
 // dP starts from -delta, as S does from -m in the forward: the subtraction is the
 // matrix product's.
 //
-// Measured, bf16, D 128: four streams of 4,620 rows x 12 heads against 512 keys dq 122 us
-// (three products, 714 TFLOP/s), dkv 138 (four, 842); 8,192 x 8,192 x 16 heads both 1,670
+// Rounded to 16 bits: P (for dV) and dS, as the MFMAs' operands; and through the forward,
+// O (delta is taken of it as it is given) and the weights whose sum lse is.  A result's
+// relative error is that of its own rounding and dS's, 0.0024, where the others average out
+// over some 200 keys, up to 0.0039 over a handful.
+//
+// Measured, bf16, D 128: four streams of 4,620 rows x 12 heads against 512 keys dq 124 us
+// (three products, 703 TFLOP/s; MFMA busy 30 % of the time), dkv 141 (four, 824; 36 %); 8,192 x 8,192 x 16 heads both 1,670
 // (823 TFLOP/s, counting five products).  No bank conflicts.
 #include "hier_cross.h"
 
@@ -579,8 +584,8 @@ __global__ __launch_bounds__(256) void cross_grad_join_kernel(Launch p) {
 }
 
 // Parts (SplitModel).  dK, dV, of the rows: 192 items of 73 tiles 132 us in one part, 152 in
-// four (three whole rounds of workgroups; the power bounds them: three quarters of the
-// CUs make as many tiles as all); 32 items of 128 tiles, D 64, 147 us with dq in one, 54
+// four (three whole rounds of workgroups, but every part starts, ends and leaves 128 KB of
+// fp32 sums to join: the fourth of the CUs that is idle in one part is not worth that); 32 items of 128 tiles, D 64, 147 us with dq in one, 54
 // in eight, 58 in sixteen.  dQ, of the keys: 12 items of 128
 // tiles (one row each) 238 us with dK and dV in one part, 57 in 26.
 int dkv_splits(const HierCrossArgs& a) {

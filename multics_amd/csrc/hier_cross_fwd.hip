@@ -18,10 +18,11 @@
 // Rows are few where a token asks: the keys are then cut into splits, whose
 // fp32 sums and maxima a second kernel joins in their order.
 //
-// Measured, bf16, D 128: 8,192 x 8,192 x 16 heads 540 us (1,017 TFLOP/s); four streams of
-// 4,620 rows x 12 heads against 512 keys 97 (600: eight tiles an item, whose first loads
-// and last stores are a third of its time; 3.5 rounds of workgroups).  Workgroups that
-// stay and ask for the next item's first tiles under the present one's last: 97.5, and
+// Measured, bf16, D 128: 8,192 x 8,192 x 16 heads 540 us (1,017 TFLOP/s; MFMA busy 47 % of
+// the time, counted in a launch alone, the vector units 34 %); four streams of
+// 4,620 rows x 12 heads against 512 keys 95 (612; MFMA 25 %: eight tiles an item, whose first
+// loads and last stores are a third of its time; 3.5 rounds of workgroups).  Workgroups that
+// stay and ask for the next item's first tiles under the present one's last: no faster there, and
 // ten streams of 660 rows 40 for 36 (registers spilled), not kept.
 #include "hier_cross.h"
 

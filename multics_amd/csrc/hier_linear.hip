@@ -14,8 +14,10 @@
 // with tanh GELU 477 -- a tile's epilogue takes 9 us beside the 35 of its products, 13
 // with the GELU's two transcendentals an element --, of K 7,680 1,304 TFLOP/s: there the
 // power limit sets the clock, and nothing but energy is left to save.  6,600 x 1,536 x 8,960 with gate and
-// residual 175: 156 tiles, so 100 of 256 CUs idle.  Gradients of 9,408 x 8,960 x 1,536: dz 121,
-// dx and dw 203 each (1,270 TFLOP/s).
+// residual 170: 156 tiles, so 100 of 256 CUs idle (a library product of that size 145, 155 with
+// gated_residual behind it).  Gradients of 9,408 x 8,960 x 1,536: dz 115, dx 203, dw 206 (1,270 and
+// 1,250 TFLOP/s).  1,536 x 1,536 for 660 / 4,620 / 18,816 rows 15 / 28 / 85, library 19 / 27 / 73:
+// short K, where a tile's epilogue is a fifth of it.
 #include "hier_gemm.h"
 
 #include <algorithm>
@@ -708,8 +710,9 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs p) {
 // at most (dg's sums then meet in sum_rows), else whole gates.
 //
 // Bound by memory and, with an activation, by the vector units beside it: 9,408 x 8,960
-// (506 MB) with tanh GELU 121 us, 4.2 TB/s; a row's loads alone 183, eight rows' 121,
-// twice the workgroups 128.
+// (506 MB) with tanh GELU 115 us, 4.4 TB/s.  Tried before a NaN's test, one after the other
+// without gaps, where it took 121: a row's loads alone 183, eight rows' 121, twice the
+// workgroups 128.
 
 struct DzArgs {
   const void* dy;

@@ -16,8 +16,10 @@
 //
 // Measured, bf16: 18,816 x 1,536 with residual 41 us (231 MB, 5.6 TB/s; a copy of as
 // much reaches 5.1), its gradient 59 + 4 of sum_rows (289 MB, 4.9 TB/s); with a row's
-// loads one after the other, each waited for by its conversion, 70 and 90.  2 x 1,536:
-// 2.6, a launch.  512 workgroups of the gradient: each sum is one row to read again.
+// loads one after the other, each waited for by its conversion, 70 and 90.  At an odd
+// address (2-byte accesses) 45 and 65, 24 for 20 without residual: whole lines all the same, but
+// eight instructions for one; 1,537 channels, a fourth chunk, 57 and 78.  2 x 1,536: 2.6,
+// a launch.  512 workgroups of the gradient: each sum is one row to read again.
 #include "hier_launch.h"
 #include "hier_types.h"
 
