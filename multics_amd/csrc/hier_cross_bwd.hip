@@ -12,7 +12,8 @@
 //         wave w + 4 of the same keys dP, dS and dK, P handed over through LDS as
 //         fp16.  P is 2^15 times the weight throughout (hence the 15 above; dK and dV
 //         are scaled back at the end): a weight is at most 1, and down to 2^-29 it keeps
-//         fp16's eleven bits, as many keys as a call may have.  (lse in fp32 leaves a weight's
+//         fp16's eleven bits, as many keys as a call may have, while fp32 holds the sums
+//         of gradients up to 10^33.  (lse in fp32 leaves a weight's
 //         exponent off by 2^-23 of the score: past scores of 5 million one may come out
 //         as 2, which fp16 does not hold.)  Items are few where the keys are
 //         (an encoder's 512 are four a head): the rows may then be cut into splits, whose

@@ -286,6 +286,39 @@ def test_modules_with_residuals_and_gates_of_other_types_and_shapes(residual, ga
         assert bool(((y.double() - want.double()).abs() <= 2.0 ** -7 * slack + 1e-6).all())
 
 
+@pytest.mark.parametrize("how", ["autocast", "fp16"])
+def test_cross_attention_of_wider_weights_and_of_fp16_trains(how):
+    """fp32 weights under autocast (the projections' bf16 goes to the kernels), and fp16 with
+    gradients (torch operations), NaN in hidden states: against the module in 64 bits."""
+    need_gpu()
+    torch.manual_seed(5)
+    attn = CrossAttention(128, 2).cuda()
+    if how == "fp16":
+        attn = attn.half()
+    wide = copy.deepcopy(attn).double()
+    t = torch.float32 if how == "autocast" else FP16
+    x, ctx, dy = _rnd(1)(2, 20, 128).to(t), _rnd(2)(2, 9, 128).to(t), _rnd(3)(2, 20, 128).to(t)
+    lens = torch.tensor([9, 4], device="cuda", dtype=torch.int32)
+
+    def run(attn, x, ctx, dy, cast, bad):
+        x = x.clone().requires_grad_()
+        with torch.autocast("cuda", torch.bfloat16, enabled=cast):
+            k, v = attn.project_context(ctx)
+            hide = torch.arange(9, device="cuda")[None, :, None, None] >= lens[:, None, None, None]
+            k, v = (torch.where(hide, torch.full_like(u, bad), u) for u in (k, v))
+            y = attn(x, kv=(k, v), kv_lens=lens, residual=x)
+        return y, torch.autograd.grad(y, [x, *attn.parameters()], dy.to(y.dtype))
+    y, grads = run(attn, x, ctx, dy, how == "autocast", float("nan"))
+    ref, want = run(wide, x.double(), ctx.double(), dy.double(), False, 0.0)
+    # some ten roundings in a row, in the norm; the module's own norm is fp32 inside, hence 2^-18
+    step = _step(BF16 if how == "autocast" else FP16)
+    names = ["x", *(n for n, _ in attn.named_parameters())]
+    assert float((y.double() - ref).norm()) <= 10 * step * float(ref.norm())
+    for name, a, b in zip(names, grads, want):
+        if name != "k.bias":            # (zero but for the norm's change from key to key)
+            assert float((a.double() - b).norm()) <= (16 * step + 2.0 ** -18) * float(b.norm()), name
+
+
 # ---- many rows ---------------------------------------------------------------------------
 
 def test_norm_of_more_rows_than_a_line_of_threads():
