@@ -41,6 +41,14 @@ def _pad(**kw):
     return _capi.HierPadRowsArgs(**{**f, **kw})
 
 
+@pytest.fixture(autouse=True)
+def _no_error_left():
+    """Whatever test runs next in this process finds no refusal of these."""
+    yield
+    args = _linear(M=0)
+    assert _capi.lib().hier_linear(C.addressof(args), None) == 0
+
+
 REFUSED = [
     ("hier_rms_norm", _norm, dict(C=0), "invalid"),
     ("hier_rms_norm", _norm, dict(C=16385, x_ss=16385, y_ss=16385), "16384"),

@@ -313,7 +313,7 @@ def test_cross_attention_of_wider_weights_and_of_fp16_trains(how):
     # some ten roundings in a row, in the norm; the module's own norm is fp32 inside, hence 2^-18
     step = _step(BF16 if how == "autocast" else FP16)
     names = ["x", *(n for n, _ in attn.named_parameters())]
-    assert float((y.double() - ref).norm()) <= 10 * step * float(ref.norm())
+    assert float((y.detach().double() - ref).detach().norm()) <= 10 * step * float(ref.detach().norm())
     for name, a, b in zip(names, grads, want):
         if name != "k.bias":            # (zero but for the norm's change from key to key)
             assert float((a.double() - b).norm()) <= (16 * step + 2.0 ** -18) * float(b.norm()), name
