@@ -824,8 +824,9 @@ int hier_linear_bwd(const HierLinearBwdArgs* args, void* stream);
 /* Sk; taken within [0, Sk]) counts a stream's keys, key_mask (bytes, NULL: */
 /* all) says which are seen; the rest of k and v is not read.  16-byte rows, */
 /* k_ss and v_ss at least D.  lse: fp32 [B][Hq][Sq] or NULL, -inf where no key */
-/* is seen.  o and lse share no memory with what is read.  `workspace` (hier_cross_workspace(args) bytes, 16-byte aligned)  */
-/* belongs to one call at a time.                                            */
+/* is seen.  o and lse share no memory with what is read.  `workspace`        */
+/* (hier_cross_workspace(args) bytes, 16-byte aligned) belongs to one call at */
+/* a time.                                                                    */
 typedef struct HierCrossArgs {
   int32_t B, Hq, Hk, D;
   int32_t type;

@@ -317,8 +317,9 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     ``"gelu_tanh"``, ``"gelu"`` or ``"silu"``.  ``residual`` is [..., N]; ``gate`` is
     [N], or [..., F, N] whose rows scale S / F rows of x's S each (a frame's tokens
     share their frame's gate, as in ``gated_residual``).  ``out`` (optional, contiguous)
-    may be ``residual`` itself and shares no memory with the inputs otherwise.  Rows of a multiple of eight channels are read in place,
-    others, and rows 2^21 elements apart or more, are copied with zeros behind.  No gradient: ``linear_act_train``."""
+    may be ``residual`` itself and shares no memory with the inputs otherwise.  Rows of a
+    multiple of eight channels are read in place, others, and rows 2^21 elements apart or
+    more, are copied with zeros behind.  No gradient: ``linear_act_train``."""
     _no_grad_call("linear_act", x, weight, bias, residual, gate)
     return _linear(x, weight, bias, activation, residual, gate, out, None)
 
@@ -505,8 +506,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     [B, Sk] (bool) is true; what else k and v hold is not read.  Returns [B, Sq, H, D]
     (``out`` where given); a row that sees no key is 0.  ``lse`` (optional, contiguous
     fp32 [B, H, Sq]) receives the natural-log softmax normaliser, -inf for such a
-    row.  ``out`` and ``lse`` share no memory with the inputs or one another.  Sq may be one token: the keys are then cut into parts that fill the GPU.
-    No gradient: ``cross_attention_train``."""
+    row.  ``out`` and ``lse`` share no memory with the inputs or one another.  Sq may be
+    one token: the keys are then cut into parts that fill the GPU.  No gradient: ``cross_attention_train``."""
     _no_grad_call("cross_attention", q, k, v)
     if lse is not None:
         _apart("lse", lse, q=q, k=k, v=v, kv_lens=kv_lens, key_mask=key_mask, out=out)

@@ -193,7 +193,8 @@ def test_outputs_in_the_memory_of_inputs():
     q, k, v = qkv.unbind(2)
     lse = torch.empty(2, 4, 50, device="cuda")
     floats = torch.empty(2 * 50 * 4 * 32, device="cuda")
-    cases = [dict(out=q), dict(out=k), dict(out=v), dict(out=q.flip(1).contiguous(), lse=qkv.view(-1).view(torch.float32)[:400].view(2, 4, 50)),
+    cases = [dict(out=q), dict(out=k), dict(out=v),
+             dict(out=q.flip(1).contiguous(), lse=qkv.view(-1).view(torch.float32)[:400].view(2, 4, 50)),
              dict(out=floats.view(BF16).view(2, 50, 4, 64), lse=floats[:400].view(2, 4, 50))]
     for kw in cases:
         with pytest.raises(ValueError, match="share memory"):
